@@ -1,0 +1,125 @@
+// Shared between the kernels of rotary positions, cache pages and attention and their entry points (hspmm_cache.hip).
+#pragma once
+#include "hspmm_device.h"
+
+namespace hspmm {
+
+// n / d for n < 2^31 by a multiplication: with l = ceil(log2 d) and m = floor(2^(31 + l) / d) + 1, n m >> (31 + l) is the
+// quotient (Granlund and Montgomery, "Division by Invariant Integers using Multiplication", 1994).
+struct Divisor {
+    uint32_t d, m, shift;
+    static Divisor of(uint32_t d)
+    {
+        uint32_t l = 0;
+        while (l < 31u && (1u << l) < d) ++l;
+        return Divisor{d, uint32_t((uint64_t(1) << (31u + l)) / d + 1u), 31u + l};
+    }
+    __host__ __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return uint32_t((uint64_t(n) * m) >> shift); }
+};
+
+// One layer of a cache (strides in elements).
+struct PagesArgs {
+    char *keys, *values;
+    const int32_t *table, *lengths;
+    uint32_t pages, sequences, table_pages, heads, head_dim;
+    Divisor page_tokens;
+    int64_t page_stride, head_stride, token_stride;
+};
+
+struct BatchArgs {
+    const int32_t *starts, *rows;
+    uint32_t sequences, tokens;
+};
+
+struct HeadsArgs {
+    char *data;
+    int64_t token_stride, head_stride, dim_stride;
+};
+
+// What a rotation's launch turns and copies: `q_heads` heads from q to q_out, turned; k_heads heads from k, turned, and from v into pages.
+struct RotaryArgs {
+    HeadsArgs q, q_out, k, v;
+    uint32_t q_heads, k_heads;
+    uint32_t head_dim, dims, interleaved, positions;
+    float sign;                          // of the sines
+    const float *table;                  // null: nothing turns
+    const int32_t *at;                   // positions of tokens; null: where they stand in the cache
+    uint32_t tokens;
+    PagesArgs pages;
+    BatchArgs batch;
+};
+// vec: elements that a lane moves at a time where a head's elements lie side by side everywhere, 0: through LDS, any strides
+hipError_t launch_rotary(int dtype, const RotaryArgs &ra, uint32_t vec, hipStream_t s);
+
+struct AttendArgs {
+    PagesArgs pages;
+    BatchArgs batch;
+    HeadsArgs q, out;
+    float *lse;
+    uint32_t q_heads;
+    Divisor shared;                      // heads of queries to one of keys
+    float scale;
+    uint32_t causal, window;
+    uint32_t splits;                     // parts that a sequence's keys are cut into
+    float *sums;                         // of more than one part: their sums
+    uint32_t *arrive;                    // and how many have left them (zero between launches)
+};
+hipError_t launch_attend_simple(int dtype, const AttendArgs &aa, hipStream_t s);
+
+// Page work: all layers.
+struct PoolArgs {
+    char *keys, *values;
+    int32_t *table, *lengths, *references, *scratch;
+    uint32_t layers, pages, heads, sequences, table_pages;
+    Divisor page_tokens;
+    uint32_t token_bytes;                // of one head
+    uint32_t heads_first;
+    uint32_t unit;                       // bytes moved at a time: 16, 4 or 2
+    int64_t page_bytes, layer_bytes;     // from one to the next
+};
+hipError_t launch_pages_extend(const PoolArgs &pa, uint32_t n, const int32_t *rows, const int32_t *add, int32_t *status, hipStream_t s);
+hipError_t launch_pages_fork(const PoolArgs &pa, uint32_t n, const int32_t *parents, const int32_t *children, int32_t *status, hipStream_t s);
+hipError_t launch_pages_free(const PoolArgs &pa, uint32_t n, const int32_t *rows, hipStream_t s);
+hipError_t launch_pages_compact(const PoolArgs &pa, int32_t *table_out, int32_t *references_out, int32_t *live, hipStream_t s);
+hipError_t launch_pages_copy(const PoolArgs &pa, uint32_t n, const int32_t *from, const int32_t *to, hipStream_t s);
+
+#ifdef __HIPCC__
+// Where token t of a batch stands: its batch row (kIdxMax: outside every chunk), sequence, position (-1 and less: in front of the cache).
+struct TokenPlace { uint32_t sequence; int32_t position; bool there; };
+
+__device__ __forceinline__ int32_t clamp_i32(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// Tokens a sequence has, within what its row of the table can hold.
+__device__ __forceinline__ int32_t tokens_held(const PagesArgs &pg, uint32_t sequence)
+{
+    const int64_t most = int64_t(pg.table_pages) * pg.page_tokens.d;
+    return clamp_i32(pg.lengths[sequence], 0, most > 0x7FFFFFFF ? 0x7FFFFFFF : int32_t(most));
+}
+
+__device__ __forceinline__ TokenPlace token_place(const BatchArgs &ba, const PagesArgs &pg, uint32_t t)
+{
+    // the last batch row that starts at or in front of t
+    uint32_t lo = 0, hi = ba.sequences;
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) / 2u;
+        if (ba.starts[mid] <= int32_t(t)) lo = mid; else hi = mid;
+    }
+    const int32_t first = ba.starts[lo], end = ba.starts[lo + 1u];
+    const uint32_t sequence = ba.rows ? uint32_t(ba.rows[lo]) : lo;
+    if (first > int32_t(t) || end <= int32_t(t) || end > int32_t(ba.tokens) || sequence >= pg.sequences) return TokenPlace{0u, -1, false};
+    return TokenPlace{sequence, tokens_held(pg, sequence) - end + int32_t(t), true};
+}
+
+// Element offset of a position's row in the pages, -1: it is not stored.
+__device__ __forceinline__ int64_t row_offset(const PagesArgs &pg, uint32_t sequence, int32_t position, uint32_t head)
+{
+    if (position < 0) return -1;
+    const uint32_t place = pg.page_tokens.quotient(uint32_t(position));
+    if (place >= pg.table_pages) return -1;
+    const uint32_t id = uint32_t(pg.table[size_t(sequence) * pg.table_pages + place]);
+    if (id >= pg.pages) return -1;
+    return int64_t(id) * pg.page_stride + int64_t(head) * pg.head_stride + int64_t(uint32_t(position) - place * pg.page_tokens.d) * pg.token_stride;
+}
+#endif
+
+}  // namespace hspmm

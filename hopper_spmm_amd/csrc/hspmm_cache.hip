@@ -1,0 +1,370 @@
+// Entry points of rotary positions, the paged cache and the attention over it (include/hspmm.h): checks of arguments, the rules
+// that choose kernels, launches.  They keep nothing: what a call uses is the caller's.
+#include "hspmm_plan.hpp"
+#include "cache_device.h"
+
+using namespace hspmm_host;
+using namespace hspmm;
+
+namespace {
+
+uint32_t element_bytes(int dtype) { return dtype == HSPMM_TF32 ? 4u : 2u; }
+
+int check_dtype(int dtype)
+{
+    if (dtype != HSPMM_FP16 && dtype != HSPMM_BF16 && dtype != HSPMM_TF32)
+        return fail(HSPMM_ERR_INVALID, "dtype %d: HSPMM_FP16, HSPMM_TF32 or HSPMM_BF16", dtype);
+    return HSPMM_OK;
+}
+
+// Compute units of the current device, which has to be a gfx950 (asked for once per device).
+int current_device(uint32_t *compute_units)
+{
+    static std::atomic<uint32_t> known[64];
+    int dev = -1;
+    HSPMM_HIP(hipGetDevice(&dev));
+    uint32_t units = dev >= 0 && dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0u;
+    if (!units) {
+        hipDeviceProp_t prop;
+        HSPMM_HIP(hipGetDeviceProperties(&prop, dev));
+        if (strncmp(prop.gcnArchName, "gfx950", 6) != 0)
+            return fail(HSPMM_ERR_UNSUPPORTED, "device %d is %s; this library is built for gfx950 only", dev, prop.gcnArchName);
+        units = uint32_t(prop.multiProcessorCount);
+        if (dev >= 0 && dev < 64) known[dev].store(units, std::memory_order_relaxed);
+    }
+    if (compute_units) *compute_units = units;
+    return HSPMM_OK;
+}
+
+int check_heads(const char *name, const hspmm_heads *x, int dtype)
+{
+    if (!x || !x->data) return fail(HSPMM_ERR_INVALID, "null %s", name);
+    if (reinterpret_cast<uintptr_t>(x->data) % element_bytes(dtype)) return fail(HSPMM_ERR_INVALID, "%s is not aligned to the element size", name);
+    if (x->token_stride < 0 || x->head_stride < 0 || x->dim_stride < 1) return fail(HSPMM_ERR_INVALID, "%s: strides below 0, or of elements below 1", name);
+    return HSPMM_OK;
+}
+
+int check_rotary(const hspmm_rotary *r, uint32_t head_dim)
+{
+    if (r->dims % 2u || r->dims > head_dim) return fail(HSPMM_ERR_INVALID, "%u of %u elements turn: an even number, at most all", r->dims, head_dim);
+    if (r->dims && (!r->table || reinterpret_cast<uintptr_t>(r->table) % 8u)) return fail(HSPMM_ERR_INVALID, "the table of rotary positions is null or not aligned to 8 bytes");
+    if (r->dims && (r->positions == 0 || r->positions > 0x7FFFFFFFu)) return fail(HSPMM_ERR_INVALID, "a table of %u positions", r->positions);
+    return HSPMM_OK;
+}
+
+int check_cache(const hspmm_cache *c)
+{
+    if (!c) return fail(HSPMM_ERR_INVALID, "null cache");
+    if (const int rc = check_dtype(c->dtype)) return rc;
+    if (c->order != HSPMM_HEADS_FIRST && c->order != HSPMM_TOKENS_FIRST) return fail(HSPMM_ERR_INVALID, "order %d of a page", c->order);
+    if (!c->layers || !c->pages || !c->page_tokens || !c->heads || !c->head_dim || !c->sequences || !c->table_pages)
+        return fail(HSPMM_ERR_INVALID, "a cache of %u layers, %u pages of %u tokens, %u heads of %u elements, %u sequences of %u pages", c->layers, c->pages,
+                    c->page_tokens, c->heads, c->head_dim, c->sequences, c->table_pages);
+    // (numbers that kernels multiply in 32 bits; a page is far below)
+    const uint64_t page = uint64_t(c->heads) * c->page_tokens;
+    if (c->pages > 0x3FFFFFFFu || c->page_tokens > 0x7FFFFFFFu || c->heads > 32768u || c->head_dim > 32768u || page > (1u << 30) || page * c->head_dim > (1u << 29) ||
+        uint64_t(c->sequences) * c->table_pages > 0x7FFFFFFFu || c->layers > 16384u)
+        return fail(HSPMM_ERR_UNSUPPORTED, "a cache of %u layers, %u pages of %u tokens, %u heads of %u elements, %u sequences of %u pages", c->layers, c->pages,
+                    c->page_tokens, c->heads, c->head_dim, c->sequences, c->table_pages);
+    const int64_t elements = int64_t(page * c->head_dim);
+    if (c->page_stride < 0 || (c->page_stride && c->page_stride < elements)) return fail(HSPMM_ERR_INVALID, "pages of %lld elements, %lld apart", (long long)elements, (long long)c->page_stride);
+    if (c->layer_stride < 0) return fail(HSPMM_ERR_INVALID, "layers %lld elements apart", (long long)c->layer_stride);
+    if (!c->keys || !c->values || !c->table || !c->lengths || !c->references || !c->scratch) return fail(HSPMM_ERR_INVALID, "a null array of the cache");
+    if (reinterpret_cast<uintptr_t>(c->keys) % 16u || reinterpret_cast<uintptr_t>(c->values) % 16u) return fail(HSPMM_ERR_INVALID, "keys and values must be aligned to 16 bytes");
+    return HSPMM_OK;
+}
+
+int64_t page_stride(const hspmm_cache *c) { return c->page_stride ? c->page_stride : int64_t(c->heads) * c->page_tokens * c->head_dim; }
+int64_t layer_stride(const hspmm_cache *c) { return c->layer_stride ? c->layer_stride : page_stride(c) * c->pages; }
+
+PagesArgs pages_of(const hspmm_cache *c, uint32_t layer)
+{
+    PagesArgs pg{};
+    const int64_t at = layer_stride(c) * layer * element_bytes(c->dtype);
+    pg.keys = static_cast<char *>(c->keys) + at;
+    pg.values = static_cast<char *>(c->values) + at;
+    pg.table = c->table; pg.lengths = c->lengths;
+    pg.pages = c->pages; pg.sequences = c->sequences; pg.table_pages = c->table_pages; pg.heads = c->heads; pg.head_dim = c->head_dim;
+    pg.page_tokens = Divisor::of(c->page_tokens);
+    pg.page_stride = page_stride(c);
+    pg.head_stride = c->order == HSPMM_HEADS_FIRST ? int64_t(c->page_tokens) * c->head_dim : c->head_dim;
+    pg.token_stride = c->order == HSPMM_HEADS_FIRST ? c->head_dim : int64_t(c->heads) * c->head_dim;
+    return pg;
+}
+
+PoolArgs pool_of(const hspmm_cache *c)
+{
+    PoolArgs pa{};
+    const uint32_t e = element_bytes(c->dtype);
+    pa.keys = static_cast<char *>(c->keys); pa.values = static_cast<char *>(c->values);
+    pa.table = c->table; pa.lengths = c->lengths; pa.references = c->references; pa.scratch = c->scratch;
+    pa.layers = c->layers; pa.pages = c->pages; pa.heads = c->heads; pa.sequences = c->sequences; pa.table_pages = c->table_pages;
+    pa.page_tokens = Divisor::of(c->page_tokens);
+    pa.token_bytes = c->head_dim * e;
+    pa.heads_first = c->order == HSPMM_HEADS_FIRST;
+    pa.page_bytes = page_stride(c) * e;
+    pa.layer_bytes = layer_stride(c) * e;
+    const uint64_t all = uint64_t(pa.token_bytes) | uint64_t(pa.page_bytes) | uint64_t(pa.layer_bytes);
+    pa.unit = all % 16u == 0u ? 16u : all % 4u == 0u ? 4u : 2u;
+    return pa;
+}
+
+int check_batch(const hspmm_cache *c, const hspmm_batch *b)
+{
+    if (!b) return fail(HSPMM_ERR_INVALID, "null batch");
+    if (b->tokens && (!b->sequences || !b->starts)) return fail(HSPMM_ERR_INVALID, "a batch of %u tokens without sequences or their starts", b->tokens);
+    if (b->tokens > 0x7FFFFFFEu || b->sequences > 0x7FFFFFFEu) return fail(HSPMM_ERR_UNSUPPORTED, "a batch of %u tokens, %u sequences", b->tokens, b->sequences);
+    if (!b->rows && b->sequences > c->sequences) return fail(HSPMM_ERR_INVALID, "a batch of %u sequences for a cache of %u", b->sequences, c->sequences);
+    return HSPMM_OK;
+}
+
+int check_list(const hspmm_cache *c, uint32_t n, const void *list, const char *name)
+{
+    if (n > c->sequences) return fail(HSPMM_ERR_INVALID, "a list of %u for a cache of %u sequences", n, c->sequences);
+    if (n && !list) return fail(HSPMM_ERR_INVALID, "null %s", name);
+    return HSPMM_OK;
+}
+
+BatchArgs batch_of(const hspmm_batch *b) { return BatchArgs{b->starts, b->rows, b->sequences, b->tokens}; }
+HeadsArgs heads_of(const hspmm_heads *x)
+{
+    return x ? HeadsArgs{static_cast<char *>(x->data), x->token_stride, x->head_stride, x->dim_stride} : HeadsArgs{nullptr, 0, 0, 1};
+}
+
+// Elements that the piece kernel moves at a time, 0: it cannot (elements apart, or pairs between two pieces).
+uint32_t rotary_piece(int dtype, const RotaryArgs &ra, const hspmm_cache *c)
+{
+    const uint32_t e = element_bytes(dtype);
+    uint64_t all = ra.head_dim | (16u / e);
+    if (ra.table) all |= ra.interleaved ? ra.dims : ra.dims / 2u;
+    const HeadsArgs *tensors[4] = {ra.q_heads ? &ra.q : nullptr, ra.q_heads ? &ra.q_out : nullptr, ra.k_heads ? &ra.k : nullptr, ra.k_heads ? &ra.v : nullptr};
+    for (const HeadsArgs *x : tensors) {
+        if (!x) continue;
+        if (x->dim_stride != 1) return 0u;
+        all |= uint64_t(x->token_stride) | uint64_t(x->head_stride) | (reinterpret_cast<uintptr_t>(x->data) / e);
+    }
+    if (c) all |= uint64_t(page_stride(c)) | uint64_t(layer_stride(c));
+    const uint32_t vec = uint32_t(all & ~(all - 1u));
+    if (vec == 1u && ra.table && ra.interleaved) return 0u;
+    // items are numbered in 31 bits
+    if (uint64_t(ra.head_dim / vec) * (ra.q_heads + 2u * ra.k_heads) * (c ? ra.tokens : 1u) >= 0x7FFFFFFFu) return 0u;
+    return vec;
+}
+
+int run_rotary(int dtype, const RotaryArgs &ra, const hspmm_cache *c, void *stream)
+{
+    const uint32_t vec = rotary_piece(dtype, ra, c);
+    if (!vec) {
+        const uint64_t groups = (uint64_t(ra.tokens) + 63u) / 64u * ((ra.head_dim + 63u) / 64u) * (ra.q_heads + 2u * ra.k_heads);
+        if (groups >= (1u << 24)) return fail(HSPMM_ERR_UNSUPPORTED, "%u tokens of %u heads at these strides: in several calls", ra.tokens, ra.q_heads + 2u * ra.k_heads);
+    }
+    HSPMM_HIP(launch_rotary(dtype, ra, vec, static_cast<hipStream_t>(stream)));
+    return HSPMM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int hspmm_rotary_table(int kind, uint32_t dims, double base, double factor, double original_length, double fast_turns, double slow_turns,
+                       uint32_t positions, float *table)
+{
+    if (kind < HSPMM_ROTARY_PLAIN || kind > HSPMM_ROTARY_YARN) return fail(HSPMM_ERR_INVALID, "rotary positions of kind %d", kind);
+    if (dims == 0 || dims % 2u || dims > 65536u) return fail(HSPMM_ERR_INVALID, "%u elements turn: an even number above 0", dims);
+    if (!(base > 1.0) || !std::isfinite(base)) return fail(HSPMM_ERR_INVALID, "base %g", base);
+    if (kind != HSPMM_ROTARY_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor))) return fail(HSPMM_ERR_INVALID, "factor %g", factor);
+    if (kind == HSPMM_ROTARY_BASE && dims == 2u) return fail(HSPMM_ERR_INVALID, "a scaled base wants more than one pair");
+    if (kind == HSPMM_ROTARY_YARN && (!(original_length > 0.0) || !(slow_turns > 0.0) || !(fast_turns > slow_turns) || !std::isfinite(original_length) || !std::isfinite(fast_turns)))
+        return fail(HSPMM_ERR_INVALID, "original length %g, turns %g and %g", original_length, fast_turns, slow_turns);
+    if (positions && !table) return fail(HSPMM_ERR_INVALID, "null table");
+    const uint32_t pairs = dims / 2u;
+    try {
+        constexpr double kTurn = 6.283185307179586476925286766559;
+        const double b = kind == HSPMM_ROTARY_BASE ? base * std::pow(factor, double(dims) / double(dims - 2u)) : base;
+        const double scale = kind == HSPMM_ROTARY_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
+        // the pair whose wavelength turns that often within the original length
+        auto pair_of = [&](double turns) { return double(dims) * std::log(original_length / (turns * kTurn)) / (2.0 * std::log(base)); };
+        double low = 0.0, high = 0.0;
+        if (kind == HSPMM_ROTARY_YARN) {
+            low = std::max(std::floor(pair_of(fast_turns)), 0.0);
+            high = std::min(std::ceil(pair_of(slow_turns)), double(dims - 1u));
+            if (high <= low) high = low + 0.001;
+        }
+        std::vector<double> f(pairs);
+        for (uint32_t i = 0; i < pairs; ++i) {
+            f[i] = std::pow(b, -2.0 * i / dims);
+            if (kind == HSPMM_ROTARY_LINEAR) f[i] /= factor;
+            if (kind == HSPMM_ROTARY_YARN) {
+                const double ramp = std::min(std::max((i - low) / (high - low), 0.0), 1.0);
+                f[i] = f[i] / factor * ramp + f[i] * (1.0 - ramp);
+            }
+        }
+        parallel_blocks(positions, 256, [&](size_t pb, size_t pe) {
+            for (size_t p = pb; p < pe; ++p)
+                for (uint32_t i = 0; i < pairs; ++i) {
+                    const double angle = double(p) * f[i];
+                    table[(p * pairs + i) * 2u] = float(std::cos(angle) * scale);
+                    table[(p * pairs + i) * 2u + 1u] = float(std::sin(angle) * scale);
+                }
+        });
+    } catch (const std::bad_alloc &) { return fail(HSPMM_ERR_ALLOC, "out of host memory"); }
+    return HSPMM_OK;
+}
+
+int hspmm_rotate(const hspmm_rotary *rotary, int dtype, uint32_t tokens, uint32_t heads, uint32_t head_dim, const hspmm_heads *x,
+                 const int32_t *positions, const hspmm_heads *y, int backward, void *stream)
+{
+    if (!rotary) return fail(HSPMM_ERR_INVALID, "null rotary positions");
+    if (int rc = check_dtype(dtype)) return rc;
+    if (!head_dim || head_dim > 32768u || heads > 32768u || tokens > 0x7FFFFFFEu) return fail(HSPMM_ERR_INVALID, "%u tokens, %u heads of %u elements", tokens, heads, head_dim);
+    if (int rc = check_rotary(rotary, head_dim)) return rc;
+    if (tokens == 0 || heads == 0) return HSPMM_OK;
+    if (int rc = check_heads("x", x, dtype)) return rc;
+    if (int rc = check_heads("y", y, dtype)) return rc;
+    if (!positions && rotary->dims) return fail(HSPMM_ERR_INVALID, "null positions");
+    if (int rc = current_device(nullptr)) return rc;
+    RotaryArgs ra{};
+    ra.q = heads_of(x); ra.q_out = heads_of(y);
+    ra.q_heads = heads; ra.head_dim = head_dim; ra.dims = rotary->dims; ra.interleaved = rotary->interleaved != 0; ra.positions = rotary->positions;
+    ra.sign = backward ? -1.f : 1.f;
+    ra.table = rotary->dims ? rotary->table : nullptr;
+    ra.at = positions;
+    ra.tokens = tokens;
+    return run_rotary(dtype, ra, nullptr, stream);
+}
+
+uint64_t hspmm_cache_scratch_words(uint32_t pages, uint32_t sequences, uint32_t table_pages)
+{
+    const uint64_t lists = uint64_t(sequences) * (4u + uint64_t(table_pages));
+    return std::max<uint64_t>(lists, 3u * uint64_t(pages) + sequences) + 16u;
+}
+
+int hspmm_cache_append(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_heads *k, const hspmm_heads *v,
+                       const hspmm_rotary *rotary, uint32_t q_heads, const hspmm_heads *q, const hspmm_heads *q_out, void *stream)
+{
+    if (int rc = check_cache(cache)) return rc;
+    if (layer >= cache->layers) return fail(HSPMM_ERR_INVALID, "layer %u of %u", layer, cache->layers);
+    if (int rc = check_batch(cache, batch)) return rc;
+    if (rotary)
+        if (int rc = check_rotary(rotary, cache->head_dim)) return rc;
+    if (q && q_heads > 32768u) return fail(HSPMM_ERR_INVALID, "%u heads of queries", q_heads);
+    if (batch->tokens == 0) return HSPMM_OK;
+    if (int rc = check_heads("k", k, cache->dtype)) return rc;
+    if (int rc = check_heads("v", v, cache->dtype)) return rc;
+    if (q && q_heads) {
+        if (int rc = check_heads("q", q, cache->dtype)) return rc;
+        if (int rc = check_heads("q_out", q_out, cache->dtype)) return rc;
+    }
+    if (int rc = current_device(nullptr)) return rc;
+    RotaryArgs ra{};
+    ra.k = heads_of(k); ra.v = heads_of(v); ra.q = heads_of(q); ra.q_out = heads_of(q ? q_out : nullptr);
+    ra.q_heads = q ? q_heads : 0u; ra.k_heads = cache->heads;
+    ra.head_dim = cache->head_dim;
+    if (rotary && rotary->dims) {
+        ra.dims = rotary->dims; ra.interleaved = rotary->interleaved != 0; ra.positions = rotary->positions;
+        ra.table = rotary->table;
+    }
+    ra.sign = 1.f;
+    ra.tokens = batch->tokens;
+    ra.pages = pages_of(cache, layer);
+    ra.batch = batch_of(batch);
+    return run_rotary(cache->dtype, ra, cache, stream);
+}
+
+static int check_attention(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
+{
+    if (int rc = check_cache(c)) return rc;
+    if (int rc = check_batch(c, b)) return rc;
+    if (!a) return fail(HSPMM_ERR_INVALID, "null attention");
+    if (!a->q_heads || a->q_heads % c->heads || a->q_heads > 32768u) return fail(HSPMM_ERR_INVALID, "%u heads of queries for %u of keys", a->q_heads, c->heads);
+    if (!std::isfinite(a->scale)) return fail(HSPMM_ERR_INVALID, "scale %g", double(a->scale));
+    if (a->window && !a->causal) return fail(HSPMM_ERR_INVALID, "a window of %u keys without causal", a->window);
+    const uint32_t piece = 16u / element_bytes(c->dtype);
+    if (c->head_dim % piece || c->head_dim > 256u) return fail(HSPMM_ERR_UNSUPPORTED, "heads of %u elements: a multiple of %u up to 256", c->head_dim, piece);
+    if (c->page_stride % piece || c->layer_stride % piece) return fail(HSPMM_ERR_UNSUPPORTED, "pages or layers that begin between two pieces of 16 bytes");
+    return HSPMM_OK;
+}
+
+int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_attention *attention, uint64_t *bytes)
+{
+    if (!bytes) return fail(HSPMM_ERR_INVALID, "null bytes");
+    if (int rc = check_attention(cache, batch, attention)) return rc;
+    *bytes = 0;
+    return HSPMM_OK;
+}
+
+int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_attention *attention, const hspmm_heads *q,
+                       const hspmm_heads *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream)
+{
+    if (int rc = check_attention(cache, batch, attention)) return rc;
+    if (layer >= cache->layers) return fail(HSPMM_ERR_INVALID, "layer %u of %u", layer, cache->layers);
+    if (batch->tokens == 0) return HSPMM_OK;
+    const uint32_t e = element_bytes(cache->dtype), piece = 16u / e;
+    if (int rc = check_heads("q", q, cache->dtype)) return rc;
+    if (int rc = check_heads("out", out, cache->dtype)) return rc;
+    if (q->dim_stride != 1 || q->token_stride % piece || q->head_stride % piece || reinterpret_cast<uintptr_t>(q->data) % 16u)
+        return fail(HSPMM_ERR_UNSUPPORTED, "q: a head's elements side by side, tokens and heads at multiples of 16 bytes");
+    if (reinterpret_cast<uintptr_t>(lse) % 4u) return fail(HSPMM_ERR_INVALID, "lse is not aligned to its elements");
+    (void)workspace; (void)workspace_bytes;
+    if (int rc = current_device(nullptr)) return rc;
+    AttendArgs aa{};
+    aa.pages = pages_of(cache, layer);
+    aa.batch = batch_of(batch);
+    aa.q = heads_of(q); aa.out = heads_of(out); aa.lse = lse;
+    aa.q_heads = attention->q_heads; aa.shared = Divisor::of(attention->q_heads / cache->heads);
+    aa.scale = attention->scale; aa.causal = attention->causal != 0; aa.window = attention->window;
+    HSPMM_HIP(launch_attend_simple(cache->dtype, aa, static_cast<hipStream_t>(stream)));
+    return HSPMM_OK;
+}
+
+int hspmm_cache_extend(const hspmm_cache *cache, uint32_t n, const int32_t *rows, const int32_t *add, int32_t *status, void *stream)
+{
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_list(cache, n, add, "add")) return rc;
+    if (int rc = current_device(nullptr)) return rc;
+    HSPMM_HIP(launch_pages_extend(pool_of(cache), n, rows, add, status, static_cast<hipStream_t>(stream)));
+    return HSPMM_OK;
+}
+
+int hspmm_cache_fork(const hspmm_cache *cache, uint32_t n, const int32_t *parents, const int32_t *children, int32_t *status, void *stream)
+{
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_list(cache, n, parents, "parents")) return rc;
+    if (int rc = check_list(cache, n, children, "children")) return rc;
+    if (n == 0 && !status) return HSPMM_OK;
+    if (int rc = current_device(nullptr)) return rc;
+    HSPMM_HIP(launch_pages_fork(pool_of(cache), n, parents, children, status, static_cast<hipStream_t>(stream)));
+    return HSPMM_OK;
+}
+
+int hspmm_cache_free(const hspmm_cache *cache, uint32_t n, const int32_t *rows, void *stream)
+{
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_list(cache, n, rows, "rows")) return rc;
+    if (n == 0) return HSPMM_OK;
+    if (int rc = current_device(nullptr)) return rc;
+    HSPMM_HIP(launch_pages_free(pool_of(cache), n, rows, static_cast<hipStream_t>(stream)));
+    return HSPMM_OK;
+}
+
+int hspmm_cache_compact(const hspmm_cache *cache, int32_t *table_out, int32_t *references_out, int32_t *live, void *stream)
+{
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = current_device(nullptr)) return rc;
+    HSPMM_HIP(launch_pages_compact(pool_of(cache), table_out ? table_out : cache->table, references_out ? references_out : cache->references, live,
+                                   static_cast<hipStream_t>(stream)));
+    return HSPMM_OK;
+}
+
+int hspmm_cache_copy(const hspmm_cache *cache, uint32_t n, const int32_t *from, const int32_t *to, void *stream)
+{
+    if (int rc = check_cache(cache)) return rc;
+    if (n > cache->pages) return fail(HSPMM_ERR_INVALID, "%u pages to copy of %u", n, cache->pages);
+    if (n && (!from || !to)) return fail(HSPMM_ERR_INVALID, "null list of pages");
+    if (n == 0) return HSPMM_OK;
+    if (int rc = current_device(nullptr)) return rc;
+    HSPMM_HIP(launch_pages_copy(pool_of(cache), n, from, to, static_cast<hipStream_t>(stream)));
+    return HSPMM_OK;
+}
+
+}  // extern "C"

@@ -504,6 +504,130 @@ int hspmm_create_grouped(hspmm_plan **plan, int dtype, uint32_t rows, uint32_t c
                          const uint32_t *tcA2B, const uint64_t *tcBit, const void *data,
                          const uint32_t *groupRowIdx, const uint8_t *atomic);
 
+/* ---- rotary positions, a paged cache of keys and values, attention over it ---- */
+
+/* No reference counterpart from here on: what lies between two products of a pruned decoder layer, in the
+ * element types of the products.  Every array below is the caller's, in device memory unless said otherwise; the
+ * functions only launch kernels on `stream` (no allocation, copy, memset or synchronize) and can be recorded in a HIP
+ * graph.  Calls on one cache that overlap in time race where one of them writes what another one uses.
+ * Numbers in device memory (starts, rows, lengths, page and position numbers) cannot be refused: the kernels
+ * keep within the arrays whatever they are. */
+
+/* A tensor tokens x heads x elements: strides in elements.  dim_stride 1 is a head's elements side by side;
+ * token_stride 1 is C of hspmm_run, features x tokens, or the B of the next one. */
+typedef struct hspmm_heads {
+    void *data;
+    int64_t token_stride, head_stride, dim_stride;
+} hspmm_heads;
+
+/* Rotary positions: the first `dims` elements of a head (even; the others are left as they are) turn in pairs by
+ * the angle of the token's position.  Pairs are elements i and i + dims / 2 or, interleaved, 2 i and 2 i + 1.
+ * table: positions x dims / 2 pairs of floats (cosine, sine), e.g. from hspmm_rotary_table; a position outside
+ * it is taken as the nearest one in it. */
+typedef struct hspmm_rotary {
+    uint32_t dims;
+    int32_t interleaved;
+    uint32_t positions;
+    const float *table;
+} hspmm_rotary;
+
+/* Frequencies of hspmm_rotary_table, f_i = base^(-2 i / dims):
+ *   PLAIN   f_i
+ *   LINEAR  f_i / factor: positions of a context `factor` times as long squeezed into the original one
+ *   BASE    base * factor^(dims / (dims - 2)) in place of base: the lowest frequency is divided by factor, the highest stays
+ *   YARN    f_i / factor for wavelengths longer than original_length / slow_turns, f_i for those shorter than
+ *           original_length / fast_turns, a linear ramp over i between the two; cosines and sines times
+ *           0.1 ln(factor) + 1 (Peng et al. 2023, "YaRN: Efficient Context Window Extension of Large Language Models") */
+#define HSPMM_ROTARY_PLAIN 0
+#define HSPMM_ROTARY_LINEAR 1
+#define HSPMM_ROTARY_BASE 2
+#define HSPMM_ROTARY_YARN 3
+/* Host only: table (host memory, positions x dims / 2 x 2 floats) in 64 bits, rounded once.  original_length,
+ * fast_turns and slow_turns are read for YARN alone. */
+int hspmm_rotary_table(int kind, uint32_t dims, double base, double factor, double original_length, double fast_turns, double slow_turns,
+                       uint32_t positions, float *table);
+
+/* y = x turned, tokens x heads x head_dim; positions[tokens].  backward: by the transposed rotation, which is the
+ * gradient of x from that of y.  Computed in fp32, rounded once.  y may be x (same strides); tensors that overlap
+ * otherwise give unspecified results. */
+int hspmm_rotate(const hspmm_rotary *rotary, int dtype, uint32_t tokens, uint32_t heads, uint32_t head_dim, const hspmm_heads *x,
+                 const int32_t *positions, const hspmm_heads *y, int backward, void *stream);
+
+/* Keys and values of `layers` layers in `pages` pages of page_tokens tokens.  A page is heads x page_tokens x
+ * head_dim elements (HSPMM_HEADS_FIRST) or page_tokens x heads x head_dim (HSPMM_TOKENS_FIRST), the same for keys and
+ * values; page_stride and layer_stride: elements from one page (layer) to the next, 0: they lie side by side.
+ * table: sequences x table_pages page numbers; place p of a row is the page of tokens p * page_tokens and on.  -1 (any
+ * number that is not a page's) is no page: its tokens are not stored and nothing sees them.
+ * lengths[sequences]: tokens of each sequence.  references[pages]: how many places of the table name a page; a page
+ * without any (<= 0) is free.  That is all there is to say which pages are free: a cache begins with lengths and
+ * references of zero and a table of -1.
+ * scratch: hspmm_cache_scratch_words words that the calls which change pages use; two such calls of one cache must
+ * not overlap.  keys and values are aligned to 16 bytes. */
+#define HSPMM_HEADS_FIRST 0
+#define HSPMM_TOKENS_FIRST 1
+typedef struct hspmm_cache {
+    int32_t dtype, order;
+    uint32_t layers, pages, page_tokens, heads, head_dim, sequences, table_pages;
+    int64_t page_stride, layer_stride;
+    void *keys, *values;
+    int32_t *table, *lengths, *references, *scratch;
+} hspmm_cache;
+uint64_t hspmm_cache_scratch_words(uint32_t pages, uint32_t sequences, uint32_t table_pages);
+
+/* A ragged batch: tokens starts[b] .. starts[b + 1] - 1 (of `tokens`) are the last ones of sequence rows[b] of a
+ * cache (rows null: of sequence b), lengths[rows[b]] counting them. */
+typedef struct hspmm_batch {
+    uint32_t sequences, tokens;
+    const int32_t *starts, *rows;
+} hspmm_batch;
+
+/* Stores keys and values (tokens x heads x head_dim) of a batch's tokens into their pages of `layer`.  rotary not
+ * null: keys are turned by their tokens' positions in their sequences first, and so are the queries q (q_heads heads)
+ * into q_out, which may be q (q null: none). */
+int hspmm_cache_append(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_heads *k, const hspmm_heads *v,
+                       const hspmm_rotary *rotary, uint32_t q_heads, const hspmm_heads *q, const hspmm_heads *q_out, void *stream);
+
+/* q_heads: a multiple of the cache's heads; query head h reads head h / (q_heads / heads).  causal: a token sees
+ * keys up to its own position only; window (causal only; 0: none): and no more than that many of them.
+ * longest_chunk, longest: the most tokens a sequence has in the batch and in the cache; they choose kernels and how the
+ * work is split, the result is right whatever they are. */
+typedef struct hspmm_attention {
+    uint32_t q_heads;
+    float scale;
+    int32_t causal;
+    uint32_t window, longest_chunk, longest;
+} hspmm_attention;
+
+/* out = softmax(scale * q k) v over the keys a token sees, tokens x q_heads x head_dim; a token that sees none gets 0.
+ * lse (tokens x q_heads, may be null): the logarithm of the softmax's denominator, -infinity where nothing is seen.
+ * Scores, softmax and sums in fp32; for 16-bit types the weights are rounded to the type before they multiply the
+ * values, as the matrix instructions want them.  What is not seen does not reach the result, infinities and NaN among it.
+ * head_dim: a multiple of 8 (fp32: 4) up to 256.  q: dim_stride 1, its strides multiples of 16 bytes, aligned to 16 bytes.
+ * workspace: hspmm_cache_attend_workspace bytes, aligned to 16 bytes; zero before its first use, and not used by
+ * two calls that overlap in time.  The calls leave it as they want to find it. */
+int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_attention *attention, const hspmm_heads *q,
+                       const hspmm_heads *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream);
+int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_attention *attention, uint64_t *bytes);
+
+/* Pages.  Pages that a call gives out are the free ones of lowest number, in the order of the call's list and of the
+ * places in a row; *status (may be null) receives how many were missing: their places are -1 and hold nothing.
+ * n: the list's length, at most the cache's sequences; a list names no sequence twice. */
+/* add[i] more tokens for sequence rows[i] (rows null: i; less than 0: none), and the pages they need. */
+int hspmm_cache_extend(const hspmm_cache *cache, uint32_t n, const int32_t *rows, const int32_t *add, int32_t *status, void *stream);
+/* Sequence children[i] becomes what sequence parents[i] was before the call: it shares the parent's full pages and gets a
+ * copy (the tokens held) of the last one where it is partly filled.  The pages it had are released; those that
+ * become free are given out by later calls only.  A parent may be named often, and be a child as well (a beam
+ * search's step); a sequence that is its own parent stays as it is. */
+int hspmm_cache_fork(const hspmm_cache *cache, uint32_t n, const int32_t *parents, const int32_t *children, int32_t *status, void *stream);
+/* Sequences rows[i] have no tokens any more; pages that nobody else names are free. */
+int hspmm_cache_free(const hspmm_cache *cache, uint32_t n, const int32_t *rows, void *stream);
+/* Moves the live pages to the low end of the pool: those at or above their number go to the free ones below it, both in
+ * ascending order.  *live (may be null) receives that number.  table_out, references_out: null, or where the new
+ * ones go, the old ones staying. */
+int hspmm_cache_compact(const hspmm_cache *cache, int32_t *table_out, int32_t *references_out, int32_t *live, void *stream);
+/* Copies pages from[i] to to[i] (all layers); no page may be both among from and to, or twice among to. */
+int hspmm_cache_copy(const hspmm_cache *cache, uint32_t n, const int32_t *from, const int32_t *to, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

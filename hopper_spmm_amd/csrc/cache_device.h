@@ -60,11 +60,20 @@ struct AttendArgs {
     Divisor shared;                      // heads of queries to one of keys
     float scale;
     uint32_t causal, window;
-    uint32_t splits;                     // parts that a sequence's keys are cut into
+    uint32_t splits, part_keys;          // parts that a tile's keys are cut into at most; keys of a part (a multiple of 32)
     float *sums;                         // of more than one part: their sums
     uint32_t *arrive;                    // and how many have left them (zero between launches)
 };
-hipError_t launch_attend_simple(int dtype, const AttendArgs &aa, hipStream_t s);
+// Tiles of (1 << rows_log) rows that a batch has at most (find_tile numbers them).
+constexpr uint32_t kAttendRowsLog = 4u;
+inline uint32_t attend_tiles(uint32_t tokens, uint32_t sequences, uint32_t shared, uint32_t rows_log)
+{
+    return uint32_t((uint64_t(tokens) * shared >> rows_log) + sequences);
+}
+constexpr uint32_t kAttendCounters = 16384u;
+// floats of a part of a tile's sums
+inline uint32_t attend_slot(uint32_t rows_log, uint32_t head_dim) { return (1u << rows_log) * ((head_dim <= 64u ? 64u : head_dim <= 128u ? 128u : 256u) + 4u); }
+hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, hipStream_t s);
 
 // Page work: all layers.
 struct PoolArgs {

@@ -278,6 +278,8 @@ static int check_attention(const hspmm_cache *c, const hspmm_batch *b, const hsp
     if (!a) return fail(HSPMM_ERR_INVALID, "null attention");
     if (!a->q_heads || a->q_heads % c->heads || a->q_heads > 32768u) return fail(HSPMM_ERR_INVALID, "%u heads of queries for %u of keys", a->q_heads, c->heads);
     if (!std::isfinite(a->scale)) return fail(HSPMM_ERR_INVALID, "scale %g", double(a->scale));
+    if (uint64_t(b->tokens) * (a->q_heads / c->heads) + b->sequences > 0x7FFFFFFFu)
+        return fail(HSPMM_ERR_UNSUPPORTED, "%u tokens with %u heads that share their keys: in several calls", b->tokens, a->q_heads / c->heads);
     if (a->window && !a->causal) return fail(HSPMM_ERR_INVALID, "a window of %u keys without causal", a->window);
     const uint32_t piece = 16u / element_bytes(c->dtype);
     if (c->head_dim % piece || c->head_dim > 256u) return fail(HSPMM_ERR_UNSUPPORTED, "heads of %u elements: a multiple of %u up to 256", c->head_dim, piece);
@@ -285,11 +287,36 @@ static int check_attention(const hspmm_cache *c, const hspmm_batch *b, const hsp
     return HSPMM_OK;
 }
 
+// How an attention is launched, by sizes alone: the same for the call and for its workspace.
+struct AttendShape {
+    uint32_t tiles, splits, part_keys;
+    uint64_t bytes;
+};
+
+static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
+{
+    const uint32_t shared = a->q_heads / c->heads;
+    AttendShape sh{};
+    sh.tiles = attend_tiles(b->tokens, b->sequences, shared, kAttendRowsLog);
+    uint64_t keys = uint64_t(c->table_pages) * c->page_tokens;
+    if (a->longest && a->longest < keys) keys = a->longest;
+    if (a->window && uint64_t(a->window) + a->longest_chunk < keys) keys = uint64_t(a->window) + a->longest_chunk;
+    const uint64_t tiles = uint64_t(b->tokens) * shared / (1u << kAttendRowsLog) + b->sequences, pairs = uint64_t(sh.tiles) * c->heads;
+    const uint64_t work = std::min<uint64_t>(tiles, uint64_t(b->sequences) * ((uint64_t(a->longest_chunk) * shared + 15u) / 16u)) * c->heads * keys;
+    uint64_t part = (work / 2048u + 127u) & ~uint64_t(127u);
+    part = std::max<uint64_t>(part, 256u);
+    sh.part_keys = uint32_t(std::min<uint64_t>(part, 1u << 30));
+    const uint64_t parts = (keys + 31u + sh.part_keys - 1u) / sh.part_keys;
+    sh.splits = pairs > kAttendCounters ? 1u : uint32_t(std::min<uint64_t>(std::max<uint64_t>(parts, 1u), 256u));
+    if (sh.splits > 1u) sh.bytes = kAttendCounters * 4u + pairs * sh.splits * attend_slot(kAttendRowsLog, c->head_dim) * 4u;
+    return sh;
+}
+
 int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_attention *attention, uint64_t *bytes)
 {
     if (!bytes) return fail(HSPMM_ERR_INVALID, "null bytes");
     if (int rc = check_attention(cache, batch, attention)) return rc;
-    *bytes = 0;
+    *bytes = batch->tokens ? attend_shape(cache, batch, attention).bytes : 0;
     return HSPMM_OK;
 }
 
@@ -305,7 +332,9 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     if (q->dim_stride != 1 || q->token_stride % piece || q->head_stride % piece || reinterpret_cast<uintptr_t>(q->data) % 16u)
         return fail(HSPMM_ERR_UNSUPPORTED, "q: a head's elements side by side, tokens and heads at multiples of 16 bytes");
     if (reinterpret_cast<uintptr_t>(lse) % 4u) return fail(HSPMM_ERR_INVALID, "lse is not aligned to its elements");
-    (void)workspace; (void)workspace_bytes;
+    const AttendShape sh = attend_shape(cache, batch, attention);
+    if (sh.bytes && (!workspace || workspace_bytes < sh.bytes || reinterpret_cast<uintptr_t>(workspace) % 16u))
+        return fail(HSPMM_ERR_INVALID, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)sh.bytes);
     if (int rc = current_device(nullptr)) return rc;
     AttendArgs aa{};
     aa.pages = pages_of(cache, layer);
@@ -313,7 +342,10 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     aa.q = heads_of(q); aa.out = heads_of(out); aa.lse = lse;
     aa.q_heads = attention->q_heads; aa.shared = Divisor::of(attention->q_heads / cache->heads);
     aa.scale = attention->scale; aa.causal = attention->causal != 0; aa.window = attention->window;
-    HSPMM_HIP(launch_attend_simple(cache->dtype, aa, static_cast<hipStream_t>(stream)));
+    aa.splits = sh.splits; aa.part_keys = sh.part_keys;
+    aa.arrive = static_cast<uint32_t *>(workspace);
+    aa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + kAttendCounters * 4u);
+    HSPMM_HIP(launch_attend_rows(cache->dtype, aa, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
 

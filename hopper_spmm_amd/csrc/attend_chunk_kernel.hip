@@ -1,0 +1,449 @@
+// Attention of many rows of queries - chunks of a prompt - over the pages of a cache, 16-bit types.
+#include "attend_common.hpp"
+
+namespace hspmm {
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <bool BF> struct Wide;
+template <> struct Wide<false> {
+    __device__ static __forceinline__ f32x16 mfma(const u32x4 a, const u32x4 b, const f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+    }
+};
+template <> struct Wide<true> {
+    __device__ static __forceinline__ f32x16 mfma(const u32x4 a, const u32x4 b, const f32x16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+};
+
+// A workgroup's LDS writes are done and every wave is here (loads from memory may be on their way).
+__device__ __forceinline__ void lds_barrier()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// A wave has 32 QT rows, a lane (h, j) = (lane / 32, lane % 32) row 32 t + j of tile t; keys come in images of 64, two halves of 32.
+//   scores: S^T = K Q^T, 32 keys x 32 rows by instructions of 16 elements; register r: key 8 (r / 4) + 4 h + r % 4
+//   sums:   O^T = V^T P^T, 32 elements x 32 rows by instructions of 16 keys: scores 8 s .. 8 s + 7 of a lane are its part of the second operand,
+//           keys in that order; the first one comes transposed from LDS (ds_read_b64_tr_b16), four keys of an element a read
+// The scores of a half are made among the exponentials of the half in front.  Images go through LDS, RING of them in turn: while image n is
+// multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image.
+template <bool BF, int DP, int QT, int W, bool Whole>
+__global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_chunk_kernel(const AttendArgs aa)
+{
+    typedef typename HalfOps<BF>::elem_t T;
+    constexpr uint32_t kThreads = 64u * W, kWaveRows = 32u * QT, kRows = kWaveRows * W, kKeys = 64u;
+    constexpr int kRowsLog = kRows == 256u ? 8 : 7;
+    static_assert(kRows == 1u << kRowsLog, "");
+    constexpr uint32_t kKeyPitch = DP * 2u + 16u, kValuePitch = DP * 2u + 64u, kImage = kKeys * (kKeyPitch + kValuePitch);
+    constexpr uint32_t kRing = DP <= 64 || (DP <= 128 && W == 8) ? 3u : 2u;
+    constexpr int kSteps = DP / 16, kTiles = DP / 32, kPieces = int(kKeys * DP / 8u / kThreads);
+    constexpr uint32_t kRowPieces = DP / 8u;
+    __shared__ __attribute__((aligned(16))) char images[kRing * kImage];
+    __shared__ uint32_t odd, arrived;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, j = lane & 31u;
+    const uint32_t head = blockIdx.x, part = blockIdx.z, D = aa.pages.head_dim, tile_number = gridDim.y - 1u - blockIdx.y;
+    const RowTile t = find_tile<kRowsLog>(aa, tile_number);
+    if (!t.there) return;
+    const int32_t lo = t.lo & ~31, span = t.hi - lo, each = int32_t(aa.part_keys);
+    int32_t parts = span > 0 ? (span + each - 1) / each : 1;
+    if (parts > int32_t(aa.splits)) parts = int32_t(aa.splits);
+    if (int32_t(part) >= parts) return;
+    const int32_t begin = lo + int32_t(part) * each, end = int32_t(part) + 1 == parts ? t.hi : begin + each;
+    const int32_t n_images = end > begin ? (end - begin + 63) / 64 : 0;
+    if (tid == 0u) odd = 0u;
+
+    const float scale = aa.scale == 0.f ? 1.f : fabsf(aa.scale) * kLog2e;
+    const uint32_t flip = aa.scale < 0.f ? 0x80008000u : 0u;
+    RowOf row[QT];
+    u32x4 q[QT][kSteps];
+    int32_t all_lo = 0, all_hi = 0x7FFFFFFF;
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+        const uint32_t m = wave * kWaveRows + 32u * u + j;
+        row[u] = row_of_tile(aa, t, head, m);
+        const char *from = aa.q.data + (int64_t(row[u].token) * aa.q.token_stride + int64_t(row[u].head) * aa.q.head_stride) * 2;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const uint32_t d = 16u * s + 8u * h;
+            q[u][s] = m < t.rows && d < D && aa.scale != 0.f ? *reinterpret_cast<const u32x4 *>(from + d * 2u) ^ flip : u32x4{0u, 0u, 0u, 0u};
+        }
+        if (m < t.rows) {
+            all_lo = max(all_lo, row[u].lo);
+            all_hi = min(all_hi, row[u].hi);
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        all_lo = max(all_lo, __shfl_xor(all_lo, d));
+        all_hi = min(all_hi, __shfl_xor(all_hi, d));
+    }
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo); all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    // the same of the workgroup's rows
+    const int32_t p0 = t.position + int32_t(aa.shared.quotient(t.first_row)), p1 = t.position + int32_t(aa.shared.quotient(t.first_row + t.rows - 1u));
+    const int32_t group_hi = aa.causal ? p0 + 1 : t.length, group_lo = aa.window && int64_t(p1) + 1 > int64_t(aa.window) ? p1 + 1 - int32_t(aa.window) : 0;
+
+    const int32_t *table = aa.pages.table + size_t(t.sequence) * aa.pages.table_pages;
+    const int64_t head_offset = int64_t(head) * aa.pages.head_stride;
+    // page numbers of the next 16 images, four an image (Whole)
+    int32_t pages_ahead = -1;
+    // a thread's pieces of an image: 16 bytes of a row of keys and of values
+    u32x4 k_piece[kPieces], v_piece[kPieces];
+    uint64_t stored_there = 0u;                                // keys of the image that are stored, a bit each
+    const uint32_t column = (tid % kRowPieces) * 8u;
+    auto request = [&](int32_t n) __attribute__((always_inline)) {
+        const int32_t key0 = begin + n * 64;
+        const uint64_t in = n >= n_images ? 0u : end - key0 >= 64 ? ~uint64_t(0) : (uint64_t(1) << (end - key0)) - 1u;
+        stored_there = 0u;
+        if constexpr (Whole) {
+            if (n % 16 == 0) {
+                const int32_t key = key0 + int32_t(lane) * 16;
+                pages_ahead = -1;
+                if (key < end) {
+                    const uint32_t place = aa.pages.page_tokens.quotient(uint32_t(key));
+                    if (place < aa.pages.table_pages) pages_ahead = table[place];
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (uint32_t(__builtin_amdgcn_readlane(pages_ahead, n % 16 * 4 + g)) < aa.pages.pages) stored_there |= uint64_t(0xFFFFu) << (16 * g);
+            stored_there &= in;
+        } else {
+            const int32_t key = key0 + int32_t(lane);
+            stored_there = __ballot(n < n_images && key < end && key_offset(aa.pages, table, 0, key) >= 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const uint32_t r = (tid + kThreads * i) / kRowPieces;
+            int64_t at;
+            if constexpr (Whole) {
+                // (a wave's rows of a piece lie in one group of 16)
+                const uint32_t g = (64u * wave + kThreads * i) / kRowPieces / 16u, key = uint32_t(key0) + 16u * g;
+                const uint32_t id = uint32_t(__builtin_amdgcn_readlane(pages_ahead, n % 16 * 4 + int(g)));
+                at = int64_t(id) * aa.pages.page_stride + head_offset + int64_t(key - aa.pages.page_tokens.quotient(key) * aa.pages.page_tokens.d) * aa.pages.token_stride +
+                     int64_t(r % 16u) * aa.pages.token_stride;
+            } else {
+                at = key0 + int32_t(r) < end ? key_offset(aa.pages, table, head_offset, key0 + int32_t(r)) : -1;
+            }
+            // (what is not stored may be anything, and no weight of zero undoes a NaN)
+            const bool there = column < D && (stored_there >> r & 1u);
+            k_piece[i] = there ? *reinterpret_cast<const u32x4 *>(aa.pages.keys + (at + column) * 2) : u32x4{0u, 0u, 0u, 0u};
+            v_piece[i] = there ? *reinterpret_cast<const u32x4 *>(aa.pages.values + (at + column) * 2) : u32x4{0u, 0u, 0u, 0u};
+        }
+    };
+    auto write_image = [&](int32_t n, uint32_t to) __attribute__((always_inline)) {
+        char *const image = images + to * kImage;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const uint32_t r = (tid + kThreads * i) / kRowPieces;
+            *reinterpret_cast<u32x4 *>(image + r * kKeyPitch + column * 2u) = k_piece[i];
+            *reinterpret_cast<u32x4 *>(image + kKeys * kKeyPitch + r * kValuePitch + column * 2u) = v_piece[i];
+        }
+        const int32_t key0 = begin + n * 64;
+        if (n < n_images && (key0 < group_lo || key0 + 64 > group_hi || ~stored_there)) {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) any |= word_not_finite<BF>(v_piece[i][w]);
+            if (any) odd = 1u;
+        }
+    };
+
+    f32x16 o[QT][kTiles];
+    float ref[QT], total[QT];
+    auto begin_sums = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[u][c][r] = 0.f;
+            ref[u] = -INFINITY;
+            total[u] = 0.f;
+        }
+    };
+    const uint32_t key_lane = j * kKeyPitch + h * 16u;
+    const uint32_t value_lane = kKeys * kKeyPitch + (4u * h + (lane & 15u) / 4u) * kValuePitch + ((lane >> 4 & 1u) * 16u + (lane & 3u) * 4u) * 2u;
+    // steps S0 .. S1 - 1 of the scores of half `half` of an image
+    auto scores = [&](auto s0, auto s1, f32x16 (&s)[QT], uint32_t image, uint32_t half) __attribute__((always_inline)) {
+        const char *const from = images + image * kImage + half * 32u * kKeyPitch + key_lane;
+        if constexpr (decltype(s0)::value == 0) {
+#pragma unroll
+            for (int u = 0; u < QT; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+        }
+#pragma unroll
+        for (int c = decltype(s0)::value; c < decltype(s1)::value; ++c) {
+            const u32x4 a = *reinterpret_cast<const u32x4 *>(from + c * 32);
+#pragma unroll
+            for (int u = 0; u < QT; ++u) s[u] = Wide<BF>::mfma(a, q[u][c], s[u]);
+        }
+    };
+    auto mask = [&](f32x16 (&s)[QT], int32_t key0, uint32_t stored) __attribute__((always_inline)) {
+        if (key0 >= all_lo && key0 + 32 <= all_hi && stored == ~0u) return;
+#pragma unroll
+        for (int u = 0; u < QT; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t a = 8u * (r / 4) + 4u * h + r % 4;
+                const int32_t key = key0 + int32_t(a);
+                if (!(key >= row[u].lo && key < row[u].hi && (stored >> a & 1u))) s[u][r] = -INFINITY;
+            }
+    };
+    // the largest score of every row; where one is far above its row's reference the sums move to a new one
+    auto move_references = [&](const f32x16 (&s)[QT]) __attribute__((always_inline)) {
+        float most[QT];
+        bool moves[QT], any = false;
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+            most[u] = s[u][0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) most[u] = fmaxf(most[u], s[u][r]);
+            most[u] = max_halves(most[u]) * scale;
+            moves[u] = most[u] > ref[u] + kReferenceSlack || (ref[u] == -INFINITY && most[u] > -INFINITY);
+            any |= moves[u];
+        }
+        if (__ballot(any)) {
+#pragma unroll
+            for (int u = 0; u < QT; ++u) {
+                const float by = moves[u] ? __builtin_amdgcn_exp2f(ref[u] - most[u]) : 1.f;
+                if (moves[u]) ref[u] = most[u];
+                total[u] *= by;
+#pragma unroll
+                for (int c = 0; c < kTiles; ++c) o[u][c] *= by;
+            }
+        }
+    };
+    auto exponentials = [&](f32x16 (&s)[QT]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+            const float base = ref[u] == -INFINITY ? 0.f : ref[u];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale, -base));
+                total[u] += s[u][r];
+            }
+        }
+    };
+    auto add = [&](const f32x16 (&s)[QT], uint32_t image, uint32_t half) __attribute__((always_inline)) {
+        const __attribute__((address_space(3))) char *const from = (const __attribute__((address_space(3))) char *)(images + image * kImage + half * 32u * kValuePitch + value_lane);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            u32x4 p[QT];
+#pragma unroll
+            for (int u = 0; u < QT; ++u)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) p[u][w] = HalfOps<BF>::pack(s[u][8 * c + 2 * w], s[u][8 * c + 2 * w + 1]);
+#pragma unroll
+            for (int e = 0; e < kTiles; ++e) {
+                const t_u32x2 a0 = __builtin_bit_cast(t_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tile_tr_ptr)(from + (16 * c) * kValuePitch + e * 64)));
+                const t_u32x2 a1 = __builtin_bit_cast(t_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tile_tr_ptr)(from + (16 * c + 8) * kValuePitch + e * 64)));
+                const u32x4 a{a0[0], a0[1], a1[0], a1[1]};
+#pragma unroll
+                for (int u = 0; u < QT; ++u) o[u][e] = Wide<BF>::mfma(a, p[u], o[u][e]);
+            }
+        }
+    };
+    using from0 = std::integral_constant<int, 0>;
+    using middle = std::integral_constant<int, kSteps / 2>;
+    using to_end = std::integral_constant<int, kSteps>;
+
+    begin_sums();
+    if (n_images) {
+        f32x16 s_a[QT], s_b[QT];
+        request(0);
+        write_image(0, 0u);
+        uint64_t stored_now = stored_there;
+        request(1);
+        write_image(1, 1u);
+        uint64_t stored_next = stored_there;
+        lds_barrier();
+        scores(from0{}, to_end{}, s_a, 0u, 0u);
+        uint32_t now = 0u, next = 1u, free = kRing - 1u;
+#pragma unroll 1
+        for (int32_t n = 0; n < n_images; ++n) {
+            const int32_t key0 = begin + n * 64;
+            request(n + 2);
+            mask(s_a, key0, uint32_t(stored_now));
+            scores(from0{}, middle{}, s_b, now, 1u);
+            move_references(s_a);
+            scores(middle{}, to_end{}, s_b, now, 1u);
+            exponentials(s_a);
+            add(s_a, now, 0u);
+            mask(s_b, key0 + 32, uint32_t(stored_now >> 32));
+            scores(from0{}, middle{}, s_a, next, 0u);
+            move_references(s_b);
+            scores(middle{}, to_end{}, s_a, next, 0u);
+            exponentials(s_b);
+            add(s_b, now, 1u);
+            if constexpr (kRing == 2u) { lds_barrier(); free = now; }
+            write_image(n + 2, free);
+            stored_now = stored_next;
+            stored_next = stored_there;
+            const uint32_t old = now;
+            now = next;
+            next = free;
+            free = old;
+            lds_barrier();
+        }
+        __syncthreads();
+        if (odd) {
+            // An infinity or a NaN that some rows do not see, which a matrix instruction would multiply by their zeros: once more, the values key by
+            // key and by the rows that see it.  Slow, and off the path of finite data.
+            begin_sums();
+            float *const weights = reinterpret_cast<float *>(images + kImage) + wave * 32u * 32u;
+            static_assert(W * 32u * 32u * 4u <= (kRing - 1u) * kImage, "weights in the place of the other images");
+#pragma unroll 1
+            for (int32_t n = 0; n < n_images; ++n) {
+                __syncthreads();
+                if (Whole && n % 16) request(n & ~15);         // (page numbers)
+                request(n);
+                write_image(n, 0u);
+                const uint64_t stored = stored_there;
+                __syncthreads();
+#pragma unroll 1
+                for (uint32_t half = 0; half < 2u; ++half) {
+                    const int32_t key0 = begin + n * 64 + int32_t(half) * 32;
+                    scores(from0{}, to_end{}, s_a, 0u, half);
+                    mask(s_a, key0, uint32_t(stored >> (32u * half)));
+                    move_references(s_a);
+                    exponentials(s_a);
+#pragma unroll
+                    for (int u = 0; u < QT; ++u) {
+                        __syncthreads();
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) weights[(8u * (r / 4) + 4u * h + r % 4) * 32u + j] = s_a[u][r];
+                        __syncthreads();
+#pragma unroll 1
+                        for (uint32_t a = 0; a < 32u; ++a) {
+                            const int32_t key = key0 + int32_t(a);
+                            const float w = weights[a * 32u + j];
+                            const T *from = reinterpret_cast<const T *>(images + kKeys * kKeyPitch + (32u * half + a) * kValuePitch) + 4u * h;
+                            if (key >= row[u].lo && key < row[u].hi) {
+#pragma unroll
+                                for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+                                    for (int r = 0; r < 16; ++r) o[u][c][r] += w * float(from[32 * c + 8 * (r / 4) + r % 4]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // what a row's two lanes have
+#pragma unroll
+    for (int u = 0; u < QT; ++u) total[u] += __shfl_xor(total[u], 32);
+    if (parts > 1) {
+        constexpr uint32_t kSlot = kRows * (DP + 4u);          // floats of a part: per row its sums, its reference and its total
+        const uint32_t pair = tile_number * gridDim.x + head;
+        const __amdgpu_buffer_rsrc_t mem = device_scope_buffer(aa.sums + size_t(pair) * aa.splits * kSlot);
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+            const uint32_t m = wave * kWaveRows + 32u * u + j;
+            if (m >= t.rows) continue;
+            const uint32_t at = (part * kSlot + m * (DP + 4u)) * 4u;
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    store_device_scope(mem, at + (32u * c + 2u * r + 4u * h) * 4u, f32x4{o[u][c][r], o[u][c][r + 1], o[u][c][r + 2], o[u][c][r + 3]});
+            if (h == 0u) store_device_scope(mem, at + DP * 4u, f32x4{ref[u], total[u], 0.f, 0.f});
+        }
+        wait_stores_acknowledged();
+        __syncthreads();
+        if (tid == 0u) arrived = __hip_atomic_fetch_add(aa.arrive + pair, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (arrived + 1u != uint32_t(parts)) return;
+        if (tid == 0u) __hip_atomic_store(aa.arrive + pair, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+            const uint32_t m = wave * kWaveRows + 32u * u + j;
+            if (m >= t.rows) continue;
+            ref[u] = -INFINITY;
+            total[u] = 0.f;
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[u][c][r] = 0.f;
+#pragma unroll 1
+            for (int32_t p = 0; p < parts; ++p) {
+                const uint32_t at = (uint32_t(p) * kSlot + m * (DP + 4u)) * 4u;
+                const f32x4 s = load_device_scope(mem, at + DP * 4u);
+                const float now = fmaxf(ref[u], s[0]);
+                const float keep = ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref[u] - now), by = s[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[0] - now);
+                total[u] = total[u] * keep + s[1] * by;
+#pragma unroll
+                for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const f32x4 x = load_device_scope(mem, at + (32u * c + 2u * r + 4u * h) * 4u);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[u][c][r + e] = o[u][c][r + e] * keep + x[e] * by;
+                    }
+                ref[u] = now;
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+        const uint32_t m = wave * kWaveRows + 32u * u + j;
+        if (m >= t.rows) continue;
+        const bool any = !(total[u] == 0.f);
+        const float by = any ? 1.f / total[u] : 0.f;
+        T *og = reinterpret_cast<T *>(aa.out.data) + int64_t(row[u].token) * aa.out.token_stride + int64_t(row[u].head) * aa.out.head_stride;
+        const bool side_by_side = aa.out.dim_stride == 1 && (reinterpret_cast<uintptr_t>(og) & 7u) == 0u;
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const uint32_t d = 32u * c + 2u * r + 4u * h;
+                if (d >= D) continue;
+                if (side_by_side) {
+                    *reinterpret_cast<t_u32x2 *>(og + d) = t_u32x2{HalfOps<BF>::pack(o[u][c][r] * by, o[u][c][r + 1] * by), HalfOps<BF>::pack(o[u][c][r + 2] * by, o[u][c][r + 3] * by)};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) og[int64_t(d + e) * aa.out.dim_stride] = T(o[u][c][r + e] * by);
+                }
+            }
+        if (aa.lse && h == 0u) aa.lse[size_t(row[u].token) * aa.q_heads + row[u].head] = any ? (ref[u] + __builtin_amdgcn_logf(total[u])) * kLn2 : -INFINITY;
+    }
+}
+
+template <bool BF, int DP, int QT, int W>
+void launch(const AttendArgs &aa, hipStream_t s)
+{
+    const dim3 grid(aa.pages.heads, attend_tiles(aa.batch.tokens, aa.batch.sequences, aa.shared.d, QT * W == 8 ? 8u : 7u), aa.splits);
+    if (aa.pages.page_tokens.d % 16u == 0u) attend_chunk_kernel<BF, DP, QT, W, true><<<grid, dim3(64 * W), 0, s>>>(aa);
+    else attend_chunk_kernel<BF, DP, QT, W, false><<<grid, dim3(64 * W), 0, s>>>(aa);
+}
+
+template <bool BF>
+void launch_type(const AttendArgs &aa, uint32_t rows_log, hipStream_t s)
+{
+    const uint32_t D = aa.pages.head_dim;
+    if (D <= 64u) rows_log == 8u ? launch<BF, 64, 1, 8>(aa, s) : launch<BF, 64, 1, 4>(aa, s);
+    else if (D <= 128u) rows_log == 8u ? launch<BF, 128, 1, 8>(aa, s) : launch<BF, 128, 1, 4>(aa, s);
+    else launch<BF, 256, 1, 4>(aa, s);
+}
+
+}  // namespace
+
+hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, uint32_t rows_log, hipStream_t s)
+{
+    if (dtype == kDtypeF16) launch_type<false>(aa, rows_log, s);
+    else launch_type<true>(aa, rows_log, s);
+    return hipGetLastError();
+}
+
+}  // namespace hspmm

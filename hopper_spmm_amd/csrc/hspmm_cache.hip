@@ -289,26 +289,33 @@ static int check_attention(const hspmm_cache *c, const hspmm_batch *b, const hsp
 
 // How an attention is launched, by sizes alone: the same for the call and for its workspace.
 struct AttendShape {
-    uint32_t tiles, splits, part_keys;
+    uint32_t rows_log;                   // of a tile: kAttendRowsLog the rows kernel, 7 and 8 the chunk kernel
+    uint32_t splits, part_keys;
     uint64_t bytes;
 };
 
 static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
 {
     const uint32_t shared = a->q_heads / c->heads;
+    const uint64_t rows = uint64_t(std::min(a->longest_chunk, b->tokens)) * shared;
     AttendShape sh{};
-    sh.tiles = attend_tiles(b->tokens, b->sequences, shared, kAttendRowsLog);
+    sh.rows_log = c->dtype == HSPMM_TF32 || rows <= 32u ? kAttendRowsLog : rows <= 128u || c->head_dim > 128u ? 7u : 8u;
+    // keys that a tile's rows see at most
     uint64_t keys = uint64_t(c->table_pages) * c->page_tokens;
     if (a->longest && a->longest < keys) keys = a->longest;
-    if (a->window && uint64_t(a->window) + a->longest_chunk < keys) keys = uint64_t(a->window) + a->longest_chunk;
-    const uint64_t tiles = uint64_t(b->tokens) * shared / (1u << kAttendRowsLog) + b->sequences, pairs = uint64_t(sh.tiles) * c->heads;
-    const uint64_t work = std::min<uint64_t>(tiles, uint64_t(b->sequences) * ((uint64_t(a->longest_chunk) * shared + 15u) / 16u)) * c->heads * keys;
-    uint64_t part = (work / 2048u + 127u) & ~uint64_t(127u);
-    part = std::max<uint64_t>(part, 256u);
+    if (a->window && uint64_t(a->window) + (1u << sh.rows_log) < keys) keys = uint64_t(a->window) + (1u << sh.rows_log);
+    const uint64_t numbered = attend_tiles(b->tokens, b->sequences, shared, sh.rows_log);
+    // tiles that have rows, at most: numbers are left out
+    const uint64_t tiles = std::min<uint64_t>(numbered, uint64_t(b->sequences) * ((rows + (1u << sh.rows_log) - 1u) >> sh.rows_log));
+    // workgroups wanted: the rows kernel has two a compute unit, and sequences are of many lengths
+    const bool chunk = sh.rows_log != kAttendRowsLog;
+    const uint64_t wanted = chunk ? 512u : 2048u, least = chunk ? 512u : 256u;
+    uint64_t part = (tiles * c->heads * keys / wanted + 127u) & ~uint64_t(127u);
+    part = std::max<uint64_t>(part, least);
     sh.part_keys = uint32_t(std::min<uint64_t>(part, 1u << 30));
     const uint64_t parts = (keys + 31u + sh.part_keys - 1u) / sh.part_keys;
-    sh.splits = pairs > kAttendCounters ? 1u : uint32_t(std::min<uint64_t>(std::max<uint64_t>(parts, 1u), 256u));
-    if (sh.splits > 1u) sh.bytes = kAttendCounters * 4u + pairs * sh.splits * attend_slot(kAttendRowsLog, c->head_dim) * 4u;
+    sh.splits = numbered * c->heads > kAttendCounters ? 1u : uint32_t(std::min<uint64_t>(std::max<uint64_t>(parts, 1u), 256u));
+    if (sh.splits > 1u) sh.bytes = kAttendCounters * 4u + numbered * c->heads * sh.splits * attend_slot(sh.rows_log, c->head_dim) * 4u;
     return sh;
 }
 
@@ -345,7 +352,8 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     aa.splits = sh.splits; aa.part_keys = sh.part_keys;
     aa.arrive = static_cast<uint32_t *>(workspace);
     aa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + kAttendCounters * 4u);
-    HSPMM_HIP(launch_attend_rows(cache->dtype, aa, static_cast<hipStream_t>(stream)));
+    if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, static_cast<hipStream_t>(stream)));
+    else HSPMM_HIP(launch_attend_chunk(cache->dtype, aa, sh.rows_log, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
 

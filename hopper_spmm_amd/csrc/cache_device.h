@@ -95,7 +95,7 @@ hipError_t launch_pages_compact(const PoolArgs &pa, int32_t *table_out, int32_t 
 hipError_t launch_pages_copy(const PoolArgs &pa, uint32_t n, const int32_t *from, const int32_t *to, hipStream_t s);
 
 #ifdef __HIPCC__
-// Where token t of a batch stands: its batch row (kIdxMax: outside every chunk), sequence, position (-1 and less: in front of the cache).
+// Where a token of a batch stands: its sequence and position (below 0: in front of the cache); not there: outside every chunk.
 struct TokenPlace { uint32_t sequence; int32_t position; bool there; };
 
 __device__ __forceinline__ int32_t clamp_i32(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : v > hi ? hi : v; }
@@ -107,16 +107,11 @@ __device__ __forceinline__ int32_t tokens_held(const PagesArgs &pg, uint32_t seq
     return clamp_i32(pg.lengths[sequence], 0, most > 0x7FFFFFFF ? 0x7FFFFFFF : int32_t(most));
 }
 
-__device__ __forceinline__ TokenPlace token_place(const BatchArgs &ba, const PagesArgs &pg, uint32_t t)
+// Token t as one of batch row b's, if it is.
+__device__ __forceinline__ TokenPlace place_in(const BatchArgs &ba, const PagesArgs &pg, uint32_t b, uint32_t t)
 {
-    // the last batch row that starts at or in front of t
-    uint32_t lo = 0, hi = ba.sequences;
-    while (hi - lo > 1u) {
-        const uint32_t mid = (lo + hi) / 2u;
-        if (ba.starts[mid] <= int32_t(t)) lo = mid; else hi = mid;
-    }
-    const int32_t first = ba.starts[lo], end = ba.starts[lo + 1u];
-    const uint32_t sequence = ba.rows ? uint32_t(ba.rows[lo]) : lo;
+    const int32_t first = ba.starts[b], end = ba.starts[b + 1u];
+    const uint32_t sequence = ba.rows ? uint32_t(ba.rows[b]) : b;
     if (first > int32_t(t) || end <= int32_t(t) || end > int32_t(ba.tokens) || sequence >= pg.sequences) return TokenPlace{0u, -1, false};
     return TokenPlace{sequence, tokens_held(pg, sequence) - end + int32_t(t), true};
 }

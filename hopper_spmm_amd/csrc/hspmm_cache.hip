@@ -146,8 +146,6 @@ uint32_t rotary_piece(int dtype, const RotaryArgs &ra, const hspmm_cache *c)
     if (c) all |= uint64_t(page_stride(c)) | uint64_t(layer_stride(c));
     const uint32_t vec = uint32_t(all & ~(all - 1u));
     if (vec == 1u && ra.table && ra.interleaved) return 0u;
-    // items are numbered in 31 bits
-    if (uint64_t(ra.head_dim / vec) * (ra.q_heads + 2u * ra.k_heads) * (c ? ra.tokens : 1u) >= 0x7FFFFFFFu) return 0u;
     return vec;
 }
 

@@ -38,72 +38,118 @@ __device__ __forceinline__ const float2 *angle_row(const RotaryArgs &ra, int32_t
     return reinterpret_cast<const float2 *>(ra.table) + size_t(clamp_i32(position, 0, int32_t(ra.positions) - 1)) * (ra.dims / 2u);
 }
 
-// Heads whose elements lie side by side in x and in y: a lane moves V of them at a time, with their partners where those are
-// V elements of their own (HALF).  A token's items: per turned head and, HALF, pair of pieces (else piece) one, per piece that only is copied one.
+// Where token t of a batch stands, t the same in every lane: the wave looks at 64 batch rows at a time.
+__device__ __forceinline__ TokenPlace wave_token_place(const BatchArgs &ba, const PagesArgs &pg, uint32_t t)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t lo = 0, n = ba.sequences;
+    while (n > 1u) {
+        const uint32_t step = (n + 63u) / 64u, b = lane * step;
+        const uint32_t below = uint32_t(__popcll(__ballot(b < n && ba.starts[lo + (b < n ? b : 0u)] <= int32_t(t))));
+        const uint32_t skip = (below ? below - 1u : 0u) * step;
+        lo += skip;
+        n = n - skip < step ? n - skip : step;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    return place_in(ba, pg, lo, t);
+}
+
+// Heads whose elements lie side by side in x and in y: a lane moves V of them at a time, with their partners where those are V elements of their
+// own (HALF).  A wave has a token and a range of its heads, so that where the token stands is found once; its lanes lie along a head's pieces (a pair of pieces
+// that turn, else a piece) and along heads, and keep their angles from head to head.  kAhead pieces of a lane are asked for before the first is turned.
 template <int DT, int V, bool HALF>
-__global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs ra, const Divisor by_items, const Divisor by_turned, const Divisor by_copied,
-                                                     const uint32_t turned_items, const uint64_t all)
+__global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs ra, const uint32_t heads_each, const uint32_t turned_items, const uint32_t copied_items)
 {
     typedef typename Elem<DT>::T T;
     struct alignas(V * sizeof(T)) Piece { T e[V]; };
-    const uint32_t pairs = HALF && ra.table ? ra.dims / 2u / V : 0u;                 // items of a turned head that are two pieces
-    for (uint64_t i = uint64_t(blockIdx.x) * 256u + threadIdx.x; i < all; i += uint64_t(gridDim.x) * 256u) {
-        const uint32_t t = by_items.quotient(uint32_t(i));
-        uint32_t item = uint32_t(i) - t * by_items.d;
-        uint32_t h, c;
-        if (item < turned_items) {
-            h = by_turned.quotient(item);
-            c = item - h * by_turned.d;
-        } else {
-            item -= turned_items;
-            const uint32_t v = by_copied.quotient(item);
-            h = ra.q_heads + ra.k_heads + v;
-            c = item - v * by_copied.d;
-        }
+    constexpr int kAhead = 4;
+    const uint32_t lane = threadIdx.x & 63u, t = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
+    if (t >= ra.tokens) return;
+    const uint32_t h0 = blockIdx.y * heads_each, all = ra.q_heads + 2u * ra.k_heads, h1 = h0 + heads_each < all ? h0 + heads_each : all;
+    TokenPlace place{0u, 0, true};
+    int64_t at = -1;                                                             // of head 0 in the pages
+    if (ra.batch.starts) {
+        place = wave_token_place(ra.batch, ra.pages, t);
+        if (!place.there) return;
+        at = row_offset(ra.pages, place.sequence, place.position, 0u);
+    }
+    const uint32_t pairs = HALF && ra.table ? ra.dims / 2u / V : 0u;            // items of a turned head that are two pieces
+    const float2 *angles = ra.table ? angle_row(ra, ra.at ? ra.at[t] : place.position) : nullptr;
+    const uint32_t turned = ra.q_heads + ra.k_heads;
+    auto source = [&](uint32_t h) __attribute__((always_inline)) {
         const HeadRole role = head_role(ra, h);
-        TokenPlace place{0u, 0, true};
-        if (ra.batch.starts) place = token_place(ra.batch, ra.pages, t);
-        if (!place.there) continue;
-        const T *x = reinterpret_cast<const T *>(role.from->data) + int64_t(t) * role.from->token_stride + int64_t(role.head) * role.from->head_stride;
-        T *y;
-        if (role.query) {
-            y = reinterpret_cast<T *>(ra.q_out.data) + int64_t(t) * ra.q_out.token_stride + int64_t(role.head) * ra.q_out.head_stride;
-        } else {
-            const int64_t at = row_offset(ra.pages, place.sequence, place.position, role.head);
-            if (at < 0) continue;
-            y = reinterpret_cast<T *>(role.key ? ra.pages.keys : ra.pages.values) + at;
-        }
-        const bool turns = ra.table && (role.query || role.key);
-        const float2 *angles = turns ? angle_row(ra, ra.at ? ra.at[t] : place.position) : nullptr;
-        if (turns && HALF && c < pairs) {
-            const uint32_t a = c * V, b = a + ra.dims / 2u;
-            const Piece p = *reinterpret_cast<const Piece *>(x + a), q = *reinterpret_cast<const Piece *>(x + b);
-            Piece r, s;
+        return reinterpret_cast<const T *>(role.from->data) + int64_t(t) * role.from->token_stride + int64_t(role.head) * role.from->head_stride;
+    };
+    // null: the token is not stored
+    auto target = [&](uint32_t h) __attribute__((always_inline)) -> T * {
+        if (h < ra.q_heads) return reinterpret_cast<T *>(ra.q_out.data) + int64_t(t) * ra.q_out.token_stride + int64_t(h) * ra.q_out.head_stride;
+        if (at < 0) return nullptr;
+        const bool key = h < turned;
+        return reinterpret_cast<T *>(key ? ra.pages.keys : ra.pages.values) + at + int64_t(h - (key ? ra.q_heads : turned)) * ra.pages.head_stride;
+    };
+    // heads [first, end) of `items` items each
+    auto walk = [&](uint32_t first, uint32_t end, uint32_t items, auto turns) __attribute__((always_inline)) {
+        constexpr bool kTurns = decltype(turns)::value;
+        const uint32_t abreast = items < 64u ? 64u / items : 1u, mine = items < 64u ? lane / items : 0u;
+        for (uint32_t c = items < 64u ? lane - mine * items : lane; c < items; c += 64u) {
+            if (mine >= abreast) break;
+            const bool pair = kTurns && HALF && c < pairs;
+            const uint32_t a = pair ? c * V : (c + (kTurns ? pairs : 0u)) * V, b = a + ra.dims / 2u;
+            float2 cs[V];
+            if constexpr (kTurns) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float2 y2 = turn(float(p.e[e]), float(q.e[e]), angles[a + e], ra.sign);
-                r.e[e] = T(y2.x);
-                s.e[e] = T(y2.y);
+                for (int e = 0; e < V; ++e) {
+                    cs[e] = float2{1.f, 0.f};
+                    if constexpr (HALF) {
+                        if (pair) cs[e] = angles[a + e];
+                    } else if (e % 2 == 0) {
+                        if (ra.table && a + e < ra.dims) cs[e] = angles[(a + e) / 2u];
+                    }
+                }
             }
-            *reinterpret_cast<Piece *>(y + a) = r;
-            *reinterpret_cast<Piece *>(y + b) = s;
-            continue;
-        }
-        if (turns && HALF) c += pairs;
-        Piece p = *reinterpret_cast<const Piece *>(x + c * V);
-        if constexpr (!HALF && V > 1) {
-            if (turns) {
+            for (uint32_t h = first + mine; h < end; h += kAhead * abreast) {
+                Piece p[kAhead], q[kAhead];
 #pragma unroll
-                for (int e = 0; e < V; e += 2) {
-                    if (c * V + e >= ra.dims) break;
-                    const float2 y2 = turn(float(p.e[e]), float(p.e[e + 1]), angles[(c * V + e) / 2u], ra.sign);
-                    p.e[e] = T(y2.x);
-                    p.e[e + 1] = T(y2.y);
+                for (int k = 0; k < kAhead; ++k) {
+                    const uint32_t hk = h + k * abreast;
+                    if (hk >= end) break;
+                    const T *x = source(hk);
+                    p[k] = *reinterpret_cast<const Piece *>(x + a);
+                    if (pair) q[k] = *reinterpret_cast<const Piece *>(x + b);
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const uint32_t hk = h + k * abreast;
+                    if (hk >= end) break;
+                    T *y = target(hk);
+                    if (!y) continue;
+                    if constexpr (kTurns && HALF) {
+                        if (pair) {
+#pragma unroll
+                            for (int e = 0; e < V; ++e) {
+                                const float2 y2 = turn(float(p[k].e[e]), float(q[k].e[e]), cs[e], ra.sign);
+                                p[k].e[e] = T(y2.x);
+                                q[k].e[e] = T(y2.y);
+                            }
+                            *reinterpret_cast<Piece *>(y + b) = q[k];
+                        }
+                    }
+                    if constexpr (kTurns && !HALF && V > 1) {
+#pragma unroll
+                        for (int e = 0; e < V; e += 2) {
+                            if (!ra.table || a + e >= ra.dims) break;
+                            const float2 y2 = turn(float(p[k].e[e]), float(p[k].e[e + 1]), cs[e], ra.sign);
+                            p[k].e[e] = T(y2.x);
+                            p[k].e[e + 1] = T(y2.y);
+                        }
+                    }
+                    *reinterpret_cast<Piece *>(y + a) = p[k];
                 }
             }
         }
-        *reinterpret_cast<Piece *>(y + c * V) = p;
-    }
+    };
+    if (h0 < turned) walk(h0, h1 < turned ? h1 : turned, turned_items, std::true_type{});
+    if (h1 > turned) walk(h0 > turned ? h0 : turned, h1, copied_items, std::false_type{});
 }
 
 // Any strides: a workgroup has tt (up to 64, a power of two) tokens of one head and 32 of its pairs (all elements count in pairs here, those that do not turn, too).
@@ -112,9 +158,12 @@ template <int DT>
 __global__ __launch_bounds__(256) void rotary_strided_kernel(const RotaryArgs ra, const uint32_t tt_log)
 {
     typedef typename Elem<DT>::T T;
-    constexpr uint32_t kPairs = 32u;
+    constexpr uint32_t kPairs = 32u, kMine = 64u * kPairs / 256u, kStarts = 512u;
     __shared__ T image[64u * (2u * kPairs + 2u)];
-    const uint32_t tt = 1u << tt_log, t0 = blockIdx.x << tt_log, pair0 = blockIdx.y * kPairs;
+    __shared__ int64_t rows[64];                    // a token's row in the pages (head 0), -1: not stored
+    __shared__ int32_t position_of[64], starts[kStarts + 1u];
+    __shared__ bool there[64];
+    const uint32_t tt = 1u << tt_log, t0 = blockIdx.x << tt_log, pair0 = blockIdx.y * kPairs, tid = threadIdx.x;
     const HeadRole role = head_role(ra, blockIdx.z);
     const uint32_t all_pairs = ra.head_dim / 2u + (ra.head_dim & 1u), dims = ra.table && (role.query || role.key) ? ra.dims : 0u;
     const bool by_token = role.from->dim_stride != 1;
@@ -123,46 +172,76 @@ __global__ __launch_bounds__(256) void rotary_strided_kernel(const RotaryArgs ra
         if (ra.interleaved || 2u * p >= dims) return 2u * p + second;
         return p + second * (dims / 2u);
     };
-    for (uint32_t i = threadIdx.x; i < tt * kPairs; i += 256u) {
-        const uint32_t ti = by_token ? i & (tt - 1u) : i / kPairs, pi = by_token ? i >> tt_log : i % kPairs, t = t0 + ti, p = pair0 + pi;
-        if (t >= ra.tokens || p >= all_pairs) continue;
-        const T *x = reinterpret_cast<const T *>(role.from->data) + int64_t(t) * role.from->token_stride + int64_t(role.head) * role.from->head_stride;
-        const uint32_t a = element(p, 0u), b = element(p, 1u);
-        T u = x[int64_t(a) * role.from->dim_stride], w = T(0.f);
-        if (b < ra.head_dim) w = x[int64_t(b) * role.from->dim_stride];
-        if (2u * p < dims) {
-            int32_t at;
-            if (ra.at) at = ra.at[t];
-            else {
-                const TokenPlace place = token_place(ra.batch, ra.pages, t);
-                if (!place.there) continue;
-                at = place.position;
+    auto token_and_pair = [&](uint32_t i, uint32_t *ti, uint32_t *pi) __attribute__((always_inline)) {
+        *ti = by_token ? i & (tt - 1u) : i / kPairs;
+        *pi = by_token ? i >> tt_log : i % kPairs;
+        return i < tt * kPairs && t0 + *ti < ra.tokens && pair0 + *pi < all_pairs;
+    };
+    // this thread's pairs, asked for before it is known where their tokens stand
+    T u[kMine], w[kMine];
+#pragma unroll
+    for (uint32_t k = 0; k < kMine; ++k) {
+        uint32_t ti, pi;
+        u[k] = w[k] = T(0.f);
+        if (!token_and_pair(tid + 256u * k, &ti, &pi)) continue;
+        const T *x = reinterpret_cast<const T *>(role.from->data) + int64_t(t0 + ti) * role.from->token_stride + int64_t(role.head) * role.from->head_stride;
+        const uint32_t a = element(pair0 + pi, 0u), b = element(pair0 + pi, 1u);
+        u[k] = x[int64_t(a) * role.from->dim_stride];
+        if (b < ra.head_dim) w[k] = x[int64_t(b) * role.from->dim_stride];
+    }
+    BatchArgs batch = ra.batch;
+    const bool near = batch.starts && batch.sequences <= kStarts;
+    if (near) {
+        for (uint32_t i = tid; i <= batch.sequences; i += 256u) starts[i] = batch.starts[i];
+        __syncthreads();
+    }
+    if (tid < tt) {
+        const uint32_t t = t0 + tid;
+        TokenPlace place{0u, 0, t < ra.tokens};
+        int64_t at = -1;
+        if (batch.starts && t < ra.tokens) {
+            uint32_t lo = 0, hi = batch.sequences;
+            while (hi - lo > 1u) {
+                const uint32_t mid = (lo + hi) / 2u;
+                if ((near ? starts[mid] : batch.starts[mid]) <= int32_t(t)) lo = mid; else hi = mid;
             }
-            const float2 y2 = turn(float(u), float(w), angle_row(ra, at)[p], ra.sign);
-            u = T(y2.x);
-            w = T(y2.y);
+            place = place_in(batch, ra.pages, lo, t);
+            if (place.there) at = row_offset(ra.pages, place.sequence, place.position, 0u);
         }
-        image[ti * (2u * kPairs + 2u) + 2u * pi] = u;
-        image[ti * (2u * kPairs + 2u) + 2u * pi + 1u] = w;
+        rows[tid] = at;
+        there[tid] = place.there;
+        position_of[tid] = ra.at && t < ra.tokens ? ra.at[t] : place.position;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < kMine; ++k) {
+        uint32_t ti, pi;
+        if (!token_and_pair(tid + 256u * k, &ti, &pi)) continue;
+        const uint32_t p = pair0 + pi;
+        if (2u * p < dims && there[ti]) {
+            const float2 y2 = turn(float(u[k]), float(w[k]), angle_row(ra, position_of[ti])[p], ra.sign);
+            u[k] = T(y2.x);
+            w[k] = T(y2.y);
+        }
+        image[ti * (2u * kPairs + 2u) + 2u * pi] = u[k];
+        image[ti * (2u * kPairs + 2u) + 2u * pi + 1u] = w[k];
     }
     __syncthreads();
     const bool out_by_token = role.query && ra.q_out.dim_stride != 1;
-    for (uint32_t i = threadIdx.x; i < tt * 2u * kPairs; i += 256u) {
+#pragma unroll
+    for (uint32_t k = 0; k < 2u * kMine; ++k) {
+        const uint32_t i = tid + 256u * k;
         uint32_t ti, pi, second;
         if (out_by_token) { ti = i & (tt - 1u); pi = (i >> tt_log) / 2u; second = (i >> tt_log) & 1u; }
         else if (ra.interleaved || 2u * (pair0 + kPairs) > dims) { ti = i / (2u * kPairs); pi = i / 2u % kPairs; second = i & 1u; }
         else { ti = i / (2u * kPairs); second = i / kPairs & 1u; pi = i % kPairs; }
         const uint32_t t = t0 + ti, p = pair0 + pi, e = element(p, second);
-        if (t >= ra.tokens || p >= all_pairs || e >= ra.head_dim) continue;
-        TokenPlace place{0u, 0, true};
-        if (ra.batch.starts) place = token_place(ra.batch, ra.pages, t);
-        if (!place.there) continue;
+        if (i >= tt * 2u * kPairs || t >= ra.tokens || p >= all_pairs || e >= ra.head_dim || !there[ti]) continue;
         const T v = image[ti * (2u * kPairs + 2u) + 2u * pi + second];
         if (role.query) {
             reinterpret_cast<T *>(ra.q_out.data)[int64_t(t) * ra.q_out.token_stride + int64_t(role.head) * ra.q_out.head_stride + int64_t(e) * ra.q_out.dim_stride] = v;
-        } else {
-            const int64_t at = row_offset(ra.pages, place.sequence, place.position, role.head);
-            if (at >= 0) reinterpret_cast<T *>(role.key ? ra.pages.keys : ra.pages.values)[at + e] = v;
+        } else if (rows[ti] >= 0) {
+            reinterpret_cast<T *>(role.key ? ra.pages.keys : ra.pages.values)[rows[ti] + int64_t(role.head) * ra.pages.head_stride + e] = v;
         }
     }
 }
@@ -170,24 +249,13 @@ __global__ __launch_bounds__(256) void rotary_strided_kernel(const RotaryArgs ra
 template <int DT, int V, bool HALF>
 void launch_pieces(const RotaryArgs &ra, hipStream_t s)
 {
-    const uint32_t pieces = ra.head_dim / V, turned = HALF && ra.table ? pieces - ra.dims / 2u / V : pieces;
-    const uint32_t turned_items = (ra.q_heads + ra.k_heads) * turned, items = turned_items + ra.k_heads * pieces;
-    // (numbers of items stay below 2^31: tokens in several launches beyond)
-    const uint32_t most = 0x7FFFFFFFu / items;
-    for (uint32_t t = 0; t < ra.tokens; t += most) {
-        RotaryArgs part = ra;
-        if (ra.tokens > most) {
-            part.tokens = ra.tokens - t < most ? ra.tokens - t : most;
-            // (only rotations of whole tensors are that large: a batch's tokens are numbered as a whole)
-            const int64_t el = DT == kDtypeF32 ? 4 : 2;
-            part.q.data += int64_t(t) * ra.q.token_stride * el;
-            part.q_out.data += int64_t(t) * ra.q_out.token_stride * el;
-            part.at += t;
-        }
-        const uint64_t all = uint64_t(part.tokens) * items, groups = (all + 255u) / 256u;
-        rotary_kernel<DT, V, HALF><<<dim3(uint32_t(groups < (1u << 20) ? groups : 1u << 20)), dim3(256), 0, s>>>(
-            part, Divisor::of(items), Divisor::of(turned), Divisor::of(pieces), turned_items, all);
-    }
+    const uint32_t pieces = ra.head_dim / V, turned = HALF && ra.table ? pieces - ra.dims / 2u / V : pieces, heads = ra.q_heads + 2u * ra.k_heads;
+    // Few tokens: their heads are shared out to several waves, as long as each has a round of its lanes.
+    const uint32_t groups = (ra.tokens + 3u) / 4u, round = turned < 64u ? 64u / turned : 1u;
+    uint32_t shares = groups < 512u ? 512u / groups : 1u;
+    if (shares > (heads + round - 1u) / round) shares = (heads + round - 1u) / round;
+    const uint32_t each = (heads + shares - 1u) / shares;
+    rotary_kernel<DT, V, HALF><<<dim3(groups, (heads + each - 1u) / each), dim3(256), 0, s>>>(ra, each, turned, pieces);
 }
 
 template <int DT>

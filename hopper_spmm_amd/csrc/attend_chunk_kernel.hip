@@ -92,54 +92,73 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
 
     const int32_t *table = aa.pages.table + size_t(t.sequence) * aa.pages.table_pages;
     const int64_t head_offset = int64_t(head) * aa.pages.head_stride;
-    // page numbers of the next 16 images, four an image (Whole)
-    int32_t pages_ahead = -1;
+    // Where keys lie, in bytes from keys and values: of groups of 16 keys, four an image, of 16 images at a time, a lane each (Whole), or of
+    // the keys of an image; and which of them are stored, a bit each.
+    uint32_t ahead_low = 0u, ahead_high = 0u;
+    uint64_t ahead_there = 0u;
+    auto look_up = [&](int32_t key) __attribute__((always_inline)) {
+        const int64_t at = key < end ? key_offset(aa.pages, table, head_offset, key) : -1;
+        ahead_there = __ballot(at >= 0);
+        const uint64_t bytes = at >= 0 ? uint64_t(at) * 2u : 0u;
+        ahead_low = uint32_t(bytes);
+        ahead_high = uint32_t(bytes >> 32);
+    };
     // a thread's pieces of an image: 16 bytes of a row of keys and of values
     u32x4 k_piece[kPieces], v_piece[kPieces];
-    uint64_t stored_there = 0u;                                // keys of the image that are stored, a bit each
+    uint32_t groups_there = 0u;                                // of the image in the registers (Whole)
+    uint64_t keys_there = 0u;
     const uint32_t column = (tid % kRowPieces) * 8u;
+    // (of lanes behind the last element, and of keys that are not stored, something is read and not used)
+    const uint32_t in_column = (column < D ? column : 0u) * 2u;
+    const uint32_t in_group = Whole ? uint32_t(int64_t((tid / kRowPieces) % 16u) * aa.pages.token_stride) * 2u + in_column : in_column;
     auto request = [&](int32_t n) __attribute__((always_inline)) {
-        const int32_t key0 = begin + n * 64;
-        const uint64_t in = n >= n_images ? 0u : end - key0 >= 64 ? ~uint64_t(0) : (uint64_t(1) << (end - key0)) - 1u;
-        stored_there = 0u;
+        constexpr uint32_t kPieceRows = kThreads / kRowPieces;                   // rows between a thread's pieces
         if constexpr (Whole) {
-            if (n % 16 == 0) {
-                const int32_t key = key0 + int32_t(lane) * 16;
-                pages_ahead = -1;
-                if (key < end) {
-                    const uint32_t place = aa.pages.page_tokens.quotient(uint32_t(key));
-                    if (place < aa.pages.table_pages) pages_ahead = table[place];
-                }
-            }
+            if (n % 16 == 0) look_up(begin + n * 64 + int32_t(lane) * 16);
+            const int32_t first = n % 16 * 4;
+            groups_there = uint32_t(ahead_there >> first) & 15u;
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                if (uint32_t(__builtin_amdgcn_readlane(pages_ahead, n % 16 * 4 + g)) < aa.pages.pages) stored_there |= uint64_t(0xFFFFu) << (16 * g);
-            stored_there &= in;
-        } else {
-            const int32_t key = key0 + int32_t(lane);
-            stored_there = __ballot(n < n_images && key < end && key_offset(aa.pages, table, 0, key) >= 0);
-        }
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const uint32_t r = (tid + kThreads * i) / kRowPieces;
-            int64_t at;
-            if constexpr (Whole) {
+            for (int i = 0; i < kPieces; ++i) {
                 // (a wave's rows of a piece lie in one group of 16)
-                const uint32_t g = (64u * wave + kThreads * i) / kRowPieces / 16u, key = uint32_t(key0) + 16u * g;
-                const uint32_t id = uint32_t(__builtin_amdgcn_readlane(pages_ahead, n % 16 * 4 + int(g)));
-                at = int64_t(id) * aa.pages.page_stride + head_offset + int64_t(key - aa.pages.page_tokens.quotient(key) * aa.pages.page_tokens.d) * aa.pages.token_stride +
-                     int64_t(r % 16u) * aa.pages.token_stride;
-            } else {
-                at = key0 + int32_t(r) < end ? key_offset(aa.pages, table, head_offset, key0 + int32_t(r)) : -1;
+                const int32_t g = first + int32_t((64u * wave + kThreads * i) / kRowPieces / 16u);
+                const uint64_t from = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(ahead_low), g))) | uint64_t(uint32_t(__builtin_amdgcn_readlane(int(ahead_high), g))) << 32;
+                const uint32_t at = in_group + (kPieceRows < 16u ? uint32_t(int64_t(i * kPieceRows % 16u) * aa.pages.token_stride) * 2u : 0u);
+                k_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.keys + from + at);
+                v_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.values + from + at);
             }
-            // (what is not stored may be anything, and no weight of zero undoes a NaN)
-            const bool there = column < D && (stored_there >> r & 1u);
-            k_piece[i] = there ? *reinterpret_cast<const u32x4 *>(aa.pages.keys + (at + column) * 2) : u32x4{0u, 0u, 0u, 0u};
-            v_piece[i] = there ? *reinterpret_cast<const u32x4 *>(aa.pages.values + (at + column) * 2) : u32x4{0u, 0u, 0u, 0u};
+        } else {
+            look_up(begin + n * 64 + int32_t(lane));
+            keys_there = ahead_there;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int r = int(tid / kRowPieces + kPieceRows * i);
+                const uint64_t from = uint64_t(uint32_t(__shfl(int(ahead_low), r))) | uint64_t(uint32_t(__shfl(int(ahead_high), r))) << 32;
+                k_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.keys + from + in_group);
+                v_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.values + from + in_group);
+            }
         }
+    };
+    // the stored keys of image n, which is in the registers
+    auto stored_keys = [&](int32_t n) __attribute__((always_inline)) {
+        const int32_t left = end - (begin + n * 64);
+        const uint64_t in = left >= 64 ? ~uint64_t(0) : left > 0 ? (uint64_t(1) << left) - 1u : 0u;
+        if constexpr (!Whole) return keys_there & in;
+        if (groups_there == 15u) return in;
+        uint64_t there = 0u;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            if (groups_there >> g & 1u) there |= uint64_t(0xFFFFu) << (16 * g);
+        return there & in;
     };
     auto write_image = [&](int32_t n, uint32_t to) __attribute__((always_inline)) {
         char *const image = images + to * kImage;
+        const uint64_t stored_there = stored_keys(n);
+        if (~stored_there || D < uint32_t(DP)) {
+            // (what is not stored may be anything, and no weight of zero undoes a NaN)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+                if (column >= D || !(stored_there >> ((tid + kThreads * i) / kRowPieces) & 1u)) k_piece[i] = v_piece[i] = u32x4{0u, 0u, 0u, 0u};
+        }
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const uint32_t r = (tid + kThreads * i) / kRowPieces;
@@ -155,6 +174,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
                 for (int w = 0; w < 4; ++w) any |= word_not_finite<BF>(v_piece[i][w]);
             if (any) odd = 1u;
         }
+        return stored_there;
     };
 
     f32x16 o[QT][kTiles];
@@ -172,32 +192,38 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
     };
     const uint32_t key_lane = j * kKeyPitch + h * 16u;
     const uint32_t value_lane = kKeys * kKeyPitch + (4u * h + (lane & 15u) / 4u) * kValuePitch + ((lane >> 4 & 1u) * 16u + (lane & 3u) * 4u) * 2u;
-    // steps S0 .. S1 - 1 of the scores of half `half` of an image
-    auto scores = [&](auto s0, auto s1, f32x16 (&s)[QT], uint32_t image, uint32_t half) __attribute__((always_inline)) {
-        const char *const from = images + image * kImage + half * 32u * kKeyPitch + key_lane;
-        if constexpr (decltype(s0)::value == 0) {
+    // The first operands of half of the scores' instructions, asked for well ahead of them.
+    struct KeyOperands { u32x4 a[kSteps / 2]; };
+    auto ask_keys = [&](KeyOperands &f, auto second, uint32_t image, uint32_t half) __attribute__((always_inline)) {
+        const char *const from = images + image * kImage + half * 32u * kKeyPitch + key_lane + decltype(second)::value * (kSteps / 2) * 32;
+#pragma unroll
+        for (int c = 0; c < kSteps / 2; ++c) f.a[c] = *reinterpret_cast<const u32x4 *>(from + c * 32);
+    };
+    auto scores = [&](auto second, f32x16 (&s)[QT], const KeyOperands &f) __attribute__((always_inline)) {
+        constexpr int c0 = decltype(second)::value * (kSteps / 2);
+        if constexpr (c0 == 0) {
 #pragma unroll
             for (int u = 0; u < QT; ++u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
         }
 #pragma unroll
-        for (int c = decltype(s0)::value; c < decltype(s1)::value; ++c) {
-            const u32x4 a = *reinterpret_cast<const u32x4 *>(from + c * 32);
+        for (int c = 0; c < kSteps / 2; ++c)
 #pragma unroll
-            for (int u = 0; u < QT; ++u) s[u] = Wide<BF>::mfma(a, q[u][c], s[u]);
-        }
+            for (int u = 0; u < QT; ++u) s[u] = Wide<BF>::mfma(f.a[c], q[u][c0 + c], s[u]);
     };
     auto mask = [&](f32x16 (&s)[QT], int32_t key0, uint32_t stored) __attribute__((always_inline)) {
         if (key0 >= all_lo && key0 + 32 <= all_hi && stored == ~0u) return;
+        const uint32_t mine = stored >> (4u * h);
 #pragma unroll
-        for (int u = 0; u < QT; ++u)
+        for (int u = 0; u < QT; ++u) {
+            const int32_t low = row[u].lo - key0 - int32_t(4u * h), high = row[u].hi - key0 - int32_t(4u * h);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const uint32_t a = 8u * (r / 4) + 4u * h + r % 4;
-                const int32_t key = key0 + int32_t(a);
-                if (!(key >= row[u].lo && key < row[u].hi && (stored >> a & 1u))) s[u][r] = -INFINITY;
+                constexpr int kOf[16] = {0, 1, 2, 3, 8, 9, 10, 11, 16, 17, 18, 19, 24, 25, 26, 27};
+                if (!(kOf[r] >= low && kOf[r] < high && (mine >> kOf[r] & 1u))) s[u][r] = -INFINITY;
             }
+        }
     };
     // the largest score of every row; where one is far above its row's reference the sums move to a new one
     auto move_references = [&](const f32x16 (&s)[QT]) __attribute__((always_inline)) {
@@ -212,7 +238,8 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
             moves[u] = most[u] > ref[u] + kReferenceSlack || (ref[u] == -INFINITY && most[u] > -INFINITY);
             any |= moves[u];
         }
-        if (__ballot(any)) {
+        if (__builtin_expect(__ballot(any) != 0u, 0)) {
+            asm volatile("");                                  // (a branch, not 32 QT DP / 64 multiplications by one every time)
 #pragma unroll
             for (int u = 0; u < QT; ++u) {
                 const float by = moves[u] ? __builtin_amdgcn_exp2f(ref[u] - most[u]) : 1.f;
@@ -234,61 +261,77 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
             }
         }
     };
-    auto add = [&](const f32x16 (&s)[QT], uint32_t image, uint32_t half) __attribute__((always_inline)) {
+    // The same of the sums' instructions for 16 keys.
+    struct ValueOperands { u32x4 a[kTiles]; };
+    auto ask_values = [&](ValueOperands &f, auto second, uint32_t image, uint32_t half) __attribute__((always_inline)) {
+        constexpr int c = decltype(second)::value;
         const __attribute__((address_space(3))) char *const from = (const __attribute__((address_space(3))) char *)(images + image * kImage + half * 32u * kValuePitch + value_lane);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            u32x4 p[QT];
-#pragma unroll
-            for (int u = 0; u < QT; ++u)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) p[u][w] = HalfOps<BF>::pack(s[u][8 * c + 2 * w], s[u][8 * c + 2 * w + 1]);
-#pragma unroll
-            for (int e = 0; e < kTiles; ++e) {
-                const t_u32x2 a0 = __builtin_bit_cast(t_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tile_tr_ptr)(from + (16 * c) * kValuePitch + e * 64)));
-                const t_u32x2 a1 = __builtin_bit_cast(t_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tile_tr_ptr)(from + (16 * c + 8) * kValuePitch + e * 64)));
-                const u32x4 a{a0[0], a0[1], a1[0], a1[1]};
-#pragma unroll
-                for (int u = 0; u < QT; ++u) o[u][e] = Wide<BF>::mfma(a, p[u], o[u][e]);
-            }
+        for (int e = 0; e < kTiles; ++e) {
+            const t_u32x2 a0 = __builtin_bit_cast(t_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tile_tr_ptr)(from + (16 * c) * kValuePitch + e * 64)));
+            const t_u32x2 a1 = __builtin_bit_cast(t_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tile_tr_ptr)(from + (16 * c + 8) * kValuePitch + e * 64)));
+            f.a[e] = u32x4{a0[0], a0[1], a1[0], a1[1]};
         }
     };
-    using from0 = std::integral_constant<int, 0>;
-    using middle = std::integral_constant<int, kSteps / 2>;
-    using to_end = std::integral_constant<int, kSteps>;
+    auto add = [&](auto second, const f32x16 (&s)[QT], const ValueOperands &f) __attribute__((always_inline)) {
+        constexpr int c = decltype(second)::value;
+        u32x4 p[QT];
+#pragma unroll
+        for (int u = 0; u < QT; ++u)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) p[u][w] = pack_two<BF>(s[u][8 * c + 2 * w], s[u][8 * c + 2 * w + 1]);
+#pragma unroll
+        for (int e = 0; e < kTiles; ++e)
+#pragma unroll
+            for (int u = 0; u < QT; ++u) o[u][e] = Wide<BF>::mfma(f.a[e], p[u], o[u][e]);
+    };
+    using first = std::integral_constant<int, 0>;
+    using second = std::integral_constant<int, 1>;
+    KeyOperands keys_1, keys_2;
+    // A half: scores `s` become weights and are added, the scores of the half behind it are made meanwhile (its first operands are asked for
+    // already); at the end those of the one behind that are asked for.
+    auto half_step = [&](f32x16 (&s)[QT], f32x16 (&s_other)[QT], int32_t key0, uint32_t stored, uint32_t image, uint32_t half, uint32_t other_image, uint32_t other_half,
+                         uint32_t third_image, uint32_t third_half) __attribute__((always_inline)) {
+        mask(s, key0, stored);
+        ask_keys(keys_2, second{}, other_image, other_half);
+        __builtin_amdgcn_sched_barrier(0);
+        scores(first{}, s_other, keys_1);
+        move_references(s);
+        ValueOperands values_1, values_2;
+        ask_values(values_1, first{}, image, half);
+        __builtin_amdgcn_sched_barrier(0);
+        scores(second{}, s_other, keys_2);
+        exponentials(s);
+        __builtin_amdgcn_sched_barrier(0);
+        ask_values(values_2, second{}, image, half);
+        add(first{}, s, values_1);
+        ask_keys(keys_1, first{}, third_image, third_half);
+        add(second{}, s, values_2);
+    };
 
     begin_sums();
     if (n_images) {
         f32x16 s_a[QT], s_b[QT];
         request(0);
-        write_image(0, 0u);
-        uint64_t stored_now = stored_there;
+        uint64_t stored_now = write_image(0, 0u);
         request(1);
-        write_image(1, 1u);
-        uint64_t stored_next = stored_there;
+        uint64_t stored_next = write_image(1, 1u);
         lds_barrier();
-        scores(from0{}, to_end{}, s_a, 0u, 0u);
+        ask_keys(keys_1, first{}, 0u, 0u);
+        ask_keys(keys_2, second{}, 0u, 0u);
+        scores(first{}, s_a, keys_1);
+        scores(second{}, s_a, keys_2);
+        ask_keys(keys_1, first{}, 0u, 1u);
         uint32_t now = 0u, next = 1u, free = kRing - 1u;
 #pragma unroll 1
         for (int32_t n = 0; n < n_images; ++n) {
             const int32_t key0 = begin + n * 64;
             request(n + 2);
-            mask(s_a, key0, uint32_t(stored_now));
-            scores(from0{}, middle{}, s_b, now, 1u);
-            move_references(s_a);
-            scores(middle{}, to_end{}, s_b, now, 1u);
-            exponentials(s_a);
-            add(s_a, now, 0u);
-            mask(s_b, key0 + 32, uint32_t(stored_now >> 32));
-            scores(from0{}, middle{}, s_a, next, 0u);
-            move_references(s_b);
-            scores(middle{}, to_end{}, s_a, next, 0u);
-            exponentials(s_b);
-            add(s_b, now, 1u);
+            half_step(s_a, s_b, key0, uint32_t(stored_now), now, 0u, now, 1u, next, 0u);
+            half_step(s_b, s_a, key0 + 32, uint32_t(stored_now >> 32), now, 1u, next, 0u, next, 1u);
             if constexpr (kRing == 2u) { lds_barrier(); free = now; }
-            write_image(n + 2, free);
             stored_now = stored_next;
-            stored_next = stored_there;
+            stored_next = write_image(n + 2, free);
             const uint32_t old = now;
             now = next;
             next = free;
@@ -305,15 +348,17 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
 #pragma unroll 1
             for (int32_t n = 0; n < n_images; ++n) {
                 __syncthreads();
-                if (Whole && n % 16) request(n & ~15);         // (page numbers)
+                if (Whole && n % 16) look_up(begin + (n & ~15) * 64 + int32_t(lane) * 16);
                 request(n);
-                write_image(n, 0u);
-                const uint64_t stored = stored_there;
+                const uint64_t stored = write_image(n, 0u);
                 __syncthreads();
 #pragma unroll 1
                 for (uint32_t half = 0; half < 2u; ++half) {
                     const int32_t key0 = begin + n * 64 + int32_t(half) * 32;
-                    scores(from0{}, to_end{}, s_a, 0u, half);
+                    ask_keys(keys_1, first{}, 0u, half);
+                    ask_keys(keys_2, second{}, 0u, half);
+                    scores(first{}, s_a, keys_1);
+                    scores(second{}, s_a, keys_2);
                     mask(s_a, key0, uint32_t(stored >> (32u * half)));
                     move_references(s_a);
                     exponentials(s_a);
@@ -410,7 +455,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
                 const uint32_t d = 32u * c + 2u * r + 4u * h;
                 if (d >= D) continue;
                 if (side_by_side) {
-                    *reinterpret_cast<t_u32x2 *>(og + d) = t_u32x2{HalfOps<BF>::pack(o[u][c][r] * by, o[u][c][r + 1] * by), HalfOps<BF>::pack(o[u][c][r + 2] * by, o[u][c][r + 3] * by)};
+                    *reinterpret_cast<t_u32x2 *>(og + d) = t_u32x2{pack_two<BF>(o[u][c][r] * by, o[u][c][r + 1] * by), pack_two<BF>(o[u][c][r + 2] * by, o[u][c][r + 3] * by)};
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) og[int64_t(d + e) * aa.out.dim_stride] = T(o[u][c][r + e] * by);
@@ -429,20 +474,20 @@ void launch(const AttendArgs &aa, hipStream_t s)
 }
 
 template <bool BF>
-void launch_type(const AttendArgs &aa, uint32_t rows_log, hipStream_t s)
+void launch_type(const AttendArgs &aa, hipStream_t s)
 {
     const uint32_t D = aa.pages.head_dim;
-    if (D <= 64u) rows_log == 8u ? launch<BF, 64, 1, 8>(aa, s) : launch<BF, 64, 1, 4>(aa, s);
-    else if (D <= 128u) rows_log == 8u ? launch<BF, 128, 1, 8>(aa, s) : launch<BF, 128, 1, 4>(aa, s);
+    if (D <= 64u) launch<BF, 64, 1, 8>(aa, s);
+    else if (D <= 128u) launch<BF, 128, 1, 8>(aa, s);
     else launch<BF, 256, 1, 4>(aa, s);
 }
 
 }  // namespace
 
-hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, uint32_t rows_log, hipStream_t s)
+hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, hipStream_t s)
 {
-    if (dtype == kDtypeF16) launch_type<false>(aa, rows_log, s);
-    else launch_type<true>(aa, rows_log, s);
+    if (dtype == kDtypeF16) launch_type<false>(aa, s);
+    else launch_type<true>(aa, s);
     return hipGetLastError();
 }
 

@@ -96,6 +96,14 @@ __device__ __forceinline__ float max_quarters(float v)
     return max_halves(fmaxf(__builtin_bit_cast(float, uint32_t(r[0])), __builtin_bit_cast(float, uint32_t(r[1]))));
 }
 
+// Two floats rounded to a word of 16-bit elements (nearest, ties to even), in one instruction.
+template <bool BF> __device__ __forceinline__ uint32_t pack_two(float lo, float hi)
+{
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef typename HalfOps<BF>::elem_t pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, pair));
+}
+
 // Whether a word holds a 16-bit element that is not finite.
 template <bool BF> __device__ __forceinline__ bool word_not_finite(uint32_t w)
 {

@@ -69,8 +69,8 @@ struct Rows16 {
         u32x4 w;
 #pragma unroll
         for (int t = 0; t < kParts; ++t) {
-            w[2 * t] = HalfOps<BF>::pack(p[t][0], p[t][1]);
-            w[2 * t + 1] = HalfOps<BF>::pack(p[t][2], p[t][3]);
+            w[2 * t] = pack_two<BF>(p[t][0], p[t][1]);
+            w[2 * t + 1] = pack_two<BF>(p[t][2], p[t][3]);
         }
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
@@ -325,6 +325,7 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
         most = max_quarters(most);
         const bool moves = most > ref + kReferenceSlack || (ref == -INFINITY && most > -INFINITY);
         if (__ballot(moves)) {
+            asm volatile("");                                  // (a branch, not multiplications by one every time)
             const float by = moves ? __builtin_amdgcn_exp2f(ref - most) : 1.f;
             if (moves) ref = most;
             total *= by;

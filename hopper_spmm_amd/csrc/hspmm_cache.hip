@@ -297,7 +297,7 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     const uint32_t shared = a->q_heads / c->heads;
     const uint64_t rows = uint64_t(std::min(a->longest_chunk, b->tokens)) * shared;
     AttendShape sh{};
-    sh.rows_log = c->dtype == HSPMM_TF32 || rows <= 32u ? kAttendRowsLog : rows <= 128u || c->head_dim > 128u ? 7u : 8u;
+    sh.rows_log = c->dtype == HSPMM_TF32 || rows <= 32u ? kAttendRowsLog : attend_chunk_rows_log(c->head_dim);
     // keys that a tile's rows see at most
     uint64_t keys = uint64_t(c->table_pages) * c->page_tokens;
     if (a->longest && a->longest < keys) keys = a->longest;
@@ -307,7 +307,7 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     const uint64_t tiles = std::min<uint64_t>(numbered, uint64_t(b->sequences) * ((rows + (1u << sh.rows_log) - 1u) >> sh.rows_log));
     // workgroups wanted: the rows kernel has two a compute unit, and sequences are of many lengths
     const bool chunk = sh.rows_log != kAttendRowsLog;
-    const uint64_t wanted = chunk ? 512u : 2048u, least = chunk ? 512u : 256u;
+    const uint64_t wanted = chunk ? 256u : 2048u, least = chunk ? 512u : 256u;
     uint64_t part = (tiles * c->heads * keys / wanted + 127u) & ~uint64_t(127u);
     part = std::max<uint64_t>(part, least);
     sh.part_keys = uint32_t(std::min<uint64_t>(part, 1u << 30));
@@ -351,7 +351,7 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     aa.arrive = static_cast<uint32_t *>(workspace);
     aa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + kAttendCounters * 4u);
     if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, static_cast<hipStream_t>(stream)));
-    else HSPMM_HIP(launch_attend_chunk(cache->dtype, aa, sh.rows_log, static_cast<hipStream_t>(stream)));
+    else HSPMM_HIP(launch_attend_chunk(cache->dtype, aa, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
 

@@ -29,23 +29,24 @@ __device__ __forceinline__ void lds_barrier()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// A wave has 32 QT rows, a lane (h, j) = (lane / 32, lane % 32) row 32 t + j of tile t; keys come in images of 64, two halves of 32.
+// A wave has 32 rows, a lane (h, j) = (lane / 32, lane % 32) row j; keys come in images of 64, two halves of 32.
 //   scores: S^T = K Q^T, 32 keys x 32 rows by instructions of 16 elements; register r: key 8 (r / 4) + 4 h + r % 4
 //   sums:   O^T = V^T P^T, 32 elements x 32 rows by instructions of 16 keys: scores 8 s .. 8 s + 7 of a lane are its part of the second operand,
 //           keys in that order; the first one comes transposed from LDS (ds_read_b64_tr_b16), four keys of an element a read
-// The scores of a half are made among the exponentials of the half in front.  Images go through LDS, RING of them in turn: while image n is
-// multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image.
-template <bool BF, int DP, int QT, int W, bool Whole>
-__global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_chunk_kernel(const AttendArgs aa)
+// The scores of a half are made among the exponentials of the half in front.  Images go through LDS, kRing of them in turn: while image n is
+// multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image (with two places: two).
+template <bool BF, int DP, int W, bool Whole>
+__global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void attend_chunk_kernel(const AttendArgs aa)
 {
     typedef typename HalfOps<BF>::elem_t T;
-    constexpr uint32_t kThreads = 64u * W, kWaveRows = 32u * QT, kRows = kWaveRows * W, kKeys = 64u;
-    constexpr int kRowsLog = kRows == 256u ? 8 : 7;
-    static_assert(kRows == 1u << kRowsLog, "");
-    constexpr uint32_t kKeyPitch = DP * 2u + 16u, kValuePitch = DP * 2u + 64u, kImage = kKeys * (kKeyPitch + kValuePitch);
-    constexpr uint32_t kRing = DP <= 64 || (DP <= 128 && W == 8) ? 3u : 2u;
-    constexpr int kSteps = DP / 16, kTiles = DP / 32, kPieces = int(kKeys * DP / 8u / kThreads);
-    constexpr uint32_t kRowPieces = DP / 8u;
+    constexpr uint32_t kThreads = 64u * W, kRows = 32u * W, kKeys = 64u;
+    constexpr int kRowsLog = W == 8 ? 8 : 7;
+    // (rows whose operands are read together begin in different banks: 16 of keys 16 bytes apart, four of values 64)
+    constexpr uint32_t kKeyPitch = DP * 2u + 16u, kValuePitch = DP * 2u + (DP % 128 == 0 || DP == 64 ? 64u : 0u), kImage = kKeys * (kKeyPitch + kValuePitch);
+    static_assert(kKeyPitch / 16u % 2u == 1u && kValuePitch / 64u % 2u == 1u && kValuePitch % 64u == 0u, "");
+    constexpr uint32_t kRing = kImage <= 50u * 1024u ? 3u : 2u;
+    constexpr uint32_t kRowPieces = DP / 8u, kImagePieces = kKeys * kRowPieces;
+    constexpr int kSteps = DP / 16, kTiles = DP / 32, kPieces = int((kImagePieces + kThreads - 1u) / kThreads);
     __shared__ __attribute__((aligned(16))) char images[kRing * kImage];
     __shared__ uint32_t odd, arrived;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, j = lane & 31u;
@@ -62,24 +63,20 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
 
     const float scale = aa.scale == 0.f ? 1.f : fabsf(aa.scale) * kLog2e;
     const uint32_t flip = aa.scale < 0.f ? 0x80008000u : 0u;
-    RowOf row[QT];
-    u32x4 q[QT][kSteps];
-    int32_t all_lo = 0, all_hi = 0x7FFFFFFF;
-#pragma unroll
-    for (int u = 0; u < QT; ++u) {
-        const uint32_t m = wave * kWaveRows + 32u * u + j;
-        row[u] = row_of_tile(aa, t, head, m);
-        const char *from = aa.q.data + (int64_t(row[u].token) * aa.q.token_stride + int64_t(row[u].head) * aa.q.head_stride) * 2;
+    const uint32_t m = wave * 32u + j;
+    const bool is_row = m < t.rows;
+    const RowOf row = row_of_tile(aa, t, head, m);
+    u32x4 q[kSteps];
+    {
+        const char *from = aa.q.data + (int64_t(row.token) * aa.q.token_stride + int64_t(row.head) * aa.q.head_stride) * 2;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const uint32_t d = 16u * s + 8u * h;
-            q[u][s] = m < t.rows && d < D && aa.scale != 0.f ? *reinterpret_cast<const u32x4 *>(from + d * 2u) ^ flip : u32x4{0u, 0u, 0u, 0u};
-        }
-        if (m < t.rows) {
-            all_lo = max(all_lo, row[u].lo);
-            all_hi = min(all_hi, row[u].hi);
+            q[s] = is_row && d < D && aa.scale != 0.f ? *reinterpret_cast<const u32x4 *>(from + d * 2u) ^ flip : u32x4{0u, 0u, 0u, 0u};
         }
     }
+    // keys that all of the wave's rows see
+    int32_t all_lo = is_row ? row.lo : 0, all_hi = is_row ? row.hi : 0x7FFFFFFF;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         all_lo = max(all_lo, __shfl_xor(all_lo, d));
@@ -107,35 +104,45 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
     u32x4 k_piece[kPieces], v_piece[kPieces];
     uint32_t groups_there = 0u;                                // of the image in the registers (Whole)
     uint64_t keys_there = 0u;
-    const uint32_t column = (tid % kRowPieces) * 8u;
-    // (of lanes behind the last element, and of keys that are not stored, something is read and not used)
-    const uint32_t in_column = (column < D ? column : 0u) * 2u;
-    const uint32_t in_group = Whole ? uint32_t(int64_t((tid / kRowPieces) % 16u) * aa.pages.token_stride) * 2u + in_column : in_column;
+    // Piece i of a thread: eight elements from `column` on of a row.  Of lanes behind the last element, and of keys that are not stored,
+    // something is read and not used.
+    auto piece_row = [&](int i) __attribute__((always_inline)) {
+        const uint32_t p = tid + kThreads * i;
+        return (kImagePieces % kThreads == 0u || p < kImagePieces ? p : kImagePieces - 1u) / kRowPieces;
+    };
+    auto piece_column = [&](int i) __attribute__((always_inline)) { return (tid + kThreads * i) % kRowPieces * 8u; };
+    auto is_piece = [&](int i) __attribute__((always_inline)) { return kImagePieces % kThreads == 0u || tid + kThreads * i < kImagePieces; };
+    uint32_t in_group[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const uint32_t c = piece_column(i);
+        in_group[i] = (Whole ? uint32_t(int64_t(piece_row(i) % 16u) * aa.pages.token_stride) * 2u : 0u) + (c < D ? c : 0u) * 2u;
+    }
     auto request = [&](int32_t n) __attribute__((always_inline)) {
-        constexpr uint32_t kPieceRows = kThreads / kRowPieces;                   // rows between a thread's pieces
         if constexpr (Whole) {
             if (n % 16 == 0) look_up(begin + n * 64 + int32_t(lane) * 16);
             const int32_t first = n % 16 * 4;
             groups_there = uint32_t(ahead_there >> first) & 15u;
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                // (a wave's rows of a piece lie in one group of 16)
-                const int32_t g = first + int32_t((64u * wave + kThreads * i) / kRowPieces / 16u);
-                const uint64_t from = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(ahead_low), g))) | uint64_t(uint32_t(__builtin_amdgcn_readlane(int(ahead_high), g))) << 32;
-                const uint32_t at = in_group + (kPieceRows < 16u ? uint32_t(int64_t(i * kPieceRows % 16u) * aa.pages.token_stride) * 2u : 0u);
-                k_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.keys + from + at);
-                v_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.values + from + at);
-            }
         } else {
             look_up(begin + n * 64 + int32_t(lane));
             keys_there = ahead_there;
+        }
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int r = int(tid / kRowPieces + kPieceRows * i);
-                const uint64_t from = uint64_t(uint32_t(__shfl(int(ahead_low), r))) | uint64_t(uint32_t(__shfl(int(ahead_high), r))) << 32;
-                k_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.keys + from + in_group);
-                v_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.values + from + in_group);
+        for (int i = 0; i < kPieces; ++i) {
+            uint64_t from;
+            if constexpr (Whole) {
+                // (the rows of a wave's pieces lie in one group of 16: 2 DP / 64 waves have a group's pieces)
+                static_assert(16u * kRowPieces % 64u == 0u, "");
+                constexpr uint32_t kGroupWaves = 16u * kRowPieces / 64u;
+                const uint32_t g = (wave + uint32_t(W) * i) / kGroupWaves;
+                const int32_t at = n % 16 * 4 + int32_t(g < 4u ? g : 3u);
+                from = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(ahead_low), at))) | uint64_t(uint32_t(__builtin_amdgcn_readlane(int(ahead_high), at))) << 32;
+            } else {
+                const int at = int(piece_row(i));
+                from = uint64_t(uint32_t(__shfl(int(ahead_low), at))) | uint64_t(uint32_t(__shfl(int(ahead_high), at))) << 32;
             }
+            k_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.keys + from + in_group[i]);
+            v_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.values + from + in_group[i]);
         }
     };
     // the stored keys of image n, which is in the registers
@@ -157,13 +164,13 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
             // (what is not stored may be anything, and no weight of zero undoes a NaN)
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
-                if (column >= D || !(stored_there >> ((tid + kThreads * i) / kRowPieces) & 1u)) k_piece[i] = v_piece[i] = u32x4{0u, 0u, 0u, 0u};
+                if (piece_column(i) >= D || !(stored_there >> piece_row(i) & 1u)) k_piece[i] = v_piece[i] = u32x4{0u, 0u, 0u, 0u};
         }
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const uint32_t r = (tid + kThreads * i) / kRowPieces;
-            *reinterpret_cast<u32x4 *>(image + r * kKeyPitch + column * 2u) = k_piece[i];
-            *reinterpret_cast<u32x4 *>(image + kKeys * kKeyPitch + r * kValuePitch + column * 2u) = v_piece[i];
+            if (!is_piece(i)) continue;
+            *reinterpret_cast<u32x4 *>(image + piece_row(i) * kKeyPitch + piece_column(i) * 2u) = k_piece[i];
+            *reinterpret_cast<u32x4 *>(image + kKeys * kKeyPitch + piece_row(i) * kValuePitch + piece_column(i) * 2u) = v_piece[i];
         }
         const int32_t key0 = begin + n * 64;
         if (n < n_images && (key0 < group_lo || key0 + 64 > group_hi || ~stored_there)) {
@@ -177,18 +184,15 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
         return stored_there;
     };
 
-    f32x16 o[QT][kTiles];
-    float ref[QT], total[QT];
+    f32x16 o[kTiles];
+    float ref, total;
     auto begin_sums = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
+        for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-            for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[u][c][r] = 0.f;
-            ref[u] = -INFINITY;
-            total[u] = 0.f;
-        }
+            for (int r = 0; r < 16; ++r) o[c][r] = 0.f;
+        ref = -INFINITY;
+        total = 0.f;
     };
     const uint32_t key_lane = j * kKeyPitch + h * 16u;
     const uint32_t value_lane = kKeys * kKeyPitch + (4u * h + (lane & 15u) / 4u) * kValuePitch + ((lane >> 4 & 1u) * 16u + (lane & 3u) * 4u) * 2u;
@@ -199,66 +203,47 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
 #pragma unroll
         for (int c = 0; c < kSteps / 2; ++c) f.a[c] = *reinterpret_cast<const u32x4 *>(from + c * 32);
     };
-    auto scores = [&](auto second, f32x16 (&s)[QT], const KeyOperands &f) __attribute__((always_inline)) {
+    auto scores = [&](auto second, f32x16 &s, const KeyOperands &f) __attribute__((always_inline)) {
         constexpr int c0 = decltype(second)::value * (kSteps / 2);
         if constexpr (c0 == 0) {
 #pragma unroll
-            for (int u = 0; u < QT; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+            for (int r = 0; r < 16; ++r) s[r] = 0.f;
         }
 #pragma unroll
-        for (int c = 0; c < kSteps / 2; ++c)
-#pragma unroll
-            for (int u = 0; u < QT; ++u) s[u] = Wide<BF>::mfma(f.a[c], q[u][c0 + c], s[u]);
+        for (int c = 0; c < kSteps / 2; ++c) s = Wide<BF>::mfma(f.a[c], q[c0 + c], s);
     };
-    auto mask = [&](f32x16 (&s)[QT], int32_t key0, uint32_t stored) __attribute__((always_inline)) {
+    auto mask = [&](f32x16 &s, int32_t key0, uint32_t stored) __attribute__((always_inline)) {
         if (key0 >= all_lo && key0 + 32 <= all_hi && stored == ~0u) return;
         const uint32_t mine = stored >> (4u * h);
+        const int32_t low = row.lo - key0 - int32_t(4u * h), high = row.hi - key0 - int32_t(4u * h);
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            const int32_t low = row[u].lo - key0 - int32_t(4u * h), high = row[u].hi - key0 - int32_t(4u * h);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                constexpr int kOf[16] = {0, 1, 2, 3, 8, 9, 10, 11, 16, 17, 18, 19, 24, 25, 26, 27};
-                if (!(kOf[r] >= low && kOf[r] < high && (mine >> kOf[r] & 1u))) s[u][r] = -INFINITY;
-            }
+        for (int r = 0; r < 16; ++r) {
+            constexpr int kOf[16] = {0, 1, 2, 3, 8, 9, 10, 11, 16, 17, 18, 19, 24, 25, 26, 27};
+            if (!(kOf[r] >= low && kOf[r] < high && (mine >> kOf[r] & 1u))) s[r] = -INFINITY;
         }
     };
     // the largest score of every row; where one is far above its row's reference the sums move to a new one
-    auto move_references = [&](const f32x16 (&s)[QT]) __attribute__((always_inline)) {
-        float most[QT];
-        bool moves[QT], any = false;
+    auto move_references = [&](const f32x16 &s) __attribute__((always_inline)) {
+        float most = s[0];
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            most[u] = s[u][0];
+        for (int r = 1; r < 16; ++r) most = fmaxf(most, s[r]);
+        most = max_halves(most) * scale;
+        const bool moves = most > ref + kReferenceSlack || (ref == -INFINITY && most > -INFINITY);
+        if (__builtin_expect(__ballot(moves) != 0u, 0)) {
+            asm volatile("");                                  // (a branch, not DP / 2 multiplications by one every time)
+            const float by = moves ? __builtin_amdgcn_exp2f(ref - most) : 1.f;
+            if (moves) ref = most;
+            total *= by;
 #pragma unroll
-            for (int r = 1; r < 16; ++r) most[u] = fmaxf(most[u], s[u][r]);
-            most[u] = max_halves(most[u]) * scale;
-            moves[u] = most[u] > ref[u] + kReferenceSlack || (ref[u] == -INFINITY && most[u] > -INFINITY);
-            any |= moves[u];
-        }
-        if (__builtin_expect(__ballot(any) != 0u, 0)) {
-            asm volatile("");                                  // (a branch, not 32 QT DP / 64 multiplications by one every time)
-#pragma unroll
-            for (int u = 0; u < QT; ++u) {
-                const float by = moves[u] ? __builtin_amdgcn_exp2f(ref[u] - most[u]) : 1.f;
-                if (moves[u]) ref[u] = most[u];
-                total[u] *= by;
-#pragma unroll
-                for (int c = 0; c < kTiles; ++c) o[u][c] *= by;
-            }
+            for (int c = 0; c < kTiles; ++c) o[c] *= by;
         }
     };
-    auto exponentials = [&](f32x16 (&s)[QT]) __attribute__((always_inline)) {
+    auto exponentials = [&](f32x16 &s) __attribute__((always_inline)) {
+        const float base = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            const float base = ref[u] == -INFINITY ? 0.f : ref[u];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale, -base));
-                total[u] += s[u][r];
-            }
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, -base));
+            total += s[r];
         }
     };
     // The same of the sums' instructions for 16 keys.
@@ -273,24 +258,20 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
             f.a[e] = u32x4{a0[0], a0[1], a1[0], a1[1]};
         }
     };
-    auto add = [&](auto second, const f32x16 (&s)[QT], const ValueOperands &f) __attribute__((always_inline)) {
+    auto add = [&](auto second, const f32x16 &s, const ValueOperands &f) __attribute__((always_inline)) {
         constexpr int c = decltype(second)::value;
-        u32x4 p[QT];
+        u32x4 p;
 #pragma unroll
-        for (int u = 0; u < QT; ++u)
+        for (int w = 0; w < 4; ++w) p[w] = pack_two<BF>(s[8 * c + 2 * w], s[8 * c + 2 * w + 1]);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) p[u][w] = pack_two<BF>(s[u][8 * c + 2 * w], s[u][8 * c + 2 * w + 1]);
-#pragma unroll
-        for (int e = 0; e < kTiles; ++e)
-#pragma unroll
-            for (int u = 0; u < QT; ++u) o[u][e] = Wide<BF>::mfma(f.a[e], p[u], o[u][e]);
+        for (int e = 0; e < kTiles; ++e) o[e] = Wide<BF>::mfma(f.a[e], p, o[e]);
     };
     using first = std::integral_constant<int, 0>;
     using second = std::integral_constant<int, 1>;
     KeyOperands keys_1, keys_2;
     // A half: scores `s` become weights and are added, the scores of the half behind it are made meanwhile (its first operands are asked for
     // already); at the end those of the one behind that are asked for.
-    auto half_step = [&](f32x16 (&s)[QT], f32x16 (&s_other)[QT], int32_t key0, uint32_t stored, uint32_t image, uint32_t half, uint32_t other_image, uint32_t other_half,
+    auto half_step = [&](f32x16 &s, f32x16 &s_other, int32_t key0, uint32_t stored, uint32_t image, uint32_t half, uint32_t other_image, uint32_t other_half,
                          uint32_t third_image, uint32_t third_half) __attribute__((always_inline)) {
         mask(s, key0, stored);
         ask_keys(keys_2, second{}, other_image, other_half);
@@ -311,7 +292,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
 
     begin_sums();
     if (n_images) {
-        f32x16 s_a[QT], s_b[QT];
+        f32x16 s_a, s_b;
         request(0);
         uint64_t stored_now = write_image(0, 0u);
         request(1);
@@ -362,23 +343,20 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
                     mask(s_a, key0, uint32_t(stored >> (32u * half)));
                     move_references(s_a);
                     exponentials(s_a);
+                    __syncthreads();
 #pragma unroll
-                    for (int u = 0; u < QT; ++u) {
-                        __syncthreads();
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) weights[(8u * (r / 4) + 4u * h + r % 4) * 32u + j] = s_a[u][r];
-                        __syncthreads();
+                    for (int r = 0; r < 16; ++r) weights[(8u * (r / 4) + 4u * h + r % 4) * 32u + j] = s_a[r];
+                    __syncthreads();
 #pragma unroll 1
-                        for (uint32_t a = 0; a < 32u; ++a) {
-                            const int32_t key = key0 + int32_t(a);
-                            const float w = weights[a * 32u + j];
-                            const T *from = reinterpret_cast<const T *>(images + kKeys * kKeyPitch + (32u * half + a) * kValuePitch) + 4u * h;
-                            if (key >= row[u].lo && key < row[u].hi) {
+                    for (uint32_t a = 0; a < 32u; ++a) {
+                        const int32_t key = key0 + int32_t(a);
+                        const float w = weights[a * 32u + j];
+                        const T *from = reinterpret_cast<const T *>(images + kKeys * kKeyPitch + (32u * half + a) * kValuePitch) + 4u * h;
+                        if (key >= row.lo && key < row.hi) {
 #pragma unroll
-                                for (int c = 0; c < kTiles; ++c)
+                            for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-                                    for (int r = 0; r < 16; ++r) o[u][c][r] += w * float(from[32 * c + 8 * (r / 4) + r % 4]);
-                            }
+                                for (int r = 0; r < 16; ++r) o[c][r] += w * float(from[32 * c + 8 * (r / 4) + r % 4]);
                         }
                     }
                 }
@@ -387,23 +365,21 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
     }
 
     // what a row's two lanes have
-#pragma unroll
-    for (int u = 0; u < QT; ++u) total[u] += __shfl_xor(total[u], 32);
+    total += __shfl_xor(total, 32);
     if (parts > 1) {
-        constexpr uint32_t kSlot = kRows * (DP + 4u);          // floats of a part: per row its sums, its reference and its total
+        // A part's sums as the lanes hold them: 16 bytes a lane side by side, then the rows' references and totals.
+        constexpr uint32_t kWaveSlot = 32u * (DP + 4u), kSlot = kRows * (DP + 4u);
         const uint32_t pair = tile_number * gridDim.x + head;
         const __amdgpu_buffer_rsrc_t mem = device_scope_buffer(aa.sums + size_t(pair) * aa.splits * kSlot);
-#pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            const uint32_t m = wave * kWaveRows + 32u * u + j;
-            if (m >= t.rows) continue;
-            const uint32_t at = (part * kSlot + m * (DP + 4u)) * 4u;
+        const bool wave_there = wave * 32u < t.rows;
+        auto sums_at = [&](uint32_t p, int c, int r) __attribute__((always_inline)) { return (p * kSlot + wave * kWaveSlot + (c * 4u + r / 4u) * 256u + lane * 4u) * 4u; };
+        auto scalars_at = [&](uint32_t p) __attribute__((always_inline)) { return (p * kSlot + wave * kWaveSlot + 32u * DP + j * 4u) * 4u; };
+        if (wave_there) {
 #pragma unroll
             for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    store_device_scope(mem, at + (32u * c + 2u * r + 4u * h) * 4u, f32x4{o[u][c][r], o[u][c][r + 1], o[u][c][r + 2], o[u][c][r + 3]});
-            if (h == 0u) store_device_scope(mem, at + DP * 4u, f32x4{ref[u], total[u], 0.f, 0.f});
+                for (int r = 0; r < 16; r += 4) store_device_scope(mem, sums_at(part, c, r), f32x4{o[c][r], o[c][r + 1], o[c][r + 2], o[c][r + 3]});
+            if (h == 0u) store_device_scope(mem, scalars_at(part), f32x4{ref, total, 0.f, 0.f});
         }
         wait_stores_acknowledged();
         __syncthreads();
@@ -411,75 +387,64 @@ __global__ __launch_bounds__(64 * W, DP <= 128 && QT == 1 ? 2 : 1) void attend_c
         __syncthreads();
         if (arrived + 1u != uint32_t(parts)) return;
         if (tid == 0u) __hip_atomic_store(aa.arrive + pair, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            const uint32_t m = wave * kWaveRows + 32u * u + j;
-            if (m >= t.rows) continue;
-            ref[u] = -INFINITY;
-            total[u] = 0.f;
+        if (!wave_there) return;
+        begin_sums();
+#pragma unroll 1
+        for (int32_t p = 0; p < parts; ++p) {
+            const f32x4 s = load_device_scope(mem, scalars_at(uint32_t(p)));
+            f32x4 x[kTiles][4];
 #pragma unroll
             for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[u][c][r] = 0.f;
-#pragma unroll 1
-            for (int32_t p = 0; p < parts; ++p) {
-                const uint32_t at = (uint32_t(p) * kSlot + m * (DP + 4u)) * 4u;
-                const f32x4 s = load_device_scope(mem, at + DP * 4u);
-                const float now = fmaxf(ref[u], s[0]);
-                const float keep = ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref[u] - now), by = s[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[0] - now);
-                total[u] = total[u] * keep + s[1] * by;
+                for (int r = 0; r < 16; r += 4) x[c][r / 4] = load_device_scope(mem, sums_at(uint32_t(p), c, r));
+            const float top = fmaxf(ref, s[0]);
+            const float keep = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - top), by = s[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[0] - top);
+            total = total * keep + s[1] * by;
 #pragma unroll
-                for (int c = 0; c < kTiles; ++c)
+            for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-                    for (int r = 0; r < 16; r += 4) {
-                        const f32x4 x = load_device_scope(mem, at + (32u * c + 2u * r + 4u * h) * 4u);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[u][c][r + e] = o[u][c][r + e] * keep + x[e] * by;
-                    }
-                ref[u] = now;
-            }
+                for (int r = 0; r < 16; ++r) o[c][r] = o[c][r] * keep + x[c][r / 4][r % 4] * by;
+            ref = top;
         }
     }
+    if (!is_row) return;
+    const bool any = !(total == 0.f);
+    const float by = any ? 1.f / total : 0.f;
+    T *og = reinterpret_cast<T *>(aa.out.data) + int64_t(row.token) * aa.out.token_stride + int64_t(row.head) * aa.out.head_stride;
+    const bool side_by_side = aa.out.dim_stride == 1 && (reinterpret_cast<uintptr_t>(og) & 7u) == 0u;
 #pragma unroll
-    for (int u = 0; u < QT; ++u) {
-        const uint32_t m = wave * kWaveRows + 32u * u + j;
-        if (m >= t.rows) continue;
-        const bool any = !(total[u] == 0.f);
-        const float by = any ? 1.f / total[u] : 0.f;
-        T *og = reinterpret_cast<T *>(aa.out.data) + int64_t(row[u].token) * aa.out.token_stride + int64_t(row[u].head) * aa.out.head_stride;
-        const bool side_by_side = aa.out.dim_stride == 1 && (reinterpret_cast<uintptr_t>(og) & 7u) == 0u;
+    for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-        for (int c = 0; c < kTiles; ++c)
+        for (int r = 0; r < 16; r += 4) {
+            const uint32_t d = 32u * c + 2u * r + 4u * h;
+            if (d >= D) continue;
+            if (side_by_side) {
+                *reinterpret_cast<t_u32x2 *>(og + d) = t_u32x2{pack_two<BF>(o[c][r] * by, o[c][r + 1] * by), pack_two<BF>(o[c][r + 2] * by, o[c][r + 3] * by)};
+            } else {
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const uint32_t d = 32u * c + 2u * r + 4u * h;
-                if (d >= D) continue;
-                if (side_by_side) {
-                    *reinterpret_cast<t_u32x2 *>(og + d) = t_u32x2{pack_two<BF>(o[u][c][r] * by, o[u][c][r + 1] * by), pack_two<BF>(o[u][c][r + 2] * by, o[u][c][r + 3] * by)};
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) og[int64_t(d + e) * aa.out.dim_stride] = T(o[u][c][r + e] * by);
-                }
+                for (int e = 0; e < 4; ++e) og[int64_t(d + e) * aa.out.dim_stride] = T(o[c][r + e] * by);
             }
-        if (aa.lse && h == 0u) aa.lse[size_t(row[u].token) * aa.q_heads + row[u].head] = any ? (ref[u] + __builtin_amdgcn_logf(total[u])) * kLn2 : -INFINITY;
-    }
+        }
+    if (aa.lse && h == 0u) aa.lse[size_t(row.token) * aa.q_heads + row.head] = any ? (ref + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
 }
 
-template <bool BF, int DP, int QT, int W>
+template <bool BF, int DP, int W>
 void launch(const AttendArgs &aa, hipStream_t s)
 {
-    const dim3 grid(aa.pages.heads, attend_tiles(aa.batch.tokens, aa.batch.sequences, aa.shared.d, QT * W == 8 ? 8u : 7u), aa.splits);
-    if (aa.pages.page_tokens.d % 16u == 0u) attend_chunk_kernel<BF, DP, QT, W, true><<<grid, dim3(64 * W), 0, s>>>(aa);
-    else attend_chunk_kernel<BF, DP, QT, W, false><<<grid, dim3(64 * W), 0, s>>>(aa);
+    const dim3 grid(aa.pages.heads, attend_tiles(aa.batch.tokens, aa.batch.sequences, aa.shared.d, W == 8 ? 8u : 7u), aa.splits);
+    if (aa.pages.page_tokens.d % 16u == 0u) attend_chunk_kernel<BF, DP, W, true><<<grid, dim3(64 * W), 0, s>>>(aa);
+    else attend_chunk_kernel<BF, DP, W, false><<<grid, dim3(64 * W), 0, s>>>(aa);
 }
 
 template <bool BF>
 void launch_type(const AttendArgs &aa, hipStream_t s)
 {
     const uint32_t D = aa.pages.head_dim;
-    if (D <= 64u) launch<BF, 64, 1, 8>(aa, s);
-    else if (D <= 128u) launch<BF, 128, 1, 8>(aa, s);
-    else launch<BF, 256, 1, 4>(aa, s);
+    if (D <= 64u) launch<BF, 64, 8>(aa, s);
+    else if (D <= 96u) launch<BF, 96, 8>(aa, s);
+    else if (D <= 128u) launch<BF, 128, 8>(aa, s);
+    else if (D <= 160u) launch<BF, 160, 4>(aa, s);
+    else launch<BF, 256, 4>(aa, s);
 }
 
 }  // namespace

@@ -411,25 +411,58 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
         __syncthreads();
         if (arrived + 1u != uint32_t(parts)) return;
         if (tid == 0u) __hip_atomic_store(aa.arrive + pair, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (m < t.rows) {
-            float ref_all = -INFINITY;
-            sum = 0.f;
+        // The parts' sums, in turn by as many sets of threads as the rows leave, kAtOnce parts on their way at a time; then the sets' own, in LDS.
+        constexpr uint32_t kAtOnce = 4u;
+        uint32_t rows_log = 0u;
+        while ((1u << rows_log) < t.rows || (uint32_t(parts) <= kAtOnce && rows_log < 4u)) ++rows_log;
+        const uint32_t sets = 16u >> rows_log, set = m >> rows_log, row_here = m & ((1u << rows_log) - 1u);
+        float top = -INFINITY;
+        sum = 0.f;
 #pragma unroll
-            for (uint32_t e = 0; e < kEach; ++e) acc[e] = 0.f;
-            for (int32_t p = 0; p < parts; ++p) {
-                const uint32_t at = (uint32_t(p) * kSlot + m * (DP + 4u)) * 4u;
-                const f32x4 s = load_device_scope(mem, at + DP * 4u);
-                f32x4 x[kEach / 4u];
+        for (uint32_t e = 0; e < kEach; ++e) acc[e] = 0.f;
+        if (row_here < t.rows)
+            for (uint32_t p0 = set; p0 < uint32_t(parts); p0 += kAtOnce * sets) {
+                f32x4 s[kAtOnce], x[kAtOnce][kEach / 4u];
 #pragma unroll
-                for (uint32_t e = 0; e < kEach / 4u; ++e) x[e] = load_device_scope(mem, at + (d0 + 4u * e) * 4u);
-                const float now = fmaxf(ref_all, s[0]);
-                const float keep = ref_all == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref_all - now), by = s[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[0] - now);
-                sum = sum * keep + s[1] * by;
+                for (uint32_t k = 0; k < kAtOnce; ++k) {
+                    const uint32_t p = p0 + k * sets, at = ((p < uint32_t(parts) ? p : p0) * kSlot + row_here * (DP + 4u)) * 4u;
+                    s[k] = load_device_scope(mem, at + DP * 4u);
 #pragma unroll
-                for (uint32_t e = 0; e < kEach; ++e) acc[e] = acc[e] * keep + x[e / 4u][e % 4u] * by;
-                ref_all = now;
+                    for (uint32_t e = 0; e < kEach / 4u; ++e) x[k][e] = load_device_scope(mem, at + (d0 + 4u * e) * 4u);
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < kAtOnce; ++k) {
+                    if (p0 + k * sets >= uint32_t(parts)) break;
+                    const float now = fmaxf(top, s[k][0]);
+                    const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now), by = s[k][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[k][0] - now);
+                    sum = sum * keep + s[k][1] * by;
+#pragma unroll
+                    for (uint32_t e = 0; e < kEach; ++e) acc[e] = acc[e] * keep + x[k][e / 4u][e % 4u] * by;
+                    top = now;
+                }
             }
-            most = ref_all;
+        most = top;
+        if (sets > 1u) {
+            // (the waves' references, totals and sums are used up: their place, a set's at [set][row])
+            float *const ref_of = &refs[0][0], *const total_of = &totals[0][0];
+            if (tid % 16u == 0u) { ref_of[m] = top; total_of[m] = sum; }
+#pragma unroll
+            for (uint32_t e = 0; e < kEach; ++e) sums[m * kPitch + d0 + e] = acc[e];
+            __syncthreads();
+            if (m < t.rows) {
+                most = -INFINITY;
+                for (uint32_t k = 0; k < sets; ++k) most = fmaxf(most, ref_of[(k << rows_log) + m]);
+                sum = 0.f;
+#pragma unroll
+                for (uint32_t e = 0; e < kEach; ++e) acc[e] = 0.f;
+                for (uint32_t k = 0; k < sets; ++k) {
+                    const uint32_t at = (k << rows_log) + m;
+                    const float by = ref_of[at] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref_of[at] - most);
+                    sum += total_of[at] * by;
+#pragma unroll
+                    for (uint32_t e = 0; e < kEach; ++e) acc[e] += sums[at * kPitch + d0 + e] * by;
+                }
+            }
         }
     }
     if (m < t.rows) {

@@ -305,12 +305,15 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     const uint64_t numbered = attend_tiles(b->tokens, b->sequences, shared, sh.rows_log);
     // tiles that have rows, at most: numbers are left out
     const uint64_t tiles = std::min<uint64_t>(numbered, uint64_t(b->sequences) * ((rows + (1u << sh.rows_log) - 1u) >> sh.rows_log));
-    // workgroups wanted: the rows kernel has two a compute unit, and sequences are of many lengths
-    const bool chunk = sh.rows_log != kAttendRowsLog;
-    const uint64_t wanted = chunk ? 256u : 2048u, least = chunk ? 512u : 256u;
-    uint64_t part = (tiles * c->heads * keys / wanted + 127u) & ~uint64_t(127u);
-    part = std::max<uint64_t>(part, least);
-    sh.part_keys = uint32_t(std::min<uint64_t>(part, 1u << 30));
+    // Keys of a part.  Rows kernel: as few as give every compute unit two workgroups, 128 at least (every wave a tile or two) and 512 at most, more only
+    // where that is over 4096 workgroups: sequences are of many lengths, and the last ones should not be long.  us by parts of 128 / 256 / 512 keys: one token
+    // over 1000 keys, 8 heads 8.1 / 9.2 / 11.9; over 30000 58 / 39 / 30; 8 sequences of up to 8000 56 / 44 / 42.
+    // Chunk kernel: a workgroup a compute unit; a part's sums are 132 KB, as much as 260 keys.  us by 256 / 512 workgroups: 100 tokens for each of 4
+    // sequences of 4000 54 / 70; 512 tokens over 8512 keys, head_dim 64 33 / 48.
+    const uint64_t work = tiles * c->heads * keys;
+    auto whole = [](uint64_t k) { return (k + 127u) & ~uint64_t(127u); };
+    const uint64_t part = sh.rows_log == kAttendRowsLog ? std::max(whole(work / 4096u), std::min<uint64_t>(whole(work / 512u), 512u)) : whole(work / 256u);
+    sh.part_keys = uint32_t(std::min<uint64_t>(std::max<uint64_t>(part, sh.rows_log == kAttendRowsLog ? 128u : 512u), 1u << 30));
     const uint64_t parts = (keys + 31u + sh.part_keys - 1u) / sh.part_keys;
     sh.splits = numbered * c->heads > kAttendCounters ? 1u : uint32_t(std::min<uint64_t>(std::max<uint64_t>(parts, 1u), 256u));
     if (sh.splits > 1u) sh.bytes = kAttendCounters * 4u + numbered * c->heads * sh.splits * attend_slot(sh.rows_log, c->head_dim) * 4u;

@@ -153,96 +153,127 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs ra, const 
 }
 
 // Any strides: a workgroup has tt (up to 64, a power of two) tokens of one head and 32 of its pairs (all elements count in pairs here, those that do not turn, too).
-// Lanes lie along tokens where x is read or y is written with tokens side by side, along pairs else; between the two the elements go through LDS.
+// Lanes lie along tokens where x is read, or y is written, with tokens side by side, along pairs else; between the two the elements go through LDS.  Pairs
+// turn on their way out, so that lanes along pairs read angles side by side.  A small batch's starts are asked for first, then the elements: where tokens stand is
+// found while those are on their way.
+constexpr uint32_t kStridedThreads = 512u;
 template <int DT>
-__global__ __launch_bounds__(256) void rotary_strided_kernel(const RotaryArgs ra, const uint32_t tt_log)
+__global__ __launch_bounds__(kStridedThreads) void rotary_strided_kernel(const RotaryArgs ra, const uint32_t tt_log)
 {
     typedef typename Elem<DT>::T T;
-    constexpr uint32_t kPairs = 32u, kMine = 64u * kPairs / 256u, kStarts = 512u;
-    __shared__ T image[64u * (2u * kPairs + 2u)];
+    constexpr uint32_t kPairs = 32u, kMine = 64u * kPairs / kStridedThreads, kPitch = 2u * kPairs + 2u;
+    __shared__ T image[64u * kPitch];
     __shared__ int64_t rows[64];                    // a token's row in the pages (head 0), -1: not stored
-    __shared__ int32_t position_of[64], starts[kStarts + 1u];
+    __shared__ int32_t position_of[64], starts[256], held[256];
+    __shared__ uint32_t sequence_of[64], sequences[256];
     __shared__ bool there[64];
     const uint32_t tt = 1u << tt_log, t0 = blockIdx.x << tt_log, pair0 = blockIdx.y * kPairs, tid = threadIdx.x;
     const HeadRole role = head_role(ra, blockIdx.z);
     const uint32_t all_pairs = ra.head_dim / 2u + (ra.head_dim & 1u), dims = ra.table && (role.query || role.key) ? ra.dims : 0u;
-    const bool by_token = role.from->dim_stride != 1;
+    const BatchArgs batch = ra.batch;
+    // (a small batch: a thread has a batch row, thread batch.sequences the end of the last one)
+    const bool near = batch.starts && batch.sequences < 256u;
+    int32_t my_start = 0, my_held = 0;
+    uint32_t my_sequence = kIdxMax;
+    if (near && tid <= batch.sequences) {
+        my_start = batch.starts[tid];
+        if (tid < batch.sequences) {
+            my_sequence = batch.rows ? uint32_t(batch.rows[tid]) : tid;
+            if (my_sequence < ra.pages.sequences) my_held = tokens_held(ra.pages, my_sequence);
+        }
+    }
     // element of pair p's first or second half
     auto element = [&](uint32_t p, uint32_t second) __attribute__((always_inline)) {
         if (ra.interleaved || 2u * p >= dims) return 2u * p + second;
         return p + second * (dims / 2u);
     };
-    auto token_and_pair = [&](uint32_t i, uint32_t *ti, uint32_t *pi) __attribute__((always_inline)) {
+    auto token_and_pair = [&](uint32_t i, bool by_token, uint32_t *ti, uint32_t *pi) __attribute__((always_inline)) {
         *ti = by_token ? i & (tt - 1u) : i / kPairs;
         *pi = by_token ? i >> tt_log : i % kPairs;
         return i < tt * kPairs && t0 + *ti < ra.tokens && pair0 + *pi < all_pairs;
     };
-    // this thread's pairs, asked for before it is known where their tokens stand
+    const bool in_by_token = role.from->dim_stride != 1, out_by_token = role.query && ra.q_out.dim_stride != 1;
     T u[kMine], w[kMine];
 #pragma unroll
     for (uint32_t k = 0; k < kMine; ++k) {
         uint32_t ti, pi;
         u[k] = w[k] = T(0.f);
-        if (!token_and_pair(tid + 256u * k, &ti, &pi)) continue;
+        if (!token_and_pair(tid + kStridedThreads * k, in_by_token, &ti, &pi)) continue;
         const T *x = reinterpret_cast<const T *>(role.from->data) + int64_t(t0 + ti) * role.from->token_stride + int64_t(role.head) * role.from->head_stride;
         const uint32_t a = element(pair0 + pi, 0u), b = element(pair0 + pi, 1u);
         u[k] = x[int64_t(a) * role.from->dim_stride];
         if (b < ra.head_dim) w[k] = x[int64_t(b) * role.from->dim_stride];
     }
-    BatchArgs batch = ra.batch;
-    const bool near = batch.starts && batch.sequences <= kStarts;
     if (near) {
-        for (uint32_t i = tid; i <= batch.sequences; i += 256u) starts[i] = batch.starts[i];
+        if (tid <= batch.sequences) {
+            starts[tid] = my_start;
+            held[tid] = my_held;
+            sequences[tid] = my_sequence;
+        }
         __syncthreads();
     }
     if (tid < tt) {
         const uint32_t t = t0 + tid;
         TokenPlace place{0u, 0, t < ra.tokens};
-        int64_t at = -1;
         if (batch.starts && t < ra.tokens) {
             uint32_t lo = 0, hi = batch.sequences;
             while (hi - lo > 1u) {
                 const uint32_t mid = (lo + hi) / 2u;
                 if ((near ? starts[mid] : batch.starts[mid]) <= int32_t(t)) lo = mid; else hi = mid;
             }
-            place = place_in(batch, ra.pages, lo, t);
-            if (place.there) at = row_offset(ra.pages, place.sequence, place.position, 0u);
+            if (near) {
+                const int32_t first = starts[lo], end = starts[lo + 1u];
+                place.there = first <= int32_t(t) && end > int32_t(t) && end <= int32_t(batch.tokens) && sequences[lo] < ra.pages.sequences;
+                place.sequence = sequences[lo];
+                place.position = held[lo] - end + int32_t(t);
+            } else {
+                place = place_in(batch, ra.pages, lo, t);
+            }
         }
-        rows[tid] = at;
         there[tid] = place.there;
+        sequence_of[tid] = place.sequence;
         position_of[tid] = ra.at && t < ra.tokens ? ra.at[t] : place.position;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kMine; ++k) {
+        uint32_t ti, pi;
+        if (!token_and_pair(tid + kStridedThreads * k, in_by_token, &ti, &pi)) continue;
+        image[ti * kPitch + 2u * pi] = u[k];
+        image[ti * kPitch + 2u * pi + 1u] = w[k];
+    }
+    __syncthreads();
+    // (its page's number and the angles, side by side)
+    if (tid < tt) rows[tid] = batch.starts && !role.query && there[tid] ? row_offset(ra.pages, sequence_of[tid], position_of[tid], 0u) : -1;
+    float2 cs[kMine];
+#pragma unroll
+    for (uint32_t k = 0; k < kMine; ++k) {
+        uint32_t ti, pi;
+        cs[k] = float2{1.f, 0.f};
+        if (token_and_pair(tid + kStridedThreads * k, out_by_token, &ti, &pi) && 2u * (pair0 + pi) < dims && there[ti]) cs[k] = angle_row(ra, position_of[ti])[pair0 + pi];
     }
     __syncthreads();
 #pragma unroll
     for (uint32_t k = 0; k < kMine; ++k) {
         uint32_t ti, pi;
-        if (!token_and_pair(tid + 256u * k, &ti, &pi)) continue;
-        const uint32_t p = pair0 + pi;
-        if (2u * p < dims && there[ti]) {
-            const float2 y2 = turn(float(u[k]), float(w[k]), angle_row(ra, position_of[ti])[p], ra.sign);
-            u[k] = T(y2.x);
-            w[k] = T(y2.y);
+        if (!token_and_pair(tid + kStridedThreads * k, out_by_token, &ti, &pi) || !there[ti]) continue;
+        const uint32_t t = t0 + ti, p = pair0 + pi, a = element(p, 0u), b = element(p, 1u);
+        T first = image[ti * kPitch + 2u * pi], second = image[ti * kPitch + 2u * pi + 1u];
+        if (2u * p < dims) {
+            const float2 y2 = turn(float(first), float(second), cs[k], ra.sign);
+            first = T(y2.x);
+            second = T(y2.y);
         }
-        image[ti * (2u * kPairs + 2u) + 2u * pi] = u[k];
-        image[ti * (2u * kPairs + 2u) + 2u * pi + 1u] = w[k];
-    }
-    __syncthreads();
-    const bool out_by_token = role.query && ra.q_out.dim_stride != 1;
-#pragma unroll
-    for (uint32_t k = 0; k < 2u * kMine; ++k) {
-        const uint32_t i = tid + 256u * k;
-        uint32_t ti, pi, second;
-        if (out_by_token) { ti = i & (tt - 1u); pi = (i >> tt_log) / 2u; second = (i >> tt_log) & 1u; }
-        else if (ra.interleaved || 2u * (pair0 + kPairs) > dims) { ti = i / (2u * kPairs); pi = i / 2u % kPairs; second = i & 1u; }
-        else { ti = i / (2u * kPairs); second = i / kPairs & 1u; pi = i % kPairs; }
-        const uint32_t t = t0 + ti, p = pair0 + pi, e = element(p, second);
-        if (i >= tt * 2u * kPairs || t >= ra.tokens || p >= all_pairs || e >= ra.head_dim || !there[ti]) continue;
-        const T v = image[ti * (2u * kPairs + 2u) + 2u * pi + second];
+        T *y;
+        int64_t stride = 1;
         if (role.query) {
-            reinterpret_cast<T *>(ra.q_out.data)[int64_t(t) * ra.q_out.token_stride + int64_t(role.head) * ra.q_out.head_stride + int64_t(e) * ra.q_out.dim_stride] = v;
-        } else if (rows[ti] >= 0) {
-            reinterpret_cast<T *>(role.key ? ra.pages.keys : ra.pages.values)[rows[ti] + int64_t(role.head) * ra.pages.head_stride + e] = v;
+            stride = ra.q_out.dim_stride;
+            y = reinterpret_cast<T *>(ra.q_out.data) + int64_t(t) * ra.q_out.token_stride + int64_t(role.head) * ra.q_out.head_stride;
+        } else {
+            if (rows[ti] < 0) continue;
+            y = reinterpret_cast<T *>(role.key ? ra.pages.keys : ra.pages.values) + rows[ti] + int64_t(role.head) * ra.pages.head_stride;
         }
+        y[int64_t(a) * stride] = first;
+        if (b < ra.head_dim) y[int64_t(b) * stride] = second;
     }
 }
 
@@ -271,7 +302,7 @@ hipError_t launch_type(const RotaryArgs &ra, uint32_t vec, hipStream_t s)
         uint32_t tt_log = 0;
         while (tt_log < 6u && (1u << tt_log) < ra.tokens) ++tt_log;
         const uint32_t all_pairs = (ra.head_dim + 1u) / 2u;
-        rotary_strided_kernel<DT><<<dim3((ra.tokens + (1u << tt_log) - 1u) >> tt_log, (all_pairs + 31u) / 32u, ra.q_heads + 2u * ra.k_heads), dim3(256), 0, s>>>(ra, tt_log);
+        rotary_strided_kernel<DT><<<dim3((ra.tokens + (1u << tt_log) - 1u) >> tt_log, (all_pairs + 31u) / 32u, ra.q_heads + 2u * ra.k_heads), dim3(kStridedThreads), 0, s>>>(ra, tt_log);
     }
     }
     return hipGetLastError();

@@ -219,7 +219,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void attend_chunk_kernel(co
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             constexpr int kOf[16] = {0, 1, 2, 3, 8, 9, 10, 11, 16, 17, 18, 19, 24, 25, 26, 27};
-            if (!(kOf[r] >= low && kOf[r] < high && (mine >> kOf[r] & 1u))) s[r] = -INFINITY;
+            s[r] = select(bool(int(kOf[r] < low) | int(kOf[r] >= high) | int(!(mine >> kOf[r] & 1u))), -INFINITY, s[r]);
         }
     };
     // the largest score of every row; where one is far above its row's reference the sums move to a new one
@@ -352,12 +352,11 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void attend_chunk_kernel(co
                         const int32_t key = key0 + int32_t(a);
                         const float w = weights[a * 32u + j];
                         const T *from = reinterpret_cast<const T *>(images + kKeys * kKeyPitch + (32u * half + a) * kValuePitch) + 4u * h;
-                        if (key >= row.lo && key < row.hi) {
+                        const bool hidden = int(key < row.lo) | int(key >= row.hi);
 #pragma unroll
-                            for (int c = 0; c < kTiles; ++c)
+                        for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-                                for (int r = 0; r < 16; ++r) o[c][r] += w * float(from[32 * c + 8 * (r / 4) + r % 4]);
-                        }
+                            for (int r = 0; r < 16; ++r) o[c][r] += select(hidden, 0.f, w * float(from[32 * c + 8 * (r / 4) + r % 4]));
                     }
                 }
             }

@@ -84,6 +84,14 @@ __device__ __forceinline__ int64_t key_offset(const PagesArgs &pg, const int32_t
     return int64_t(id) * pg.page_stride + head_offset + int64_t(uint32_t(key) - place * pg.page_tokens.d) * pg.token_stride;
 }
 
+// yes or no by the condition, in one instruction.  (Elements of a matrix instruction's result are never written in a branch that some lanes take: where
+// results lie in accumulation registers the compiler has been seen to write the neighbouring elements there, too.)
+__device__ __forceinline__ float select(bool condition, float yes, float no)
+{
+    asm("" : "+v"(no));
+    return condition ? yes : no;
+}
+
 // The larger of the values of two (four) lanes 32 (and 16) apart, in all of them.
 __device__ __forceinline__ float max_halves(float v)
 {

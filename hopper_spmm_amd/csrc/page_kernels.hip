@@ -75,20 +75,26 @@ __device__ uint32_t find_free(const int32_t *references, uint32_t pages, uint32_
     return found < need ? found : need;
 }
 
-// Copies `bytes` (a multiple of the unit) by the workgroup's threads.
-template <class U>
+// Copies `bytes` (a multiple of the unit) by `threads` threads, four units of each on their way at a time.  Nothing that is written is read again in the
+// launch, and of whole pages nothing is read twice either: past the L2 (a pool of 2048 pages of 2 MB, 476 of them moved, 402 -> 389 us, 5.1 TB/s).  A partly
+// filled page may be several children's (shared): its loads stay (48 x 4 beams, all layers, 72 -> 68 us).
+template <class U, bool Shared>
 __device__ __forceinline__ void copy_run(char *to, const char *from, uint32_t bytes, uint32_t thread, uint32_t threads)
 {
-    const uint32_t n = bytes / sizeof(U), step = 4u * threads;
-    uint32_t i = thread;
-    for (; i + 3u * threads < n; i += step) {
-        U v[4];
+    constexpr uint32_t kAtOnce = 4u;
+    const uint32_t n = bytes / sizeof(U);
+    for (uint32_t i = thread; i < n; i += kAtOnce * threads) {
+        U v[kAtOnce];
 #pragma unroll
-        for (uint32_t k = 0; k < 4u; ++k) v[k] = reinterpret_cast<const U *>(from)[i + k * threads];
+        for (uint32_t k = 0; k < kAtOnce; ++k)
+            if (i + k * threads < n) {
+                const U *at = reinterpret_cast<const U *>(from) + i + k * threads;
+                v[k] = Shared ? *at : __builtin_nontemporal_load(at);
+            }
 #pragma unroll
-        for (uint32_t k = 0; k < 4u; ++k) reinterpret_cast<U *>(to)[i + k * threads] = v[k];
+        for (uint32_t k = 0; k < kAtOnce; ++k)
+            if (i + k * threads < n) __builtin_nontemporal_store(v[k], reinterpret_cast<U *>(to) + i + k * threads);
     }
-    for (; i < n; i += threads) reinterpret_cast<U *>(to)[i] = reinterpret_cast<const U *>(from)[i];
 }
 
 // The first `tokens` tokens of a page of one layer's keys or values.
@@ -100,14 +106,14 @@ __device__ __forceinline__ void copy_tokens(const PoolArgs &pa, uint32_t part, u
     char *d = base + int64_t(to) * pa.page_bytes;
     const char *s = base + int64_t(from) * pa.page_bytes;
     if (tokens == pa.page_tokens.d && head0 == 0u && head1 == pa.heads) {
-        copy_run<U>(d, s, tokens * pa.heads * pa.token_bytes, threadIdx.x, blockDim.x);
+        copy_run<U, false>(d, s, tokens * pa.heads * pa.token_bytes, threadIdx.x, blockDim.x);
     } else if (!pa.heads_first) {
-        if (head0 == 0u) copy_run<U>(d, s, tokens * pa.heads * pa.token_bytes, threadIdx.x, blockDim.x);
+        if (head0 == 0u) copy_run<U, true>(d, s, tokens * pa.heads * pa.token_bytes, threadIdx.x, blockDim.x);
     } else {
         // a head's tokens lie side by side: a wave has a head at a time
         const uint32_t pitch = pa.page_tokens.d * pa.token_bytes, waves = blockDim.x / 64u;
         for (uint32_t h = head0 + threadIdx.x / 64u; h < head1; h += waves)
-            copy_run<U>(d + size_t(h) * pitch, s + size_t(h) * pitch, tokens * pa.token_bytes, threadIdx.x & 63u, 64u);
+            copy_run<U, true>(d + size_t(h) * pitch, s + size_t(h) * pitch, tokens * pa.token_bytes, threadIdx.x & 63u, 64u);
     }
 }
 

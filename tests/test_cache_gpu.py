@@ -212,7 +212,15 @@ ATTENTIONS = [  # chunks, tokens held before, heads, shared, dim, page tokens, w
     ([4, 100, 1], [0, 31, 200], 2, 2, 64, 16, 0, False),
     ([300], [1000], 1, 4, 128, 32, 0, True),
     ([1] * 40, list(range(0, 800, 20)), 4, 2, 64, 16, 0, True),
-    ([33, 33], [0, 95], 8, 1, 8, 5, 0, True)]
+    ([33, 33], [0, 95], 8, 1, 8, 5, 0, True),
+    ([50, 90], [200, 0], 1, 2, 88, 16, 0, True),
+    ([70, 1, 200], [0, 500, 33], 2, 1, 96, 32, 60, True),
+    ([45, 140], [100, 0], 1, 2, 160, 16, 0, True),
+    ([90], [300], 1, 1, 136, 24, 50, True),
+    ([64], [40], 1, 1, 248, 48, 0, True),
+    ([1, 1], [9000, 17], 1, 4, 128, 16, 0, True),
+    ([1], [5000], 2, 1, 64, 10, 0, True),
+    ([40], [6000], 1, 4, 128, 16, 0, True)]
 
 
 def attention_case(torch, hs, dtype, case, order=0, seed=0, layers=1):
@@ -314,7 +322,7 @@ def test_pages_that_are_gone_are_not_seen(torch_cuda, hs, dtype, case):
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
-@pytest.mark.parametrize("case", [2, 4, 6, 8, 9, 10])
+@pytest.mark.parametrize("case", [2, 4, 6, 8, 9, 10, 17, 18, 19, 20])
 def test_what_is_masked_does_not_reach_the_result(torch_cuda, hs, dtype, case):
     # infinities and NaN in keys and values: only the tokens that see them have them
     torch = torch_cuda
@@ -341,6 +349,14 @@ def test_what_is_masked_does_not_reach_the_result(torch_cuda, hs, dtype, case):
         st.store(0, int(s), 1, b)
         hit.append(mine)
     hit = np.concatenate(hit)
+    # (by the chunk's own kernel, and by that of a few rows)
+    few = hs.Attention(attention.q_heads, attention.scale, causal=causal, window=window, longest_chunk=1, longest=attention.longest)
+    for a in (attention, few):
+        masked_holds(torch, hs, st, batch, a, q, k, v, new, old, scale, window, causal, hit)
+
+
+def masked_holds(torch, hs, st, batch, attention, q, k, v, new, old, scale, window, causal, hit):
+    dtype = st.dtype
     out, lse = attend(torch, hs, st, batch, attention, q)
     clean = [[np.where(np.isfinite(x), x, 0.0) for x in y] for y in (k, v)]
     want = expected(q, *clean, new, old, scale, causal, window)
@@ -604,3 +620,138 @@ def test_a_pool_without_pages_left(torch_cuda, hs):
     st.handle.fork(3, parents.data_ptr(), children.data_ptr(), status.data_ptr(), stream)
     assert int(status) == books.fork([0, 0, 1], [2, 3, 1])
     books.same(torch, st)
+
+
+# ---- how it is called --------------------------------------------------------------------------------------------------
+
+
+def test_workspaces_are_asked_for_and_left_as_they_were(torch_cuda, hs):
+    torch = torch_cuda
+    st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, 2, 21)
+    need = st.handle.attend_workspace(batch, attention)
+    assert need > 0
+    qd = device(torch, q, 2)
+    out = torch.empty_like(qd)
+    for size in (0, need - 1):
+        w = torch.zeros(max(size, 16), dtype=torch.uint8, device="cuda")
+        with pytest.raises(hs.HspmmError) as e:
+            st.handle.attend(0, batch, attention, heads_view(hs, qd), heads_view(hs, out), workspace=w.data_ptr() if size else 0, workspace_bytes=size)
+        assert e.value.code == 1 and str(need) in str(e.value)
+    # one workspace, calls of different shapes in turn: counters in front of the sums are zero again
+    w = torch.zeros(need + 4096, dtype=torch.uint8, device="cuda")
+    want = expected(q, k, v, new, old, scale, causal, window)
+    for _ in range(3):
+        o, l = attend(torch, hs, st, batch, attention, q, workspace=w)
+        assert_attended(2, o, l, want, k, v, q.shape[2])
+        small = hs.Attention(attention.q_heads, attention.scale, longest_chunk=1, longest=300)
+        o, l = attend(torch, hs, st, batch, small, q, workspace=w)
+        assert_attended(2, o, l, want, k, v, q.shape[2])
+        torch.cuda.synchronize()
+        assert int(w[:65536].count_nonzero()) == 0
+
+
+def test_streams_and_a_recorded_step(torch_cuda, hs):
+    # extend, append and attend on a stream of their own, and recorded in a graph that replays with other inputs in place
+    torch = torch_cuda
+    rng = np.random.default_rng(4)
+    S, page, heads, dim, steps = 6, 16, 2, 64, 5
+    st = State(torch, hs, 0, 64, page, heads, dim, S, 10)
+    table = torch.from_numpy(hs.rotary_table(dim, 200)).cuda()
+    r = hs.Rotary(dim, 200, table.data_ptr())
+    starts, one = ints(torch, np.arange(S + 1)), ints(torch, np.ones(S))
+    batch = hs.Batch(S, S, starts.data_ptr())
+    a = hs.Attention(heads * 2, 0.125, longest_chunk=1, longest=150)
+    w = torch.zeros(max(1, st.handle.attend_workspace(batch, a)), dtype=torch.uint8, device="cuda")
+    q, k, v = (torch.zeros(S, h, dim, dtype=torch.float16, device="cuda") for h in (heads * 2, heads, heads))
+    q2, out = torch.zeros_like(q), torch.zeros_like(q)
+    prompt = [int(x) for x in rng.integers(0, 120, S)]
+
+    def step(stream):
+        st.handle.extend(S, 0, one.data_ptr(), 0, stream)
+        st.handle.append(0, batch, heads_view(hs, k), heads_view(hs, v), rotary=r, q_heads=heads * 2, q=heads_view(hs, q), q_out=heads_view(hs, q2), stream=stream)
+        st.handle.attend(0, batch, a, heads_view(hs, q2), heads_view(hs, out), workspace=w.data_ptr(), workspace_bytes=w.numel(), stream=stream)
+
+    def begin():
+        st.table.fill_(-1)
+        st.lengths.zero_()
+        st.references.zero_()
+        for p in st.pool:
+            p.copy_(filled)
+        st.handle.extend(S, 0, ints(torch, prompt).data_ptr(), 0, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+
+    filled = torch.randn(st.pool[0].shape, device="cuda").half()
+    inputs = [[torch.randn(x.shape, device="cuda").half() for x in (q, k, v)] for _ in range(steps)]
+    begin()
+    side = torch.cuda.Stream()
+    results = []
+    for x in inputs:
+        for to, y in zip((q, k, v), x):
+            to.copy_(y)
+        side.wait_stream(torch.cuda.current_stream())
+        step(side.cuda_stream)
+        torch.cuda.current_stream().wait_stream(side)
+        results.append(out.clone())
+        out.zero_()
+    begin()
+    with torch.cuda.stream(side):
+        step(side.cuda_stream)                                # (eagerly once: the device is known)
+    torch.cuda.synchronize()
+    begin()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        step(side.cuda_stream)
+    begin()
+    for x, want in zip(inputs, results):
+        for to, y in zip((q, k, v), x):
+            to.copy_(y)
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert st.lengths.tolist() == [p + steps for p in prompt]
+
+
+def test_two_streams_with_workspaces_of_their_own(torch_cuda, hs):
+    torch = torch_cuda
+    st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, 2, 23)
+    want = expected(q, k, v, new, old, scale, causal, window)
+    qd = device(torch, q, 2)
+    need = st.handle.attend_workspace(batch, attention)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs, spaces = [torch.zeros_like(qd) for _ in range(2)], [torch.zeros(need, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    lses = [torch.zeros(qd.shape[:2], device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for s, o, l, w in zip(streams, outs, lses, spaces):
+            st.handle.attend(0, batch, attention, heads_view(hs, qd), heads_view(hs, o), lse=l.data_ptr(), workspace=w.data_ptr(), workspace_bytes=need, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for o, l in zip(outs, lses):
+        assert_attended(2, o, l, want, k, v, q.shape[2])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+@pytest.mark.parametrize("dtype,case", [(0, 2), (2, 8), (1, 8), (0, 18)])
+def test_other_scales(torch_cuda, hs, scale, dtype, case):
+    torch = torch_cuda
+    st, batch, attention, q, k, v, new, old, rows, _, window, causal = attention_case(torch, hs, dtype, case, seed=1)
+    other = hs.Attention(attention.q_heads, scale, causal=causal, window=window, longest_chunk=max(new), longest=attention.longest)
+    out, lse = attend(torch, hs, st, batch, other, q)
+    assert_attended(dtype, out, lse, expected(q, k, v, new, old, np.float64(np.float32(scale)), causal, window), k, v, q.shape[2])
+
+
+def test_tokens_of_no_chunk_are_left_alone(torch_cuda, hs):
+    # chunks that begin in front of the batch, end behind it or belong to no sequence
+    torch = torch_cuda
+    st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, 2, 5)
+    T = q.shape[0]
+    starts, rd = ints(torch, [0, 3, 4, T + 5]), ints(torch, [int(rows[0]), 1 << 20, int(rows[2])])
+    out = torch.full(q.shape, 7.0, device="cuda").bfloat16()
+    qd = device(torch, q, 2)
+    for chunk in (1, 100):
+        a = hs.Attention(attention.q_heads, attention.scale, longest_chunk=chunk, longest=400)
+        b = hs.Batch(3, T, starts.data_ptr(), rd.data_ptr())
+        w = torch.zeros(max(1, st.handle.attend_workspace(b, a)), dtype=torch.uint8, device="cuda")
+        st.handle.attend(0, b, a, heads_view(hs, qd), heads_view(hs, out), workspace=w.data_ptr(), workspace_bytes=w.numel(), stream=torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert (out[3:] == 7).all() and not (out[:3] == 7).all()

@@ -36,7 +36,7 @@ __device__ __forceinline__ void lds_barrier()
 // The scores of a half are made among the exponentials of the half in front.  Images go through LDS, kRing of them in turn: while image n is
 // multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image (with two places: two).
 template <bool BF, int DP, int W, bool Whole>
-__global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void attend_chunk_kernel(const AttendArgs aa)
+__global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel(const AttendArgs aa)
 {
     typedef typename HalfOps<BF>::elem_t T;
     constexpr uint32_t kThreads = 64u * W, kRows = 32u * W, kKeys = 64u;
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void attend_chunk_kernel(co
     // (rows whose operands are read together begin in different banks: 16 of keys 16 bytes apart, four of values 64)
     constexpr uint32_t kKeyPitch = DP * 2u + 16u, kValuePitch = DP * 2u + (DP % 128 == 0 || DP == 64 ? 64u : 0u), kImage = kKeys * (kKeyPitch + kValuePitch);
     static_assert(kKeyPitch / 16u % 2u == 1u && kValuePitch / 64u % 2u == 1u && kValuePitch % 64u == 0u, "");
-    constexpr uint32_t kRing = kImage <= 50u * 1024u ? 3u : 2u;
+    constexpr uint32_t kRing = 3u * kImage <= (DP <= 128 && W == 4 ? 80u : 160u) * 1024u - 8u ? 3u : 2u;
     constexpr uint32_t kRowPieces = DP / 8u, kImagePieces = kKeys * kRowPieces;
     constexpr int kSteps = DP / 16, kTiles = DP / 32, kPieces = int((kImagePieces + kThreads - 1u) / kThreads);
     __shared__ __attribute__((aligned(16))) char images[kRing * kImage];
@@ -436,22 +436,22 @@ void launch(const AttendArgs &aa, hipStream_t s)
 }
 
 template <bool BF>
-void launch_type(const AttendArgs &aa, hipStream_t s)
+void launch_type(const AttendArgs &aa, uint32_t rows_log, hipStream_t s)
 {
     const uint32_t D = aa.pages.head_dim;
-    if (D <= 64u) launch<BF, 64, 8>(aa, s);
-    else if (D <= 96u) launch<BF, 96, 8>(aa, s);
-    else if (D <= 128u) launch<BF, 128, 8>(aa, s);
+    if (D <= 64u) launch<BF, 64, 4>(aa, s);
+    else if (D <= 96u) launch<BF, 96, 4>(aa, s);
+    else if (D <= 128u) rows_log == 8u ? launch<BF, 128, 8>(aa, s) : launch<BF, 128, 4>(aa, s);
     else if (D <= 160u) launch<BF, 160, 4>(aa, s);
     else launch<BF, 256, 4>(aa, s);
 }
 
 }  // namespace
 
-hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, hipStream_t s)
+hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, uint32_t rows_log, hipStream_t s)
 {
-    if (dtype == kDtypeF16) launch_type<false>(aa, s);
-    else launch_type<true>(aa, s);
+    if (dtype == kDtypeF16) launch_type<false>(aa, rows_log, s);
+    else launch_type<true>(aa, rows_log, s);
     return hipGetLastError();
 }
 

@@ -297,7 +297,12 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     const uint32_t shared = a->q_heads / c->heads;
     const uint64_t rows = uint64_t(std::min(a->longest_chunk, b->tokens)) * shared;
     AttendShape sh{};
-    sh.rows_log = c->dtype == HSPMM_TF32 || rows <= 32u ? kAttendRowsLog : attend_chunk_rows_log(c->head_dim);
+    // 256 rows only for heads of 97 to 128 elements and tiles for two rounds: with 128 rows two workgroups share a compute unit, but there only two images
+    // fit for each.  us with 128 / 256 rows: 4096 tokens over 16384 keys, 32 heads, 512 tiles of 256, 1007 / 931; 17 chunks of up to 700 tokens over up
+    // to 5700, 12 heads, 344 tiles, 204 / 229; heads of 64, 2048 tokens over 8048, 177 / 184.
+    const uint64_t wide = uint64_t(c->heads) * ((uint64_t(b->tokens) * shared >> 8) + (b->sequences + 1u) / 2u);
+    if (c->dtype == HSPMM_TF32 || rows <= 32u) sh.rows_log = kAttendRowsLog;
+    else sh.rows_log = c->head_dim > 96u && c->head_dim <= 128u && rows > 128u && wide >= 512u ? 8u : 7u;
     // keys that a tile's rows see at most
     uint64_t keys = uint64_t(c->table_pages) * c->page_tokens;
     if (a->longest && a->longest < keys) keys = a->longest;
@@ -308,11 +313,15 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     // Keys of a part.  Rows kernel: as few as give every compute unit two workgroups, 128 at least (every wave a tile or two) and 512 at most, more only
     // where that is over 4096 workgroups: sequences are of many lengths, and the last ones should not be long.  us by parts of 128 / 256 / 512 keys: one token
     // over 1000 keys, 8 heads 8.1 / 9.2 / 11.9; over 30000 58 / 39 / 30; 8 sequences of up to 8000 56 / 44 / 42.
-    // Chunk kernel: a workgroup a compute unit; a part's sums are 132 KB, as much as 260 keys.  us by 256 / 512 workgroups: 100 tokens for each of 4
-    // sequences of 4000 54 / 70; 512 tokens over 8512 keys, head_dim 64 33 / 48.
+    // Chunk kernel: as many as run at a time (two a compute unit with 128 rows and heads of up to 128 elements); a part's sums are as much as 130 keys.
+    // Of two, twice as many where there are tiles for half of them anyway, which are of different lengths.  us by 512 / 1024 workgroups: 100 tokens for
+    // each of 4 sequences of 4000 52 / 64; 512 tokens over 8512 keys, head_dim 64 38 / 48; the 17 chunks above 204 / 175.  (One a compute unit, head_dim
+    // 256, 1024 tokens over 2048 older keys, by 256 / 512 264 / 338.)
     const uint64_t work = tiles * c->heads * keys;
+    const bool two = sh.rows_log == 7u && c->head_dim <= 128u;
     auto whole = [](uint64_t k) { return (k + 127u) & ~uint64_t(127u); };
-    const uint64_t part = sh.rows_log == kAttendRowsLog ? std::max(whole(work / 4096u), std::min<uint64_t>(whole(work / 512u), 512u)) : whole(work / 256u);
+    const uint64_t part = sh.rows_log == kAttendRowsLog ? std::max(whole(work / 4096u), std::min<uint64_t>(whole(work / 512u), 512u)) :
+                                                          whole(work / (!two ? 256u : tiles * c->heads < 256u ? 512u : 1024u));
     sh.part_keys = uint32_t(std::min<uint64_t>(std::max<uint64_t>(part, sh.rows_log == kAttendRowsLog ? 128u : 512u), 1u << 30));
     const uint64_t parts = (keys + 31u + sh.part_keys - 1u) / sh.part_keys;
     sh.splits = numbered * c->heads > kAttendCounters ? 1u : uint32_t(std::min<uint64_t>(std::max<uint64_t>(parts, 1u), 256u));
@@ -354,7 +363,7 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     aa.arrive = static_cast<uint32_t *>(workspace);
     aa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + kAttendCounters * 4u);
     if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, static_cast<hipStream_t>(stream)));
-    else HSPMM_HIP(launch_attend_chunk(cache->dtype, aa, static_cast<hipStream_t>(stream)));
+    else HSPMM_HIP(launch_attend_chunk(cache->dtype, aa, sh.rows_log, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
 

@@ -220,7 +220,10 @@ ATTENTIONS = [  # chunks, tokens held before, heads, shared, dim, page tokens, w
     ([64], [40], 1, 1, 248, 48, 0, True),
     ([1, 1], [9000, 17], 1, 4, 128, 16, 0, True),
     ([1], [5000], 2, 1, 64, 10, 0, True),
-    ([40], [6000], 1, 4, 128, 16, 0, True)]
+    ([40], [6000], 1, 4, 128, 16, 0, True),
+    # tiles of 256 rows: for many tiles only
+    ([1] * 29 + [150, 2], [7] * 29 + [130, 0], 32, 1, 128, 16, 0, True),
+    ([140] + [2] * 35, [300] + [0, 3, 50, 8, 1] * 7, 32, 1, 104, 24, 60, True)]
 
 
 def attention_case(torch, hs, dtype, case, order=0, seed=0, layers=1):
@@ -297,7 +300,7 @@ def test_attend(torch_cuda, hs, dtype, case):
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
-@pytest.mark.parametrize("case", [4, 5, 9, 12, 13])
+@pytest.mark.parametrize("case", [4, 5, 9, 12, 13, 24, 25])
 def test_pages_that_are_gone_are_not_seen(torch_cuda, hs, dtype, case):
     torch = torch_cuda
     st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, dtype, case, seed=7)
@@ -322,7 +325,7 @@ def test_pages_that_are_gone_are_not_seen(torch_cuda, hs, dtype, case):
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
-@pytest.mark.parametrize("case", [2, 4, 6, 8, 9, 10, 17, 18, 19, 20])
+@pytest.mark.parametrize("case", [2, 4, 6, 8, 9, 10, 17, 18, 19, 20, 24, 25])
 def test_what_is_masked_does_not_reach_the_result(torch_cuda, hs, dtype, case):
     # infinities and NaN in keys and values: only the tokens that see them have them
     torch = torch_cuda

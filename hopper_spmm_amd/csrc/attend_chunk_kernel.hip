@@ -33,6 +33,11 @@ __device__ __forceinline__ void lds_barrier()
 //   scores: S^T = K Q^T, 32 keys x 32 rows by instructions of 16 elements; register r: key 8 (r / 4) + 4 h + r % 4
 //   sums:   O^T = V^T P^T, 32 elements x 32 rows by instructions of 16 keys: scores 8 s .. 8 s + 7 of a lane are its part of the second operand,
 //           keys in that order; the first one comes transposed from LDS (ds_read_b64_tr_b16), four keys of an element a read
+// Per key and row 4 D operations, an exponential and some ten other instructions.  Matrix instructions bound it where keys are many: 4096 tokens over
+// 16384 keys, 32 heads on 8, head_dim 128, bf16, 940 us, 1020 TFLOP/s (a library's product of 8192^3: 1170); 2048 tokens over 8048 keys, heads of 96 / 64:
+// 220 / 180 us, 800 / 650 TFLOP/s, as exponentials weigh more.  What is left there is the exponentials' share of a wave's issue that no matrix
+// instruction of the other wave covers.  Short spans: an image's arrival and the last workgroups; 17 chunks of up to 700 tokens, window 1000, 72 us, 350
+// TFLOP/s.  A wave has 32 rows (64 do not fit in its registers), two waves a SIMD: one multiplies while the other one takes exponentials.
 // The scores of a half are made among the exponentials of the half in front.  Images go through LDS, kRing of them in turn: while image n is
 // multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image (with two places: two).
 template <bool BF, int DP, int W, bool Whole>
@@ -50,7 +55,10 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     __shared__ __attribute__((aligned(16))) char images[kRing * kImage];
     __shared__ uint32_t odd, arrived;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, j = lane & 31u;
-    const uint32_t head = blockIdx.x, part = blockIdx.z, D = aa.pages.head_dim, tile_number = gridDim.y - 1u - blockIdx.y;
+    // (the last tiles first: where a token sees what is in front of it they are the longest)
+    const uint32_t part = blockIdx.y, D = aa.pages.head_dim;
+    const Cell cell = cell_of(aa, gridDim.x - 1u - blockIdx.x, part);
+    const uint32_t head = cell.head, tile_number = cell.tile;
     const RowTile t = find_tile<kRowsLog>(aa, tile_number);
     if (!t.there) return;
     const int32_t lo = t.lo & ~31, span = t.hi - lo, each = int32_t(aa.part_keys);
@@ -368,7 +376,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     if (parts > 1) {
         // A part's sums as the lanes hold them: 16 bytes a lane side by side, then the rows' references and totals.
         constexpr uint32_t kWaveSlot = 32u * (DP + 4u), kSlot = kRows * (DP + 4u);
-        const uint32_t pair = tile_number * gridDim.x + head;
+        const uint32_t pair = tile_number * aa.heads.d + head;
         const __amdgpu_buffer_rsrc_t mem = device_scope_buffer(aa.sums + size_t(pair) * aa.splits * kSlot);
         const bool wave_there = wave * 32u < t.rows;
         auto sums_at = [&](uint32_t p, int c, int r) __attribute__((always_inline)) { return (p * kSlot + wave * kWaveSlot + (c * 4u + r / 4u) * 256u + lane * 4u) * 4u; };
@@ -430,7 +438,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
 template <bool BF, int DP, int W>
 void launch(const AttendArgs &aa, hipStream_t s)
 {
-    const dim3 grid(aa.pages.heads, attend_tiles(aa.batch.tokens, aa.batch.sequences, aa.shared.d, W == 8 ? 8u : 7u), aa.splits);
+    const dim3 grid(aa.tiles * aa.heads.d, aa.splits);
     if (aa.pages.page_tokens.d % 16u == 0u) attend_chunk_kernel<BF, DP, W, true><<<grid, dim3(64 * W), 0, s>>>(aa);
     else attend_chunk_kernel<BF, DP, W, false><<<grid, dim3(64 * W), 0, s>>>(aa);
 }

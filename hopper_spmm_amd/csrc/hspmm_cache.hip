@@ -288,7 +288,7 @@ static int check_attention(const hspmm_cache *c, const hspmm_batch *b, const hsp
 // How an attention is launched, by sizes alone: the same for the call and for its workspace.
 struct AttendShape {
     uint32_t rows_log;                   // of a tile: kAttendRowsLog the rows kernel, 7 and 8 the chunk kernel
-    uint32_t splits, part_keys;
+    uint32_t tiles, splits, part_keys;
     uint64_t bytes;
 };
 
@@ -297,16 +297,22 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     const uint32_t shared = a->q_heads / c->heads;
     const uint64_t rows = uint64_t(std::min(a->longest_chunk, b->tokens)) * shared;
     AttendShape sh{};
+    // keys that a sequence's tokens see at most, and those of a tile of so many rows
+    uint64_t keys = uint64_t(c->table_pages) * c->page_tokens;
+    if (a->longest && a->longest < keys) keys = a->longest;
+    auto seen = [&](uint32_t tile_rows) { return a->window && uint64_t(a->window) + tile_rows < keys ? uint64_t(a->window) + tile_rows : keys; };
+    // The rows kernel for up to 16 rows, and where there is little to do: a tile of it is sixteen rows, and its waves share out the keys.  us of it / of the
+    // chunk kernel by tiles of 16 rows x heads x keys: 18 K (60 tokens from the beginning, 32 heads) 7.0 / 10.6; 96 K (8 tokens for each of 3 sequences
+    // of 2000, 32 heads on 8) 18.6 / 25; 180 K (300 tokens from the beginning) 15.2 / 16.7; 192 K (3 sequences of 4000) 29 / 27; 320 K 19.8 / 18.8;
+    // 2048 K (32 sequences of 4000) 198 / 144.
+    const uint64_t rows_work = uint64_t(b->sequences) * ((rows + 15u) / 16u) * c->heads * seen(16u);
     // 256 rows only for heads of 97 to 128 elements and tiles for two rounds: with 128 rows two workgroups share a compute unit, but there only two images
     // fit for each.  us with 128 / 256 rows: 4096 tokens over 16384 keys, 32 heads, 512 tiles of 256, 1007 / 931; 17 chunks of up to 700 tokens over up
     // to 5700, 12 heads, 344 tiles, 204 / 229; heads of 64, 2048 tokens over 8048, 177 / 184.
     const uint64_t wide = uint64_t(c->heads) * ((uint64_t(b->tokens) * shared >> 8) + (b->sequences + 1u) / 2u);
-    if (c->dtype == HSPMM_TF32 || rows <= 32u) sh.rows_log = kAttendRowsLog;
+    if (c->dtype == HSPMM_TF32 || rows <= 16u || rows_work <= 190000u) sh.rows_log = kAttendRowsLog;
     else sh.rows_log = c->head_dim > 96u && c->head_dim <= 128u && rows > 128u && wide >= 512u ? 8u : 7u;
-    // keys that a tile's rows see at most
-    uint64_t keys = uint64_t(c->table_pages) * c->page_tokens;
-    if (a->longest && a->longest < keys) keys = a->longest;
-    if (a->window && uint64_t(a->window) + (1u << sh.rows_log) < keys) keys = uint64_t(a->window) + (1u << sh.rows_log);
+    keys = seen(1u << sh.rows_log);
     const uint64_t numbered = attend_tiles(b->tokens, b->sequences, shared, sh.rows_log);
     // tiles that have rows, at most: numbers are left out
     const uint64_t tiles = std::min<uint64_t>(numbered, uint64_t(b->sequences) * ((rows + (1u << sh.rows_log) - 1u) >> sh.rows_log));
@@ -325,16 +331,26 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     sh.part_keys = uint32_t(std::min<uint64_t>(std::max<uint64_t>(part, sh.rows_log == kAttendRowsLog ? 128u : 512u), 1u << 30));
     const uint64_t parts = (keys + 31u + sh.part_keys - 1u) / sh.part_keys;
     sh.splits = numbered * c->heads > kAttendCounters ? 1u : uint32_t(std::min<uint64_t>(std::max<uint64_t>(parts, 1u), 256u));
+    sh.tiles = uint32_t(numbered);
     if (sh.splits > 1u) sh.bytes = kAttendCounters * 4u + numbered * c->heads * sh.splits * attend_slot(sh.rows_log, c->head_dim) * 4u;
     return sh;
+}
+
+// (a launch has fewer than 2^32 threads, 512 a workgroup at most)
+static int check_tiles(const hspmm_cache *c, const hspmm_batch *b, const AttendShape &sh)
+{
+    if (uint64_t(sh.tiles) * c->heads < (1u << 23)) return HSPMM_OK;
+    return fail(HSPMM_ERR_UNSUPPORTED, "%u tokens of %u sequences with %u heads of keys: in several calls", b->tokens, b->sequences, c->heads);
 }
 
 int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_attention *attention, uint64_t *bytes)
 {
     if (!bytes) return fail(HSPMM_ERR_INVALID, "null bytes");
     if (int rc = check_attention(cache, batch, attention)) return rc;
-    *bytes = batch->tokens ? attend_shape(cache, batch, attention).bytes : 0;
-    return HSPMM_OK;
+    if (batch->tokens == 0) { *bytes = 0; return HSPMM_OK; }
+    const AttendShape sh = attend_shape(cache, batch, attention);
+    *bytes = sh.bytes;
+    return check_tiles(cache, batch, sh);
 }
 
 int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_attention *attention, const hspmm_heads *q,
@@ -350,6 +366,7 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
         return fail(HSPMM_ERR_UNSUPPORTED, "q: a head's elements side by side, tokens and heads at multiples of 16 bytes");
     if (reinterpret_cast<uintptr_t>(lse) % 4u) return fail(HSPMM_ERR_INVALID, "lse is not aligned to its elements");
     const AttendShape sh = attend_shape(cache, batch, attention);
+    if (int rc = check_tiles(cache, batch, sh)) return rc;
     if (sh.bytes && (!workspace || workspace_bytes < sh.bytes || reinterpret_cast<uintptr_t>(workspace) % 16u))
         return fail(HSPMM_ERR_INVALID, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)sh.bytes);
     if (int rc = current_device(nullptr)) return rc;
@@ -359,7 +376,7 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     aa.q = heads_of(q); aa.out = heads_of(out); aa.lse = lse;
     aa.q_heads = attention->q_heads; aa.shared = Divisor::of(attention->q_heads / cache->heads);
     aa.scale = attention->scale; aa.causal = attention->causal != 0; aa.window = attention->window;
-    aa.splits = sh.splits; aa.part_keys = sh.part_keys;
+    aa.heads = Divisor::of(cache->heads); aa.tiles = sh.tiles; aa.splits = sh.splits; aa.part_keys = sh.part_keys;
     aa.arrive = static_cast<uint32_t *>(workspace);
     aa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + kAttendCounters * 4u);
     if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, static_cast<hipStream_t>(stream)));

@@ -1,5 +1,8 @@
 // Work on the pages of a cache: giving out, sharing, releasing, moving and copying them.  What decides is integers - the
-// table, lengths and references -, what takes time is the pages' bytes, each read and written once, all layers in one launch.
+// table, lengths and references -, what takes time is the pages' bytes, each read and written once, all layers in one launch.  us: 476 pages of 2 MB
+// moved 389, 5.1 TB/s (a large copy: 4.8); 192 beams of partly filled pages, all of 32 layers, 68 for 284 MB, 4.2 TB/s; small ones 10, which is two
+// launches, as which pages are free has to be known before one is written: what is decided cannot be decided again by every workgroup that copies
+// while others change the table and the references.
 #include "cache_device.h"
 
 namespace hspmm {

@@ -223,7 +223,10 @@ ATTENTIONS = [  # chunks, tokens held before, heads, shared, dim, page tokens, w
     ([40], [6000], 1, 4, 128, 16, 0, True),
     # tiles of 256 rows: for many tiles only
     ([1] * 29 + [150, 2], [7] * 29 + [130, 0], 32, 1, 128, 16, 0, True),
-    ([140] + [2] * 35, [300] + [0, 3, 50, 8, 1] * 7, 32, 1, 104, 24, 60, True)]
+    ([140] + [2] * 35, [300] + [0, 3, 50, 8, 1] * 7, 32, 1, 104, 24, 60, True),
+    # windows, and so many tiles that the chunk's own kernel serves them
+    ([200] + [1] * 20, [700] + [30] * 20, 16, 2, 64, 24, 60, True),
+    ([90, 5] + [1] * 18, [0, 300] + [64] * 18, 16, 2, 160, 16, 100, True)]
 
 
 def attention_case(torch, hs, dtype, case, order=0, seed=0, layers=1):
@@ -231,7 +234,7 @@ def attention_case(torch, hs, dtype, case, order=0, seed=0, layers=1):
     rng = np.random.default_rng(1000 * case + seed)
     n, lengths = len(new), np.add(new, old)
     used = int(sum(-(-x // page) for x in lengths))
-    st = State(torch, hs, dtype, used + 2, page, heads, dim, n + 1, int(max(-(-lengths // page))) + 2, layers=layers, order=order)
+    st = State(torch, hs, dtype, used + 2, page, heads, dim, n + 1, 100000 // page + 2, layers=layers, order=order)
     rows = rng.permutation(n + 1)[:n]
     by_row = np.zeros(n + 1, int)
     by_row[rows] = lengths
@@ -247,6 +250,12 @@ def attention_case(torch, hs, dtype, case, order=0, seed=0, layers=1):
     scale = 1.0 / math.sqrt(dim)
     attention = hs.Attention(heads * shared, scale, causal=causal, window=window, longest_chunk=max(new), longest=int(lengths.max()))
     return st, batch, attention, q, k, v, new, old, rows, np.float64(np.float32(scale)), window, causal
+
+
+def many(hs, st, batch, attention):
+    """The same with hints of many rows and of so many keys that the chunk's own kernel serves, in parts of 512 keys."""
+    tiles = st.heads * batch.sequences * -(-batch.tokens * (attention.q_heads // st.heads) // 128)
+    return hs.Attention(attention.q_heads, attention.scale, causal=attention.causal, window=attention.window, longest_chunk=5000, longest=100000 // tiles)
 
 
 def attend(torch, hs, st, batch, attention, q, layout="tokens", layer=0, lse=True, hints=True, workspace=None):
@@ -293,14 +302,15 @@ def test_attend(torch_cuda, hs, dtype, case):
         # the hints choose kernels and parts, not the result; lse may be left out; bits do not change from call to call
         again, _ = attend(torch, hs, st, batch, attention, q, layout, layer=layers - 1, lse=False)
         assert torch.equal(out, again)
-        for chunk, longest in ((1, 0), (1, 1 << 30), (5000, 100000), (0, 1)):
-            other = hs.Attention(attention.q_heads, attention.scale, causal=causal, window=window, longest_chunk=chunk, longest=longest)
+        others = [hs.Attention(attention.q_heads, attention.scale, causal=causal, window=window, longest_chunk=chunk, longest=longest)
+                  for chunk, longest in ((1, 0), (1, 1 << 30), (5000, 100000), (0, 1))]
+        for other in others + [many(hs, st, batch, attention)]:
             out, lse = attend(torch, hs, st, batch, other, q, "gaps" if q.shape[2] > 3 else layout, layer=layers - 1)
             assert_attended(dtype, out, lse, want, k, v, q.shape[2])
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
-@pytest.mark.parametrize("case", [4, 5, 9, 12, 13, 24, 25])
+@pytest.mark.parametrize("case", [4, 5, 9, 12, 13, 24, 25, 26, 27])
 def test_pages_that_are_gone_are_not_seen(torch_cuda, hs, dtype, case):
     torch = torch_cuda
     st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, dtype, case, seed=7)
@@ -319,13 +329,14 @@ def test_pages_that_are_gone_are_not_seen(torch_cuda, hs, dtype, case):
         parts.append(attend64(q[at:at + n], a, b, np.arange(o, o + n), scale, causal, window, t[None]))
         at += n
     want = [np.concatenate(x) for x in zip(*parts)]
-    out, lse = attend(torch, hs, st, batch, attention, q)
-    assert_attended(dtype, out, lse, want, k, v, q.shape[2])
-    assert np.isneginf(to64(lse)).any()
+    for a in (attention, many(hs, st, batch, attention)):
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert_attended(dtype, out, lse, want, k, v, q.shape[2])
+        assert np.isneginf(to64(lse)).any()
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
-@pytest.mark.parametrize("case", [2, 4, 6, 8, 9, 10, 17, 18, 19, 20, 24, 25])
+@pytest.mark.parametrize("case", [2, 4, 6, 8, 9, 10, 17, 18, 19, 20, 24, 25, 26, 27])
 def test_what_is_masked_does_not_reach_the_result(torch_cuda, hs, dtype, case):
     # infinities and NaN in keys and values: only the tokens that see them have them
     torch = torch_cuda
@@ -354,7 +365,7 @@ def test_what_is_masked_does_not_reach_the_result(torch_cuda, hs, dtype, case):
     hit = np.concatenate(hit)
     # (by the chunk's own kernel, and by that of a few rows)
     few = hs.Attention(attention.q_heads, attention.scale, causal=causal, window=window, longest_chunk=1, longest=attention.longest)
-    for a in (attention, few):
+    for a in (attention, few, many(hs, st, batch, attention)):
         masked_holds(torch, hs, st, batch, a, q, k, v, new, old, scale, window, causal, hit)
 
 
@@ -377,6 +388,7 @@ def test_infinite_values_stay_in_their_element(torch_cuda, hs, dtype):
     j = 1100
     v[0][j, 0, 5] = np.inf
     st.store(0, int(rows[0]), 1, v[0])
+    attention = many(hs, st, batch, attention)
     out, lse = attend(torch, hs, st, batch, attention, q)
     got = to64(out)
     sees = np.arange(old[0], old[0] + new[0]) >= j
@@ -399,14 +411,16 @@ def test_scores_far_apart(torch_cuda, hs, dtype):
         kk[0][j] *= 30
         kk = [rounded(torch, kk[0], dtype)]
         st.store(0, int(rows[0]), 0, kk[0])
-        out, lse = attend(torch, hs, st, batch, attention, q)
-        assert_attended(dtype, out, lse, expected(q, kk, v, new, old, scale, causal, window), kk, v, q.shape[2])
+        for a in (attention, many(hs, st, batch, attention)):
+            out, lse = attend(torch, hs, st, batch, a, q)
+            assert_attended(dtype, out, lse, expected(q, kk, v, new, old, scale, causal, window), kk, v, q.shape[2])
     kk = [np.ones_like(k[0])]
     st.store(0, int(rows[0]), 0, kk[0])
     for sign in (1.0, -1.0):
         qq = rounded(torch, sign * np.full_like(q, 40.0), dtype)
-        out, lse = attend(torch, hs, st, batch, attention, qq)
-        assert_attended(dtype, out, lse, expected(qq, kk, v, new, old, scale, causal, window), kk, v, q.shape[2])
+        for a in (attention, many(hs, st, batch, attention)):
+            out, lse = attend(torch, hs, st, batch, a, qq)
+            assert_attended(dtype, out, lse, expected(qq, kk, v, new, old, scale, causal, window), kk, v, q.shape[2])
 
 
 def test_sequences_shorter_than_their_chunk(torch_cuda, hs):
@@ -414,10 +428,11 @@ def test_sequences_shorter_than_their_chunk(torch_cuda, hs):
     torch = torch_cuda
     st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, 2, 8)
     st.lengths[int(rows[0])] = 50                              # a chunk of 130
-    out, lse = attend(torch, hs, st, batch, attention, q)
     want = expected(q, [k[0][:50]] + k[1:], v[:1] and [v[0][:50]] + v[1:], new, [-80] + old[1:], scale, causal, window)
-    assert_attended(2, out, lse, want, k, v, q.shape[2])
-    assert (to64(out)[:80] == 0).all()
+    for a in (attention, many(hs, st, batch, attention)):
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert_attended(2, out, lse, want, k, v, q.shape[2])
+        assert (to64(out)[:80] == 0).all()
 
 
 def test_pages_beyond_32_bits(torch_cuda, hs):
@@ -426,7 +441,7 @@ def test_pages_beyond_32_bits(torch_cuda, hs):
     rng = np.random.default_rng(2)
     page, heads, dim = 64, 2, 128
     pages = (1 << 32) // (page * heads * dim) + 64
-    st = State(torch, hs, 2, pages, page, heads, dim, 2, 8, fill=0.0)
+    st = State(torch, hs, 2, pages, page, heads, dim, 2, 2048, fill=0.0)
     ids = pages - 1 - np.arange(4)
     st.table[0, :4] = ints(torch, ids)
     st.lengths[0] = 200
@@ -442,10 +457,11 @@ def test_pages_beyond_32_bits(torch_cuda, hs):
         s2 = ints(torch, [0, chunk])
         b2 = hs.Batch(1, chunk, s2.data_ptr())
         a = hs.Attention(heads * 2, 0.1, longest_chunk=chunk, longest=200)
-        out, lse = attend(torch, hs, st, b2, a, qq)
         st.kept = st.kept + (s2,)
         want = attend64(qq, k, v, np.arange(200 - chunk, 200), np.float64(np.float32(0.1)), True, 0)
-        assert_attended(2, out, lse, want, [k], [v], dim)
+        for b in (a, many(hs, st, b2, a)):
+            out, lse = attend(torch, hs, st, b2, b, qq)
+            assert_attended(2, out, lse, want, [k], [v], dim)
 
 
 # ---- pages -----------------------------------------------------------------------------------------------------------
@@ -630,8 +646,10 @@ def test_a_pool_without_pages_left(torch_cuda, hs):
 
 def test_workspaces_are_asked_for_and_left_as_they_were(torch_cuda, hs):
     torch = torch_cuda
-    st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, 2, 21)
-    need = st.handle.attend_workspace(batch, attention)
+    st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, 2, 23)
+    chunks = many(hs, st, batch, attention)
+    need = min(st.handle.attend_workspace(batch, a) for a in (attention, chunks))
+    most = max(st.handle.attend_workspace(batch, a) for a in (attention, chunks))
     assert need > 0
     qd = device(torch, q, 2)
     out = torch.empty_like(qd)
@@ -639,16 +657,15 @@ def test_workspaces_are_asked_for_and_left_as_they_were(torch_cuda, hs):
         w = torch.zeros(max(size, 16), dtype=torch.uint8, device="cuda")
         with pytest.raises(hs.HspmmError) as e:
             st.handle.attend(0, batch, attention, heads_view(hs, qd), heads_view(hs, out), workspace=w.data_ptr() if size else 0, workspace_bytes=size)
-        assert e.value.code == 1 and str(need) in str(e.value)
+        assert e.value.code == 1 and str(st.handle.attend_workspace(batch, attention)) in str(e.value)
     # one workspace, calls of different shapes in turn: counters in front of the sums are zero again
-    w = torch.zeros(need + 4096, dtype=torch.uint8, device="cuda")
+    w = torch.zeros(most + 4096, dtype=torch.uint8, device="cuda")
     want = expected(q, k, v, new, old, scale, causal, window)
+    small = hs.Attention(attention.q_heads, attention.scale, longest_chunk=1, longest=300)
     for _ in range(3):
-        o, l = attend(torch, hs, st, batch, attention, q, workspace=w)
-        assert_attended(2, o, l, want, k, v, q.shape[2])
-        small = hs.Attention(attention.q_heads, attention.scale, longest_chunk=1, longest=300)
-        o, l = attend(torch, hs, st, batch, small, q, workspace=w)
-        assert_attended(2, o, l, want, k, v, q.shape[2])
+        for a in (attention, small, chunks):
+            o, l = attend(torch, hs, st, batch, a, q, workspace=w)
+            assert_attended(2, o, l, want, k, v, q.shape[2])
         torch.cuda.synchronize()
         assert int(w[:65536].count_nonzero()) == 0
 
@@ -715,9 +732,12 @@ def test_streams_and_a_recorded_step(torch_cuda, hs):
     assert st.lengths.tolist() == [p + steps for p in prompt]
 
 
-def test_two_streams_with_workspaces_of_their_own(torch_cuda, hs):
+@pytest.mark.parametrize("chunks", [False, True])
+def test_two_streams_with_workspaces_of_their_own(torch_cuda, hs, chunks):
     torch = torch_cuda
     st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, 2, 23)
+    if chunks:
+        attention = many(hs, st, batch, attention)
     want = expected(q, k, v, new, old, scale, causal, window)
     qd = device(torch, q, 2)
     need = st.handle.attend_workspace(batch, attention)
@@ -739,8 +759,9 @@ def test_other_scales(torch_cuda, hs, scale, dtype, case):
     torch = torch_cuda
     st, batch, attention, q, k, v, new, old, rows, _, window, causal = attention_case(torch, hs, dtype, case, seed=1)
     other = hs.Attention(attention.q_heads, scale, causal=causal, window=window, longest_chunk=max(new), longest=attention.longest)
-    out, lse = attend(torch, hs, st, batch, other, q)
-    assert_attended(dtype, out, lse, expected(q, k, v, new, old, np.float64(np.float32(scale)), causal, window), k, v, q.shape[2])
+    for a in (other, many(hs, st, batch, other)):
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert_attended(dtype, out, lse, expected(q, k, v, new, old, np.float64(np.float32(scale)), causal, window), k, v, q.shape[2])
 
 
 def test_tokens_of_no_chunk_are_left_alone(torch_cuda, hs):
@@ -751,8 +772,7 @@ def test_tokens_of_no_chunk_are_left_alone(torch_cuda, hs):
     starts, rd = ints(torch, [0, 3, 4, T + 5]), ints(torch, [int(rows[0]), 1 << 20, int(rows[2])])
     out = torch.full(q.shape, 7.0, device="cuda").bfloat16()
     qd = device(torch, q, 2)
-    for chunk in (1, 100):
-        a = hs.Attention(attention.q_heads, attention.scale, longest_chunk=chunk, longest=400)
+    for a in (hs.Attention(attention.q_heads, attention.scale, longest_chunk=1, longest=400), many(hs, st, batch, attention)):
         b = hs.Batch(3, T, starts.data_ptr(), rd.data_ptr())
         w = torch.zeros(max(1, st.handle.attend_workspace(b, a)), dtype=torch.uint8, device="cuda")
         st.handle.attend(0, b, a, heads_view(hs, qd), heads_view(hs, out), workspace=w.data_ptr(), workspace_bytes=w.numel(), stream=torch.cuda.current_stream().cuda_stream)

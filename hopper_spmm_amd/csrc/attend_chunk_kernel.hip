@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, j = lane & 31u;
     // (the last tiles first: where a token sees what is in front of it they are the longest)
     const uint32_t part = blockIdx.y, D = aa.pages.head_dim;
-    const Cell cell = cell_of(aa, gridDim.x - 1u - blockIdx.x, part);
+    const Cell cell = cell_of(aa, gridDim.x - 1u - blockIdx.x, 0u);
     const uint32_t head = cell.head, tile_number = cell.tile;
     const RowTile t = find_tile<kRowsLog>(aa, tile_number);
     if (!t.there) return;

@@ -64,12 +64,14 @@ __device__ __forceinline__ RowTile find_tile(const AttendArgs &aa, uint32_t tile
 
 // The tile and the head of a workgroup: heads side by side, as they are of one length, then tiles, then parts.  Workgroups go to the eight L2 domains and,
 // there, to groups of compute units in turn, whatever they have to do, so what repeats in the numbers must not repeat in time: where chunks fill their
-// tiles every (k + 1)th number is empty, so each eight tiles are turned by one against those in front; where a sequence is long all its parts are there, so
-// its tiles move on by one from part to part.  48 sequences of up to 8000 keys, 16 rows each: 358 us by tiles, then heads, then parts, 178 so; 4 rows 173, 163.
+// tiles every (k + 1)th number is empty, so each eight tiles are turned by one against those in front (40 chunks of 32 tokens, 16 heads on 4: 69 -> 43 us);
+// where a sequence is long all its parts are there, so the rows kernel's tiles move on by one from part to part (`moved`; the chunk kernel, whose parts
+// are few, loses by it: 512 tokens over 8512 keys 40 -> 45 us).  48 sequences of up to 8000 keys, 16 rows each: 358 us by tiles, then heads, then
+// parts, 178 so; 4 rows 173, 163.
 struct Cell { uint32_t tile, head; };
-__device__ __forceinline__ Cell cell_of(const AttendArgs &aa, uint32_t number, uint32_t part)
+__device__ __forceinline__ Cell cell_of(const AttendArgs &aa, uint32_t number, uint32_t moved)
 {
-    const uint32_t column = aa.heads.quotient(number), at = (column + part) % aa.tiles;
+    const uint32_t column = aa.heads.quotient(number), at = moved ? (column + moved) % aa.tiles : column;
     return Cell{(at | 7u) < aa.tiles ? (at & ~7u) | ((at + (at >> 3)) & 7u) : at, number - column * aa.heads.d};
 }
 

@@ -1,9 +1,10 @@
 // Work on the pages of a cache: giving out, sharing, releasing, moving and copying them.  What decides is integers - the
 // table, lengths and references -, what takes time is the pages' bytes, each read and written once, all layers in one launch.  us: 476 pages of 2 MB
-// moved 389, 5.1 TB/s (a large copy: 4.8); 192 beams of partly filled pages, all of 32 layers, 68 for 284 MB, 4.2 TB/s; small ones 10, which is two
+// moved 389, 5.1 TB/s (a large copy: 4.8); 192 beams of partly filled pages, all of 32 layers, 55 for 284 MB, 5.1 TB/s; small ones 10, which is two
 // launches, as which pages are free has to be known before one is written: what is decided cannot be decided again by every workgroup that copies
 // while others change the table and the references.
 #include "cache_device.h"
+#include <algorithm>
 
 namespace hspmm {
 
@@ -185,6 +186,7 @@ __device__ __forceinline__ ForkScratch fork_scratch(const PoolArgs &pa)
     int32_t *s = pa.scratch;
     return ForkScratch{s, s + pa.sequences, s + 2u * pa.sequences, s + 3u * pa.sequences, s + 4u * size_t(pa.sequences)};
 }
+constexpr uint32_t kForkRows = 32768u;          // entries along y of the second launch
 __device__ __forceinline__ bool fork_takes_page(const PoolArgs &pa, uint32_t parent, uint32_t child, int32_t tokens)
 {
     return parent != kIdxMax && child != kIdxMax && parent != child && uint32_t(tokens) != pa.page_tokens.quotient(uint32_t(tokens)) * pa.page_tokens.d;
@@ -226,16 +228,19 @@ __global__ __launch_bounds__(kScanThreads) void pages_fork_kernel(const PoolArgs
     if (status && threadIdx.x == 0u) *status = int32_t(need - found);
 }
 
-// Second launch: workgroup (i, part): part 0 entry i's row and references, the others copy its last page's tokens.
+// Second launch: workgroup (part, i): part 0 entry i's row and references, the others copy its last page's tokens.  (An entry's parts follow each other:
+// workgroups go to the eight L2 domains in turn, and where every fourth entry is its own parent, entries in turn would leave two of them with nothing.)
 template <class U>
-__global__ __launch_bounds__(256) void pages_fork_copy_kernel(const PoolArgs pa, const int32_t *parents, const int32_t *children, const uint32_t heads_each, const uint32_t head_parts)
+__global__ __launch_bounds__(256) void pages_fork_copy_kernel(const PoolArgs pa, const uint32_t n, const int32_t *parents, const int32_t *children, const uint32_t heads_each, const uint32_t head_parts)
 {
     const ForkScratch fs = fork_scratch(pa);
-    const uint32_t i = blockIdx.x, parent = row_of(pa, parents, i), child = row_of(pa, children, i);
+    const uint32_t i = blockIdx.z * kForkRows + blockIdx.y;
+    if (i >= n) return;
+    const uint32_t parent = row_of(pa, parents, i), child = row_of(pa, children, i);
     if (parent == kIdxMax || child == kIdxMax || parent == child) return;
     const int32_t tokens = fs.tokens[i], page = fs.page[i];
     const uint32_t full = pa.page_tokens.quotient(uint32_t(tokens)), rest = uint32_t(tokens) - full * pa.page_tokens.d;
-    if (blockIdx.y == 0u) {
+    if (blockIdx.x == 0u) {
         for (uint32_t p = threadIdx.x; p < pa.table_pages; p += blockDim.x) {
             int32_t &at = pa.table[size_t(child) * pa.table_pages + p];
             const uint32_t old = uint32_t(at);
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(256) void pages_fork_copy_kernel(const PoolArgs pa,
         if (threadIdx.x == 0u) pa.lengths[child] = tokens;
         return;
     }
-    const uint32_t from = uint32_t(fs.from[i]), part = (blockIdx.y - 1u) / head_parts, h0 = (blockIdx.y - 1u) % head_parts * heads_each;
+    const uint32_t from = uint32_t(fs.from[i]), part = (blockIdx.x - 1u) / head_parts, h0 = (blockIdx.x - 1u) % head_parts * heads_each;
     if (!rest || uint32_t(page) >= pa.pages || from >= pa.pages) return;
     copy_tokens<U>(pa, part, uint32_t(page), from, rest, h0, h0 + heads_each < pa.heads ? h0 + heads_each : pa.heads);
 }
@@ -386,7 +391,7 @@ hipError_t launch_pages_fork(const PoolArgs &pa, uint32_t n, const int32_t *pare
     const uint32_t each = (pa.heads + parts - 1u) / parts;
     parts = (pa.heads + each - 1u) / each;
     by_unit(pa, [&](auto u) {
-        pages_fork_copy_kernel<decltype(u)><<<dim3(n, 1u + pa.layers * 2u * parts), dim3(256), 0, s>>>(pa, parents, children, each, parts);
+        pages_fork_copy_kernel<decltype(u)><<<dim3(1u + pa.layers * 2u * parts, std::min(n, kForkRows), (n + kForkRows - 1u) / kForkRows), dim3(256), 0, s>>>(pa, n, parents, children, each, parts);
     });
     return hipGetLastError();
 }

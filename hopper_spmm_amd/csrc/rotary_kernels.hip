@@ -1,10 +1,11 @@
 // Rotary positions, and new keys and values into the pages of a cache.
 //   y_a = x_a cos - x_b sin, y_b = x_a sin + x_b cos for the pairs (a, b) of a head's first `dims` elements, in fp32
 // from 16-bit or fp32 elements, rounded once.  Every element is read and written once: memory bounds it (a large copy: 4.8 TB/s).  us: 16384 tokens of 32
-// heads of 128, fp16, 52, 5.2 TB/s; 12000 tokens of 50 heads of 80, fp32, into pages of 24, 96, 4.0 TB/s; 4096 tokens of 48 heads of 128, bf16, into pages
+// heads of 128, fp16, 52, 5.2 TB/s; 12000 tokens of 50 heads of 80, fp32, into pages of 24, 87, 4.4 TB/s; 4096 tokens of 48 heads of 128, bf16, into pages
 // 20, from features x tokens 37; few tokens 7, which is the host's call.
 #include "cache_device.h"
 #include "spmm_tile_common.hpp"
+#include <algorithm>
 
 namespace hspmm {
 
@@ -295,9 +296,12 @@ template <int DT, int V, bool HALF>
 void launch_pieces(const RotaryArgs &ra, hipStream_t s)
 {
     const uint32_t pieces = ra.head_dim / V, turned = HALF && ra.table ? pieces - ra.dims / 2u / V : pieces, heads = ra.q_heads + 2u * ra.k_heads;
-    // Few tokens: their heads are shared out to several waves, as long as each has a round of its lanes.
+    // Few tokens: their heads are shared out to several waves, as long as each has a round of its lanes.  Many heads, too, as soon as each has 500 pieces,
+    // about two rounds of kAhead: shorter waves leave less of the chip idle at the end, but each finds its token's place.  us in 1 / 2 / 3 shares: 1000 pieces
+    // (12000 tokens of 50 heads of 80, fp32) 96 / 87 / 90, 1536 (8192 tokens of 48 heads of 128, fp32) 86 / 84 / 83.5, 768 (16384 tokens, bf16)
+    // 82 / 84 / 84, 512 (16384 tokens of 32 heads) 54 / 56 / 60.
     const uint32_t groups = (ra.tokens + 3u) / 4u, round = turned < 64u ? 64u / turned : 1u;
-    uint32_t shares = groups < 512u ? 512u / groups : 1u;
+    uint32_t shares = std::max(groups < 512u ? 512u / groups : 1u, uint32_t(std::min<uint64_t>(uint64_t(heads) * pieces / 500u, 4096u)));
     if (shares > (heads + round - 1u) / round) shares = (heads + round - 1u) / round;
     const uint32_t each = (heads + shares - 1u) / shares;
     rotary_kernel<DT, V, HALF><<<dim3(groups, (heads + each - 1u) / each), dim3(256), 0, s>>>(ra, each, turned, pieces);

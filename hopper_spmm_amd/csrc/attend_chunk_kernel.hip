@@ -37,7 +37,7 @@ __device__ __forceinline__ void lds_barrier()
 // 16384 keys, 32 heads on 8, head_dim 128, bf16, 940 us, 1020 TFLOP/s (a library's product of 8192^3: 1170); 2048 tokens over 8048 keys, heads of 96 / 64:
 // 220 / 180 us, 800 / 650 TFLOP/s, as exponentials weigh more.  What is left there is the exponentials' share of a wave's issue that no matrix
 // instruction of the other wave covers.  Short spans: an image's arrival and the last workgroups; 17 chunks of up to 700 tokens, window 1000, 72 us, 350
-// TFLOP/s.  A wave has 32 rows (64 do not fit in its registers), two waves a SIMD: one multiplies while the other one takes exponentials.
+// TFLOP/s.  A wave has 32 rows, two waves a SIMD: one multiplies while the other one takes exponentials.
 // The scores of a half are made among the exponentials of the half in front.  Images go through LDS, kRing of them in turn: while image n is
 // multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image (with two places: two).
 template <bool BF, int DP, int W, bool Whole>

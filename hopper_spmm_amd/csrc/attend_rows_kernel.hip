@@ -36,7 +36,7 @@ struct Rows16 {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const uint32_t d = 32u * s + 8u * (lane >> 4);
-            k[t][s] = at >= 0 && d < D ? __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(keys + (at + d) * 2)) : u32x4{0u, 0u, 0u, 0u};
+            k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(keys + (at + (d < D ? d : 0u)) * 2));
         }
     }
     __device__ __forceinline__ void load_values(int t, int r, const char *values, int64_t at, uint32_t lane, uint32_t D)
@@ -44,17 +44,35 @@ struct Rows16 {
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
             const uint32_t d = uint32_t(16 * kPiece * b) + uint32_t(kPiece) * (lane & 15u);
-            const char *p = values + (at + d) * 2;
-            const bool in = at >= 0 && d < D;
+            const char *p = values + (at + (d < D ? d : 0u)) * 2;
             uint32_t *to = v[4 * t + r][b];
             if constexpr (kPiece == 8) {
-                const u32x4 x = in ? __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p)) : u32x4{0u, 0u, 0u, 0u};
+                const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
                 to[0] = x[0]; to[1] = x[1]; to[2] = x[2]; to[3] = x[3];
             } else {
-                const t_u32x2 x = in ? __builtin_nontemporal_load(reinterpret_cast<const t_u32x2 *>(p)) : t_u32x2{0u, 0u};
+                const t_u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const t_u32x2 *>(p));
                 to[0] = x[0]; to[1] = x[1];
             }
         }
+    }
+    // elements behind the last one
+    __device__ __forceinline__ void clear_keys(uint32_t lane, uint32_t D)
+    {
+#pragma unroll
+        for (int t = 0; t < kParts; ++t)
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+                if (32u * s + 8u * (lane >> 4) >= D) k[t][s] = u32x4{0u, 0u, 0u, 0u};
+    }
+    // keys that are not stored
+    __device__ __forceinline__ void clear_values(uint32_t stored)
+    {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int n = 0; n < kPiece / 2; ++n) v[r][b][n] = stored >> (16 * (r / 4) + r % 4) & 1u ? v[r][b][n] : 0u;
     }
     __device__ __forceinline__ void scores(const Query &Q, f32x4 (&s)[kParts]) const
     {
@@ -130,7 +148,7 @@ struct Rows32 {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const uint32_t d = 16u * s + 4u * (lane >> 4);
-            k[s] = at >= 0 && d < D ? *reinterpret_cast<const f32x4 *>(keys + (at + d) * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
+            k[s] = *reinterpret_cast<const f32x4 *>(keys + (at + (d < D ? d : 0u)) * 4);
         }
     }
     __device__ __forceinline__ void load_values(int, int r, const char *values, int64_t at, uint32_t lane, uint32_t D)
@@ -138,8 +156,23 @@ struct Rows32 {
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
             const uint32_t d = 64u * b + 4u * (lane & 15u);
-            v[r][b] = at >= 0 && d < D ? *reinterpret_cast<const f32x4 *>(values + (at + d) * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
+            v[r][b] = *reinterpret_cast<const f32x4 *>(values + (at + (d < D ? d : 0u)) * 4);
         }
+    }
+    __device__ __forceinline__ void clear_keys(uint32_t lane, uint32_t D)
+    {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+            if (16u * s + 4u * (lane >> 4) >= D) k[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void clear_values(uint32_t stored)
+    {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[r][b][e] = stored >> r & 1u ? v[r][b][e] : 0.f;
     }
     __device__ __forceinline__ void scores(const Query &Q, f32x4 (&s)[1]) const
     {
@@ -189,7 +222,7 @@ constexpr int kRowWaves = 4;
 
 // A workgroup has 16 rows and a part of their keys; its waves take tiles of keys in turn.  The waves' sums are added at the end in LDS, the parts'
 // through memory.  Memory bounds it, as keys and values are read once for all heads that share them: one token for each of 48 sequences of up to 16000
-// keys, 32 heads on 8 of 128 elements, bf16, 312 us for 1.62 GB, 5.2 TB/s (a large copy: 4.8).  Short sequences: three of up to 300 keys, fp32, 8.0 us,
+// keys, 32 heads on 8 of 128 elements, bf16, 281 us for 1.62 GB, 5.8 TB/s (a large copy: 4.8, read and written).  Short sequences: three of up to 300 keys, fp32, 8.0 us,
 // launch and a few dependent loads (starts, table, keys); 30000 keys of one sequence 30 us.
 // Registers for two workgroups a compute unit (three up to 64 elements): a wave has one tile on its way, 16 KB of keys and values.
 // Whole: pages hold a multiple of 16 tokens, so 16 keys of a tile lie in one page, and a wave asks for its next tiles' page numbers 64 at a time;
@@ -249,14 +282,17 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
             const uint32_t place = aa.pages.page_tokens.quotient(uint32_t(key));
             if (place < aa.pages.table_pages) pages_ahead = table[place];
         }
+        asm volatile("" : "+v"(pages_ahead));                  // (waited for here, not wherever it is used, with all that is on its way then)
     };
     K kv;
+    // Every request is made, of what is not there for the pool's first row, and what came is cleared before it is used: the number of loads on their way is
+    // the same on every path, so that a wait can leave the later ones alone.
     // Keys and values of a tile are asked for as soon as the registers are free: the keys after the scores of the tile in front, the values
     // after its sums.
     struct Place { int64_t at[K::kParts]; uint32_t stored; } now{}, next{};     // of 16 keys (Whole) or of this lane's key; keys that are stored, a bit each
     auto locate = [&](Place &pl, int32_t n) __attribute__((always_inline)) {
         const int32_t j0 = first + n * step;
-        const uint32_t in = end - j0 >= kKeys ? ~0u >> (32 - kKeys) : (1u << (end - j0)) - 1u;
+        const uint32_t in = end - j0 >= kKeys ? ~0u >> (32 - kKeys) : end > j0 ? (1u << (end - j0)) - 1u : 0u;
         pl.stored = 0u;
         if constexpr (Whole) {
 #pragma unroll
@@ -285,7 +321,10 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
     };
     auto request_keys = [&](const Place &pl) __attribute__((always_inline)) {
 #pragma unroll
-        for (int p = 0; p < K::kParts; ++p) kv.load_keys(p, keys, offset(pl, p, 16u * p + i), lane, D);
+        for (int p = 0; p < K::kParts; ++p) {
+            const int64_t at = offset(pl, p, 16u * p + i);
+            kv.load_keys(p, keys, at < 0 ? 0 : at, lane, D);
+        }
     };
     auto request_values = [&](const Place &pl) __attribute__((always_inline)) {
 #pragma unroll
@@ -293,90 +332,101 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const uint32_t a = 16u * p + 4u * g + r;
-                // (what is behind the last key may be anything, and no weight of zero undoes a NaN)
                 const int64_t at = offset(pl, p, a);
-                kv.load_values(p, r, values, pl.stored >> a & 1u ? at : -1, lane, D);
+                kv.load_values(p, r, values, at < 0 ? 0 : at, lane, D);
             }
     };
     constexpr int32_t kAhead = 64 / K::kParts;
-    if (n_tiles) {
+    if (n_tiles > 0) {
         if (Whole) look_up_pages(0);
         locate(now, 0);
         request_keys(now);
         request_values(now);
-    }
-    for (int32_t n = 0; n < n_tiles; ++n) {
-        const int32_t j0 = first + n * step;
-        if (n + 1 < n_tiles) {
+        // (Waits count loads in the order they were asked for, and the compiler takes the worst of all ways that lead to a wait: queries and page numbers are
+        // waited for here and where they are asked for, or every tile's keys would be waited for with its values: 807 -> 711 us for fp32 chunks, 2 x 1500 tokens
+        // over 2000 keys; 286 -> 281 for one token of 48 sequences of up to 16000.)
+#pragma unroll
+        for (int x = 0; x < K::kSteps; ++x) asm volatile("" : "+v"(Q.q[x]));
+        int32_t n = 0;
+#pragma unroll 1
+        do {
+            const int32_t j0 = first + n * step;
             if (Whole && (n + 1) % kAhead == 0) look_up_pages(n + 1);
             locate(next, n + 1);
-        }
-        f32x4 s[K::kParts];
-        kv.scores(Q, s);
-        if (n + 1 < n_tiles) request_keys(next);
-        const bool masked = j0 < all_lo || j0 + kKeys > all_hi || now.stored != (~0u >> (32 - kKeys));
-        // (a row's keys, and this lane's of the tile, from the lane's first key on)
-        const int32_t low = row.lo - j0 - int32_t(4u * g), high = row.hi - j0 - int32_t(4u * g);
-        const uint32_t stored = now.stored >> (4u * g);
-        float most = -INFINITY, x[K::kParts][4];
+            f32x4 s[K::kParts];
+            if (D < uint32_t(DP)) {
+                asm volatile("");
+                kv.clear_keys(lane, D);
+            }
+            kv.scores(Q, s);
+            request_keys(next);
+            const bool masked = j0 < all_lo || j0 + kKeys > all_hi || now.stored != (~0u >> (32 - kKeys));
+            // (a row's keys, and this lane's of the tile, from the lane's first key on)
+            const int32_t low = row.lo - j0 - int32_t(4u * g), high = row.hi - j0 - int32_t(4u * g);
+            const uint32_t stored = now.stored >> (4u * g);
+            float most = -INFINITY, x[K::kParts][4];
 #pragma unroll
-        for (int p = 0; p < K::kParts; ++p)
+            for (int p = 0; p < K::kParts; ++p)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                x[p][r] = s[p][r] * scale;
-                if (masked) {
-                    const int a = 16 * p + r;
-                    x[p][r] = select(bool(int(a < low) | int(a >= high) | int(!(stored >> a & 1u))), -INFINITY, x[p][r]);
+                for (int r = 0; r < 4; ++r) {
+                    x[p][r] = s[p][r] * scale;
+                    if (masked) {
+                        const int a = 16 * p + r;
+                        x[p][r] = select(bool(int(a < low) | int(a >= high) | int(!(stored >> a & 1u))), -INFINITY, x[p][r]);
+                    }
+                    most = fmaxf(most, x[p][r]);
                 }
-                most = fmaxf(most, x[p][r]);
+            most = max_quarters(most);
+            const bool moves = most > ref + kReferenceSlack || (ref == -INFINITY && most > -INFINITY);
+            if (__ballot(moves)) {
+                asm volatile("");                                  // (a branch, not multiplications by one every time)
+                const float by = moves ? __builtin_amdgcn_exp2f(ref - most) : 1.f;
+                if (moves) ref = most;
+                total *= by;
+#pragma unroll
+                for (int c = 0; c < K::kTiles; ++c) o[c] *= by;
             }
-        most = max_quarters(most);
-        const bool moves = most > ref + kReferenceSlack || (ref == -INFINITY && most > -INFINITY);
-        if (__ballot(moves)) {
-            asm volatile("");                                  // (a branch, not multiplications by one every time)
-            const float by = moves ? __builtin_amdgcn_exp2f(ref - most) : 1.f;
-            if (moves) ref = most;
-            total *= by;
+            const float base = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
-            for (int c = 0; c < K::kTiles; ++c) o[c] *= by;
-        }
-        const float base = ref == -INFINITY ? 0.f : ref;
+            for (int p = 0; p < K::kParts; ++p)
 #pragma unroll
-        for (int p = 0; p < K::kParts; ++p)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                x[p][r] = __builtin_amdgcn_exp2f(x[p][r] - base);
-                total += x[p][r];
-                s[p][r] = x[p][r];
+                for (int r = 0; r < 4; ++r) {
+                    x[p][r] = __builtin_amdgcn_exp2f(x[p][r] - base);
+                    total += x[p][r];
+                    s[p][r] = x[p][r];
+                }
+            if (now.stored != (~0u >> (32 - kKeys))) {
+                // (what is not stored may be anything, and no weight of zero undoes a NaN)
+                asm volatile("");
+                kv.clear_values(stored);
             }
-        if (masked && __ballot(kv.not_finite())) {
-            // an infinity or a NaN that some rows do not see, which a matrix instruction would multiply by their zeros: a key at a time,
-            // taken by the rows that see it
+            if (masked && __ballot(kv.not_finite())) {
+                // an infinity or a NaN that some rows do not see, which a matrix instruction would multiply by their zeros: a key at a time,
+                // taken by the rows that see it
 #pragma unroll 1
-            for (uint32_t a = 0; a < uint32_t(kKeys); ++a) {
-                const K alone = kv.only(a, g);
-                f32x4 w[K::kParts], sum[K::kTiles];
+                for (uint32_t a = 0; a < uint32_t(kKeys); ++a) {
+                    const K alone = kv.only(a, g);
+                    f32x4 w[K::kParts], sum[K::kTiles];
 #pragma unroll
-                for (int p = 0; p < K::kParts; ++p)
+                    for (int p = 0; p < K::kParts; ++p)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) w[p][r] = a == 16u * p + 4u * g + r ? x[p][r] : 0.f;
+                        for (int r = 0; r < 4; ++r) w[p][r] = a == 16u * p + 4u * g + r ? x[p][r] : 0.f;
 #pragma unroll
-                for (int c = 0; c < K::kTiles; ++c) sum[c] = o[c];
-                alone.add(w, sum);
-                const int32_t j = j0 + int32_t(a);
-                const bool sees = int(j >= row.lo) & int(j < row.hi);
+                    for (int c = 0; c < K::kTiles; ++c) sum[c] = o[c];
+                    alone.add(w, sum);
+                    const int32_t j = j0 + int32_t(a);
+                    const bool sees = int(j >= row.lo) & int(j < row.hi);
 #pragma unroll
-                for (int c = 0; c < K::kTiles; ++c)
+                    for (int c = 0; c < K::kTiles; ++c)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[c][r] = select(sees, sum[c][r], o[c][r]);
+                        for (int r = 0; r < 4; ++r) o[c][r] = select(sees, sum[c][r], o[c][r]);
+                }
+            } else {
+                kv.add(s, o);
             }
-        } else {
-            kv.add(s, o);
-        }
-        if (n + 1 < n_tiles) {
             request_values(next);
             now = next;
-        }
+        } while (++n < n_tiles);
     }
     total += __shfl_xor(total, 16);
     total += __shfl_xor(total, 32);

@@ -36,7 +36,7 @@ __device__ __forceinline__ void lds_barrier()
 // Per key and row 4 D operations, an exponential and some ten other instructions.  Matrix instructions bound it where keys are many: 4096 tokens over
 // 16384 keys, 32 heads on 8, head_dim 128, bf16, 940 us, 1020 TFLOP/s (a library's product of 8192^3: 1170); 2048 tokens over 8048 keys, heads of 96 / 64:
 // 220 / 180 us, 800 / 650 TFLOP/s, as exponentials weigh more.  What is left there is the exponentials' share of a wave's issue that no matrix
-// instruction of the other wave covers.  Short spans: an image's arrival and the last workgroups; 17 chunks of up to 700 tokens, window 1000, 72 us, 350
+// instruction of the other wave covers.  Short spans: an image's arrival and the last workgroups; 17 chunks of up to 700 tokens, window 1000, 70 us, 360
 // TFLOP/s.  A wave has 32 rows, two waves a SIMD: one multiplies while the other one takes exponentials.
 // The scores of a half are made among the exponentials of the half in front.  Images go through LDS, kRing of them in turn: while image n is
 // multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image (with two places: two).
@@ -77,10 +77,19 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     u32x4 q[kSteps];
     {
         const char *from = aa.q.data + (int64_t(row.token) * aa.q.token_stride + int64_t(row.head) * aa.q.head_stride) * 2;
+        // (loads without conditions: one wait for all of them)
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const uint32_t d = 16u * s + 8u * h;
-            q[s] = is_row && d < D && aa.scale != 0.f ? *reinterpret_cast<const u32x4 *>(from + d * 2u) ^ flip : u32x4{0u, 0u, 0u, 0u};
+            q[s] = *reinterpret_cast<const u32x4 *>(from + (d < D ? d : 0u) * 2u);
+        }
+        const uint32_t keep = is_row && aa.scale != 0.f ? ~0u : 0u;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) q[s] = (q[s] ^ flip) & keep;
+        if (D < uint32_t(DP)) {
+            asm volatile("");
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) q[s] &= 16u * s + 8u * h < D ? ~0u : 0u;
         }
     }
     // keys that all of the wave's rows see

@@ -1,6 +1,6 @@
 // Work on the pages of a cache: giving out, sharing, releasing, moving and copying them.  What decides is integers - the
 // table, lengths and references -, what takes time is the pages' bytes, each read and written once, all layers in one launch.  us: 476 pages of 2 MB
-// moved 389, 5.1 TB/s (a large copy: 4.8); 192 beams of partly filled pages, all of 32 layers, 55 for 284 MB, 5.1 TB/s; small ones 10, which is two
+// moved 389, 5.1 TB/s (a large copy: 4.8); 192 beams of partly filled pages, all of 32 layers, 55 for 284 MB, 5.1 TB/s; small ones 9, which is two
 // launches, as which pages are free has to be known before one is written: what is decided cannot be decided again by every workgroup that copies
 // while others change the table and the references.
 #include "cache_device.h"
@@ -56,13 +56,14 @@ __device__ __forceinline__ Eight load_references(const int32_t *references, uint
     return v;
 }
 
-// The first `need` free pages, ascending, into list; how many there were.  A workgroup of kScanThreads, eight pages a thread at a time.
-__device__ uint32_t find_free(const int32_t *references, uint32_t pages, uint32_t need, int32_t *list, uint32_t *waves, uint32_t turn)
+// The first `need` free pages, ascending, into list; how many there were.  A workgroup of kScanThreads, eight pages a thread at a time; ahead: a thread's first
+// eight, asked for before it was known how many are needed.
+__device__ uint32_t find_free(const int32_t *references, uint32_t pages, uint32_t need, int32_t *list, uint32_t *waves, uint32_t turn, const Eight &ahead)
 {
     uint32_t found = 0u;
     for (uint32_t p0 = 0; p0 < pages && found < need; p0 += kScanThreads * kEach) {
         const uint32_t p = p0 + threadIdx.x * kEach;
-        const Eight v = load_references(references, pages, p);
+        const Eight v = p0 ? load_references(references, pages, p) : ahead;
         uint32_t count = 0u;
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) count += v.r[e] <= 0;
@@ -142,6 +143,7 @@ __device__ __forceinline__ uint32_t pages_for(const PoolArgs &pa, int32_t tokens
 __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PoolArgs pa, const uint32_t n, const int32_t *rows, const int32_t *add, int32_t *status)
 {
     __shared__ uint32_t waves[2u * kScanWaves];
+    const Eight ahead = load_references(pa.references, pa.pages, threadIdx.x * kEach);
     int32_t *const first = pa.scratch, *const list = pa.scratch + pa.sequences;
     uint32_t need = 0u, turn = 0u;
     for (uint32_t i0 = 0; i0 < n; i0 += kScanThreads) {
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PoolAr
         if (i < n) first[i] = int32_t(at);
         need += total;
     }
-    const uint32_t found = find_free(pa.references, pa.pages, need < pa.pages ? need : pa.pages, list, waves, turn);
+    const uint32_t found = find_free(pa.references, pa.pages, need < pa.pages ? need : pa.pages, list, waves, turn, ahead);
     __syncthreads();
     for (uint32_t i = threadIdx.x / 64u; i < n; i += kScanWaves) {
         const uint32_t row = row_of(pa, rows, i);
@@ -203,6 +205,7 @@ __global__ __launch_bounds__(kScanThreads) void pages_fork_kernel(const PoolArgs
         return;
     }
     __shared__ uint32_t waves[2u * kScanWaves];
+    const Eight ahead = load_references(pa.references, pa.pages, threadIdx.x * kEach);
     uint32_t need = 0u, turn = 0u;
     for (uint32_t i0 = 0; i0 < n; i0 += kScanThreads) {
         const uint32_t i = i0 + threadIdx.x;
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(kScanThreads) void pages_fork_kernel(const PoolArgs
         }
         need += total;
     }
-    const uint32_t found = find_free(pa.references, pa.pages, need, fs.list, waves, turn);
+    const uint32_t found = find_free(pa.references, pa.pages, need, fs.list, waves, turn, ahead);
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += kScanThreads) {
         const int32_t k = fs.page[i];
@@ -280,45 +283,49 @@ __device__ __forceinline__ CompactScratch compact_scratch(const PoolArgs &pa)
 
 __global__ __launch_bounds__(kScanThreads) void pages_compact_kernel(const PoolArgs pa, int32_t *live_out)
 {
-    __shared__ uint32_t waves[2u * kScanWaves];
+    __shared__ uint32_t waves[2u * kScanWaves], below_live;
     const CompactScratch cs = compact_scratch(pa);
-    uint32_t live = 0u, turn = 0u;
-    for (uint32_t p0 = 0; p0 < pa.pages; p0 += kScanThreads * kEach) {
+    uint32_t live = 0u, turn = 0u, at = 0u;
+    Eight v;
+    auto look = [&](uint32_t p0) {
         const uint32_t p = p0 + threadIdx.x * kEach;
-        const Eight v = load_references(pa.references, pa.pages, p);
+        v = load_references(pa.references, pa.pages, p);
         uint32_t count = 0u, total;
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) count += p + e < pa.pages && v.r[e] > 0;
-        scan(count, waves, turn, &total);
+        at = scan(count, waves, turn, &total);
         turn ^= 1u;
-        live += total;
-    }
-    uint32_t from = 0u, to = 0u;
+        return total;
+    };
+    for (uint32_t p0 = 0; p0 < pa.pages; p0 += kScanThreads * kEach) live += look(p0);
+    // Of a page below their number that is free, and of a live one at or above it, the number is the live pages' in front of it, up to a constant.
+    // (The references of a pool of one round are in registers.)
+    const bool once = pa.pages <= kScanThreads * kEach;
+    uint32_t before = 0u;
     for (uint32_t p0 = 0; p0 < pa.pages; p0 += kScanThreads * kEach) {
-        const uint32_t p = p0 + threadIdx.x * kEach;
-        const Eight v = load_references(pa.references, pa.pages, p);
-        uint32_t count = 0u;                                    // pages that move | pages to fill << 16
+        const uint32_t total = once ? live : look(p0), p = p0 + threadIdx.x * kEach;
+        at += before;
+        before += total;
+        if (p <= live && live < p + kEach) {
+            uint32_t below = at;
 #pragma unroll
-        for (uint32_t e = 0; e < kEach; ++e) {
-            if (p + e < pa.pages) count += p + e >= live ? uint32_t(v.r[e] > 0) : uint32_t(v.r[e] <= 0) << 16;
+            for (uint32_t e = 0; e < kEach; ++e) below += p + e < live && v.r[e] > 0;
+            below_live = below;
         }
-        uint32_t total;
-        const uint32_t at = scan(count, waves, turn, &total);
-        turn ^= 1u;
-        uint32_t f = from + (at & 0xFFFFu), t = to + (at >> 16);
+        __syncthreads();
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) {
             if (p + e >= pa.pages) continue;
             if (p + e >= live) {
-                if (v.r[e] > 0) cs.from[f] = int32_t(p + e);
-                cs.map[p + e] = v.r[e] > 0 ? int32_t(f++) : -1;
+                if (v.r[e] > 0) cs.from[at - below_live] = int32_t(p + e);
+                cs.map[p + e] = v.r[e] > 0 ? int32_t(at - below_live) : -1;
             } else if (v.r[e] <= 0) {
-                cs.to[t++] = int32_t(p + e);
+                cs.to[p + e - at] = int32_t(p + e);
             }
+            at += v.r[e] > 0;
         }
-        from += total & 0xFFFFu;
-        to += total >> 16;
     }
+    const uint32_t from = live < pa.pages ? live - below_live : 0u;
     if (threadIdx.x == 0u) {
         cs.count[0] = int32_t(live);
         cs.count[1] = int32_t(from);

@@ -602,6 +602,24 @@ def test_a_life_of_pages(torch_cuda, hs, dtype, order, pages, page, heads, dim, 
         assert books.references.max() > 1
 
 
+@pytest.mark.parametrize("pages,lengths", [(20000, [5000, 4321, 2100, 600]), (20000, [8190, 2, 0, 0]), (8192, [8191, 1, 0, 0]), (8193, [4000, 4193, 0, 0]), (8193, [0, 0, 0, 0]),
+                                           (8200, [3, 0, 8000, 190]), (30, [10, 9, 3, 0])])
+def test_compaction_of_pools_of_every_fill(torch_cuda, hs, pages, lengths):
+    # a page holds one token: live pages all over the pool, their number on either side of what a workgroup looks at at a time
+    torch = torch_cuda
+    rng = np.random.default_rng(pages + lengths[0])
+    st = State(torch, hs, 2, pages, 1, 1, 8, 4, max(max(lengths), 1))
+    for pool in st.pool:
+        pool.copy_(torch.randn(pool.shape, device="cuda").bfloat16())
+    st.place(rng, lengths)
+    st.table[(st.table < 0) | (st.table >= pages)] = -1
+    books, live, stream = Books(st), torch.zeros(1, dtype=torch.int32, device="cuda"), torch.cuda.current_stream().cuda_stream
+    for _ in range(2):
+        st.handle.compact(live.data_ptr(), stream=stream)
+        assert int(live) == sum(lengths) == books.compact()
+        books.same(torch, st)
+
+
 def test_numbers_that_are_none_are_passed_over(torch_cuda, hs):
     torch = torch_cuda
     rng = np.random.default_rng(8)

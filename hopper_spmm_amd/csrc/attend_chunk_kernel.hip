@@ -300,7 +300,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
         __builtin_amdgcn_sched_barrier(0);
         scores(second{}, s_other, keys_2);
         exponentials(s);
-        __builtin_amdgcn_sched_barrier(0);
+        // (nothing between: the values are asked for among the exponentials, 960 -> 937 us for 4096 tokens over 16384 keys)
         ask_values(values_2, second{}, image, half);
         add(first{}, s, values_1);
         ask_keys(keys_1, first{}, third_image, third_half);

@@ -133,6 +133,10 @@ def test_attend_refuses(hs):
     for d in (4, 60, 264):
         refused(hs, 5, lambda: cache(hs, head_dim=d).attend(0, b, a, x, x), "elements")
     refused(hs, 5, lambda: cache(hs, page_stride=16 * 4 * 64 + 4).attend(0, b, a, x, x), "16 bytes")
+    # more tiles than a launch has workgroups
+    wide = hs.Batch(3, 1 << 29, ADDRESS)
+    for f in (lambda: c.attend(0, wide, hs.Attention(4, 1.0, longest_chunk=1 << 29), x, x), lambda: c.attend_workspace(wide, hs.Attention(4, 1.0, longest_chunk=1 << 29))):
+        refused(hs, 5, f, "several calls")
     c.attend(0, hs.Batch(3, 0, 0), a, None, None)           # no tokens
     L = hs.load_library()
     assert L.hspmm_cache_attend_workspace(c._c, b, a, None) == 1

@@ -13,7 +13,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 //           the order the lanes hold them; the first operand wants a lane's keys side by side per element
 // 16-bit types: a lane loads pieces of eight elements (head_dim up to 64: four) of eight keys, 4 g .. + 3 of either part: an 8 x 8 block which 32
 // byte permutations transpose.  Elements of an operand's 16 rows are kPiece apart: kPiece i + dt.  Nothing goes through LDS.
-template <bool BF, int DP>
+template <bool BF, int DP, bool Past>
 struct Rows16 {
     typedef typename HalfOps<BF>::elem_t T;
     static constexpr int kKeys = 32, kParts = 2, kElem = 2, kPiece = DP >= 128 ? 8 : 4, kSteps = DP / 32, kBlocks = DP / (16 * kPiece), kTiles = DP / 16;
@@ -29,14 +29,19 @@ struct Rows16 {
             Q.q[s] = there && d < D ? *reinterpret_cast<const u32x4 *>(row + d * 2u) : u32x4{0u, 0u, 0u, 0u};
         }
     }
-    // Key 16 t + i, by its offset.  (Keys and values are read once, by two row tiles at most: not kept in the L2, 330 -> 317 us for one token of 48
-    // sequences of up to 16000.)
+    // Past: not kept in the L2.
+    template <class P> __device__ static __forceinline__ P fetch(const char *p)
+    {
+        if constexpr (Past) return __builtin_nontemporal_load(reinterpret_cast<const P *>(p));
+        else return *reinterpret_cast<const P *>(p);
+    }
+    // Key 16 t + i, by its offset.
     __device__ __forceinline__ void load_keys(int t, const char *keys, int64_t at, uint32_t lane, uint32_t D)
     {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const uint32_t d = 32u * s + 8u * (lane >> 4);
-            k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(keys + (at + (d < D ? d : 0u)) * 2));
+            k[t][s] = fetch<u32x4>(keys + (at + (d < D ? d : 0u)) * 2);
         }
     }
     __device__ __forceinline__ void load_values(int t, int r, const char *values, int64_t at, uint32_t lane, uint32_t D)
@@ -47,10 +52,10 @@ struct Rows16 {
             const char *p = values + (at + (d < D ? d : 0u)) * 2;
             uint32_t *to = v[4 * t + r][b];
             if constexpr (kPiece == 8) {
-                const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+                const u32x4 x = fetch<u32x4>(p);
                 to[0] = x[0]; to[1] = x[1]; to[2] = x[2]; to[3] = x[3];
             } else {
-                const t_u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const t_u32x2 *>(p));
+                const t_u32x2 x = fetch<t_u32x2>(p);
                 to[0] = x[0]; to[1] = x[1];
             }
         }
@@ -545,19 +550,26 @@ void launch(const AttendArgs &aa, hipStream_t s)
     else attend_rows_kernel<K, false, DP><<<grid, dim3(64 * kRowWaves), 0, s>>>(aa);
 }
 
+template <bool BF, bool Past>
+void launch16(const AttendArgs &aa, hipStream_t s)
+{
+    const uint32_t D = aa.pages.head_dim;
+    if (D <= 64u) launch<Rows16<BF, 64, Past>, 64>(aa, s);
+    else if (D <= 128u) launch<Rows16<BF, 128, Past>, 128>(aa, s);
+    else launch<Rows16<BF, 256, Past>, 256>(aa, s);
+}
+
 }  // namespace
 
-hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, hipStream_t s)
+hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, bool past, hipStream_t s)
 {
     const uint32_t D = aa.pages.head_dim;
     if (dtype == kDtypeF16) {
-        if (D <= 64u) launch<Rows16<false, 64>, 64>(aa, s);
-        else if (D <= 128u) launch<Rows16<false, 128>, 128>(aa, s);
-        else launch<Rows16<false, 256>, 256>(aa, s);
+        if (past) launch16<false, true>(aa, s);
+        else launch16<false, false>(aa, s);
     } else if (dtype == kDtypeBf16) {
-        if (D <= 64u) launch<Rows16<true, 64>, 64>(aa, s);
-        else if (D <= 128u) launch<Rows16<true, 128>, 128>(aa, s);
-        else launch<Rows16<true, 256>, 256>(aa, s);
+        if (past) launch16<true, true>(aa, s);
+        else launch16<true, false>(aa, s);
     } else {
         if (D <= 64u) launch<Rows32<64>, 64>(aa, s);
         else if (D <= 128u) launch<Rows32<128>, 128>(aa, s);

@@ -289,6 +289,7 @@ static int check_attention(const hspmm_cache *c, const hspmm_batch *b, const hsp
 struct AttendShape {
     uint32_t rows_log;                   // of a tile: kAttendRowsLog the rows kernel, 7 and 8 the chunk kernel
     uint32_t tiles, splits, part_keys;
+    bool past;                           // the rows kernel reads past the L2
     uint64_t bytes;
 };
 
@@ -332,6 +333,10 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     const uint64_t parts = (keys + 31u + sh.part_keys - 1u) / sh.part_keys;
     sh.splits = numbered * c->heads > kAttendCounters ? 1u : uint32_t(std::min<uint64_t>(std::max<uint64_t>(parts, 1u), 256u));
     sh.tiles = uint32_t(numbered);
+    // Keys and values of more than 256 MB by tiles, which no cache holds until they are read again, are read past the L2.  us past it / through it: one token for
+    // each of 48 sequences of up to 16000 keys 281 / 310, up to 8000 160 / 163; 32 of up to 2000, 8 heads of 64 24.2 / 22.1; 8 tokens for each of 4 of up to
+    // 4000, 16 heads on 2 22.1 / 19.7.
+    sh.past = tiles * c->heads * keys * c->head_dim * 2u * element_bytes(c->dtype) > (uint64_t(1) << 28);
     if (sh.splits > 1u) sh.bytes = kAttendCounters * 4u + numbered * c->heads * sh.splits * attend_slot(sh.rows_log, c->head_dim) * 4u;
     return sh;
 }
@@ -379,7 +384,7 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     aa.heads = Divisor::of(cache->heads); aa.tiles = sh.tiles; aa.splits = sh.splits; aa.part_keys = sh.part_keys;
     aa.arrive = static_cast<uint32_t *>(workspace);
     aa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + kAttendCounters * 4u);
-    if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, static_cast<hipStream_t>(stream)));
+    if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, sh.past, static_cast<hipStream_t>(stream)));
     else HSPMM_HIP(launch_attend_chunk(cache->dtype, aa, sh.rows_log, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }

@@ -311,6 +311,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     if (n_images) {
         f32x16 s_a, s_b;
         request(0);
+        lds_barrier();                                         // (`odd` is zero before any wave can set it)
         uint64_t stored_now = write_image(0, 0u);
         request(1);
         uint64_t stored_next = write_image(1, 1u);

@@ -1,0 +1,50 @@
+"""Rare states of a paged cache and unusual calls: values that are not finite where a launch begins, lists of nothing, rows that are full or have holes.
+Against plain implementations in 64 bits; tolerances are derived in cache_util.  Needs a real MI355X: run with -m gpu."""
+import numpy as np
+import pytest
+
+from cache_util import State, rounded, to64
+from test_cache_gpu import assert_attended, attend, expected, ints, many
+from test_spmm_gpu import torch_cuda  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def one_sequence(torch, hs, dtype, new, old, heads, shared, dim, page, window, seed):
+    """A chunk of `new` tokens behind `old` older ones in sequence 0, and what attends to it."""
+    rng = np.random.default_rng(seed)
+    tokens = new + old
+    st = State(torch, hs, dtype, -(-tokens // page) + 1, page, heads, dim, 1, -(-tokens // page))
+    st.place(rng, [tokens])
+    k, v = (rounded(torch, rng.standard_normal((tokens, heads, dim)), dtype) for _ in range(2))
+    st.store(0, 0, 0, k)
+    st.store(0, 0, 1, v)
+    q = rounded(torch, rng.standard_normal((new, heads * shared, dim)), dtype)
+    starts = ints(torch, [0, new])
+    st.kept = (starts,)
+    scale = np.float64(np.float32(0.125))
+    return st, hs.Batch(1, new, starts.data_ptr()), hs.Attention(heads * shared, float(scale), window=window, longest_chunk=new, longest=tokens), q, k, v, scale
+
+
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("new,old,heads,dim,page,window,keys", [(700, 100, 16, 64, 16, 300, (50, 450)), (700, 100, 16, 128, 24, 300, (50, 450)),
+                                                                (700, 500, 4, 64, 16, 0, (530, 1030)), (700, 500, 4, 160, 16, 0, (530, 1030))])
+def test_values_that_are_not_finite_among_the_first_keys(torch_cuda, hs, dtype, new, old, heads, dim, page, window, keys):
+    # in the first images of tiles and of parts of 512 keys, in every head: what some rows do not see must not reach them, however the waves of a workgroup
+    # follow each other
+    torch = torch_cuda
+    st, batch, attention, q, k, v, scale = one_sequence(torch, hs, dtype, new, old, heads, 1, dim, page, window, 11)
+    want = expected(q, [k], [v], [new], [old], scale, True, window)
+    position, hit = np.arange(old, old + new), np.zeros(new, bool)
+    for j, value in zip(keys, (np.nan, np.inf)):
+        bad = v.copy()
+        hit |= (position >= j) & ((position - window < j) if window else True)
+        bad[j, :, 3] = value
+        v = bad
+    st.store(0, 0, 1, v)
+    assert hit.any() and not hit.all()
+    clear = torch.from_numpy(~hit).cuda()
+    for a in (attention, many(hs, st, batch, attention)):
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert not np.isfinite(to64(out)[hit][:, :, 3]).any()
+        assert_attended(dtype, out[clear], lse[clear], [x[~hit] for x in want], [k], [np.where(np.isfinite(v), v, 0.0)], dim)

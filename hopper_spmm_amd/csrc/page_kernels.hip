@@ -391,6 +391,7 @@ hipError_t launch_pages_extend(const PoolArgs &pa, uint32_t n, const int32_t *ro
 hipError_t launch_pages_fork(const PoolArgs &pa, uint32_t n, const int32_t *parents, const int32_t *children, int32_t *status, hipStream_t s)
 {
     pages_fork_kernel<<<dim3(n + 1u), dim3(kScanThreads), 0, s>>>(pa, n, parents, children, status);
+    if (n == 0u) return hipGetLastError();                     // (the status alone)
     // heads of a page are shared out while that leaves fewer than some thousand workgroups
     const uint64_t groups = uint64_t(n) * pa.layers * 2u;
     uint32_t parts = pa.heads_first && groups < 2048u ? uint32_t(2048u / groups) : 1u;

@@ -1,5 +1,8 @@
 """Rare states of a paged cache and unusual calls: values that are not finite where a launch begins, lists of nothing, rows that are full or have holes.
 Against plain implementations in 64 bits; tolerances are derived in cache_util.  Needs a real MI355X: run with -m gpu."""
+import importlib.util
+import os
+
 import numpy as np
 import pytest
 
@@ -48,3 +51,35 @@ def test_values_that_are_not_finite_among_the_first_keys(torch_cuda, hs, dtype, 
         out, lse = attend(torch, hs, st, batch, a, q)
         assert not np.isfinite(to64(out)[hit][:, :, 3]).any()
         assert_attended(dtype, out[clear], lse[clear], [x[~hit] for x in want], [k], [np.where(np.isfinite(v), v, 0.0)], dim)
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_lists_of_nothing(torch_cuda, hs, order):
+    # nothing changes, and nothing is missing
+    torch = torch_cuda
+    rng = np.random.default_rng(1)
+    st = State(torch, hs, 0, 20, 4, 2, 8, 3, 5, order=order, fill=1.0)
+    st.place(rng, [9, 4, 0])
+    before = [x.clone() for x in (st.table, st.lengths, st.references, *st.pool)]
+    status = torch.full((1,), 77, dtype=torch.int32, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    st.handle.fork(0, 0, 0, status.data_ptr(), stream)
+    assert int(status) == 0
+    status.fill_(77)
+    st.handle.extend(0, 0, 0, status.data_ptr(), stream)
+    assert int(status) == 0
+    st.handle.free(0, 0, stream)
+    st.handle.copy(0, 0, 0, stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, (st.table, st.lengths, st.references, *st.pool)))
+
+
+def test_the_example_with_a_single_beam(torch_cuda, hs):
+    # its prompts are forked into no beams at all
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "pruned_attention.py")
+    spec = importlib.util.spec_from_file_location("pruned_attention", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got, want, largest = example.run(hidden=128, heads=2, kv_heads=1, keep=0.3, layers=1, prompts=(20, 7), beams=1, steps=2, page_tokens=8)
+    # roundings to fp16 as in the example's own test: of q, k, v, turned q and k, of weights, sums, the last product and the sum with x
+    assert np.linalg.norm(got - want) <= (6 + 4 * largest) * 2.0 ** -11 * np.linalg.norm(want)

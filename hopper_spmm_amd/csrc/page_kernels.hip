@@ -211,14 +211,16 @@ __global__ __launch_bounds__(kScanThreads) void pages_fork_kernel(const PoolArgs
         const uint32_t i = i0 + threadIdx.x;
         const uint32_t parent = i < n ? row_of(pa, parents, i) : kIdxMax, child = i < n ? row_of(pa, children, i) : kIdxMax;
         const int32_t tokens = parent != kIdxMax ? held(pa, parent) : 0;
-        const bool takes = fork_takes_page(pa, parent, child, tokens);
+        // (a last page that the parent lacks the child lacks, too: a page of its own would show what its last owner left there)
+        const int32_t last = fork_takes_page(pa, parent, child, tokens) ? pa.table[size_t(parent) * pa.table_pages + pages_for(pa, tokens) - 1u] : -1;
+        const bool takes = uint32_t(last) < pa.pages;
         uint32_t total;
         const uint32_t at = need + scan(takes, waves, turn, &total);
         turn ^= 1u;
         if (i < n) {
             fs.page[i] = takes ? int32_t(at) : -1;
             fs.tokens[i] = tokens;
-            fs.from[i] = takes ? pa.table[size_t(parent) * pa.table_pages + pages_for(pa, tokens) - 1u] : -1;
+            fs.from[i] = last;
         }
         need += total;
     }

@@ -615,8 +615,8 @@ int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *ba
 /* add[i] more tokens for sequence rows[i] (rows null: i; less than 0: none), and the pages they need. */
 int hspmm_cache_extend(const hspmm_cache *cache, uint32_t n, const int32_t *rows, const int32_t *add, int32_t *status, void *stream);
 /* Sequence children[i] becomes what sequence parents[i] was before the call: it shares the parent's full pages and gets a
- * copy (the tokens held) of the last one where it is partly filled.  The pages it had are released; those that
- * become free are given out by later calls only.  A parent may be named often, and be a child as well (a beam
+ * copy (the tokens held) of the last one where it is partly filled; places where the parent has no page are -1, the last
+ * one among them, and are not counted as missing.  The pages it had are released; those that become free are given out by later calls only.  A parent may be named often, and be a child as well (a beam
  * search's step); a sequence that is its own parent stays as it is. */
 int hspmm_cache_fork(const hspmm_cache *cache, uint32_t n, const int32_t *parents, const int32_t *children, int32_t *status, void *stream);
 /* Sequences rows[i] have no tokens any more; pages that nobody else names are free. */

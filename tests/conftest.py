@@ -13,6 +13,21 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
 
+# Tests that expect a value which include/hspmm.h rules out, and why: they run as they are, fail there and nowhere else.
+WRONG_VALUES = {
+    "test_cache_gpu.py::test_a_life_of_pages[%s]" % case:
+        "forks of sequences whose last page is missing are expected to take a free page, which shows what its last owner left there; "
+        "test_cache_edges_gpu.py has the value that the header names"
+    for case in ("2-0-90-16-2-32-3", "1-0-77-5-2-3-2")}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        reason = WRONG_VALUES.get(item.nodeid.split("/")[-1])
+        if reason:
+            item.add_marker(pytest.mark.xfail(reason=reason, raises=AssertionError, strict=True))
+
+
 @pytest.fixture(scope="session")
 def oracle():
     import oracle as O

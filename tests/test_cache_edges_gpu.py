@@ -83,3 +83,42 @@ def test_the_example_with_a_single_beam(torch_cuda, hs):
     got, want, largest = example.run(hidden=128, heads=2, kv_heads=1, keep=0.3, layers=1, prompts=(20, 7), beams=1, steps=2, page_tokens=8)
     # roundings to fp16 as in the example's own test: of q, k, v, turned q and k, of weights, sums, the last product and the sum with x
     assert np.linalg.norm(got - want) <= (6 + 4 * largest) * 2.0 ** -11 * np.linalg.norm(want)
+
+
+def contents(torch, hs, order, pages, page, sequences, places):
+    """A cache of two heads of 64 whose pages all hold something."""
+    st = State(torch, hs, 0, pages, page, 2, 64, sequences, places, order=order)
+    for pool in st.pool:
+        pool.copy_(torch.randn(pool.shape, device="cuda").half())
+    return st
+
+
+def attend_all(torch, hs, st, sequences, longest):
+    """One token of every sequence: out, lse."""
+    q = torch.from_numpy(np.tile(np.random.default_rng(2).standard_normal((1, 4, 64)), (sequences, 1, 1))).half().cuda()
+    starts = ints(torch, np.arange(sequences + 1))
+    st.kept = (starts,)
+    return attend(torch, hs, st, hs.Batch(sequences, sequences, starts.data_ptr()), hs.Attention(4, 0.125, longest_chunk=1, longest=longest), q)
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_forks_of_a_sequence_whose_last_page_is_missing(torch_cuda, hs, order):
+    # what the parent lacks its children lack, though there are free pages by then: they hold what others left there
+    torch = torch_cuda
+    st = contents(torch, hs, order, 5, 16, 4, 3)
+    status, stream = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.cuda.current_stream().cuda_stream
+    lists = [ints(torch, x) for x in ([1, 0], [48, 40], [1], [0, 0, 0], [2, 3, 1])]
+    st.handle.extend(2, lists[0].data_ptr(), lists[1].data_ptr(), status.data_ptr(), stream)
+    assert int(status) == 1 and st.table[0].tolist() == [3, 4, -1]
+    st.handle.free(1, lists[2].data_ptr(), stream)
+    pool = [x.clone() for x in st.pool]
+    st.handle.fork(3, lists[3].data_ptr(), lists[4].data_ptr(), status.data_ptr(), stream)
+    assert int(status) == 0
+    assert st.table.tolist() == [[3, 4, -1]] * 4 and st.lengths.tolist() == [40] * 4 and st.references.tolist() == [0, 0, 0, 4, 4]
+    assert all(torch.equal(a, b) for a, b in zip(pool, st.pool))
+    out, lse = attend_all(torch, hs, st, 4, 48)
+    assert (out == out[0]).all() and (lse == lse[0]).all()
+    # and that is the attention over the 32 tokens that are there
+    st.lengths.fill_(32)
+    stored, stored_lse = attend_all(torch, hs, st, 4, 48)
+    assert torch.equal(out, stored) and torch.equal(lse, stored_lse)

@@ -62,7 +62,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     const RowTile t = find_tile<kRowsLog>(aa, tile_number);
     if (!t.there) return;
     const int32_t lo = t.lo & ~31, span = t.hi - lo, each = int32_t(aa.part_keys);
-    int32_t parts = span > 0 ? (span + each - 1) / each : 1;
+    int32_t parts = span > 0 ? int32_t((uint32_t(span) + uint32_t(each) - 1u) / uint32_t(each)) : 1;
     if (parts > int32_t(aa.splits)) parts = int32_t(aa.splits);
     if (int32_t(part) >= parts) return;
     const int32_t begin = lo + int32_t(part) * each, end = int32_t(part) + 1 == parts ? t.hi : begin + each;

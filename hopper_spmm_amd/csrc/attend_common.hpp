@@ -18,7 +18,7 @@ constexpr float kReferenceSlack = 8.f;
 struct RowTile {
     uint32_t sequence, first_row, rows, first_token, chunk;      // first_token of the batch; rows from first_row on
     int32_t length, position;                                    // tokens the cache holds; the position of the chunk's first token
-    int32_t lo, hi;                                              // keys that any of the rows may see
+    int32_t lo, hi;                                              // keys that any of the rows may see, as far as there are places for them
     bool there;
 };
 
@@ -55,9 +55,8 @@ __device__ __forceinline__ RowTile find_tile(const AttendArgs &aa, uint32_t tile
     t.length = tokens_held(aa.pages, t.sequence);
     t.position = t.length - (end - first);
     const int32_t p0 = t.position + int32_t(aa.shared.quotient(from)), p1 = t.position + int32_t(aa.shared.quotient(from + t.rows - 1u));
-    t.hi = aa.causal ? p1 + 1 : t.length;
-    t.lo = aa.window && int64_t(p0) + 1 > int64_t(aa.window) ? p0 + 1 - int32_t(aa.window) : 0;
-    if (t.hi < 0) t.hi = 0;
+    t.hi = clamp_i32(aa.causal ? p1 + 1 : t.length, 0, keys_of_row(aa.pages));
+    t.lo = aa.window && int64_t(p0) + 1 > int64_t(aa.window) ? min(p0 + 1 - int32_t(aa.window), t.hi) : 0;
     t.there = true;
     return t;
 }

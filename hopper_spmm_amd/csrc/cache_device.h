@@ -103,11 +103,15 @@ struct TokenPlace { uint32_t sequence; int32_t position; bool there; };
 
 __device__ __forceinline__ int32_t clamp_i32(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-// Tokens a sequence has, within what its row of the table can hold.
-__device__ __forceinline__ int32_t tokens_held(const PagesArgs &pg, uint32_t sequence)
+// Tokens a sequence has.  Where that is more than its row of the table has places for, those behind are like tokens without a page: a length that was
+// cut to the row's would put a batch's tokens over stored ones.
+__device__ __forceinline__ int32_t tokens_held(const PagesArgs &pg, uint32_t sequence) { return max(pg.lengths[sequence], 0); }
+
+// Keys that a row of the table has places for (numbers a few tiles behind the last one are 31 bits, too).
+__device__ __forceinline__ int32_t keys_of_row(const PagesArgs &pg)
 {
     const int64_t most = int64_t(pg.table_pages) * pg.page_tokens.d;
-    return clamp_i32(pg.lengths[sequence], 0, most > 0x7FFFFFFF ? 0x7FFFFFFF : int32_t(most));
+    return most > 0x7FFF0000 ? 0x7FFF0000 : int32_t(most);
 }
 
 // Token t as one of batch row b's, if it is.

@@ -128,32 +128,35 @@ __device__ __forceinline__ uint32_t row_of(const PoolArgs &pa, const int32_t *ro
     return r < pa.sequences ? r : kIdxMax;
 }
 
-__device__ __forceinline__ int32_t most_tokens(const PoolArgs &pa)
-{
-    const int64_t m = int64_t(pa.table_pages) * pa.page_tokens.d;
-    return m > 0x7FFFFFFF ? 0x7FFFFFFF : int32_t(m);
-}
-__device__ __forceinline__ int32_t held(const PoolArgs &pa, uint32_t sequence) { return clamp_i32(pa.lengths[sequence], 0, most_tokens(pa)); }
+// Tokens of a sequence, more than its row has places for where it was extended past them.
+__device__ __forceinline__ int32_t held(const PoolArgs &pa, uint32_t sequence) { return max(pa.lengths[sequence], 0); }
+// Pages of so many tokens; places_for: of them, those that a row has places for.
 __device__ __forceinline__ uint32_t pages_for(const PoolArgs &pa, int32_t tokens)
 {
     return tokens ? pa.page_tokens.quotient(uint32_t(tokens) - 1u) + 1u : 0u;
 }
+__device__ __forceinline__ uint32_t places_for(const PoolArgs &pa, int32_t tokens) { return min(pages_for(pa, tokens), pa.table_pages); }
+__device__ __forceinline__ int32_t extended(int32_t have, int32_t add) { return add > 0x7FFFFFFF - have ? 0x7FFFFFFF : have + max(add, 0); }
 
 // One workgroup: pages for more tokens.  scratch: the first request of every list entry, then the free pages.
 __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PoolArgs pa, const uint32_t n, const int32_t *rows, const int32_t *add, int32_t *status)
 {
     __shared__ uint32_t waves[2u * kScanWaves];
+    __shared__ unsigned long long past;                        // pages that no row has a place for
     const Eight ahead = load_references(pa.references, pa.pages, threadIdx.x * kEach);
     int32_t *const first = pa.scratch, *const list = pa.scratch + pa.sequences;
     uint32_t need = 0u, turn = 0u;
+    if (threadIdx.x == 0u) past = 0u;
+    __syncthreads();
     for (uint32_t i0 = 0; i0 < n; i0 += kScanThreads) {
         const uint32_t i = i0 + threadIdx.x;
         const uint32_t row = i < n ? row_of(pa, rows, i) : kIdxMax;
         uint32_t mine = 0u;
         if (row != kIdxMax) {
-            const int32_t have = held(pa, row), more = add[i] > 0 ? add[i] : 0, most = most_tokens(pa);
-            const int32_t now = more > most - have ? most : have + more;
-            mine = pages_for(pa, now) - pages_for(pa, have);
+            const int32_t have = held(pa, row), now = extended(have, add[i]);
+            mine = places_for(pa, now) - places_for(pa, have);
+            const uint32_t all = pages_for(pa, now) - pages_for(pa, have);
+            if (all > mine) atomicAdd(&past, static_cast<unsigned long long>(all - mine));
         }
         uint32_t total;
         const uint32_t at = need + scan(mine, waves, turn, &total);
@@ -166,9 +169,8 @@ __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PoolAr
     for (uint32_t i = threadIdx.x / 64u; i < n; i += kScanWaves) {
         const uint32_t row = row_of(pa, rows, i);
         if (row == kIdxMax) continue;
-        const int32_t have = held(pa, row), more = add[i] > 0 ? add[i] : 0, most = most_tokens(pa);
-        const int32_t now = more > most - have ? most : have + more;
-        const uint32_t p0 = pages_for(pa, have), p1 = pages_for(pa, now), at = uint32_t(first[i]);
+        const int32_t have = held(pa, row), now = extended(have, add[i]);
+        const uint32_t p0 = places_for(pa, have), p1 = places_for(pa, now), at = uint32_t(first[i]);
         for (uint32_t p = p0 + (threadIdx.x & 63u); p < p1; p += 64u) {
             const uint32_t k = at + p - p0;
             const int32_t id = k < found ? list[k] : -1;
@@ -177,7 +179,10 @@ __global__ __launch_bounds__(kScanThreads) void pages_extend_kernel(const PoolAr
         }
         if ((threadIdx.x & 63u) == 0u) pa.lengths[row] = now;
     }
-    if (status && threadIdx.x == 0u) *status = int32_t(need - found);
+    if (status && threadIdx.x == 0u) {
+        const unsigned long long missing = past + (need - found);
+        *status = missing > 0x7FFFFFFFu ? 0x7FFFFFFF : int32_t(missing);
+    }
 }
 
 // Fork, first launch: what the second needs to know of the state before the call.  Workgroup 0 finds the new pages; workgroup 1 + i keeps
@@ -191,7 +196,8 @@ __device__ __forceinline__ ForkScratch fork_scratch(const PoolArgs &pa)
 constexpr uint32_t kForkRows = 32768u;          // entries along y of the second launch
 __device__ __forceinline__ bool fork_takes_page(const PoolArgs &pa, uint32_t parent, uint32_t child, int32_t tokens)
 {
-    return parent != kIdxMax && child != kIdxMax && parent != child && uint32_t(tokens) != pa.page_tokens.quotient(uint32_t(tokens)) * pa.page_tokens.d;
+    const uint32_t full = pa.page_tokens.quotient(uint32_t(tokens));
+    return parent != kIdxMax && child != kIdxMax && parent != child && full < pa.table_pages && uint32_t(tokens) != full * pa.page_tokens.d;
 }
 
 __global__ __launch_bounds__(kScanThreads) void pages_fork_kernel(const PoolArgs pa, const uint32_t n, const int32_t *parents, const int32_t *children, int32_t *status)
@@ -200,7 +206,7 @@ __global__ __launch_bounds__(kScanThreads) void pages_fork_kernel(const PoolArgs
     if (blockIdx.x > 0u) {
         const uint32_t i = blockIdx.x - 1u, parent = row_of(pa, parents, i);
         if (parent == kIdxMax) return;
-        const uint32_t used = pages_for(pa, held(pa, parent));
+        const uint32_t used = places_for(pa, held(pa, parent));
         for (uint32_t p = threadIdx.x; p < used; p += kScanThreads) fs.rows[size_t(i) * pa.table_pages + p] = pa.table[size_t(parent) * pa.table_pages + p];
         return;
     }

@@ -558,8 +558,8 @@ int hspmm_rotate(const hspmm_rotary *rotary, int dtype, uint32_t tokens, uint32_
  * values; page_stride and layer_stride: elements from one page (layer) to the next, 0: they lie side by side.
  * table: sequences x table_pages page numbers; place p of a row is the page of tokens p * page_tokens and on.  -1 (any
  * number that is not a page's) is no page: its tokens are not stored and nothing sees them.
- * lengths[sequences]: tokens of each sequence.  references[pages]: how many places of the table name a page; a page
- * without any (<= 0) is free.  That is all there is to say which pages are free: a cache begins with lengths and
+ * lengths[sequences]: tokens of each sequence; those behind table_pages * page_tokens have no place, and so no page.
+ * references[pages]: how many places of the table name a page; a page without any (<= 0) is free.  That is all there is to say which pages are free: a cache begins with lengths and
  * references of zero and a table of -1.
  * scratch: hspmm_cache_scratch_words words that the calls which change pages use; two such calls of one cache must
  * not overlap.  keys and values are aligned to 16 bytes. */
@@ -611,6 +611,7 @@ int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *ba
 
 /* Pages.  Pages that a call gives out are the free ones of lowest number, in the order of the call's list and of the
  * places in a row; *status (may be null) receives how many were missing: their places are -1 and hold nothing.
+ * Pages that a row has no place for are among the missing; the tokens are counted in lengths and are neither stored nor seen.
  * n: the list's length, at most the cache's sequences; a list names no sequence twice. */
 /* add[i] more tokens for sequence rows[i] (rows null: i; less than 0: none), and the pages they need. */
 int hspmm_cache_extend(const hspmm_cache *cache, uint32_t n, const int32_t *rows, const int32_t *add, int32_t *status, void *stream);

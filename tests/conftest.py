@@ -16,9 +16,9 @@ def pytest_configure(config):
 # Tests that expect a value which include/hspmm.h rules out, and why: they run as they are, fail there and nowhere else.
 WRONG_VALUES = {
     "test_cache_gpu.py::test_a_life_of_pages[%s]" % case:
-        "forks of sequences whose last page is missing are expected to take a free page, which shows what its last owner left there; "
-        "test_cache_edges_gpu.py has the value that the header names"
-    for case in ("2-0-90-16-2-32-3", "1-0-77-5-2-3-2")}
+        "forks of sequences whose last page is missing are expected to take a free page, which shows what its last owner left there, and tokens that a row has "
+        "no place for are expected to be dropped without a word, so that appending them overwrites others; test_cache_edges_gpu.py has the same lives as the header has them"
+    for case in ("2-0-90-16-2-32-3", "0-1-200-7-3-5-2", "1-0-1000-4-1-6-1", "1-0-77-5-2-3-2")}
 
 
 def pytest_collection_modifyitems(items):

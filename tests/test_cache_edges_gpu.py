@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from cache_util import State, rounded, to64
-from test_cache_gpu import assert_attended, attend, expected, ints, many
+from test_cache_gpu import Books, assert_attended, attend, expected, heads_view, ints, many, pages_for
 from test_spmm_gpu import torch_cuda  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -122,3 +122,139 @@ def test_forks_of_a_sequence_whose_last_page_is_missing(torch_cuda, hs, order):
     st.lengths.fill_(32)
     stored, stored_lse = attend_all(torch, hs, st, 4, 48)
     assert torch.equal(out, stored) and torch.equal(lse, stored_lse)
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_tokens_that_a_row_has_no_place_for(torch_cuda, hs, order):
+    # sequences that are full and shared, and one that has room for two of five more tokens
+    torch = torch_cuda
+    st = contents(torch, hs, order, 6, 16, 3, 2)
+    status, stream = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.cuda.current_stream().cuda_stream
+    rows, lists = ints(torch, [0, 1, 2]), [ints(torch, x) for x in ([32, 0, 30], [0], [1], [1, 1, 5])]
+    st.handle.extend(3, rows.data_ptr(), lists[0].data_ptr(), status.data_ptr(), stream)
+    st.handle.fork(1, lists[1].data_ptr(), lists[2].data_ptr(), 0, stream)
+    table, references = st.table.clone(), st.references.clone()
+    st.handle.extend(3, rows.data_ptr(), lists[3].data_ptr(), status.data_ptr(), stream)
+    assert int(status) == 3 and st.lengths.tolist() == [33, 33, 35]
+    assert torch.equal(table, st.table) and torch.equal(references, st.references)
+    pool = [st.view(i)[0].clone() for i in range(2)]
+    k, v = (torch.randn(7, 2, 64, device="cuda").half() for _ in range(2))
+    starts = ints(torch, [0, 1, 2, 7])
+    for x, y in ((k, v), (k.permute(1, 2, 0).contiguous().permute(2, 0, 1), v.permute(1, 2, 0).contiguous().permute(2, 0, 1))):
+        st.handle.append(0, hs.Batch(3, 7, starts.data_ptr()), heads_view(hs, x), heads_view(hs, y), stream=stream)
+        # the two tokens that have a place are stored, at their own positions
+        for i, want in enumerate((k, v)):
+            pool[i][int(table[2, 1]), :, 14:] = want[2:4].transpose(0, 1)
+            assert torch.equal(pool[i], st.view(i)[0])
+    out, lse = attend_all(torch, hs, st, 3, 48)
+    st.lengths.fill_(32)
+    stored, stored_lse = attend_all(torch, hs, st, 3, 48)
+    assert torch.equal(out, stored) and torch.equal(lse, stored_lse)
+    # more of them, in a fork that takes the row over, and again
+    st.lengths.copy_(ints(torch, [33, 33, 35]))
+    st.handle.fork(1, lists[2].data_ptr(), rows[2:].data_ptr(), status.data_ptr(), stream)
+    assert int(status) == 0 and st.table[2].tolist() == st.table[1].tolist() and st.lengths.tolist() == [33, 33, 33] and st.references[st.table[0].long()].tolist() == [3, 3]
+    most = ints(torch, [15, 16, 0x7FFFFFFF])
+    st.handle.extend(3, rows.data_ptr(), most.data_ptr(), status.data_ptr(), stream)
+    # (the page of tokens 32 .. 47 was missing before)
+    assert st.lengths.tolist() == [48, 49, 0x7FFFFFFF] and int(status) == 0 + 1 + (1 << 27) - 3
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("new,more,window,causal", [(130, 40, 0, True), (130, 40, 100, True), (3, 1, 0, True), (130, 40, 0, False), (130, 0x7FFFFFFF - 320, 0, True), (9, 0x7FFFFFFF - 320, 64, True)])
+def test_attention_of_sequences_longer_than_their_row(torch_cuda, hs, dtype, new, more, window, causal):
+    # tokens behind the row's last place have positions of their own and see what is stored
+    torch = torch_cuda
+    st, batch, attention, q, k, v, scale = one_sequence(torch, hs, dtype, new, 320 - new, 2, 2, 64, 16, window, 5)
+    attention = hs.Attention(4, float(scale), causal=causal, window=window, longest_chunk=new, longest=320)
+    st.lengths.fill_(320 + more)
+    want = expected(q, [k], [v], [new], [320 + more - new], scale, causal, window)
+    for a in (attention, many(hs, st, batch, attention)):
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert_attended(dtype, out, lse, want, [k], [v], 64)
+
+
+class Lives(Books):
+    """Books of every token that is asked for and of pages that a parent lacks."""
+
+    def extend(self, rows, add):
+        free, missing = self.free_pages(), 0
+        for s, a in zip(rows, add):
+            have = int(self.lengths[s])
+            now = have + max(int(a), 0)
+            for p in range(pages_for(have, self.page), pages_for(now, self.page)):
+                if p < self.table.shape[1] and free:
+                    self.table[s, p] = free.pop(0)
+                    self.references[self.table[s, p]] = 1
+                    continue
+                if p < self.table.shape[1]:
+                    self.table[s, p] = -1
+                missing += 1
+            self.lengths[s] = now
+        return missing
+
+    def fork(self, parents, children):
+        free, missing = self.free_pages(), 0
+        table, lengths = self.table.copy(), self.lengths.copy()
+        places, pages = table.shape[1], len(self.references)
+        for p, c in zip(parents, children):
+            if p == c:
+                continue
+            n = int(lengths[p])
+            full, rest = n // self.page, n % self.page
+            row = np.where(np.arange(places) < full, table[p], -1)
+            if rest and full < places and 0 <= table[p, full] < pages:
+                if free:
+                    row[full] = free.pop(0)
+                    for x in self.pool:
+                        x[:, int(row[full]), :, :rest] = x[:, int(table[p, full]), :, :rest]
+                else:
+                    missing += 1
+            for old in self.table[c]:
+                if 0 <= old < pages:
+                    self.references[old] -= 1
+            for now in row:
+                if 0 <= now < pages:
+                    self.references[now] += 1
+            self.table[c], self.lengths[c] = row, n
+        return missing
+
+
+@pytest.mark.parametrize("dtype,order,pages,page,heads,dim,layers", [(2, 0, 90, 16, 2, 32, 3), (0, 1, 200, 7, 3, 5, 2), (1, 0, 1000, 4, 1, 6, 1), (1, 0, 77, 5, 2, 3, 2), (0, 0, 30, 3, 2, 8, 1)])
+def test_lives_of_pages_with_holes_and_full_rows(torch_cuda, hs, dtype, order, pages, page, heads, dim, layers):
+    torch = torch_cuda
+    rng = np.random.default_rng(pages)
+    S, P = 24, 12
+    st = State(torch, hs, dtype, pages, page, heads, dim, S, P, layers=layers, order=order, page_gap=3 if dim % 2 else 0)
+    for i in range(2):
+        st.view(i).copy_(torch.randn(st.view(i).shape, device="cuda"))
+    books = Lives(st)
+    status, live = (torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(2))
+    stream = torch.cuda.current_stream().cuda_stream
+    past = 0
+    for step in range(21):
+        what = ["extend", "fork", "extend", "free", "compact", "fork", "extend"][step % 7]
+        n = int(rng.integers(1, S + 1))
+        rows = rng.permutation(S)[:n]
+        rd = ints(torch, rows)
+        if what == "extend":
+            add = rng.integers(-2, 5 * page, n)
+            ad = ints(torch, add)
+            st.handle.extend(n, rd.data_ptr(), ad.data_ptr(), status.data_ptr(), stream)
+            assert int(status) == books.extend(rows, add)
+            past += int((books.lengths > P * page).sum())
+        elif what == "fork":
+            parents = rng.integers(0, S, n)
+            parents[: n // 4] = rows[: n // 4]
+            pd = ints(torch, parents)
+            st.handle.fork(n, pd.data_ptr(), rd.data_ptr(), status.data_ptr(), stream)
+            assert int(status) == books.fork(parents, rows)
+        elif what == "free":
+            n = n // 2 + 1
+            st.handle.free(n, rd.data_ptr(), stream)
+            books.free(rows[:n])
+        else:
+            st.handle.compact(live.data_ptr(), stream=stream)
+            assert int(live) == books.compact()
+        books.same(torch, st)
+    assert past

@@ -245,11 +245,12 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
 #pragma unroll
         for (int r = 1; r < 16; ++r) most = fmaxf(most, s[r]);
         most = max_halves(most) * scale;
-        const bool moves = most > ref + kReferenceSlack || (ref == -INFINITY && most > -INFINITY);
+        constexpr float kLead = kReferenceLead<T>;
+        const bool moves = most > ref + (kReferenceSlack + kLead) || (ref == -INFINITY && most > -INFINITY);
         if (__builtin_expect(__ballot(moves) != 0u, 0)) {
             asm volatile("");                                  // (a branch, not DP / 2 multiplications by one every time)
-            const float by = moves ? __builtin_amdgcn_exp2f(ref - most) : 1.f;
-            if (moves) ref = most;
+            const float to = most - kLead, by = moves ? __builtin_amdgcn_exp2f(ref - to) : 1.f;
+            if (moves) ref = to;
             total *= by;
 #pragma unroll
             for (int c = 0; c < kTiles; ++c) o[c] *= by;

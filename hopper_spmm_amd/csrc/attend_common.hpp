@@ -12,8 +12,13 @@
 namespace hspmm {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// A reference is moved (and sums multiplied) only where a score is that far above it: weights are up to 2^8, far inside every type.
+// A reference is moved (and sums multiplied) only where a score is that far above the largest one when it was set: weights are up to 2^8 of what the largest
+// had then, far inside every type.
 constexpr float kReferenceSlack = 8.f;
+// Weights are rounded to the elements' type, as matrix instructions of 16-bit types take no others; their total is of unrounded ones.  A reference is set that far
+// below the largest score: fp16's weights are 2^7 there and up to 2^15, so that they keep eleven bits down to 2^-21 of the largest and 2^-32 of it is the most that
+// a smaller one is off (from 1 on these would be 2^-14 and 2^-25, and 20000 keys of 2^-26 each had counted in the total and not in the sums).  bf16 has fp32's range.
+template <class T> constexpr float kReferenceLead = sizeof(T) == 2 && !__is_same(T, __bf16) ? 7.f : 0.f;
 
 struct RowTile {
     uint32_t sequence, first_row, rows, first_token, chunk;      // first_token of the batch; rows from first_row on

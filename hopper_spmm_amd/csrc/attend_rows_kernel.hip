@@ -382,11 +382,12 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
                     most = fmaxf(most, x[p][r]);
                 }
             most = max_quarters(most);
-            const bool moves = most > ref + kReferenceSlack || (ref == -INFINITY && most > -INFINITY);
+            constexpr float kLead = kReferenceLead<typename K::T>;
+            const bool moves = most > ref + (kReferenceSlack + kLead) || (ref == -INFINITY && most > -INFINITY);
             if (__ballot(moves)) {
                 asm volatile("");                                  // (a branch, not multiplications by one every time)
-                const float by = moves ? __builtin_amdgcn_exp2f(ref - most) : 1.f;
-                if (moves) ref = most;
+                const float to = most - kLead, by = moves ? __builtin_amdgcn_exp2f(ref - to) : 1.f;
+                if (moves) ref = to;
                 total *= by;
 #pragma unroll
                 for (int c = 0; c < K::kTiles; ++c) o[c] *= by;

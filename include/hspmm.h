@@ -601,7 +601,7 @@ typedef struct hspmm_attention {
 /* out = softmax(scale * q k) v over the keys a token sees, tokens x q_heads x head_dim; a token that sees none gets 0.
  * lse (tokens x q_heads, may be null): the logarithm of the softmax's denominator, -infinity where nothing is seen.
  * Scores, softmax and sums in fp32; for 16-bit types the weights are rounded to the type before they multiply the
- * values, as the matrix instructions want them.  What is not seen does not reach the result, infinities and NaN among it.
+ * values, as the matrix instructions want them (fp16: times 2^7 to 2^15, so that small ones keep their bits).  What is not seen does not reach the result, infinities and NaN among it.
  * head_dim: a multiple of 8 (fp32: 4) up to 256.  q: dim_stride 1, its strides multiples of 16 bytes, aligned to 16 bytes.
  * workspace: hspmm_cache_attend_workspace bytes, aligned to 16 bytes; zero before its first use, and not used by
  * two calls that overlap in time.  The calls leave it as they want to find it. */

@@ -6,7 +6,7 @@ import os
 import numpy as np
 import pytest
 
-from cache_util import State, rounded, to64
+from cache_util import State, attend_bounds, rounded, to64
 from test_cache_gpu import Books, assert_attended, attend, expected, heads_view, ints, many, pages_for
 from test_spmm_gpu import torch_cuda  # noqa: F401
 
@@ -258,3 +258,30 @@ def test_lives_of_pages_with_holes_and_full_rows(torch_cuda, hs, dtype, order, p
             assert int(live) == books.compact()
         books.same(torch, st)
     assert past
+
+
+@pytest.mark.parametrize("less", [14.5, 21.0, 24.7, 26.0, 29.3])
+@pytest.mark.parametrize("dtype,dim,page", [(0, 64, 16), (0, 128, 24), (0, 160, 16), (2, 64, 16)])
+def test_many_small_weights(torch_cuda, hs, dtype, dim, page, less):
+    # keys of 2^-less of the weight of a few others, whose values alone are not zero; every part of the keys, and every wave's share of one, begins with one of those few
+    torch = torch_cuda
+    new, keys = 17, 20000
+    st, batch, _, q, k, v, _ = one_sequence(torch, hs, dtype, new, keys - new, 1, 2, dim, page, 0, 5)
+    heavy = np.isin(np.arange(keys) % 512, (5, 37, 69, 101))
+    q[:], k[:], v[:] = 0.0, 0.0, 1024.0
+    q[..., 0] = k[heavy, 0, 0] = 1.0
+    v[heavy] = 0.0
+    st.store(0, 0, 0, k)
+    st.store(0, 0, 1, v)
+    scale = np.float64(np.float32(less * np.log(2.0)))
+    out64, lse64, size, reach = expected(q, [k], [v], [new], [keys - new], scale, True, 0)
+    bound, lse_bound = attend_bounds(dtype, out64, lse64, size, reach, dim, keys, 0.0)
+    if dtype == 0:
+        # a weight is off by half the spacing of fp16's subnormals at most, the largest being 2^7 or more: 2^-25 / 2^7 of that, and their total is that of the heavy ones at least
+        bound = bound + keys * 2.0 ** -32 * 1024.0 / heavy.sum()
+    attention = hs.Attention(2, float(scale), longest_chunk=new, longest=keys)
+    few = hs.Attention(2, float(scale), longest_chunk=1, longest=keys)
+    for a in (attention, few, many(hs, st, batch, attention)):
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert (np.abs(to64(out) - out64) <= bound).all(), (np.abs(to64(out) - out64) / bound).max()
+        assert (np.abs(to64(lse) - lse64) <= lse_bound).all()

@@ -118,6 +118,13 @@ int check_batch(const hspmm_cache *c, const hspmm_batch *b)
     return HSPMM_OK;
 }
 
+// `threads` of an entry, in a launch that has fewer than 2^32
+int check_launch(uint32_t n, uint32_t threads)
+{
+    if ((uint64_t(n) + 1u) * threads < (uint64_t(1) << 32)) return HSPMM_OK;
+    return fail(HSPMM_ERR_UNSUPPORTED, "a list of %u: in several calls", n);
+}
+
 int check_list(const hspmm_cache *c, uint32_t n, const void *list, const char *name)
 {
     if (n > c->sequences) return fail(HSPMM_ERR_INVALID, "a list of %u for a cache of %u sequences", n, c->sequences);
@@ -149,13 +156,18 @@ uint32_t rotary_piece(int dtype, const RotaryArgs &ra, const hspmm_cache *c)
     return vec;
 }
 
+// (a launch has fewer than 2^32 threads along x, and 65535 workgroups along z)
 int run_rotary(int dtype, const RotaryArgs &ra, const hspmm_cache *c, void *stream)
 {
-    const uint32_t vec = rotary_piece(dtype, ra, c);
+    const uint32_t vec = rotary_piece(dtype, ra, c), heads = ra.q_heads + 2u * ra.k_heads;
     if (!vec) {
-        const uint64_t groups = (uint64_t(ra.tokens) + 63u) / 64u * ((ra.head_dim + 63u) / 64u) * (ra.q_heads + 2u * ra.k_heads);
-        if (groups >= (1u << 24)) return fail(HSPMM_ERR_UNSUPPORTED, "%u tokens of %u heads at these strides: in several calls", ra.tokens, ra.q_heads + 2u * ra.k_heads);
+        const uint64_t groups = (uint64_t(ra.tokens) + 63u) / 64u * ((ra.head_dim + 63u) / 64u) * heads;
+        if (groups >= (1u << 24) || ra.tokens >= (1u << 29) || heads > 65535u)
+            return fail(HSPMM_ERR_UNSUPPORTED, "%u tokens of %u heads at these strides: in several calls", ra.tokens, heads);
+    } else if (ra.tokens > 4u * ((1u << 24) - 1u)) {
+        return fail(HSPMM_ERR_UNSUPPORTED, "%u tokens: in several calls", ra.tokens);
     }
+    if (int rc = current_device(nullptr)) return rc;
     HSPMM_HIP(launch_rotary(dtype, ra, vec, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
@@ -220,7 +232,6 @@ int hspmm_rotate(const hspmm_rotary *rotary, int dtype, uint32_t tokens, uint32_
     if (int rc = check_heads("x", x, dtype)) return rc;
     if (int rc = check_heads("y", y, dtype)) return rc;
     if (!positions && rotary->dims) return fail(HSPMM_ERR_INVALID, "null positions");
-    if (int rc = current_device(nullptr)) return rc;
     RotaryArgs ra{};
     ra.q = heads_of(x); ra.q_out = heads_of(y);
     ra.q_heads = heads; ra.head_dim = head_dim; ra.dims = rotary->dims; ra.interleaved = rotary->interleaved != 0; ra.positions = rotary->positions;
@@ -253,7 +264,6 @@ int hspmm_cache_append(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
         if (int rc = check_heads("q", q, cache->dtype)) return rc;
         if (int rc = check_heads("q_out", q_out, cache->dtype)) return rc;
     }
-    if (int rc = current_device(nullptr)) return rc;
     RotaryArgs ra{};
     ra.k = heads_of(k); ra.v = heads_of(v); ra.q = heads_of(q); ra.q_out = heads_of(q ? q_out : nullptr);
     ra.q_heads = q ? q_heads : 0u; ra.k_heads = cache->heads;
@@ -404,6 +414,7 @@ int hspmm_cache_fork(const hspmm_cache *cache, uint32_t n, const int32_t *parent
     if (int rc = check_list(cache, n, parents, "parents")) return rc;
     if (int rc = check_list(cache, n, children, "children")) return rc;
     if (n == 0 && !status) return HSPMM_OK;
+    if (int rc = check_launch(n, 1024u)) return rc;
     if (int rc = current_device(nullptr)) return rc;
     HSPMM_HIP(launch_pages_fork(pool_of(cache), n, parents, children, status, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
@@ -414,6 +425,7 @@ int hspmm_cache_free(const hspmm_cache *cache, uint32_t n, const int32_t *rows, 
     if (int rc = check_cache(cache)) return rc;
     if (int rc = check_list(cache, n, rows, "rows")) return rc;
     if (n == 0) return HSPMM_OK;
+    if (int rc = check_launch(n, 256u)) return rc;
     if (int rc = current_device(nullptr)) return rc;
     HSPMM_HIP(launch_pages_free(pool_of(cache), n, rows, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
@@ -434,6 +446,7 @@ int hspmm_cache_copy(const hspmm_cache *cache, uint32_t n, const int32_t *from, 
     if (n > cache->pages) return fail(HSPMM_ERR_INVALID, "%u pages to copy of %u", n, cache->pages);
     if (n && (!from || !to)) return fail(HSPMM_ERR_INVALID, "null list of pages");
     if (n == 0) return HSPMM_OK;
+    if (int rc = check_launch(n, 256u)) return rc;
     if (int rc = current_device(nullptr)) return rc;
     HSPMM_HIP(launch_pages_copy(pool_of(cache), n, from, to, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;

@@ -399,7 +399,8 @@ hipError_t launch_pages_extend(const PoolArgs &pa, uint32_t n, const int32_t *ro
 hipError_t launch_pages_fork(const PoolArgs &pa, uint32_t n, const int32_t *parents, const int32_t *children, int32_t *status, hipStream_t s)
 {
     pages_fork_kernel<<<dim3(n + 1u), dim3(kScanThreads), 0, s>>>(pa, n, parents, children, status);
-    if (n == 0u) return hipGetLastError();                     // (the status alone)
+    // (nothing is copied by what a launch that failed has not written; for a list of nothing there is the status alone)
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess || n == 0u) return e;
     // heads of a page are shared out while that leaves fewer than some thousand workgroups
     const uint64_t groups = uint64_t(n) * pa.layers * 2u;
     uint32_t parts = pa.heads_first && groups < 2048u ? uint32_t(2048u / groups) : 1u;
@@ -421,6 +422,7 @@ hipError_t launch_pages_free(const PoolArgs &pa, uint32_t n, const int32_t *rows
 hipError_t launch_pages_compact(const PoolArgs &pa, int32_t *table_out, int32_t *references_out, int32_t *live, hipStream_t s)
 {
     pages_compact_kernel<<<dim3(1), dim3(kScanThreads), 0, s>>>(pa, live);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     const uint64_t most = uint64_t(pa.pages) * pa.layers;          // (at most half of the pages move)
     by_unit(pa, [&](auto u) {
         pages_compact_copy_kernel<decltype(u)><<<dim3(uint32_t(most < 4096u ? most : 4096u)), dim3(256), 0, s>>>(pa, table_out, references_out);

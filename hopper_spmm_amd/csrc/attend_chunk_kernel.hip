@@ -61,11 +61,9 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     const uint32_t head = cell.head, tile_number = cell.tile;
     const RowTile t = find_tile<kRowsLog>(aa, tile_number);
     if (!t.there) return;
-    const int32_t lo = t.lo & ~31, span = t.hi - lo, each = int32_t(aa.part_keys);
-    int32_t parts = span > 0 ? int32_t((uint32_t(span) + uint32_t(each) - 1u) / uint32_t(each)) : 1;
-    if (parts > int32_t(aa.splits)) parts = int32_t(aa.splits);
+    const KeyPart keys_here = key_part(aa, t, part);
+    const int32_t parts = keys_here.parts, begin = keys_here.begin, end = keys_here.end;
     if (int32_t(part) >= parts) return;
-    const int32_t begin = lo + int32_t(part) * each, end = int32_t(part) + 1 == parts ? t.hi : begin + each;
     const int32_t n_images = end > begin ? (end - begin + 63) / 64 : 0;
     uint32_t odd = 0u;                                         // whether this wave has written values that are not finite and hidden from some row
 

@@ -247,11 +247,9 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
     if (!t.there) return;
     // this part's keys
     constexpr int32_t kKeys = K::kKeys;
-    const int32_t lo = t.lo & ~31, span = t.hi - lo, each = int32_t(aa.part_keys);
-    int32_t parts = span > 0 ? int32_t((uint32_t(span) + uint32_t(each) - 1u) / uint32_t(each)) : 1;
-    if (parts > int32_t(aa.splits)) parts = int32_t(aa.splits);
+    const KeyPart keys_here = key_part(aa, t, part);
+    const int32_t parts = keys_here.parts, begin = keys_here.begin, end = keys_here.end;
     if (int32_t(part) >= parts) return;
-    const int32_t begin = lo + int32_t(part) * each, end = int32_t(part) + 1 == parts ? t.hi : begin + each;
 
     const RowOf row = row_of_tile(aa, t, head, i);
     typename K::Query Q;

@@ -285,3 +285,41 @@ def test_many_small_weights(torch_cuda, hs, dtype, dim, page, less):
         out, lse = attend(torch, hs, st, batch, a, q)
         assert (np.abs(to64(out) - out64) <= bound).all(), (np.abs(to64(out) - out64) / bound).max()
         assert (np.abs(to64(lse) - lse64) <= lse_bound).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("new,shared,page,window", [(1, 4, 64, 0), (20, 2, 100, 0), (3, 1, 16, 100000)])
+def test_more_keys_than_parts_reach(torch_cuda, hs, dtype, new, shared, page, window):
+    torch = torch_cuda
+    keys = 140003
+    st, batch, attention, q, k, v, scale = one_sequence(torch, hs, dtype, new, keys - new, 1, shared, 64, page, window, 3)
+    want = expected(q, [k], [v], [new], [keys - new], scale, True, window)
+    for longest, chunk in ((keys, new), (300, new), (70000, 5000), (0, 1)):
+        a = hs.Attention(shared, float(scale), window=window, longest_chunk=chunk, longest=longest)
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert_attended(dtype, out, lse, want, [k], [v], 64)
+
+
+def test_long_sequences_are_shared_out(torch_cuda, hs):
+    # eight times the keys take less than ten times as long, which they do not where one workgroup has what the others leave
+    torch = torch_cuda
+    took = []
+    for keys in (1 << 15, 1 << 18):
+        st = State(torch, hs, 2, keys // 64, 64, 1, 128, 1, keys // 64, fill=0.5)
+        st.place(np.random.default_rng(0), [keys])
+        starts, q = ints(torch, [0, 1]), torch.randn(1, 4, 128, device="cuda").bfloat16()
+        st.kept = (starts,)
+        batch, attention = hs.Batch(1, 1, starts.data_ptr()), hs.Attention(4, 0.1, longest_chunk=1, longest=keys)
+        out, w = torch.empty_like(q), torch.zeros(st.handle.attend_workspace(batch, attention), dtype=torch.uint8, device="cuda")
+        times = []
+        for _ in range(8):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            for _ in range(4):
+                st.handle.attend(0, batch, attention, heads_view(hs, q), heads_view(hs, out), workspace=w.data_ptr(), workspace_bytes=w.numel(),
+                                 stream=torch.cuda.current_stream().cuda_stream)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        took.append(min(times))
+    assert took[1] < 10 * took[0], took

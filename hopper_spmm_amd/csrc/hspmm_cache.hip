@@ -17,22 +17,18 @@ int check_dtype(int dtype)
     return HSPMM_OK;
 }
 
-// Compute units of the current device, which has to be a gfx950 (asked for once per device).
-int current_device(uint32_t *compute_units)
+// The current device has to be a gfx950 (asked for once per device).
+int check_device()
 {
-    static std::atomic<uint32_t> known[64];
+    static std::atomic<bool> known[64];
     int dev = -1;
     HSPMM_HIP(hipGetDevice(&dev));
-    uint32_t units = dev >= 0 && dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0u;
-    if (!units) {
-        hipDeviceProp_t prop;
-        HSPMM_HIP(hipGetDeviceProperties(&prop, dev));
-        if (strncmp(prop.gcnArchName, "gfx950", 6) != 0)
-            return fail(HSPMM_ERR_UNSUPPORTED, "device %d is %s; this library is built for gfx950 only", dev, prop.gcnArchName);
-        units = uint32_t(prop.multiProcessorCount);
-        if (dev >= 0 && dev < 64) known[dev].store(units, std::memory_order_relaxed);
-    }
-    if (compute_units) *compute_units = units;
+    if (dev >= 0 && dev < 64 && known[dev].load(std::memory_order_relaxed)) return HSPMM_OK;
+    hipDeviceProp_t prop;
+    HSPMM_HIP(hipGetDeviceProperties(&prop, dev));
+    if (strncmp(prop.gcnArchName, "gfx950", 6) != 0)
+        return fail(HSPMM_ERR_UNSUPPORTED, "device %d is %s; this library is built for gfx950 only", dev, prop.gcnArchName);
+    if (dev >= 0 && dev < 64) known[dev].store(true, std::memory_order_relaxed);
     return HSPMM_OK;
 }
 
@@ -167,7 +163,7 @@ int run_rotary(int dtype, const RotaryArgs &ra, const hspmm_cache *c, void *stre
     } else if (ra.tokens > 4u * ((1u << 24) - 1u)) {
         return fail(HSPMM_ERR_UNSUPPORTED, "%u tokens: in several calls", ra.tokens);
     }
-    if (int rc = current_device(nullptr)) return rc;
+    if (int rc = check_device()) return rc;
     HSPMM_HIP(launch_rotary(dtype, ra, vec, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
@@ -384,7 +380,7 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     if (int rc = check_tiles(cache, batch, sh)) return rc;
     if (sh.bytes && (!workspace || workspace_bytes < sh.bytes || reinterpret_cast<uintptr_t>(workspace) % 16u))
         return fail(HSPMM_ERR_INVALID, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)sh.bytes);
-    if (int rc = current_device(nullptr)) return rc;
+    if (int rc = check_device()) return rc;
     AttendArgs aa{};
     aa.pages = pages_of(cache, layer);
     aa.batch = batch_of(batch);
@@ -403,7 +399,7 @@ int hspmm_cache_extend(const hspmm_cache *cache, uint32_t n, const int32_t *rows
 {
     if (int rc = check_cache(cache)) return rc;
     if (int rc = check_list(cache, n, add, "add")) return rc;
-    if (int rc = current_device(nullptr)) return rc;
+    if (int rc = check_device()) return rc;
     HSPMM_HIP(launch_pages_extend(pool_of(cache), n, rows, add, status, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
@@ -415,7 +411,7 @@ int hspmm_cache_fork(const hspmm_cache *cache, uint32_t n, const int32_t *parent
     if (int rc = check_list(cache, n, children, "children")) return rc;
     if (n == 0 && !status) return HSPMM_OK;
     if (int rc = check_launch(n, 1024u)) return rc;
-    if (int rc = current_device(nullptr)) return rc;
+    if (int rc = check_device()) return rc;
     HSPMM_HIP(launch_pages_fork(pool_of(cache), n, parents, children, status, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
@@ -426,7 +422,7 @@ int hspmm_cache_free(const hspmm_cache *cache, uint32_t n, const int32_t *rows, 
     if (int rc = check_list(cache, n, rows, "rows")) return rc;
     if (n == 0) return HSPMM_OK;
     if (int rc = check_launch(n, 256u)) return rc;
-    if (int rc = current_device(nullptr)) return rc;
+    if (int rc = check_device()) return rc;
     HSPMM_HIP(launch_pages_free(pool_of(cache), n, rows, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
@@ -434,7 +430,7 @@ int hspmm_cache_free(const hspmm_cache *cache, uint32_t n, const int32_t *rows, 
 int hspmm_cache_compact(const hspmm_cache *cache, int32_t *table_out, int32_t *references_out, int32_t *live, void *stream)
 {
     if (int rc = check_cache(cache)) return rc;
-    if (int rc = current_device(nullptr)) return rc;
+    if (int rc = check_device()) return rc;
     HSPMM_HIP(launch_pages_compact(pool_of(cache), table_out ? table_out : cache->table, references_out ? references_out : cache->references, live,
                                    static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
@@ -447,7 +443,7 @@ int hspmm_cache_copy(const hspmm_cache *cache, uint32_t n, const int32_t *from, 
     if (n && (!from || !to)) return fail(HSPMM_ERR_INVALID, "null list of pages");
     if (n == 0) return HSPMM_OK;
     if (int rc = check_launch(n, 256u)) return rc;
-    if (int rc = current_device(nullptr)) return rc;
+    if (int rc = check_device()) return rc;
     HSPMM_HIP(launch_pages_copy(pool_of(cache), n, from, to, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }

@@ -192,6 +192,7 @@ int hspmm_rotary_table(int kind, uint32_t dims, double base, double factor, doub
         auto pair_of = [&](double turns) { return double(dims) * std::log(original_length / (turns * kTurn)) / (2.0 * std::log(base)); };
         double low = 0.0, high = 0.0;
         if (kind == HSPMM_ROTARY_YARN) {
+            // (whole pairs, dims - 1 and 0.001 are the steps of the authors' published program, to which trained models hold; the paper has none of them)
             low = std::max(std::floor(pair_of(fast_turns)), 0.0);
             high = std::min(std::ceil(pair_of(slow_turns)), double(dims - 1u));
             if (high <= low) high = low + 0.001;

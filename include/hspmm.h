@@ -535,9 +535,13 @@ typedef struct hspmm_rotary {
  *   PLAIN   f_i
  *   LINEAR  f_i / factor: positions of a context `factor` times as long squeezed into the original one
  *   BASE    base * factor^(dims / (dims - 2)) in place of base: the lowest frequency is divided by factor, the highest stays
- *   YARN    f_i / factor for wavelengths longer than original_length / slow_turns, f_i for those shorter than
- *           original_length / fast_turns, a linear ramp over i between the two; cosines and sines times
- *           0.1 ln(factor) + 1 (Peng et al. 2023, "YaRN: Efficient Context Window Extension of Large Language Models") */
+ *   YARN    f_i for wavelengths shorter than original_length / fast_turns, f_i / factor for those longer than
+ *           original_length / slow_turns, a mixture of the two between; cosines and sines times 0.1 ln(factor) + 1 (Peng et al. 2023,
+ *           "YaRN: Efficient Context Window Extension of Large Language Models").  The mixture is that of the authors' published
+ *           program, which models are trained with, not the paper's, whose ramp is linear in the turns: with
+ *           i(t) = dims ln(original_length / (2 pi t)) / (2 ln base), the pair that turns t times, low = max(floor i(fast_turns), 0) and
+ *           high = min(ceil i(slow_turns), dims - 1), low + 0.001 where that is not above low, pair i has
+ *           r = (i - low) / (high - low) within 0 and 1, and the frequency (1 - r) f_i + r f_i / factor */
 #define HSPMM_ROTARY_PLAIN 0
 #define HSPMM_ROTARY_LINEAR 1
 #define HSPMM_ROTARY_BASE 2

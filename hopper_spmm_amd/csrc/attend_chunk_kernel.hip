@@ -454,9 +454,10 @@ template <bool BF>
 void launch_type(const AttendArgs &aa, uint32_t rows_log, hipStream_t s)
 {
     const uint32_t D = aa.pages.head_dim;
-    if (D <= 64u) launch<BF, 64, 4>(aa, s);
+    if (rows_log == 8u) launch<BF, 128, 8>(aa, s);
+    else if (D <= 64u) launch<BF, 64, 4>(aa, s);
     else if (D <= 96u) launch<BF, 96, 4>(aa, s);
-    else if (D <= 128u) rows_log == 8u ? launch<BF, 128, 8>(aa, s) : launch<BF, 128, 4>(aa, s);
+    else if (D <= 128u) launch<BF, 128, 4>(aa, s);
     else if (D <= 160u) launch<BF, 160, 4>(aa, s);
     else launch<BF, 256, 4>(aa, s);
 }

@@ -64,8 +64,7 @@ constexpr uint32_t kAttendCounters = 16384u;
 inline uint32_t attend_slot(uint32_t rows_log, uint32_t head_dim) { return (1u << rows_log) * ((head_dim <= 64u ? 64u : head_dim <= 128u ? 128u : 256u) + 4u); }
 // past: 16-bit keys and values are not kept in the L2
 hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, bool past, hipStream_t s);
-// 16-bit types
-// 16-bit types; tiles of 1 << rows_log rows: 128, and 256 for heads of up to 128 elements
+// 16-bit types; tiles of 1 << rows_log rows: 128, or 256 for heads of up to 128 elements
 hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, uint32_t rows_log, hipStream_t s);
 
 // Page work: all layers.

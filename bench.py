@@ -152,18 +152,25 @@ def cpu_baseline(A, B, N, flops_full):
     }
 
 
-def kernel_sources_digest():
-    """sha256 over the kernel and host sources libhspmm.so is built from: the counter figures of
+# sources that no product is made with: positions, the cache's pages and attention over it
+CACHE_SOURCES = ("attend_chunk_kernel.hip", "attend_common.hpp", "attend_rows_kernel.hip", "cache_device.h", "divisor.hpp", "hspmm_cache.hip",
+                 "page_kernels.hip", "rotary_kernels.hip")
+
+
+def kernel_sources_digest(csrc=os.path.join(ROOT, "hopper_spmm_amd", "csrc")):
+    """sha256 over the kernel and host sources of the products in libhspmm.so and the flags they are built with: the counter figures of
     profiles/traffic.json carry the digest they were measured with."""
     import glob
     import hashlib
     h = hashlib.sha256()
-    csrc = os.path.join(ROOT, "hopper_spmm_amd", "csrc")
     for path in sorted(glob.glob(os.path.join(csrc, "*"))):
-        if path.endswith((".hip", ".hpp", ".h", ".cpp")) or os.path.basename(path) == "Makefile":
-            h.update(os.path.basename(path).encode())
+        name = os.path.basename(path)
+        if name.endswith((".hip", ".hpp", ".h", ".cpp")) and name not in CACHE_SOURCES:
+            h.update(name.encode())
             with open(path, "rb") as f:
                 h.update(f.read())
+    with open(os.path.join(csrc, "Makefile")) as f:
+        h.update("".join(line for line in f if line.startswith(("ARCH", "FLAGS", "HOSTFLAGS", "           -W"))).encode())
     return h.hexdigest()
 
 

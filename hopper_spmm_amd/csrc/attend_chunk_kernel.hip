@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     constexpr uint32_t kRowPieces = DP / 8u, kImagePieces = kKeys * kRowPieces;
     constexpr int kSteps = DP / 16, kTiles = DP / 32, kPieces = int((kImagePieces + kThreads - 1u) / kThreads);
     __shared__ __attribute__((aligned(16))) char images[kRing * kImage];
-    __shared__ uint32_t arrived;
+    __shared__ uint32_t odd, arrived;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, j = lane & 31u;
     // (the last tiles first: where a token sees what is in front of it they are the longest)
     const uint32_t part = blockIdx.y, D = aa.pages.head_dim;
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     const int32_t parts = keys_here.parts, begin = keys_here.begin, end = keys_here.end;
     if (int32_t(part) >= parts) return;
     const int32_t n_images = end > begin ? (end - begin + 63) / 64 : 0;
-    uint32_t odd = 0u;                                         // whether this wave has written values that are not finite and hidden from some row
+    if (tid == 0u) odd = 0u;
 
     const float scale = aa.scale == 0.f ? 1.f : fabsf(aa.scale) * kLog2e;
     const uint32_t flip = aa.scale < 0.f ? 0x80008000u : 0u;
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
             for (int i = 0; i < kPieces; ++i)
 #pragma unroll
                 for (int w = 0; w < 4; ++w) any |= word_not_finite<BF>(v_piece[i][w]);
-            if (__ballot(any)) odd = 1u;
+            if (any) odd = 1u;
         }
         return stored_there;
     };
@@ -310,6 +310,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     if (n_images) {
         f32x16 s_a, s_b;
         request(0);
+        lds_barrier();                                         // (`odd` is zero before any wave can set it)
         uint64_t stored_now = write_image(0, 0u);
         request(1);
         uint64_t stored_next = write_image(1, 1u);
@@ -335,7 +336,8 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
             free = old;
             lds_barrier();
         }
-        if (__syncthreads_or(int(odd))) {
+        __syncthreads();
+        if (odd) {
             // An infinity or a NaN that some rows do not see, which a matrix instruction would multiply by their zeros: once more, the values key by
             // key and by the rows that see it.  Slow, and off the path of finite data.
             begin_sums();

@@ -310,16 +310,23 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     if (a->longest && a->longest < keys) keys = a->longest;
     auto seen = [&](uint32_t tile_rows) { return a->window && uint64_t(a->window) + tile_rows < keys ? uint64_t(a->window) + tile_rows : keys; };
     // The rows kernel for up to 16 rows, and where there is little to do: a tile of it is sixteen rows, and its waves share out the keys.  us of it / of the
-    // chunk kernel by tiles of 16 rows x heads x keys: 18 K (60 tokens from the beginning, 32 heads) 7.0 / 10.6; 96 K (8 tokens for each of 3 sequences
-    // of 2000, 32 heads on 8) 18.6 / 25; 180 K (300 tokens from the beginning) 15.2 / 16.7; 192 K (3 sequences of 4000) 29 / 27; 320 K 19.8 / 18.8;
-    // 2048 K (32 sequences of 4000) 198 / 144.
+    // chunk kernel by tiles of 16 rows x heads x keys, bf16, heads of 128: 8 K (60 tokens from the beginning, 32 heads) 6.6 / 9.7; 96 K (8 tokens for each of
+    // 3 sequences of up to 2000, 32 heads on 8) 15.3 / 22.7; 180 K (300 tokens from the beginning) 15.0 / 16.7; 256 K (32 sequences of up to 500) 19.7 / 28.3;
+    // 384 K (3 of 8000) 30.6 / 38.6; 384 K (3 tokens for each of 64 of 1500, 16 heads on 2) 34.0 / 32.6; 480 K (5 tokens over 30000) 55.9 / 70.8; 512 K (16 over
+    // 16000) 48.3 / 44.4; 640 K (64 over 20000, 8 heads on 4) 67.5 / 54.4; 1024 K (32 of 2000) 82 / 70; 1600 K (16 ragged chunks) 65 / 33.  Up to 400 K it lost
+    // at 4 of 24 such shapes, by 10 % at most (400 tokens from the beginning 19.9 / 18.1), above 500 K at 11 of 18, by up to a half; of 256 elements it won at
+    // 304 K (59.5 / 74) and lost at 480 K (80 / 77).
     const uint64_t rows_work = uint64_t(b->sequences) * ((rows + 15u) / 16u) * c->heads * seen(16u);
-    // 256 rows only for heads of 97 to 128 elements and tiles for two rounds: with 128 rows two workgroups share a compute unit, but there only two images
-    // fit for each.  us with 128 / 256 rows: 4096 tokens over 16384 keys, 32 heads, 512 tiles of 256, 1007 / 931; 17 chunks of up to 700 tokens over up
-    // to 5700, 12 heads, 344 tiles, 204 / 229; heads of 64, 2048 tokens over 8048, 177 / 184.
+    // 256 rows for heads of 97 to 128 elements only - with 128 rows two workgroups share a compute unit, but there only two images fit for each -, where chunks
+    // are of one length, tiles for a quarter of the compute units and keys for parts on all of them: few, short and half-filled tiles are the longer ones' loss.  us
+    // with 128 / 256 rows, by heads x tiles of 256 (`wide`), 32 heads on 8: 4096 tokens over 16384 keys (520) 1025 / 942; 8192 over 8192 (1032) 597 / 571; 2048 over
+    // 8192 (264) 281 / 266; 1024 over 4096 (136) 96 / 82; 512 over 8512 (72) 105 / 99; 16 x 512 over 2000 (1088) 232 / 237; 2048 over 2048 (264) 67 / 71; 500 over
+    // 500, 32 heads of keys (64) 22 / 27; few tiles: 256 over 8192 (40) 58 / 60, 700 over 20000, 8 heads on 4 (24) 85 / 103; ragged: 17 chunks of up to 700 over up
+    // to 5700 (592) 216 / 279, 16 of up to 300 over 600 (664) 44 / 50, 8 of up to 300 over 2000 (328) 73 / 68.  Heads of 64, 2048 tokens over 8048, 177 / 184.
     const uint64_t wide = uint64_t(c->heads) * ((uint64_t(b->tokens) * shared >> 8) + (b->sequences + 1u) / 2u);
-    if (c->dtype == HSPMM_TF32 || rows <= 16u || rows_work <= 190000u) sh.rows_log = kAttendRowsLog;
-    else sh.rows_log = c->head_dim > 96u && c->head_dim <= 128u && rows > 128u && wide >= 512u ? 8u : 7u;
+    const bool even = uint64_t(b->tokens) * 8u >= uint64_t(b->sequences) * std::min(a->longest_chunk, b->tokens) * 7u;
+    if (c->dtype == HSPMM_TF32 || rows <= 16u || rows_work <= 400000u) sh.rows_log = kAttendRowsLog;
+    else sh.rows_log = c->head_dim > 96u && c->head_dim <= 128u && rows > 128u && even && wide >= 64u && wide * seen(256u) >= 200000u ? 8u : 7u;
     keys = seen(1u << sh.rows_log);
     const uint64_t numbered = attend_tiles(b->tokens, b->sequences, shared, sh.rows_log);
     // tiles that have rows, at most: numbers are left out

@@ -30,15 +30,15 @@ def one_sequence(torch, hs, dtype, new, old, heads, shared, dim, page, window, s
 
 
 @pytest.mark.parametrize("dtype", [0, 2])
-@pytest.mark.parametrize("new,old,heads,dim,page,window,keys", [(700, 100, 16, 64, 16, 300, (50, 450)), (700, 100, 16, 128, 24, 300, (50, 450)),
-                                                                (700, 500, 4, 64, 16, 0, (530, 1030)), (700, 500, 4, 160, 16, 0, (530, 1030))])
+@pytest.mark.parametrize("new,old,heads,dim,page,window,keys", [(700, 100, 32, 64, 16, 300, (50, 450)), (700, 100, 32, 128, 24, 300, (50, 450)),
+                                                                (700, 500, 8, 64, 16, 0, (530, 1030)), (700, 500, 8, 160, 16, 0, (530, 1030))])
 def test_values_that_are_not_finite_among_the_first_keys(torch_cuda, hs, dtype, new, old, heads, dim, page, window, keys):
     # in the first images of tiles and of parts of 512 keys, in every head: what some rows do not see must not reach them, however the waves of a workgroup
     # follow each other
     torch = torch_cuda
     st, batch, attention, q, k, v, scale = one_sequence(torch, hs, dtype, new, old, heads, 1, dim, page, window, 11)
-    want = expected(q, [k], [v], [new], [old], scale, True, window)
     position, hit = np.arange(old, old + new), np.zeros(new, bool)
+    want = dense64(q, k, v, position, scale, window)
     for j, value in zip(keys, (np.nan, np.inf)):
         bad = v.copy()
         hit |= (position >= j) & ((position - window < j) if window else True)
@@ -323,3 +323,60 @@ def test_long_sequences_are_shared_out(torch_cuda, hs):
             times.append(begin.elapsed_time(end))
         took.append(min(times))
     assert took[1] < 10 * took[0], took
+
+
+def dense64(q, k, v, position, scale, window, there=True):
+    """attend64 of one sequence, causal, a head at a time."""
+    T, H, D = q.shape
+    j = np.arange(len(k))
+    seen = (j[None] <= position[:, None]) & there
+    if window:
+        seen = seen & (j[None] > position[:, None] - window)
+    out, size, lse, reach, any_seen = np.zeros((T, H, D)), np.zeros((T, H, D)), np.zeros((T, H)), np.zeros((T, H)), seen.any(1)
+    for h in range(H):
+        kk, vv = k[:, h // (H // k.shape[1])], v[:, h // (H // k.shape[1])]
+        s = np.where(seen, scale * (q[:, h] @ kk.T), -np.inf)
+        m = np.where(any_seen, s.max(1), 0.0)
+        p = np.exp(s - m[:, None])
+        total = p.sum(1)
+        p /= np.where(any_seen, total, 1.0)[:, None]
+        out[:, h], size[:, h] = p @ vv, p @ np.abs(vv)
+        lse[:, h] = np.where(any_seen, m + np.log(np.where(any_seen, total, 1.0)), -np.inf)
+        reach[:, h] = abs(scale) * np.where(seen, np.abs(q[:, h]) @ np.abs(kk).T, 0.0).max(1)
+    return out, lse, size, reach
+
+
+# a chunk and heads for so many tiles that the chunk's own kernel serves them, of 97 to 128 elements with 256 rows a tile
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("dim,page,window,old,heads", [(128, 16, 0, 1900, 16), (104, 24, 0, 100, 64), (128, 64, 400, 500, 64), (120, 7, 400, 77, 64),
+                                                       (40, 16, 330, 400, 16), (96, 16, 0, 111, 16), (88, 5, 350, 20, 16), (136, 24, 330, 10, 16), (248, 16, 0, 150, 16), (256, 32, 320, 40, 16)])
+def test_chunks_of_many_rows(torch_cuda, hs, dtype, dim, page, window, old, heads):
+    torch = torch_cuda
+    new, shared = 601, 2
+    st, batch, attention, q, k, v, scale = one_sequence(torch, hs, dtype, new, old, heads, shared, dim, page, window, 31)
+    position = np.arange(old, old + new)
+    want = dense64(q, k, v, position, scale, window)
+    hints = [attention, hs.Attention(heads * shared, float(scale), window=window, longest_chunk=new, longest=100000), hs.Attention(heads * shared, float(scale), window=window, longest_chunk=new, longest=1)]
+    for a in hints:
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert_attended(dtype, out, lse, want, [k], [v], dim)
+    # values that are not finite, in the first and the last tile's keys
+    bad, hit = v.copy(), np.zeros(new, bool)
+    for j, value in ((old + 40, np.inf), (old + new - 20, np.nan)):
+        bad[j, :, 7] = value
+        hit |= (position >= j) & ((position - window < j) if window else True)
+    st.store(0, 0, 1, bad)
+    clear = torch.from_numpy(~hit).cuda()
+    for a in hints[:2]:
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert not np.isfinite(to64(out)[hit][:, :, 7]).any()
+        assert_attended(dtype, out[clear], lse[clear], [x[~hit] for x in want], [k], [np.where(np.isfinite(bad), bad, 0.0)], dim)
+    st.store(0, 0, 1, v)
+    # pages that are gone
+    used = -(-(old + new) // page)
+    gone = np.random.default_rng(4).random(used) < 0.3
+    st.table[0, :used][torch.from_numpy(gone).cuda()] = -1
+    want = dense64(q, k, v, position, scale, window, ~gone[np.arange(old + new) // page])
+    for a in hints[:2]:
+        out, lse = attend(torch, hs, st, batch, a, q)
+        assert_attended(dtype, out, lse, want, [k], [v], dim)

@@ -227,8 +227,8 @@ constexpr int kRowWaves = 4;
 
 // A workgroup has 16 rows and a part of their keys; its waves take tiles of keys in turn.  The waves' sums are added at the end in LDS, the parts'
 // through memory.  Memory bounds it, as keys and values are read once for all heads that share them: one token for each of 48 sequences of up to 16000
-// keys, 32 heads on 8 of 128 elements, bf16, 281 us for 1.62 GB, 5.8 TB/s (a large copy: 4.8, read and written).  Short sequences: three of up to 300 keys, fp32, 8.0 us,
-// launch and a few dependent loads (starts, table, keys); 30000 keys of one sequence 30 us.
+// keys, 32 heads on 8 of 128 elements, bf16, 281 us for 1.62 GB, 5.8 TB/s (a large copy: 4.8, read and written).  Short sequences: three of up to 300 keys, fp32, 7.8 us,
+// launch and a few dependent loads (starts, table, keys); 30000 keys of one sequence 31 us, 2^18 194, 5.5 TB/s.
 // Registers for two workgroups a compute unit (three up to 64 elements): a wave has one tile on its way, 16 KB of keys and values.
 // Whole: pages hold a multiple of 16 tokens, so 16 keys of a tile lie in one page, and a wave asks for its next tiles' page numbers 64 at a time;
 // else every lane finds a key's row and hands it to the lanes that load it.

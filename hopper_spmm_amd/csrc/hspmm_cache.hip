@@ -336,7 +336,7 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     // over 1000 keys, 8 heads 8.1 / 9.2 / 11.9; over 30000 58 / 39 / 30; 8 sequences of up to 8000 56 / 44 / 42.
     // Chunk kernel: as many as run at a time (two a compute unit with 128 rows and heads of up to 128 elements); a part's sums are as much as 130 keys.
     // Of two, twice as many where there are tiles for half of them anyway, which are of different lengths.  us by 512 / 1024 workgroups: 100 tokens for
-    // each of 4 sequences of 4000 52 / 64; 512 tokens over 8512 keys, head_dim 64 38 / 48; the 17 chunks above 204 / 175.  (One a compute unit, head_dim
+    // each of 4 sequences of 4000 52 / 64; 512 tokens over 8512 keys, head_dim 64 38 / 48; 17 chunks of up to 700 tokens over up to 5700, 12 heads on 4, 204 / 175.  (One a compute unit, head_dim
     // 256, 1024 tokens over 2048 older keys, by 256 / 512 264 / 338.)
     const uint64_t work = tiles * c->heads * keys;
     const bool two = sh.rows_log == 7u && c->head_dim <= 128u;

@@ -1,7 +1,7 @@
 // Work on the pages of a cache: giving out, sharing, releasing, moving and copying them.  What decides is integers - the
 // table, lengths and references -, what takes time is the pages' bytes, each read and written once, all layers in one launch.  us: 476 pages of 2 MB
-// moved 389, 5.1 TB/s (a large copy: 4.8); 192 beams of partly filled pages, all of 32 layers, 55 for 284 MB, 5.1 TB/s; small ones 9, which is two
-// launches, as which pages are free has to be known before one is written: what is decided cannot be decided again by every workgroup that copies
+// moved 382, 5.2 TB/s (a large copy: 4.8); 192 beams of partly filled pages, all of 32 layers, 57 for 284 MB, 5.0 TB/s; a token more for 64 sequences 4.4, freeing
+// them 4.8; small forks and compactions 10, which is two launches, as which pages are free has to be known before one is written: what is decided cannot be decided again by every workgroup that copies
 // while others change the table and the references.
 #include "cache_device.h"
 #include <algorithm>

@@ -34,7 +34,7 @@ __device__ __forceinline__ void lds_barrier()
 //   sums:   O^T = V^T P^T, 32 elements x 32 rows by instructions of 16 keys: scores 8 s .. 8 s + 7 of a lane are its part of the second operand,
 //           keys in that order; the first one comes transposed from LDS (ds_read_b64_tr_b16), four keys of an element a read
 // Per key and row 4 D operations, an exponential and some ten other instructions.  Matrix instructions bound it where keys are many: 4096 tokens over
-// 16384 keys, 32 heads on 8, head_dim 128, bf16, 935 to 960 us, 1000 to 1030 TFLOP/s (a library's product of 8192^3: 1170); 2048 tokens over 8048 keys, heads of 96 / 64:
+// 16384 keys, 32 heads on 8, head_dim 128, bf16, 935 to 1020 us, 940 to 1030 TFLOP/s, by machine (a library's product of 8192^3: 1170); 2048 tokens over 8048 keys, heads of 96 / 64:
 // 217 / 180 us, 800 / 650 TFLOP/s, as exponentials weigh more.  What is left there is the exponentials' share of a wave's issue that no matrix
 // instruction of the other wave covers.  Short spans: an image's arrival and the last workgroups; 17 chunks of up to 700 tokens, window 1000, 70 us, 360
 // TFLOP/s.  A wave has 32 rows, two waves a SIMD: one multiplies while the other one takes exponentials.

@@ -50,6 +50,21 @@ class Attention(C.Structure):
         super().__init__(q_heads, scale, int(bool(causal)), window, longest_chunk, longest)
 
 
+class Prefix(C.Structure):
+    """Groups of a batch's rows that begin with the same tokens: rows firsts[g] .. firsts[g + 1] - 1 share the first tokens[g], which the first
+    one's pages hold; most_tokens (of the batch, of a group) and longest (of a prefix) choose kernels only."""
+    _fields_ = [("groups", C.c_uint32), ("most_tokens", C.c_uint32), ("longest", C.c_uint32), ("firsts", C.c_void_p), ("tokens", C.c_void_p)]
+
+    def __init__(self, groups, firsts, tokens, most_tokens=0, longest=0):
+        super().__init__(groups, most_tokens, longest, firsts or None, tokens or None)
+
+
+class Weights(C.Structure):
+    """Attention weight that cached keys have received, layers x sequences x heads x tokens floats (a head's tokens side by side):
+    `Weights(w.data_ptr(), *w.stride()[:3])`."""
+    _fields_ = [("data", C.c_void_p), ("layer_stride", C.c_int64), ("sequence_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
 class _Cache(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("order", C.c_int32), ("layers", C.c_uint32), ("pages", C.c_uint32), ("page_tokens", C.c_uint32),
                 ("heads", C.c_uint32), ("head_dim", C.c_uint32), ("sequences", C.c_uint32), ("table_pages", C.c_uint32),
@@ -72,6 +87,12 @@ def _library():
         L.hspmm_cache_append.argtypes = [P(_Cache), u32, P(Batch), P(Heads), P(Heads), P(Rotary), u32, P(Heads), P(Heads), vp]
         L.hspmm_cache_attend_workspace.argtypes = [P(_Cache), P(Batch), P(Attention), P(C.c_uint64)]
         L.hspmm_cache_attend.argtypes = [P(_Cache), u32, P(Batch), P(Attention), P(Heads), P(Heads), vp, vp, C.c_uint64, vp]
+        L.hspmm_cache_attend_shared_workspace.argtypes = [P(_Cache), P(Batch), P(Prefix), P(Attention), P(C.c_uint64)]
+        L.hspmm_cache_attend_shared.argtypes = [P(_Cache), u32, P(Batch), P(Prefix), P(Attention), P(Heads), P(Heads), vp, vp, C.c_uint64, vp]
+        L.hspmm_cache_weigh_workspace.argtypes = [P(_Cache), P(Batch), P(Attention), u32, P(C.c_uint64)]
+        L.hspmm_cache_weigh.argtypes = [P(_Cache), u32, P(Batch), P(Attention), P(Heads), vp, P(Weights), C.c_float, u32, vp, C.c_uint64, vp]
+        L.hspmm_cache_evict_workspace.argtypes = [P(_Cache), u32, u32, P(C.c_uint64)]
+        L.hspmm_cache_evict.argtypes = [P(_Cache), u32, vp, vp, P(Weights), u32, u32, u32, vp, vp, vp, C.c_uint64, vp]
         L.hspmm_cache_extend.argtypes = [P(_Cache), u32, vp, vp, vp, vp]
         L.hspmm_cache_fork.argtypes = [P(_Cache), u32, vp, vp, vp, vp]
         L.hspmm_cache_free.argtypes = [P(_Cache), u32, vp, vp]
@@ -113,6 +134,7 @@ class Cache:
                          keys, values, table, lengths, references, scratch)
         # (bound once: small calls are made of their host time)
         self._append, self._attend, self._fork, self._compact = L.hspmm_cache_append, L.hspmm_cache_attend, L.hspmm_cache_fork, L.hspmm_cache_compact
+        self._attend_shared, self._weigh, self._evict = L.hspmm_cache_attend_shared, L.hspmm_cache_weigh, L.hspmm_cache_evict
 
     def append(self, layer, batch, k, v, rotary=None, q_heads=0, q=None, q_out=None, stream=0):
         """hspmm_cache_append: keys and values of the batch's tokens into their pages, turned before if rotary is given; q_out = q turned."""
@@ -129,6 +151,42 @@ class Cache:
     def attend(self, layer, batch, attention, q, out, lse=0, workspace=0, workspace_bytes=0, stream=0):
         """hspmm_cache_attend: out = softmax(scale q k) v of the batch's tokens; lse: address of tokens x q_heads floats, or 0."""
         rc = self._attend(self._c, layer, batch, attention, q, out, lse, workspace, workspace_bytes, stream)
+        if rc:
+            _check(rc)
+
+    def attend_shared_workspace(self, batch, prefix, attention):
+        """Bytes of workspace (zeros at first) that `attend_shared` wants for these."""
+        n = C.c_uint64()
+        _check(_library().hspmm_cache_attend_shared_workspace(self._c, batch, prefix, attention, n))
+        return n.value
+
+    def attend_shared(self, layer, batch, prefix, attention, q, out, lse=0, workspace=0, workspace_bytes=0, stream=0):
+        """hspmm_cache_attend_shared: `attend` of groups of sequences that begin with the same tokens, whose keys and values are read once."""
+        rc = self._attend_shared(self._c, layer, batch, prefix, attention, q, out, lse, workspace, workspace_bytes, stream)
+        if rc:
+            _check(rc)
+
+    def weigh_workspace(self, batch, attention, last=0):
+        """Bytes of workspace (zeros at first) that `weigh` wants for these."""
+        n = C.c_uint64()
+        _check(_library().hspmm_cache_weigh_workspace(self._c, batch, attention, last, n))
+        return n.value
+
+    def weigh(self, layer, batch, attention, q, lse, weights, decay=1.0, last=0, workspace=0, workspace_bytes=0, stream=0):
+        """hspmm_cache_weigh: weights of cached keys = decay * weights + what the batch's tokens give them; q and lse are those of `attend`."""
+        rc = self._weigh(self._c, layer, batch, attention, q, lse, weights, decay, last, workspace, workspace_bytes, stream)
+        if rc:
+            _check(rc)
+
+    def evict_workspace(self, n, keep):
+        """Bytes of workspace (zeros at first) that `evict` wants for a list of n sequences that keep so many tokens."""
+        b = C.c_uint64()
+        _check(_library().hspmm_cache_evict_workspace(self._c, n, keep, b))
+        return b.value
+
+    def evict(self, n, parents, children, weights, keep, first=0, last=0, kept=0, status=0, workspace=0, workspace_bytes=0, stream=0):
+        """hspmm_cache_evict: sequence children[i] (children 0: the parent itself) becomes what parents[i] was, with `keep` of its tokens at most."""
+        rc = self._evict(self._c, n, parents, children, weights, keep, first, last, kept, status, workspace, workspace_bytes, stream)
         if rc:
             _check(rc)
 

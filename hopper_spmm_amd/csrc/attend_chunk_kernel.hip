@@ -40,7 +40,7 @@ __device__ __forceinline__ void lds_barrier()
 // TFLOP/s.  A wave has 32 rows, two waves a SIMD: one multiplies while the other one takes exponentials.
 // The scores of a half are made among the exponentials of the half in front.  Images go through LDS, kRing of them in turn: while image n is
 // multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image (with two places: two).
-template <bool BF, int DP, int W, bool Whole>
+template <bool BF, int DP, int W, bool Whole, AttendSpan Span>
 __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel(const AttendArgs aa)
 {
     typedef typename HalfOps<BF>::elem_t T;
@@ -59,8 +59,42 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     const uint32_t part = blockIdx.y, D = aa.pages.head_dim;
     const Cell cell = cell_of(aa, gridDim.x - 1u - blockIdx.x, 0u);
     const uint32_t head = cell.head, tile_number = cell.tile;
-    const RowTile t = find_tile<kRowsLog>(aa, tile_number);
+    RowTile t = find_tile<kRowsLog, Span>(aa, tile_number);
     if (!t.there) return;
+    const uint32_t m = wave * 32u + j;
+    const bool is_row = m < t.rows;
+    const RowOf row = row_of_tile<Span>(aa, t, head, m);
+    // keys that all of the wave's rows see
+    int32_t all_lo = is_row ? row.lo : 0, all_hi = is_row ? row.hi : 0x7FFFFFFF, any_lo = is_row ? row.lo : 0x7FFFFFFF;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        all_lo = max(all_lo, __shfl_xor(all_lo, d));
+        all_hi = min(all_hi, __shfl_xor(all_hi, d));
+        if (Span == kSpanPrefix) any_lo = min(any_lo, __shfl_xor(any_lo, d));
+    }
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo); all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    // the same of the workgroup's rows
+    int32_t group_lo, group_hi;
+    if constexpr (Span == kSpanPrefix) {
+        // (rows of several sequences)
+        __shared__ int32_t ranges[W][3];
+        if (lane == 0u) { ranges[wave][0] = all_lo; ranges[wave][1] = all_hi; ranges[wave][2] = any_lo; }
+        __syncthreads();
+        group_lo = all_lo; group_hi = all_hi;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            group_lo = max(group_lo, ranges[w][0]);
+            group_hi = min(group_hi, ranges[w][1]);
+            any_lo = min(any_lo, ranges[w][2]);
+        }
+        group_lo = __builtin_amdgcn_readfirstlane(group_lo); group_hi = __builtin_amdgcn_readfirstlane(group_hi);
+        t.lo = __builtin_amdgcn_readfirstlane(min(any_lo, t.hi));
+    } else {
+        const int32_t p0 = t.position + int32_t(aa.shared.quotient(t.first_row)), p1 = t.position + int32_t(aa.shared.quotient(t.first_row + t.rows - 1u));
+        group_hi = aa.causal ? p0 + 1 : t.length;
+        group_lo = aa.window && int64_t(p1) + 1 > int64_t(aa.window) ? p1 + 1 - int32_t(aa.window) : 0;
+        if constexpr (Span == kSpanRest) group_lo = max(group_lo, t.prefix);
+    }
     const KeyPart keys_here = key_part(aa, t, part);
     const int32_t parts = keys_here.parts, begin = keys_here.begin, end = keys_here.end;
     if (int32_t(part) >= parts) return;
@@ -69,9 +103,6 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
 
     const float scale = aa.scale == 0.f ? 1.f : fabsf(aa.scale) * kLog2e;
     const uint32_t flip = aa.scale < 0.f ? 0x80008000u : 0u;
-    const uint32_t m = wave * 32u + j;
-    const bool is_row = m < t.rows;
-    const RowOf row = row_of_tile(aa, t, head, m);
     u32x4 q[kSteps];
     {
         const char *from = aa.q.data + (int64_t(row.token) * aa.q.token_stride + int64_t(row.head) * aa.q.head_stride) * 2;
@@ -90,18 +121,6 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
             for (int s = 0; s < kSteps; ++s) q[s] &= 16u * s + 8u * h < D ? ~0u : 0u;
         }
     }
-    // keys that all of the wave's rows see
-    int32_t all_lo = is_row ? row.lo : 0, all_hi = is_row ? row.hi : 0x7FFFFFFF;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        all_lo = max(all_lo, __shfl_xor(all_lo, d));
-        all_hi = min(all_hi, __shfl_xor(all_hi, d));
-    }
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo); all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-    // the same of the workgroup's rows
-    const int32_t p0 = t.position + int32_t(aa.shared.quotient(t.first_row)), p1 = t.position + int32_t(aa.shared.quotient(t.first_row + t.rows - 1u));
-    const int32_t group_hi = aa.causal ? p0 + 1 : t.length, group_lo = aa.window && int64_t(p1) + 1 > int64_t(aa.window) ? p1 + 1 - int32_t(aa.window) : 0;
-
     const int32_t *table = aa.pages.table + size_t(t.sequence) * aa.pages.table_pages;
     const int64_t head_offset = int64_t(head) * aa.pages.head_stride;
     // Where keys lie, in bytes from keys and values: of groups of 16 keys, four an image, of 16 images at a time, a lane each (Whole), or of
@@ -424,6 +443,34 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
         }
     }
     if (!is_row) return;
+    if constexpr (Span == kSpanPrefix) {
+        float *const to = prefix_sums(aa, row);
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const uint32_t d = 32u * c + 2u * r + 4u * h;
+                if (d < D) *reinterpret_cast<f32x4 *>(to + d) = f32x4{o[c][r], o[c][r + 1], o[c][r + 2], o[c][r + 3]};
+            }
+        if (h == 0u) *reinterpret_cast<f32x4 *>(to + D) = f32x4{ref, total, 0.f, 0.f};
+        return;
+    }
+    if (Span == kSpanRest && t.prefix) {
+        const float *const from = prefix_sums(aa, row);
+        const float other = from[D], top = fmaxf(ref, other);
+        const float keep = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - top), by = other == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other - top);
+        total = total * keep + from[D + 1u] * by;
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const uint32_t d = 32u * c + 2u * r + 4u * h;
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (d < D ? d : 0u));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[c][r + e] = o[c][r + e] * keep + x[e] * by;
+            }
+        ref = top;
+    }
     const bool any = !(total == 0.f);
     const float by = any ? 1.f / total : 0.f;
     T *og = reinterpret_cast<T *>(aa.out.data) + int64_t(row.token) * aa.out.token_stride + int64_t(row.head) * aa.out.head_stride;
@@ -444,32 +491,40 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     if (aa.lse && h == 0u) aa.lse[size_t(row.token) * aa.q_heads + row.head] = any ? (ref + __builtin_amdgcn_logf(total)) * kLn2 : -INFINITY;
 }
 
-template <bool BF, int DP, int W>
-void launch(const AttendArgs &aa, hipStream_t s)
+template <bool BF, int DP, int W, AttendSpan Span>
+void launch_span(const AttendArgs &aa, hipStream_t s)
 {
     const dim3 grid(aa.tiles * aa.heads.d, aa.splits);
-    if (aa.pages.page_tokens.d % 16u == 0u) attend_chunk_kernel<BF, DP, W, true><<<grid, dim3(64 * W), 0, s>>>(aa);
-    else attend_chunk_kernel<BF, DP, W, false><<<grid, dim3(64 * W), 0, s>>>(aa);
+    if (aa.pages.page_tokens.d % 16u == 0u) attend_chunk_kernel<BF, DP, W, true, Span><<<grid, dim3(64 * W), 0, s>>>(aa);
+    else attend_chunk_kernel<BF, DP, W, false, Span><<<grid, dim3(64 * W), 0, s>>>(aa);
+}
+
+template <bool BF, int DP, int W>
+void launch(const AttendArgs &aa, AttendSpan span, hipStream_t s)
+{
+    if (span == kSpanAll) launch_span<BF, DP, W, kSpanAll>(aa, s);
+    else if (span == kSpanPrefix) launch_span<BF, DP, W, kSpanPrefix>(aa, s);
+    else launch_span<BF, DP, W, kSpanRest>(aa, s);
 }
 
 template <bool BF>
-void launch_type(const AttendArgs &aa, uint32_t rows_log, hipStream_t s)
+void launch_type(const AttendArgs &aa, AttendSpan span, uint32_t rows_log, hipStream_t s)
 {
     const uint32_t D = aa.pages.head_dim;
-    if (rows_log == 8u) launch<BF, 128, 8>(aa, s);
-    else if (D <= 64u) launch<BF, 64, 4>(aa, s);
-    else if (D <= 96u) launch<BF, 96, 4>(aa, s);
-    else if (D <= 128u) launch<BF, 128, 4>(aa, s);
-    else if (D <= 160u) launch<BF, 160, 4>(aa, s);
-    else launch<BF, 256, 4>(aa, s);
+    if (rows_log == 8u) launch<BF, 128, 8>(aa, span, s);
+    else if (D <= 64u) launch<BF, 64, 4>(aa, span, s);
+    else if (D <= 96u) launch<BF, 96, 4>(aa, span, s);
+    else if (D <= 128u) launch<BF, 128, 4>(aa, span, s);
+    else if (D <= 160u) launch<BF, 160, 4>(aa, span, s);
+    else launch<BF, 256, 4>(aa, span, s);
 }
 
 }  // namespace
 
-hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, uint32_t rows_log, hipStream_t s)
+hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, AttendSpan span, uint32_t rows_log, hipStream_t s)
 {
-    if (dtype == kDtypeF16) launch_type<false>(aa, rows_log, s);
-    else launch_type<true>(aa, rows_log, s);
+    if (dtype == kDtypeF16) launch_type<false>(aa, span, rows_log, s);
+    else launch_type<true>(aa, span, rows_log, s);
     return hipGetLastError();
 }
 

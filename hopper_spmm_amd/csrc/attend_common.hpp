@@ -24,31 +24,74 @@ struct RowTile {
     uint32_t sequence, first_row, rows, first_token, chunk;      // first_token of the batch; rows from first_row on
     int32_t length, position;                                    // tokens the cache holds; the position of the chunk's first token
     int32_t lo, hi;                                              // keys that any of the rows may see, as far as there are places for them
+    uint32_t first_batch, end_batch;                             // kSpanPrefix: the batch's rows of the group, whose sequences' chunks the rows are of
+    int32_t prefix;                                              // keys of the group's prefix (kSpanPrefix, kSpanRest)
     bool there;
 };
 
-// Tile number `tile` of (1 << ROWS_LOG) rows.  Batch row b has the tiles from (starts[b] * shared >> ROWS_LOG) + b on: more than it needs at most by
-// one, so that no list of tiles is made.  A wave looks at 64 batch rows at a time.
-template <int ROWS_LOG>
-__device__ __forceinline__ RowTile find_tile(const AttendArgs &aa, uint32_t tile)
+// The last of n ascending numbers base(0), base(1), .. that is at most `most`, 0 where none is.  A wave looks at 64 of them at a time.
+template <class F>
+__device__ __forceinline__ uint32_t last_at_most(uint32_t n, uint32_t most, F base)
 {
-    const BatchArgs &ba = aa.batch;
     const uint32_t lane = threadIdx.x & 63u;
-    auto base = [&](uint32_t b) __attribute__((always_inline)) {
-        return (uint32_t(clamp_i32(ba.starts[b], 0, int32_t(ba.tokens))) * aa.shared.d >> ROWS_LOG) + b;
-    };
-    uint32_t lo = 0, n = ba.sequences;
+    uint32_t lo = 0;
     while (n > 1u) {
         const uint32_t step = (n + 63u) / 64u, b = lane * step;
-        const uint32_t below = uint32_t(__popcll(__ballot(b < n && base(lo + b) <= tile)));
+        const uint32_t below = uint32_t(__popcll(__ballot(b < n && base(lo + b) <= most)));
         const uint32_t skip = (below ? below - 1u : 0u) * step;
         lo += skip;
         n = n - skip < step ? n - skip : step;
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+__device__ __forceinline__ uint32_t batch_sequence(const BatchArgs &ba, uint32_t b) { return ba.rows ? uint32_t(ba.rows[b]) : b; }
+
+// Group g's prefix: how many keys, whose row of the table has them, and the group's rows and tokens of the batch.  None where the group is empty or out of order.
+struct Prefix { int32_t keys; uint32_t sequence, first, end; int32_t first_token, end_token; };
+__device__ __forceinline__ Prefix prefix_of(const AttendArgs &aa, uint32_t g)
+{
+    const Prefix none{0, 0u, 0u, 0u, 0, 0};
+    const int32_t first = aa.prefix.firsts[g], end = aa.prefix.firsts[g + 1u];
+    if (first < 0 || end <= first || uint32_t(end) > aa.batch.sequences) return none;
+    const uint32_t sequence = batch_sequence(aa.batch, uint32_t(first));
+    const int32_t first_token = aa.batch.starts[first], end_token = aa.batch.starts[end];
+    if (sequence >= aa.pages.sequences || first_token < 0 || end_token > int32_t(aa.batch.tokens)) return none;
+    const int32_t held = tokens_held(aa.pages, sequence), places = keys_of_row(aa.pages);
+    return Prefix{clamp_i32(aa.prefix.tokens[g], 0, held < places ? held : places), sequence, uint32_t(first), uint32_t(end), first_token, end_token};
+}
+
+// The prefix of the group that batch row b, which has the tokens [first_token, end_token), is in.
+__device__ __forceinline__ int32_t prefix_keys(const AttendArgs &aa, uint32_t b, int32_t first_token, int32_t end_token)
+{
+    const uint32_t g = last_at_most(aa.prefix.groups, b, [&](uint32_t i) __attribute__((always_inline)) { return uint32_t(max(aa.prefix.firsts[i], 0)); });
+    const Prefix p = prefix_of(aa, g);
+    return b >= p.first && b < p.end && first_token >= p.first_token && end_token <= p.end_token ? p.keys : 0;
+}
+
+// Tile number `tile` of (1 << ROWS_LOG) rows.  Batch row b has the tiles from (starts[b] * shared >> ROWS_LOG) + b on: more than it needs at most by
+// one, so that no list of tiles is made.  kSpanPrefix: a tile's rows are a group's, of all its sequences one after another, and group g has the tiles from
+// (starts[firsts[g]] * shared >> ROWS_LOG) + g on.
+template <int ROWS_LOG, AttendSpan Span>
+__device__ __forceinline__ RowTile find_tile(const AttendArgs &aa, uint32_t tile)
+{
+    const BatchArgs &ba = aa.batch;
+    auto base = [&](uint32_t b) __attribute__((always_inline)) {
+        const uint32_t at = Span == kSpanPrefix ? uint32_t(clamp_i32(aa.prefix.firsts[b], 0, int32_t(ba.sequences))) : b;
+        return (uint32_t(clamp_i32(ba.starts[at], 0, int32_t(ba.tokens))) * aa.shared.d >> ROWS_LOG) + b;
+    };
+    const uint32_t lo = last_at_most(Span == kSpanPrefix ? aa.prefix.groups : ba.sequences, tile, base);
     RowTile t{};
-    const int32_t first = ba.starts[lo], end = ba.starts[lo + 1u];
-    t.sequence = ba.rows ? uint32_t(ba.rows[lo]) : lo;
+    int32_t first, end;
+    if constexpr (Span == kSpanPrefix) {
+        const Prefix p = prefix_of(aa, lo);
+        if (!p.keys) return t;
+        first = p.first_token; end = p.end_token;
+        t.sequence = p.sequence; t.first_batch = p.first; t.end_batch = p.end; t.prefix = p.keys;
+    } else {
+        first = ba.starts[lo]; end = ba.starts[lo + 1u];
+        t.sequence = batch_sequence(ba, lo);
+    }
     if (first < 0 || end <= first || end > int32_t(ba.tokens) || t.sequence >= aa.pages.sequences) return t;
     const uint32_t rows = uint32_t(end - first) * aa.shared.d;
     const uint32_t from = (tile - base(lo)) << ROWS_LOG;
@@ -57,12 +100,20 @@ __device__ __forceinline__ RowTile find_tile(const AttendArgs &aa, uint32_t tile
     t.rows = rows - from < (1u << ROWS_LOG) ? rows - from : 1u << ROWS_LOG;
     t.first_token = uint32_t(first);
     t.chunk = uint32_t(end - first);
+    t.there = true;
+    if constexpr (Span == kSpanPrefix) {
+        t.hi = t.prefix;
+        return t;
+    }
     t.length = tokens_held(aa.pages, t.sequence);
     t.position = t.length - (end - first);
     const int32_t p0 = t.position + int32_t(aa.shared.quotient(from)), p1 = t.position + int32_t(aa.shared.quotient(from + t.rows - 1u));
     t.hi = clamp_i32(aa.causal ? p1 + 1 : t.length, 0, keys_of_row(aa.pages));
     t.lo = aa.window && int64_t(p0) + 1 > int64_t(aa.window) ? min(p0 + 1 - int32_t(aa.window), t.hi) : 0;
-    t.there = true;
+    if constexpr (Span == kSpanRest) {
+        t.prefix = prefix_keys(aa, lo, first, end);
+        t.lo = min(max(t.lo, t.prefix), t.hi);
+    }
     return t;
 }
 
@@ -95,16 +146,40 @@ __device__ __forceinline__ Cell cell_of(const AttendArgs &aa, uint32_t number, u
 
 // A row's token (of the batch), head and the keys [lo, hi) that it may see; a row behind the last one sees none.
 struct RowOf { uint32_t token, head; int32_t lo, hi; };
+template <AttendSpan Span>
 __device__ __forceinline__ RowOf row_of_tile(const AttendArgs &aa, const RowTile &t, uint32_t head, uint32_t m)
 {
     const uint32_t at = t.first_row + (m < t.rows ? m : 0u), i = aa.shared.quotient(at);
     RowOf r;
     r.token = t.first_token + i;
     r.head = head * aa.shared.d + at - i * aa.shared.d;
-    const int32_t p = t.position + int32_t(i);
-    r.hi = m >= t.rows ? 0 : aa.causal ? p + 1 : t.length;
+    int32_t p = t.position + int32_t(i), length = t.length;
+    bool there = m < t.rows;
+    if constexpr (Span == kSpanPrefix) {
+        // the row's sequence is the last one of the group that begins at the token or in front of it
+        uint32_t b = t.first_batch, n = t.end_batch - t.first_batch;
+        while (n > 1u) {
+            const uint32_t half = n / 2u;
+            const bool after = aa.batch.starts[b + half] <= int32_t(r.token);
+            b += after ? half : 0u;
+            n = after ? n - half : half;
+        }
+        const TokenPlace at_place = place_in(aa.batch, aa.pages, b, r.token);
+        there &= at_place.there;
+        p = at_place.position;
+        length = at_place.there ? tokens_held(aa.pages, at_place.sequence) : 0;
+    }
+    r.hi = !there ? 0 : aa.causal ? p + 1 : length;
     r.lo = aa.window && int64_t(p) + 1 > int64_t(aa.window) ? p + 1 - int32_t(aa.window) : 0;
+    if constexpr (Span == kSpanPrefix) r.hi = min(r.hi, t.prefix);
+    if constexpr (Span == kSpanRest) r.lo = max(r.lo, t.prefix);
     return r;
+}
+
+// Where a row's sums over its group's prefix are.
+__device__ __forceinline__ float *prefix_sums(const AttendArgs &aa, const RowOf &r)
+{
+    return aa.prefix.sums + (size_t(r.token) * aa.q_heads + r.head) * (aa.pages.head_dim + kPrefixExtra);
 }
 
 // Element offset of the row of a key (kv head `head`), -1: not stored.

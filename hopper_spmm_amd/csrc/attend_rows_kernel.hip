@@ -232,7 +232,7 @@ constexpr int kRowWaves = 4;
 // Registers for two workgroups a compute unit (three up to 64 elements): a wave has one tile on its way, 16 KB of keys and values.
 // Whole: pages hold a multiple of 16 tokens, so 16 keys of a tile lie in one page, and a wave asks for its next tiles' page numbers 64 at a time;
 // else every lane finds a key's row and hands it to the lanes that load it.
-template <class K, bool Whole, int DP>
+template <class K, bool Whole, int DP, AttendSpan Span>
 __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attend_rows_kernel(const AttendArgs aa)
 {
     constexpr uint32_t kRows = 16u, kPitch = DP + 4u;
@@ -243,15 +243,24 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
     const uint32_t part = blockIdx.y, D = aa.pages.head_dim;
     const Cell cell = cell_of(aa, blockIdx.x, part);
     const uint32_t head = cell.head;
-    const RowTile t = find_tile<4>(aa, cell.tile);
+    RowTile t = find_tile<4, Span>(aa, cell.tile);
     if (!t.there) return;
-    // this part's keys
     constexpr int32_t kKeys = K::kKeys;
+    RowOf row;
+    if constexpr (Span == kSpanPrefix) {
+        row = row_of_tile<Span>(aa, t, head, i);
+        // (rows of several sequences: the first key that any of them sees)
+        int32_t low = i < t.rows ? row.lo : 0x7FFFFFFF;
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) low = min(low, __shfl_xor(low, d));
+        t.lo = __builtin_amdgcn_readfirstlane(min(low, t.hi));
+    }
+    // this part's keys
     const KeyPart keys_here = key_part(aa, t, part);
     const int32_t parts = keys_here.parts, begin = keys_here.begin, end = keys_here.end;
     if (int32_t(part) >= parts) return;
 
-    const RowOf row = row_of_tile(aa, t, head, i);
+    if constexpr (Span != kSpanPrefix) row = row_of_tile<Span>(aa, t, head, i);
     typename K::Query Q;
     K::load_query(Q, aa.q.data + (int64_t(row.token) * aa.q.token_stride + int64_t(row.head) * aa.q.head_stride) * K::kElem, i < t.rows, lane, D);
     const float scale = aa.scale * kLog2e;
@@ -530,7 +539,24 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
         }
     }
     if (m < t.rows) {
-        const RowOf r = row_of_tile(aa, t, head, m);
+        const RowOf r = row_of_tile<Span>(aa, t, head, m);
+        if constexpr (Span == kSpanPrefix) {
+            float *const to = prefix_sums(aa, r);
+#pragma unroll
+            for (uint32_t e = 0; e < kEach; e += 4)
+                if (d0 + e < D) *reinterpret_cast<f32x4 *>(to + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+            if (tid % 16u == 0u) *reinterpret_cast<f32x4 *>(to + D) = f32x4{most, sum, 0.f, 0.f};
+            return;
+        }
+        if (Span == kSpanRest && t.prefix) {
+            const float *const from = prefix_sums(aa, r);
+            const float other = from[D], top = fmaxf(most, other);
+            const float keep = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(most - top), by = other == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other - top);
+            sum = sum * keep + from[D + 1u] * by;
+#pragma unroll
+            for (uint32_t e = 0; e < kEach; ++e) acc[e] = acc[e] * keep + (d0 + e < D ? from[d0 + e] : 0.f) * by;
+            most = top;
+        }
         const bool any = !(sum == 0.f);
         const float by = any ? 1.f / sum : 0.f;
         typename K::T *og = reinterpret_cast<typename K::T *>(aa.out.data) + int64_t(r.token) * aa.out.token_stride + int64_t(r.head) * aa.out.head_stride;
@@ -541,38 +567,46 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
     }
 }
 
-template <class K, int DP>
-void launch(const AttendArgs &aa, hipStream_t s)
+template <class K, int DP, AttendSpan Span>
+void launch_span(const AttendArgs &aa, hipStream_t s)
 {
     const dim3 grid(aa.tiles * aa.heads.d, aa.splits);
-    if (aa.pages.page_tokens.d % 16u == 0u) attend_rows_kernel<K, true, DP><<<grid, dim3(64 * kRowWaves), 0, s>>>(aa);
-    else attend_rows_kernel<K, false, DP><<<grid, dim3(64 * kRowWaves), 0, s>>>(aa);
+    if (aa.pages.page_tokens.d % 16u == 0u) attend_rows_kernel<K, true, DP, Span><<<grid, dim3(64 * kRowWaves), 0, s>>>(aa);
+    else attend_rows_kernel<K, false, DP, Span><<<grid, dim3(64 * kRowWaves), 0, s>>>(aa);
+}
+
+template <class K, int DP>
+void launch(const AttendArgs &aa, AttendSpan span, hipStream_t s)
+{
+    if (span == kSpanAll) launch_span<K, DP, kSpanAll>(aa, s);
+    else if (span == kSpanPrefix) launch_span<K, DP, kSpanPrefix>(aa, s);
+    else launch_span<K, DP, kSpanRest>(aa, s);
 }
 
 template <bool BF, bool Past>
-void launch16(const AttendArgs &aa, hipStream_t s)
+void launch16(const AttendArgs &aa, AttendSpan span, hipStream_t s)
 {
     const uint32_t D = aa.pages.head_dim;
-    if (D <= 64u) launch<Rows16<BF, 64, Past>, 64>(aa, s);
-    else if (D <= 128u) launch<Rows16<BF, 128, Past>, 128>(aa, s);
-    else launch<Rows16<BF, 256, Past>, 256>(aa, s);
+    if (D <= 64u) launch<Rows16<BF, 64, Past>, 64>(aa, span, s);
+    else if (D <= 128u) launch<Rows16<BF, 128, Past>, 128>(aa, span, s);
+    else launch<Rows16<BF, 256, Past>, 256>(aa, span, s);
 }
 
 }  // namespace
 
-hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, bool past, hipStream_t s)
+hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, AttendSpan span, bool past, hipStream_t s)
 {
     const uint32_t D = aa.pages.head_dim;
     if (dtype == kDtypeF16) {
-        if (past) launch16<false, true>(aa, s);
-        else launch16<false, false>(aa, s);
+        if (past) launch16<false, true>(aa, span, s);
+        else launch16<false, false>(aa, span, s);
     } else if (dtype == kDtypeBf16) {
-        if (past) launch16<true, true>(aa, s);
-        else launch16<true, false>(aa, s);
+        if (past) launch16<true, true>(aa, span, s);
+        else launch16<true, false>(aa, span, s);
     } else {
-        if (D <= 64u) launch<Rows32<64>, 64>(aa, s);
-        else if (D <= 128u) launch<Rows32<128>, 128>(aa, s);
-        else launch<Rows32<256>, 256>(aa, s);
+        if (D <= 64u) launch<Rows32<64>, 64>(aa, span, s);
+        else if (D <= 128u) launch<Rows32<128>, 128>(aa, span, s);
+        else launch<Rows32<256>, 256>(aa, span, s);
     }
     return hipGetLastError();
 }

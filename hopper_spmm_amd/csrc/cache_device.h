@@ -39,6 +39,16 @@ struct RotaryArgs {
 // vec: elements that a lane moves at a time where a head's elements lie side by side everywhere, 0: through LDS, any strides
 hipError_t launch_rotary(int dtype, const RotaryArgs &ra, uint32_t vec, hipStream_t s);
 
+// Groups of a batch's rows that begin with the same tokens (hspmm_prefix).
+struct PrefixArgs {
+    const int32_t *firsts, *tokens;
+    uint32_t groups;
+    float *sums;                         // per token and head of queries: sums over the prefix (kPrefixExtra floats more than head_dim)
+};
+constexpr uint32_t kPrefixExtra = 4u;    // reference, total
+// Which keys an attention's launch has: all; those of the groups' prefixes; those behind them, after which the sums of both are added.
+enum AttendSpan { kSpanAll, kSpanPrefix, kSpanRest };
+
 struct AttendArgs {
     PagesArgs pages;
     BatchArgs batch;
@@ -52,6 +62,7 @@ struct AttendArgs {
     uint32_t splits, part_keys;          // parts that a tile's keys are cut into at most; keys of a part (a multiple of 32)
     float *sums;                         // of more than one part: their sums
     uint32_t *arrive;                    // and how many have left them (zero between launches)
+    PrefixArgs prefix;
 };
 // Tiles of (1 << rows_log) rows that a batch has at most (find_tile numbers them).
 constexpr uint32_t kAttendRowsLog = 4u;
@@ -63,9 +74,25 @@ constexpr uint32_t kAttendCounters = 16384u;
 // floats of a part of a tile's sums
 inline uint32_t attend_slot(uint32_t rows_log, uint32_t head_dim) { return (1u << rows_log) * ((head_dim <= 64u ? 64u : head_dim <= 128u ? 128u : 256u) + 4u); }
 // past: 16-bit keys and values are not kept in the L2
-hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, bool past, hipStream_t s);
+hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, AttendSpan span, bool past, hipStream_t s);
 // 16-bit types; tiles of 1 << rows_log rows: 128, or 256 for heads of up to 128 elements
-hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, uint32_t rows_log, hipStream_t s);
+hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, AttendSpan span, uint32_t rows_log, hipStream_t s);
+
+// Attention weights that cached keys have received.
+struct WeighArgs {
+    PagesArgs pages;
+    BatchArgs batch;
+    HeadsArgs q;
+    const float *lse;
+    uint32_t q_heads;
+    Divisor shared, heads;               // heads of queries to one of keys; heads of keys
+    float scale, decay;
+    uint32_t causal, window, last;       // last: tokens of a chunk that count, 0: all
+    float *weights;                      // of the layer
+    int64_t sequence_stride, head_stride;
+    uint32_t parts;                      // workgroups that share out a sequence's keys
+};
+hipError_t launch_weigh_rows(int dtype, const WeighArgs &wa, hipStream_t s);
 
 // Page work: all layers.
 struct PoolArgs {
@@ -82,6 +109,30 @@ hipError_t launch_pages_extend(const PoolArgs &pa, uint32_t n, const int32_t *ro
 hipError_t launch_pages_fork(const PoolArgs &pa, uint32_t n, const int32_t *parents, const int32_t *children, int32_t *status, hipStream_t s);
 hipError_t launch_pages_free(const PoolArgs &pa, uint32_t n, const int32_t *rows, hipStream_t s);
 hipError_t launch_pages_compact(const PoolArgs &pa, int32_t *table_out, int32_t *references_out, int32_t *live, hipStream_t s);
+// What an eviction is asked for, and where it notes things between its launches.
+struct EvictArgs {
+    uint32_t n;
+    const int32_t *parents, *children;
+    uint32_t keep, first, last;
+    float *weights;
+    int64_t weights_layer, weights_sequence, weights_head;       // strides
+    int32_t *kept, *status;
+    uint32_t *arrive;                    // zero between calls
+    int32_t *entries;                    // of every entry of the list: EvictEntry
+    int32_t *rows;                       // its parent's row of the table
+    int32_t *to;                         // the pages its tokens go to: a page, or below 0, -1 - k: the k-th of its new ones
+    int32_t *free;                       // free pages
+    float *kept_weights;                 // layers x entries x heads x keep
+    uint32_t keep_pages;                 // of `keep` tokens
+};
+constexpr uint32_t kEvictEntry = 8u;     // words of an entry
+// Workgroups that share out keys, and values, of a layer, an entry and a head: as many as give a small call some thousand, of 64 bytes of a token at least.
+inline uint32_t evict_shares(const PoolArgs &pa, uint64_t cells)
+{
+    const uint64_t wanted = cells < 2048u ? 2048u / (cells ? cells : 1u) : 1u, most = pa.token_bytes / 64u;
+    return uint32_t(wanted < most ? wanted : most ? most : 1u);
+}
+hipError_t launch_evict(const PoolArgs &pa, const EvictArgs &ea, hipStream_t s);
 hipError_t launch_pages_copy(const PoolArgs &pa, uint32_t n, const int32_t *from, const int32_t *to, hipStream_t s);
 
 #ifdef __HIPCC__

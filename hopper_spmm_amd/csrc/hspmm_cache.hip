@@ -276,6 +276,14 @@ int hspmm_cache_append(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     return run_rotary(cache->dtype, ra, cache, stream);
 }
 
+static int check_queries(const hspmm_cache *c, const hspmm_heads *q)
+{
+    const uint32_t piece = 16u / element_bytes(c->dtype);
+    if (q->dim_stride != 1 || q->token_stride % piece || q->head_stride % piece || reinterpret_cast<uintptr_t>(q->data) % 16u)
+        return fail(HSPMM_ERR_UNSUPPORTED, "q: a head's elements side by side, tokens and heads at multiples of 16 bytes");
+    return HSPMM_OK;
+}
+
 static int check_attention(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
 {
     if (int rc = check_cache(c)) return rc;
@@ -300,14 +308,13 @@ struct AttendShape {
     uint64_t bytes;
 };
 
-static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
+// sequences: of a batch, or groups of them; chunk: the most tokens that one has; keys: the most that one sees.
+static AttendShape attend_shape(const hspmm_cache *c, uint32_t sequences, uint32_t tokens, uint32_t chunk, uint64_t keys, const hspmm_attention *a)
 {
     const uint32_t shared = a->q_heads / c->heads;
-    const uint64_t rows = uint64_t(std::min(a->longest_chunk, b->tokens)) * shared;
+    const uint64_t rows = uint64_t(std::min(chunk, tokens)) * shared;
     AttendShape sh{};
-    // keys that a sequence's tokens see at most, and those of a tile of so many rows
-    uint64_t keys = uint64_t(c->table_pages) * c->page_tokens;
-    if (a->longest && a->longest < keys) keys = a->longest;
+    // those that a tile of so many rows sees
     auto seen = [&](uint32_t tile_rows) { return a->window && uint64_t(a->window) + tile_rows < keys ? uint64_t(a->window) + tile_rows : keys; };
     // The rows kernel for up to 16 rows, and where there is little to do: a tile of it is sixteen rows, and its waves share out the keys.  us of it / of the
     // chunk kernel by tiles of 16 rows x heads x keys, bf16, heads of 128: 8 K (60 tokens from the beginning, 32 heads) 6.6 / 9.7; 96 K (8 tokens for each of
@@ -316,21 +323,21 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     // 16000) 48.3 / 44.4; 640 K (64 over 20000, 8 heads on 4) 67.5 / 54.4; 1024 K (32 of 2000) 82 / 70; 1600 K (16 ragged chunks) 65 / 33.  Up to 400 K it lost
     // at 4 of 24 such shapes, by 10 % at most (400 tokens from the beginning 19.9 / 18.1), above 500 K at 11 of 18, by up to a half; of 256 elements it won at
     // 304 K (59.5 / 74) and lost at 480 K (80 / 77).
-    const uint64_t rows_work = uint64_t(b->sequences) * ((rows + 15u) / 16u) * c->heads * seen(16u);
+    const uint64_t rows_work = uint64_t(sequences) * ((rows + 15u) / 16u) * c->heads * seen(16u);
     // 256 rows for heads of 97 to 128 elements only - with 128 rows two workgroups share a compute unit, but there only two images fit for each -, where chunks
     // are of one length, tiles for a quarter of the compute units and keys for parts on all of them: few, short and half-filled tiles are the longer ones' loss.  us
     // with 128 / 256 rows, by heads x tiles of 256 (`wide`), 32 heads on 8: 4096 tokens over 16384 keys (520) 1025 / 942; 8192 over 8192 (1032) 597 / 571; 2048 over
     // 8192 (264) 281 / 266; 1024 over 4096 (136) 96 / 82; 512 over 8512 (72) 105 / 99; 16 x 512 over 2000 (1088) 232 / 237; 2048 over 2048 (264) 67 / 71; 500 over
     // 500, 32 heads of keys (64) 22 / 27; few tiles: 256 over 8192 (40) 58 / 60, 700 over 20000, 8 heads on 4 (24) 85 / 103; ragged: 17 chunks of up to 700 over up
     // to 5700 (592) 216 / 279, 16 of up to 300 over 600 (664) 44 / 50, 8 of up to 300 over 2000 (328) 73 / 68.  Heads of 64, 2048 tokens over 8048, 177 / 184.
-    const uint64_t wide = uint64_t(c->heads) * ((uint64_t(b->tokens) * shared >> 8) + (b->sequences + 1u) / 2u);
-    const bool even = uint64_t(b->tokens) * 8u >= uint64_t(b->sequences) * std::min(a->longest_chunk, b->tokens) * 7u;
+    const uint64_t wide = uint64_t(c->heads) * ((uint64_t(tokens) * shared >> 8) + (sequences + 1u) / 2u);
+    const bool even = uint64_t(tokens) * 8u >= uint64_t(sequences) * std::min(chunk, tokens) * 7u;
     if (c->dtype == HSPMM_TF32 || rows <= 16u || rows_work <= 400000u) sh.rows_log = kAttendRowsLog;
     else sh.rows_log = c->head_dim > 96u && c->head_dim <= 128u && rows > 128u && even && wide >= 64u && wide * seen(256u) >= 200000u ? 8u : 7u;
     keys = seen(1u << sh.rows_log);
-    const uint64_t numbered = attend_tiles(b->tokens, b->sequences, shared, sh.rows_log);
+    const uint64_t numbered = attend_tiles(tokens, sequences, shared, sh.rows_log);
     // tiles that have rows, at most: numbers are left out
-    const uint64_t tiles = std::min<uint64_t>(numbered, uint64_t(b->sequences) * ((rows + (1u << sh.rows_log) - 1u) >> sh.rows_log));
+    const uint64_t tiles = std::min<uint64_t>(numbered, uint64_t(sequences) * ((rows + (1u << sh.rows_log) - 1u) >> sh.rows_log));
     // Keys of a part.  Rows kernel: as few as give every compute unit two workgroups, 128 at least (every wave a tile or two) and 512 at most, more only
     // where that is over 4096 workgroups: sequences are of many lengths, and the last ones should not be long.  us by parts of 128 / 256 / 512 keys: one token
     // over 1000 keys, 8 heads 8.1 / 9.2 / 11.9; over 30000 58 / 39 / 30; 8 sequences of up to 8000 56 / 44 / 42.
@@ -355,6 +362,46 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     return sh;
 }
 
+// Keys that a sequence may have, as far as the call says.
+static uint64_t most_keys(const hspmm_cache *c, uint32_t longest)
+{
+    const uint64_t places = uint64_t(c->table_pages) * c->page_tokens;
+    return longest && longest < places ? longest : places;
+}
+
+static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
+{
+    return attend_shape(c, b->sequences, b->tokens, a->longest_chunk, most_keys(c, a->longest), a);
+}
+
+// An attention over shared prefixes: two launches, of the prefixes with a group for a sequence, and of what is behind them.
+struct SharedShape {
+    AttendShape prefix, rest;
+    uint64_t parts_bytes, bytes;         // of the workspace: counters and sums of parts, which the launches have in turn; with the prefixes' sums behind them
+};
+
+static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, const hspmm_prefix *p, const hspmm_attention *a)
+{
+    SharedShape sh{};
+    const uint64_t all = most_keys(c, a->longest), common = std::min<uint64_t>(p->longest ? p->longest : all, all);
+    hspmm_attention whole = *a;
+    whole.window = 0u;
+    sh.prefix = attend_shape(c, p->groups, b->tokens, p->most_tokens ? p->most_tokens : b->tokens, common, &whole);
+    // (keys behind the prefix: the longest sequence is taken to have the longest one)
+    sh.rest = attend_shape(c, b->sequences, b->tokens, a->longest_chunk, std::max<uint64_t>(all - common, std::min<uint64_t>(std::max(a->longest_chunk, 1u), all)), a);
+    sh.parts_bytes = (std::max(sh.prefix.bytes, sh.rest.bytes) + 15u) & ~uint64_t(15u);
+    sh.bytes = sh.parts_bytes + uint64_t(b->tokens) * a->q_heads * (c->head_dim + kPrefixExtra) * 4u;
+    return sh;
+}
+
+static int check_prefix(const hspmm_batch *b, const hspmm_prefix *p)
+{
+    if (!p) return fail(HSPMM_ERR_INVALID, "null prefix");
+    if (p->groups > b->sequences) return fail(HSPMM_ERR_INVALID, "%u groups of %u sequences", p->groups, b->sequences);
+    if (p->groups && (!p->firsts || !p->tokens)) return fail(HSPMM_ERR_INVALID, "%u groups without their sequences or tokens", p->groups);
+    return HSPMM_OK;
+}
+
 // (a launch has fewer than 2^32 threads, 512 a workgroup at most)
 static int check_tiles(const hspmm_cache *c, const hspmm_batch *b, const AttendShape &sh)
 {
@@ -372,23 +419,22 @@ int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *ba
     return check_tiles(cache, batch, sh);
 }
 
-int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_attention *attention, const hspmm_heads *q,
-                       const hspmm_heads *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream)
+}  // extern "C"
+
+// What an attention's calls check alike.
+static int check_attend_tensors(const hspmm_cache *cache, uint32_t layer, const hspmm_heads *q, const hspmm_heads *out, const float *lse)
 {
-    if (int rc = check_attention(cache, batch, attention)) return rc;
     if (layer >= cache->layers) return fail(HSPMM_ERR_INVALID, "layer %u of %u", layer, cache->layers);
-    if (batch->tokens == 0) return HSPMM_OK;
-    const uint32_t e = element_bytes(cache->dtype), piece = 16u / e;
     if (int rc = check_heads("q", q, cache->dtype)) return rc;
     if (int rc = check_heads("out", out, cache->dtype)) return rc;
-    if (q->dim_stride != 1 || q->token_stride % piece || q->head_stride % piece || reinterpret_cast<uintptr_t>(q->data) % 16u)
-        return fail(HSPMM_ERR_UNSUPPORTED, "q: a head's elements side by side, tokens and heads at multiples of 16 bytes");
+    if (int rc = check_queries(cache, q)) return rc;
     if (reinterpret_cast<uintptr_t>(lse) % 4u) return fail(HSPMM_ERR_INVALID, "lse is not aligned to its elements");
-    const AttendShape sh = attend_shape(cache, batch, attention);
-    if (int rc = check_tiles(cache, batch, sh)) return rc;
-    if (sh.bytes && (!workspace || workspace_bytes < sh.bytes || reinterpret_cast<uintptr_t>(workspace) % 16u))
-        return fail(HSPMM_ERR_INVALID, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)sh.bytes);
-    if (int rc = check_device()) return rc;
+    return HSPMM_OK;
+}
+
+static AttendArgs attend_args(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_attention *attention, const hspmm_heads *q,
+                              const hspmm_heads *out, float *lse, const AttendShape &sh, void *workspace)
+{
     AttendArgs aa{};
     aa.pages = pages_of(cache, layer);
     aa.batch = batch_of(batch);
@@ -398,8 +444,74 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     aa.heads = Divisor::of(cache->heads); aa.tiles = sh.tiles; aa.splits = sh.splits; aa.part_keys = sh.part_keys;
     aa.arrive = static_cast<uint32_t *>(workspace);
     aa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + kAttendCounters * 4u);
-    if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, sh.past, static_cast<hipStream_t>(stream)));
-    else HSPMM_HIP(launch_attend_chunk(cache->dtype, aa, sh.rows_log, static_cast<hipStream_t>(stream)));
+    return aa;
+}
+
+static hipError_t launch_attend(int dtype, const AttendArgs &aa, AttendSpan span, const AttendShape &sh, void *stream)
+{
+    if (sh.rows_log == kAttendRowsLog) return launch_attend_rows(dtype, aa, span, sh.past, static_cast<hipStream_t>(stream));
+    return launch_attend_chunk(dtype, aa, span, sh.rows_log, static_cast<hipStream_t>(stream));
+}
+
+static int check_workspace(const void *workspace, uint64_t bytes, uint64_t wanted)
+{
+    if (wanted && (!workspace || bytes < wanted || reinterpret_cast<uintptr_t>(workspace) % 16u))
+        return fail(HSPMM_ERR_INVALID, "a workspace of %llu bytes, aligned to 16, is wanted", (unsigned long long)wanted);
+    return HSPMM_OK;
+}
+
+extern "C" {
+
+int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_attention *attention, const hspmm_heads *q,
+                       const hspmm_heads *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream)
+{
+    if (int rc = check_attention(cache, batch, attention)) return rc;
+    if (layer >= cache->layers) return fail(HSPMM_ERR_INVALID, "layer %u of %u", layer, cache->layers);
+    if (batch->tokens == 0) return HSPMM_OK;
+    if (int rc = check_attend_tensors(cache, layer, q, out, lse)) return rc;
+    const AttendShape sh = attend_shape(cache, batch, attention);
+    if (int rc = check_tiles(cache, batch, sh)) return rc;
+    if (int rc = check_workspace(workspace, workspace_bytes, sh.bytes)) return rc;
+    if (int rc = check_device()) return rc;
+    const AttendArgs aa = attend_args(cache, layer, batch, attention, q, out, lse, sh, workspace);
+    HSPMM_HIP(launch_attend(cache->dtype, aa, kSpanAll, sh, stream));
+    return HSPMM_OK;
+}
+
+int hspmm_cache_attend_shared_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_prefix *prefix, const hspmm_attention *attention, uint64_t *bytes)
+{
+    if (!bytes) return fail(HSPMM_ERR_INVALID, "null bytes");
+    if (int rc = check_attention(cache, batch, attention)) return rc;
+    if (int rc = check_prefix(batch, prefix)) return rc;
+    if (prefix->groups == 0) return hspmm_cache_attend_workspace(cache, batch, attention, bytes);
+    if (batch->tokens == 0) { *bytes = 0; return HSPMM_OK; }
+    const SharedShape sh = shared_shape(cache, batch, prefix, attention);
+    *bytes = sh.bytes;
+    if (int rc = check_tiles(cache, batch, sh.prefix)) return rc;
+    return check_tiles(cache, batch, sh.rest);
+}
+
+int hspmm_cache_attend_shared(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_prefix *prefix, const hspmm_attention *attention,
+                              const hspmm_heads *q, const hspmm_heads *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream)
+{
+    if (int rc = check_attention(cache, batch, attention)) return rc;
+    if (int rc = check_prefix(batch, prefix)) return rc;
+    if (prefix->groups == 0) return hspmm_cache_attend(cache, layer, batch, attention, q, out, lse, workspace, workspace_bytes, stream);
+    if (layer >= cache->layers) return fail(HSPMM_ERR_INVALID, "layer %u of %u", layer, cache->layers);
+    if (batch->tokens == 0) return HSPMM_OK;
+    if (int rc = check_attend_tensors(cache, layer, q, out, lse)) return rc;
+    const SharedShape sh = shared_shape(cache, batch, prefix, attention);
+    if (int rc = check_tiles(cache, batch, sh.prefix)) return rc;
+    if (int rc = check_tiles(cache, batch, sh.rest)) return rc;
+    if (int rc = check_workspace(workspace, workspace_bytes, sh.bytes)) return rc;
+    if (int rc = check_device()) return rc;
+    const PrefixArgs pa{prefix->firsts, prefix->tokens, prefix->groups, reinterpret_cast<float *>(static_cast<char *>(workspace) + sh.parts_bytes)};
+    AttendArgs aa = attend_args(cache, layer, batch, attention, q, out, lse, sh.prefix, workspace);
+    aa.prefix = pa;
+    HSPMM_HIP(launch_attend(cache->dtype, aa, kSpanPrefix, sh.prefix, stream));
+    aa = attend_args(cache, layer, batch, attention, q, out, lse, sh.rest, workspace);
+    aa.prefix = pa;
+    HSPMM_HIP(launch_attend(cache->dtype, aa, kSpanRest, sh.rest, stream));
     return HSPMM_OK;
 }
 
@@ -441,6 +553,142 @@ int hspmm_cache_compact(const hspmm_cache *cache, int32_t *table_out, int32_t *r
     if (int rc = check_device()) return rc;
     HSPMM_HIP(launch_pages_compact(pool_of(cache), table_out ? table_out : cache->table, references_out ? references_out : cache->references, live,
                                    static_cast<hipStream_t>(stream)));
+    return HSPMM_OK;
+}
+
+}  // extern "C"
+
+static int check_weights(const hspmm_weights *w)
+{
+    if (!w || !w->data) return fail(HSPMM_ERR_INVALID, "null weights");
+    if (reinterpret_cast<uintptr_t>(w->data) % 4u) return fail(HSPMM_ERR_INVALID, "weights are not aligned to their elements");
+    if (w->layer_stride < 0 || w->sequence_stride < 0 || w->head_stride < 0) return fail(HSPMM_ERR_INVALID, "weights: strides below 0");
+    return HSPMM_OK;
+}
+
+// The workgroups of a sequence's keys, for every head: a wave has a tile of 32 keys or some.
+static uint32_t weigh_parts(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
+{
+    const uint64_t blocks = (most_keys(c, a->longest) + 127u) / 128u, cells = uint64_t(b->sequences) * c->heads;
+    const uint64_t parts = std::max<uint64_t>(std::min<uint64_t>(blocks, 8192u / std::max<uint64_t>(cells, 1u)), 1u);
+    return uint32_t(std::min<uint64_t>(parts, 32768u));
+}
+
+static int check_weigh(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
+{
+    if (int rc = check_attention(c, b, a)) return rc;
+    // (a launch has fewer than 2^32 threads)
+    if (uint64_t(b->sequences) * c->heads >= (1u << 23)) return fail(HSPMM_ERR_UNSUPPORTED, "%u sequences with %u heads of keys: in several calls", b->sequences, c->heads);
+    return HSPMM_OK;
+}
+
+extern "C" {
+
+int hspmm_cache_weigh_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_attention *attention, uint32_t last, uint64_t *bytes)
+{
+    (void)last;
+    if (!bytes) return fail(HSPMM_ERR_INVALID, "null bytes");
+    if (int rc = check_weigh(cache, batch, attention)) return rc;
+    *bytes = 0;
+    return HSPMM_OK;
+}
+
+int hspmm_cache_weigh(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_attention *attention, const hspmm_heads *q, const float *lse,
+                      const hspmm_weights *weights, float decay, uint32_t last, void *workspace, uint64_t workspace_bytes, void *stream)
+{
+    if (int rc = check_weigh(cache, batch, attention)) return rc;
+    if (layer >= cache->layers) return fail(HSPMM_ERR_INVALID, "layer %u of %u", layer, cache->layers);
+    if (!std::isfinite(decay)) return fail(HSPMM_ERR_INVALID, "decay %g", double(decay));
+    if (int rc = check_weights(weights)) return rc;
+    if (batch->tokens == 0) return HSPMM_OK;
+    if (int rc = check_heads("q", q, cache->dtype)) return rc;
+    if (int rc = check_queries(cache, q)) return rc;
+    if (!lse || reinterpret_cast<uintptr_t>(lse) % 4u) return fail(HSPMM_ERR_INVALID, "lse is null or not aligned to its elements");
+    if (int rc = check_workspace(workspace, workspace_bytes, 0u)) return rc;
+    if (int rc = check_device()) return rc;
+    WeighArgs wa{};
+    wa.pages = pages_of(cache, layer);
+    wa.batch = batch_of(batch);
+    wa.q = heads_of(q); wa.lse = lse;
+    wa.q_heads = attention->q_heads; wa.shared = Divisor::of(attention->q_heads / cache->heads); wa.heads = Divisor::of(cache->heads);
+    wa.scale = attention->scale; wa.decay = decay; wa.causal = attention->causal != 0; wa.window = attention->window; wa.last = last;
+    wa.weights = weights->data + weights->layer_stride * layer;
+    wa.sequence_stride = weights->sequence_stride; wa.head_stride = weights->head_stride;
+    wa.parts = weigh_parts(cache, batch, attention);
+    HSPMM_HIP(launch_weigh_rows(cache->dtype, wa, static_cast<hipStream_t>(stream)));
+    return HSPMM_OK;
+}
+
+}  // extern "C"
+
+// Words of an eviction's workspace, one behind another.
+struct EvictShape { uint64_t arrive, entries, rows, to, free, kept, weights, words; uint32_t keep_pages; };
+
+static EvictShape evict_shape(const hspmm_cache *c, uint32_t n, uint32_t keep)
+{
+    EvictShape sh{};
+    sh.keep_pages = (keep + c->page_tokens - 1u) / c->page_tokens;
+    const uint64_t lists = uint64_t(c->layers) * n * c->heads * keep, pages = uint64_t(n) * sh.keep_pages;
+    sh.entries = sh.arrive + 16u;
+    sh.rows = sh.entries + uint64_t(n) * kEvictEntry;
+    sh.to = sh.rows + uint64_t(n) * c->table_pages;
+    sh.free = sh.to + pages;
+    sh.kept = sh.free + std::min<uint64_t>(pages, c->pages);
+    sh.weights = sh.kept + lists;
+    sh.words = sh.weights + lists;
+    return sh;
+}
+
+static int check_eviction(const hspmm_cache *c, uint32_t n, uint32_t keep)
+{
+    if (int rc = check_cache(c)) return rc;
+    if (n > c->sequences) return fail(HSPMM_ERR_INVALID, "a list of %u for a cache of %u sequences", n, c->sequences);
+    if (!keep || keep > uint64_t(c->table_pages) * c->page_tokens) return fail(HSPMM_ERR_INVALID, "%u tokens to keep, of at most %llu", keep, (unsigned long long)c->table_pages * c->page_tokens);
+    // (a launch has fewer than 2^32 threads, 1024 a workgroup, or 256 and up to 2 x 16384 + 1 workgroups a head)
+    const uint64_t cells = uint64_t(n) * c->layers * c->heads;
+    PoolArgs pa{};
+    pa.token_bytes = c->head_dim * element_bytes(c->dtype);
+    if (n + cells >= (1u << 22) || n + cells * (2u * evict_shares(pa, cells) + 1u) >= (1u << 24)) return fail(HSPMM_ERR_UNSUPPORTED, "a list of %u: in several calls", n);
+    return HSPMM_OK;
+}
+
+extern "C" {
+
+int hspmm_cache_evict_workspace(const hspmm_cache *cache, uint32_t n, uint32_t keep, uint64_t *bytes)
+{
+    if (!bytes) return fail(HSPMM_ERR_INVALID, "null bytes");
+    if (int rc = check_eviction(cache, n, keep)) return rc;
+    *bytes = n ? evict_shape(cache, n, keep).words * 4u : 0u;
+    return HSPMM_OK;
+}
+
+int hspmm_cache_evict(const hspmm_cache *cache, uint32_t n, const int32_t *parents, const int32_t *children, const hspmm_weights *weights, uint32_t keep, uint32_t first,
+                      uint32_t last, int32_t *kept, int32_t *status, void *workspace, uint64_t workspace_bytes, void *stream)
+{
+    if (int rc = check_eviction(cache, n, keep)) return rc;
+    if (int rc = check_list(cache, n, parents, "parents")) return rc;
+    if (int rc = check_weights(weights)) return rc;
+    if (uint64_t(first) + last > keep) return fail(HSPMM_ERR_INVALID, "the first %u and the last %u tokens, of %u to keep", first, last, keep);
+    if (n == 0 && !status) return HSPMM_OK;
+    const EvictShape sh = evict_shape(cache, n, keep);
+    if (n)
+        if (int rc = check_workspace(workspace, workspace_bytes, sh.words * 4u)) return rc;
+    if (int rc = check_device()) return rc;
+    // (of nothing there is the status alone)
+    if (n == 0) {
+        HSPMM_HIP(launch_pages_extend(pool_of(cache), 0u, nullptr, nullptr, status, static_cast<hipStream_t>(stream)));
+        return HSPMM_OK;
+    }
+    int32_t *const words = static_cast<int32_t *>(workspace);
+    EvictArgs ea{};
+    ea.n = n; ea.parents = parents; ea.children = children; ea.keep = keep; ea.first = first; ea.last = last;
+    ea.weights = weights->data; ea.weights_layer = weights->layer_stride; ea.weights_sequence = weights->sequence_stride; ea.weights_head = weights->head_stride;
+    ea.kept = kept ? kept : words + sh.kept; ea.status = status;
+    ea.arrive = reinterpret_cast<uint32_t *>(words + sh.arrive);
+    ea.entries = words + sh.entries; ea.rows = words + sh.rows; ea.to = words + sh.to; ea.free = words + sh.free;
+    ea.kept_weights = reinterpret_cast<float *>(words + sh.weights);
+    ea.keep_pages = sh.keep_pages;
+    HSPMM_HIP(launch_evict(pool_of(cache), ea, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
 

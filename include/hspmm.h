@@ -613,6 +613,39 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
                        const hspmm_heads *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream);
 int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_attention *attention, uint64_t *bytes);
 
+/* Groups of a batch's rows whose sequences begin with the same tokens (a system prompt, the prompt of several beams):
+ * rows firsts[g] .. firsts[g + 1] - 1 of the batch share the first tokens[g] tokens, which are read by the table row of the group's
+ * first sequence, once for all of them (at most the tokens that it holds).  The other sequences' own pages of these
+ * tokens are not read.  Rows of the batch that are in no group share nothing.  firsts ascends.
+ * most_tokens: the most tokens of the batch that a group has; longest: of a prefix (0: not known); they choose kernels and how the work
+ * is split, the result is right whatever they are. */
+typedef struct hspmm_prefix {
+    uint32_t groups, most_tokens, longest;
+    const int32_t *firsts, *tokens;
+} hspmm_prefix;
+/* hspmm_cache_attend with the groups' prefixes read once.  No groups: the same call. */
+int hspmm_cache_attend_shared(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_prefix *prefix, const hspmm_attention *attention,
+                              const hspmm_heads *q, const hspmm_heads *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream);
+int hspmm_cache_attend_shared_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_prefix *prefix, const hspmm_attention *attention, uint64_t *bytes);
+
+/* The attention weight that cached keys have received: floats, layers x sequences x heads (of keys) at these strides (in
+ * floats), a head's tokens side by side: those that a sequence holds, for hspmm_cache_evict table_pages * page_tokens of them.  The
+ * caller's, zero at first; a row follows its sequence through hspmm_cache_evict, and is the caller's to copy or to clear where a
+ * sequence is forked or freed. */
+typedef struct hspmm_weights {
+    float *data;
+    int64_t layer_stride, sequence_stride, head_stride;
+} hspmm_weights;
+/* weights of `layer` <- decay * weights + sum over the batch's tokens, and the query heads that share a head of keys, of
+ * exp(scale * q k - lse), for every key of the batch's sequences; the batch's own tokens begin with 0, what is behind a
+ * sequence's last token stays as it is.  What a token does not see, or has no page, receives nothing from it.
+ * q, lse: those of hspmm_cache_attend (or _shared), with the same attention.  last: of a sequence's tokens in the batch only that
+ * many last ones count (0: all).  Products as in attend, the rest in fp32.
+ * workspace: as for attend, of hspmm_cache_weigh_workspace bytes; zero before its first use. */
+int hspmm_cache_weigh(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_attention *attention, const hspmm_heads *q, const float *lse,
+                      const hspmm_weights *weights, float decay, uint32_t last, void *workspace, uint64_t workspace_bytes, void *stream);
+int hspmm_cache_weigh_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_attention *attention, uint32_t last, uint64_t *bytes);
+
 /* Pages.  Pages that a call gives out are the free ones of lowest number, in the order of the call's list and of the
  * places in a row; *status (may be null) receives how many were missing: their places are -1 and hold nothing.
  * Pages that a row has no place for are among the missing; the tokens are counted in lengths and are neither stored nor seen.
@@ -626,6 +659,20 @@ int hspmm_cache_extend(const hspmm_cache *cache, uint32_t n, const int32_t *rows
 int hspmm_cache_fork(const hspmm_cache *cache, uint32_t n, const int32_t *parents, const int32_t *children, int32_t *status, void *stream);
 /* Sequences rows[i] have no tokens any more; pages that nobody else names are free. */
 int hspmm_cache_free(const hspmm_cache *cache, uint32_t n, const int32_t *rows, void *stream);
+/* Sequence children[i] (children null: the parent itself) becomes what sequence parents[i] was before the call, with no more than
+ * `keep` of its tokens.  Of the tokens that have pages every layer and head of keys keeps, by itself, the first `first`, the last `last` and of the
+ * others those of the greatest weights; ties go to the lowest number, NaN is less than anything.  (Tokens without a page are
+ * dropped; `first` and `last` count them.)  What is kept stays in order and takes the slots from 0 on; the weights move with it,
+ * behind them the child's are 0.  Keys are not turned again: where positions matter later tokens are turned by hspmm_rotate with
+ * their own, and appended as they are.
+ * A sequence that is its own child and has no more than `keep` tokens stays as it is; one with more is rewritten in the pages it has, but for those that
+ * others name as well, or where it is another entry's parent, too: there, and for other children, pages are given out.  A child that the pool has no pages for stays as it was; *status
+ * receives how many pages were missing.  Pages released become free as in hspmm_cache_fork.
+ * kept (layers x n x heads x keep, may be null): the numbers of the tokens kept, -1 behind them.
+ * workspace: hspmm_cache_evict_workspace bytes, aligned to 16 bytes; zero before its first use, and not used by two calls that overlap in time. */
+int hspmm_cache_evict(const hspmm_cache *cache, uint32_t n, const int32_t *parents, const int32_t *children, const hspmm_weights *weights, uint32_t keep, uint32_t first,
+                      uint32_t last, int32_t *kept, int32_t *status, void *workspace, uint64_t workspace_bytes, void *stream);
+int hspmm_cache_evict_workspace(const hspmm_cache *cache, uint32_t n, uint32_t keep, uint64_t *bytes);
 /* Moves the live pages to the low end of the pool: those at or above their number go to the free ones below it, both in
  * ascending order.  *live (may be null) receives that number.  table_out, references_out: null, or where the new
  * ones go, the old ones staying. */

@@ -5,22 +5,6 @@ namespace hspmm {
 
 namespace {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-template <bool BF> struct Wide;
-template <> struct Wide<false> {
-    __device__ static __forceinline__ f32x16 mfma(const u32x4 a, const u32x4 b, const f32x16 c)
-    {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
-    }
-};
-template <> struct Wide<true> {
-    __device__ static __forceinline__ f32x16 mfma(const u32x4 a, const u32x4 b, const f32x16 c)
-    {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-    }
-};
-
 // A workgroup's LDS writes are done and every wave is here (loads from memory may be on their way).
 __device__ __forceinline__ void lds_barrier()
 {

@@ -90,9 +90,16 @@ struct WeighArgs {
     uint32_t causal, window, last;       // last: tokens of a chunk that count, 0: all
     float *weights;                      // of the layer
     int64_t sequence_stride, head_stride;
-    uint32_t parts;                      // workgroups that share out a sequence's keys
+    uint32_t parts;                      // rows kernel: workgroups that share out a sequence's keys; chunk kernel: parts of the rows, at most
+    Divisor blocks;                      // chunk kernel: of kWeighKeys keys, of the longest sequence that the call speaks of
+    uint32_t part_rows;                  // rows of a part
+    float *sums;                         // of more than one part: their sums
+    uint32_t *arrive;                    // and how many have left them (zero between launches)
 };
 hipError_t launch_weigh_rows(int dtype, const WeighArgs &wa, hipStream_t s);
+constexpr uint32_t kWeighKeys = 128u;    // of a workgroup of the chunk kernel
+// 16-bit types
+hipError_t launch_weigh_chunk(int dtype, const WeighArgs &wa, hipStream_t s);
 
 // Page work: all layers.
 struct PoolArgs {

@@ -566,12 +566,32 @@ static int check_weights(const hspmm_weights *w)
     return HSPMM_OK;
 }
 
-// The workgroups of a sequence's keys, for every head: a wave has a tile of 32 keys or some.
-static uint32_t weigh_parts(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
+// How a call of hspmm_cache_weigh is launched, by sizes alone: the same for the call and for its workspace.
+struct WeighShape {
+    bool chunk;                          // by the chunk kernel
+    uint32_t parts, blocks, part_rows;
+    uint64_t cells, bytes;
+};
+
+static WeighShape weigh_shape(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a, uint32_t last)
 {
-    const uint64_t blocks = (most_keys(c, a->longest) + 127u) / 128u, cells = uint64_t(b->sequences) * c->heads;
-    const uint64_t parts = std::max<uint64_t>(std::min<uint64_t>(blocks, 8192u / std::max<uint64_t>(cells, 1u)), 1u);
-    return uint32_t(std::min<uint64_t>(parts, 32768u));
+    WeighShape sh{};
+    const uint64_t keys = most_keys(c, a->longest), heads = uint64_t(b->sequences) * c->heads;
+    const uint64_t tokens = std::min(a->longest_chunk, b->tokens), rows = std::max<uint64_t>((last && last < tokens ? last : tokens) * (a->q_heads / c->heads), 1u);
+    auto up = [](uint64_t n, uint64_t to) { return (n + to - 1u) / to; };
+    sh.chunk = c->dtype != HSPMM_TF32 && rows > 16u;
+    if (!sh.chunk) {
+        // a wave has a tile of 32 keys or some
+        sh.parts = uint32_t(std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(up(keys, 128u), 8192u / std::max<uint64_t>(heads, 1u)), 1u), 32768u));
+        return sh;
+    }
+    sh.blocks = uint32_t(std::min<uint64_t>(up(keys, kWeighKeys), std::max<uint64_t>((uint64_t(1) << 22) / std::max<uint64_t>(heads, 1u), 1u)));
+    sh.cells = heads * sh.blocks;
+    // parts of the rows: as many as make some thousand workgroups, 256 rows at least
+    sh.part_rows = uint32_t(std::max<uint64_t>(up(up(rows * sh.cells, 1536u), 64u) * 64u, 256u));
+    sh.parts = uint32_t(std::min<uint64_t>(up(rows, sh.part_rows), 256u));
+    if (sh.parts > 1u) sh.bytes = ((sh.cells * 4u + 15u) & ~uint64_t(15u)) + sh.cells * sh.parts * kWeighKeys * 4u;
+    return sh;
 }
 
 static int check_weigh(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a)
@@ -586,10 +606,9 @@ extern "C" {
 
 int hspmm_cache_weigh_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_attention *attention, uint32_t last, uint64_t *bytes)
 {
-    (void)last;
     if (!bytes) return fail(HSPMM_ERR_INVALID, "null bytes");
     if (int rc = check_weigh(cache, batch, attention)) return rc;
-    *bytes = 0;
+    *bytes = batch->tokens ? weigh_shape(cache, batch, attention, last).bytes : 0u;
     return HSPMM_OK;
 }
 
@@ -604,7 +623,8 @@ int hspmm_cache_weigh(const hspmm_cache *cache, uint32_t layer, const hspmm_batc
     if (int rc = check_heads("q", q, cache->dtype)) return rc;
     if (int rc = check_queries(cache, q)) return rc;
     if (!lse || reinterpret_cast<uintptr_t>(lse) % 4u) return fail(HSPMM_ERR_INVALID, "lse is null or not aligned to its elements");
-    if (int rc = check_workspace(workspace, workspace_bytes, 0u)) return rc;
+    const WeighShape sh = weigh_shape(cache, batch, attention, last);
+    if (int rc = check_workspace(workspace, workspace_bytes, sh.bytes)) return rc;
     if (int rc = check_device()) return rc;
     WeighArgs wa{};
     wa.pages = pages_of(cache, layer);
@@ -614,8 +634,15 @@ int hspmm_cache_weigh(const hspmm_cache *cache, uint32_t layer, const hspmm_batc
     wa.scale = attention->scale; wa.decay = decay; wa.causal = attention->causal != 0; wa.window = attention->window; wa.last = last;
     wa.weights = weights->data + weights->layer_stride * layer;
     wa.sequence_stride = weights->sequence_stride; wa.head_stride = weights->head_stride;
-    wa.parts = weigh_parts(cache, batch, attention);
-    HSPMM_HIP(launch_weigh_rows(cache->dtype, wa, static_cast<hipStream_t>(stream)));
+    wa.parts = sh.parts;
+    if (!sh.chunk) {
+        HSPMM_HIP(launch_weigh_rows(cache->dtype, wa, static_cast<hipStream_t>(stream)));
+        return HSPMM_OK;
+    }
+    wa.blocks = Divisor::of(sh.blocks); wa.part_rows = sh.part_rows;
+    wa.arrive = static_cast<uint32_t *>(workspace);
+    wa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + ((sh.cells * 4u + 15u) & ~uint64_t(15u)));
+    HSPMM_HIP(launch_weigh_chunk(cache->dtype, wa, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
 

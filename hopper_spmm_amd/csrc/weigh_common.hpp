@@ -64,4 +64,16 @@ __device__ __forceinline__ RowRange rows_that_see(const WeighArgs &wa, const Wei
     return r;
 }
 
+// The sum over 16 lanes side by side, in all of them.
+__device__ __forceinline__ float sum_row(float v)
+{
+#define HSPMM_ROTATED(n) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + n, 0xF, 0xF, false))
+    v += HSPMM_ROTATED(8);
+    v += HSPMM_ROTATED(4);
+    v += HSPMM_ROTATED(2);
+    v += HSPMM_ROTATED(1);
+#undef HSPMM_ROTATED
+    return v;
+}
+
 }  // namespace hspmm

@@ -96,18 +96,6 @@ struct Keys32 {
     }
 };
 
-// The sum over 16 lanes side by side, in all of them.
-__device__ __forceinline__ float sum_row(float v)
-{
-#define HSPMM_ROTATED(n) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + n, 0xF, 0xF, false))
-    v += HSPMM_ROTATED(8);
-    v += HSPMM_ROTATED(4);
-    v += HSPMM_ROTATED(2);
-    v += HSPMM_ROTATED(1);
-#undef HSPMM_ROTATED
-    return v;
-}
-
 constexpr int kWeighWaves = 4;
 
 // A wave has tiles of 32 keys in turn and all rows that count, sixteen at a time.

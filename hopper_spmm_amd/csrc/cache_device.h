@@ -96,7 +96,8 @@ struct WeighArgs {
     float *sums;                         // of more than one part: their sums
     uint32_t *arrive;                    // and how many have left them (zero between launches)
 };
-hipError_t launch_weigh_rows(int dtype, const WeighArgs &wa, hipStream_t s);
+// few: up to 16 rows at a time
+hipError_t launch_weigh_rows(int dtype, const WeighArgs &wa, bool few, hipStream_t s);
 constexpr uint32_t kWeighKeys = 128u;    // of a workgroup of the chunk kernel
 // 16-bit types
 hipError_t launch_weigh_chunk(int dtype, const WeighArgs &wa, hipStream_t s);
@@ -136,7 +137,7 @@ constexpr uint32_t kEvictEntry = 8u;     // words of an entry
 // Workgroups that share out keys, and values, of a layer, an entry and a head: as many as give a small call some thousand, of 64 bytes of a token at least.
 inline uint32_t evict_shares(const PoolArgs &pa, uint64_t cells)
 {
-    const uint64_t wanted = cells < 2048u ? 2048u / (cells ? cells : 1u) : 1u, most = pa.token_bytes / 64u;
+    const uint64_t wanted = cells < 4096u ? 4096u / (cells ? cells : 1u) : 1u, most = pa.token_bytes / 64u;
     return uint32_t(wanted < most ? wanted : most ? most : 1u);
 }
 hipError_t launch_evict(const PoolArgs &pa, const EvictArgs &ea, hipStream_t s);

@@ -49,43 +49,52 @@ __device__ void evict_plan(const PoolArgs &pa, const EvictArgs &ea, uint32_t i)
     __shared__ uint32_t waves[2u * kScanWaves], last_one;
     uint32_t turn = 0u;
     const uint32_t tid = threadIdx.x, parent = parent_of(pa, ea, i), child = child_of(pa, ea, i);
+    // (asked for before it is known which workgroup looks at them)
+    const Eight ahead = load_references(pa.references, pa.pages, tid * kEach);
     EvictEntry e{-1, 0, 0, 0, {0, 0, 0, 0}};
     if (parent != kIdxMax && child != kIdxMax) {
         const int32_t length = held(pa, parent);
         const uint32_t used = places_for(pa, length);
         const int32_t *row = pa.table + size_t(parent) * pa.table_pages;
-        uint32_t stored = 0u, named = 0u, total;
-        for (uint32_t p = tid; p < used; p += kScanThreads) {
-            const int32_t id = row[p];
-            ea.rows[size_t(i) * pa.table_pages + p] = uint32_t(id) < pa.pages ? id : -1;
-            if (uint32_t(id) < pa.pages) stored += tokens_of_place(pa, p, length);
+        const bool own = parent == child;
+        int32_t *const to = ea.to + size_t(i) * ea.keep_pages;
+        // the k-th page that the parent has takes the k-th page of tokens where that can be in place, else a new one does
+        uint32_t pages_there = 0u, stored = 0u, total;
+        for (uint32_t p0 = 0; p0 < used; p0 += kScanThreads) {
+            const uint32_t p = p0 + tid;
+            const int32_t id = p < used ? row[p] : -1;
+            const bool there = uint32_t(id) < pa.pages;
+            if (p < used) ea.rows[size_t(i) * pa.table_pages + p] = there ? id : -1;
+            // (a bit more where the last place, which may be filled in part, has a page)
+            const uint32_t k = pages_there + (scan(uint32_t(there) + (there && p + 1u == used ? 1u << 16 : 0u), waves, turn, &total) & 0xFFFFu);
+            turn ^= 1u;
+            pages_there += total & 0xFFFFu;
+            stored += (total & 0xFFFFu) * pa.page_tokens.d - (total >> 16 ? pa.page_tokens.d - tokens_of_place(pa, used - 1u, length) : 0u);
+            if (there && k < ea.keep_pages) to[k] = own ? id : -1 - int32_t(k);
         }
-        for (uint32_t k = tid; k < ea.n; k += kScanThreads) named += parent_of(pa, ea, k) == parent;
-        scan(stored, waves, turn, &total);
-        turn ^= 1u;
-        stored = total;
-        scan(named, waves, turn, &total);
-        turn ^= 1u;
-        e.in_place = parent == child && total == 1u;
-        if (parent != child || uint32_t(length) > ea.keep) {
+        if (!own || uint32_t(length) > ea.keep) {
             e.tokens = int32_t(stored < ea.keep ? stored : ea.keep);
             const uint32_t pages = pages_for(pa, e.tokens);
-            // the k-th page that the parent has takes the k-th page of tokens where that can be in place, else a new one does
-            uint32_t before = 0u, before_new = 0u;
-            for (uint32_t p0 = 0; p0 < used && before < pages; p0 += kScanThreads) {
-                const uint32_t p = p0 + tid;
-                const int32_t id = p < used ? row[p] : -1;
-                const bool there = uint32_t(id) < pa.pages;
-                const uint32_t k = before + scan(there, waves, turn, &total);
+            e.need = int32_t(pages);
+            if (own) {
+                uint32_t named = 0u;
+                for (uint32_t k = tid; k < ea.n; k += kScanThreads) named += parent_of(pa, ea, k) == parent;
+                scan(named, waves, turn, &total);
                 turn ^= 1u;
-                before += total;
-                const bool takes = there && k < pages, fresh = takes && !(e.in_place && pa.references[id] == 1);
-                const uint32_t rank = before_new + scan(fresh, waves, turn, &total);
-                turn ^= 1u;
-                before_new += total;
-                if (takes) ea.to[size_t(i) * ea.keep_pages + k] = fresh ? -1 - int32_t(rank) : id;
+                e.in_place = total == 1u;
+                // (the pages that follow in `to` are this workgroup's own writes, of other threads: behind the barrier of the sum above)
+                uint32_t before = 0u;
+                for (uint32_t k0 = 0; k0 < pages; k0 += kScanThreads) {
+                    const uint32_t k = k0 + tid;
+                    const int32_t id = k < pages ? to[k] : 0;
+                    const bool fresh = k < pages && !(e.in_place && pa.references[id] == 1);
+                    const uint32_t rank = before + scan(fresh, waves, turn, &total);
+                    turn ^= 1u;
+                    before += total;
+                    if (fresh) to[k] = -1 - int32_t(rank);
+                }
+                e.need = int32_t(before);
             }
-            e.need = int32_t(before_new);
         }
     }
     if (tid == 0u) {
@@ -98,7 +107,6 @@ __device__ void evict_plan(const PoolArgs &pa, const EvictArgs &ea, uint32_t i)
     __syncthreads();
     if (!last_one) return;
     if (tid == 0u) __hip_atomic_store(ea.arrive, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const Eight ahead = load_references(pa.references, pa.pages, tid * kEach);
     uint64_t need = 0u;
     for (uint32_t i0 = 0; i0 < ea.n; i0 += kScanThreads) {
         const uint32_t k = i0 + tid;
@@ -127,7 +135,9 @@ __device__ void evict_plan(const PoolArgs &pa, const EvictArgs &ea, uint32_t i)
 constexpr uint32_t kDigits = 3u, kBins = 2048u;
 __device__ __forceinline__ uint32_t digit_of(uint32_t u, uint32_t digit) { return digit == 0u ? u >> 21 : digit == 1u ? u >> 10 & 2047u : u & 1023u; }
 
-// Which tokens of a layer, an entry and a head are kept.
+// Which tokens of a layer, an entry and a head are kept.  kHeld: tokens a thread has in registers, so that of up to 1024 times as many each weight is read once; of more, the threads look at
+// 1024 side by side at a time, and again for every digit.
+template <uint32_t kHeld>
 __device__ void evict_choose(const PoolArgs &pa, const EvictArgs &ea, uint32_t cell)
 {
     __shared__ uint32_t waves[2u * kScanWaves], bins[kBins], found[2];
@@ -141,22 +151,46 @@ __device__ void evict_choose(const PoolArgs &pa, const EvictArgs &ea, uint32_t c
     const float *weights = ea.weights + int64_t(layer) * ea.weights_layer + int64_t(parent == kIdxMax ? 0u : parent) * ea.weights_sequence + int64_t(head) * ea.weights_head;
     const uint32_t tokens = uint32_t(length) < used * pa.page_tokens.d ? uint32_t(length) : used * pa.page_tokens.d;      // that there are places for
     const int32_t last = length - int32_t(ea.last);            // (below 0 where all are among the last ones)
-    auto is_stored = [&](uint32_t j) __attribute__((always_inline)) { return uint32_t(table[pa.page_tokens.quotient(j)]) < pa.pages; };
     auto is_kept_anyway = [&](uint32_t j) __attribute__((always_inline)) { return j < ea.first || int32_t(j) >= last; };
+    const bool held_here = tokens <= kHeld * kScanThreads;
+    // (a thread's tokens follow each other: one sum over the threads is enough to put them in order)
+    const uint32_t each = (tokens + kScanThreads - 1u) / kScanThreads, mine = held_here ? tid * each : 0u;
+    float w[kHeld];
+    if (held_here) {
+#pragma unroll
+        for (uint32_t e = 0; e < kHeld; ++e) w[e] = weights[e < each && mine + e < tokens ? mine + e : 0u];
+    }
+    // whether every place has a page, else they are looked up token by token
+    uint32_t missing = 0u, total;
+    for (uint32_t p = tid; p < used; p += kScanThreads) missing += uint32_t(table[p]) >= pa.pages;
+    scan(missing, waves, turn, &total);
+    turn ^= 1u;
+    const bool whole = total == 0u;
+    auto is_stored = [&](uint32_t j) __attribute__((always_inline)) { return whole || uint32_t(table[pa.page_tokens.quotient(j)]) < pa.pages; };
     // how many are stored, and how many of those are kept anyway
-    uint32_t stored = 0u, anyway = 0u, total;
-    for (uint32_t j = tid; j < tokens; j += kScanThreads)
-        if (is_stored(j)) {
-            ++stored;
-            anyway += is_kept_anyway(j);
-        }
-    scan(stored, waves, turn, &total);
-    turn ^= 1u;
-    stored = total;
-    scan(anyway, waves, turn, &total);
-    turn ^= 1u;
-    anyway = total;
+    uint32_t stored = tokens, anyway = min(ea.first, tokens) + (last < int32_t(tokens) ? tokens - uint32_t(max(last, int32_t(min(ea.first, tokens)))) : 0u);
+    if (!whole) {
+        stored = anyway = 0u;
+        for (uint32_t j = tid; j < tokens; j += kScanThreads)
+            if (is_stored(j)) {
+                ++stored;
+                anyway += is_kept_anyway(j);
+            }
+        scan(stored, waves, turn, &total);
+        turn ^= 1u;
+        stored = total;
+        scan(anyway, waves, turn, &total);
+        turn ^= 1u;
+        anyway = total;
+    }
     const uint32_t stays = stored < ea.keep ? stored : ea.keep;
+    // of a thread's tokens: stored ones that are kept anyway, and the others, a bit each
+    uint32_t sure_bits = 0u, open_bits = 0u;
+    if (held_here) {
+#pragma unroll
+        for (uint32_t e = 0; e < kHeld; ++e)
+            if (e < each && mine + e < tokens && is_stored(mine + e)) (is_kept_anyway(mine + e) ? sure_bits : open_bits) |= 1u << e;
+    }
     // the smallest weight that is taken, and how many tokens of it; all of them where no choice is to be made
     uint32_t least = 0u, ties = ~0u;
     if (stays < stored) {
@@ -169,10 +203,17 @@ __device__ void evict_choose(const PoolArgs &pa, const EvictArgs &ea, uint32_t c
                 const uint32_t shift = digit == 0u ? 32u : digit == 1u ? 21u : 10u;
                 for (uint32_t k = tid; k < kBins; k += kScanThreads) bins[k] = 0u;
                 __syncthreads();
-                for (uint32_t j = tid; j < tokens; j += kScanThreads) {
-                    if (!is_stored(j) || is_kept_anyway(j)) continue;
-                    const uint32_t u = ordered(weights[j]);
+                auto count = [&](float weight) __attribute__((always_inline)) {
+                    const uint32_t u = ordered(weight);
                     if (digit == 0u || u >> shift == prefix) atomicAdd(&bins[digit_of(u, digit)], 1u);
+                };
+                if (held_here) {
+#pragma unroll
+                    for (uint32_t e = 0; e < kHeld; ++e)
+                        if (open_bits >> e & 1u) count(w[e]);
+                } else {
+                    for (uint32_t j = tid; j < tokens; j += kScanThreads)
+                        if (is_stored(j) && !is_kept_anyway(j)) count(weights[j]);
                 }
                 __syncthreads();
                 // counts from the greatest digit down: a thread has two
@@ -191,36 +232,58 @@ __device__ void evict_choose(const PoolArgs &pa, const EvictArgs &ea, uint32_t c
         }
     }
     // in the tokens' order
-    uint32_t before = 0u, equal = 0u;
-    for (uint32_t j0 = 0; j0 < tokens; j0 += kScanThreads) {
-        const uint32_t j = j0 + tid;
-        bool sure = false, tie = false;
-        float w = 0.f;
-        if (j < tokens && is_stored(j)) {
-            w = weights[j];
-            const uint32_t u = ordered(w);
-            sure = is_kept_anyway(j) || u > least;
-            tie = !sure && u == least;
+    auto keep = [&](uint32_t at, uint32_t j, float weight) __attribute__((always_inline)) {
+        ea.kept[out + at] = int32_t(j);
+        ea.kept_weights[out + at] = weight;
+    };
+    if (held_here) {
+        uint32_t tie_bits = 0u;
+#pragma unroll
+        for (uint32_t e = 0; e < kHeld; ++e)
+            if (open_bits >> e & 1u) {
+                const uint32_t u = ordered(w[e]);
+                if (u > least) sure_bits |= 1u << e;
+                else if (u == least) tie_bits |= 1u << e;
+            }
+        // (both counts in a word: there are 16384 at most)
+        const uint32_t both = scan(uint32_t(__popc(sure_bits)) | uint32_t(__popc(tie_bits)) << 16, waves, turn, &total);
+        uint32_t sure = both & 0xFFFFu, tie = both >> 16;
+#pragma unroll
+        for (uint32_t e = 0; e < kHeld; ++e) {
+            const bool is_sure = sure_bits >> e & 1u, is_tie = tie_bits >> e & 1u;
+            if (is_sure || (is_tie && tie < ties)) keep(sure + min(tie, ties), mine + e, w[e]);
+            sure += is_sure;
+            tie += is_tie;
         }
-        // (both counts in a word: a workgroup has 1024 tokens)
-        const uint32_t both = scan(uint32_t(sure) | uint32_t(tie) << 16, waves, turn, &total);
-        turn ^= 1u;
-        const uint32_t ties_before = equal + (both >> 16);
-        if (sure || (tie && ties_before < ties)) {
-            const uint32_t at = before + (both & 0xFFFFu) + (ties_before < ties ? ties_before : ties);
-            ea.kept[out + at] = int32_t(j);
-            ea.kept_weights[out + at] = w;
+    } else {
+        uint32_t before = 0u, equal = 0u;
+        for (uint32_t j0 = 0; j0 < tokens; j0 += kScanThreads) {
+            const uint32_t j = j0 + tid;
+            bool sure = false, tie = false;
+            float weight = 0.f;
+            if (j < tokens && is_stored(j)) {
+                weight = weights[j];
+                const uint32_t u = ordered(weight);
+                sure = is_kept_anyway(j) || u > least;
+                tie = !sure && u == least;
+            }
+            // (both counts in a word: a workgroup has 1024 tokens)
+            const uint32_t both = scan(uint32_t(sure) | uint32_t(tie) << 16, waves, turn, &total);
+            turn ^= 1u;
+            const uint32_t ties_before = equal + (both >> 16);
+            if (sure || (tie && ties_before < ties)) keep(before + (both & 0xFFFFu) + min(ties_before, ties), j, weight);
+            before += total & 0xFFFFu;
+            equal += total >> 16;
         }
-        before += total & 0xFFFFu;
-        equal += total >> 16;
     }
     for (uint32_t k = stays + tid; k < ea.keep; k += kScanThreads) ea.kept[out + k] = -1;
 }
 
-__global__ __launch_bounds__(kScanThreads) void evict_choose_kernel(const PoolArgs pa, const EvictArgs ea)
+template <uint32_t kHeld>
+__global__ __launch_bounds__(kScanThreads, kHeld <= 8u ? 8 : 4) void evict_choose_kernel(const PoolArgs pa, const EvictArgs ea)
 {
     if (blockIdx.x < ea.n) evict_plan(pa, ea, blockIdx.x);
-    else evict_choose(pa, ea, blockIdx.x - ea.n);
+    else evict_choose<kHeld>(pa, ea, blockIdx.x - ea.n);
 }
 
 constexpr uint32_t kMoveThreads = 256u, kMoveAtOnce = 8u;
@@ -274,7 +337,7 @@ __device__ void evict_move(const PoolArgs &pa, const EvictArgs &ea, uint32_t row
             }
 #pragma unroll
             for (uint32_t k = 0; k < kMoveAtOnce; ++k)
-                if (to[k]) *reinterpret_cast<U *>(to[k]) = v[k];
+                if (to[k]) __builtin_nontemporal_store(v[k], reinterpret_cast<U *>(to[k]));
         }
     }
 }
@@ -323,7 +386,8 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(const PoolArgs
 hipError_t launch_evict(const PoolArgs &pa, const EvictArgs &ea, hipStream_t s)
 {
     const uint64_t cells = uint64_t(ea.n) * pa.layers * pa.heads;
-    evict_choose_kernel<<<dim3(uint32_t(ea.n + cells)), dim3(kScanThreads), 0, s>>>(pa, ea);
+    if (uint64_t(pa.table_pages) * pa.page_tokens.d <= 8u * kScanThreads) evict_choose_kernel<8u><<<dim3(uint32_t(ea.n + cells)), dim3(kScanThreads), 0, s>>>(pa, ea);
+    else evict_choose_kernel<16u><<<dim3(uint32_t(ea.n + cells)), dim3(kScanThreads), 0, s>>>(pa, ea);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     const uint32_t shares = evict_shares(pa, cells);
     by_unit(pa, [&](auto u) { evict_move_kernel<decltype(u)><<<dim3(uint32_t(ea.n + cells * (2u * shares + 1u))), dim3(kMoveThreads), 0, s>>>(pa, ea, shares); });

@@ -568,7 +568,7 @@ static int check_weights(const hspmm_weights *w)
 
 // How a call of hspmm_cache_weigh is launched, by sizes alone: the same for the call and for its workspace.
 struct WeighShape {
-    bool chunk;                          // by the chunk kernel
+    bool chunk, few;                     // by the chunk kernel; by the rows kernel, sixteen rows at a time
     uint32_t parts, blocks, part_rows;
     uint64_t cells, bytes;
 };
@@ -579,10 +579,13 @@ static WeighShape weigh_shape(const hspmm_cache *c, const hspmm_batch *b, const 
     const uint64_t keys = most_keys(c, a->longest), heads = uint64_t(b->sequences) * c->heads;
     const uint64_t tokens = std::min(a->longest_chunk, b->tokens), rows = std::max<uint64_t>((last && last < tokens ? last : tokens) * (a->q_heads / c->heads), 1u);
     auto up = [](uint64_t n, uint64_t to) { return (n + to - 1u) / to; };
-    sh.chunk = c->dtype != HSPMM_TF32 && rows > 16u;
+    sh.few = rows <= 16u;
+    sh.chunk = c->dtype != HSPMM_TF32 && rows > 128u;
     if (!sh.chunk) {
-        // a wave has a tile of 32 keys or some
-        sh.parts = uint32_t(std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(up(keys, 128u), 8192u / std::max<uint64_t>(heads, 1u)), 1u), 32768u));
+        // a wave has a tile of 32 keys or some.  us by 1024 / 2048 / 4096 / 8192 / 16384 workgroups: a token for each of 48 sequences of up to 16000 214 / 195 / 184 / 177 / 182;
+        // where a workgroup has rows to load first, the last 32 tokens of 17 of up to 5700 19.6 / 20.2 / 21.0 / 22.0
+        const uint64_t groups = (sh.few ? 8192u : 1024u) / std::max<uint64_t>(heads, 1u);
+        sh.parts = uint32_t(std::min<uint64_t>(std::max<uint64_t>(std::min<uint64_t>(up(keys, 128u), groups), 1u), 32768u));
         return sh;
     }
     sh.blocks = uint32_t(std::min<uint64_t>(up(keys, kWeighKeys), std::max<uint64_t>((uint64_t(1) << 22) / std::max<uint64_t>(heads, 1u), 1u)));
@@ -636,7 +639,7 @@ int hspmm_cache_weigh(const hspmm_cache *cache, uint32_t layer, const hspmm_batc
     wa.sequence_stride = weights->sequence_stride; wa.head_stride = weights->head_stride;
     wa.parts = sh.parts;
     if (!sh.chunk) {
-        HSPMM_HIP(launch_weigh_rows(cache->dtype, wa, static_cast<hipStream_t>(stream)));
+        HSPMM_HIP(launch_weigh_rows(cache->dtype, wa, sh.few, static_cast<hipStream_t>(stream)));
         return HSPMM_OK;
     }
     wa.blocks = Divisor::of(sh.blocks); wa.part_rows = sh.part_rows;

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     const uint32_t part = blockIdx.y, D = aa.pages.head_dim;
     const Cell cell = cell_of(aa, gridDim.x - 1u - blockIdx.x, 0u);
     const uint32_t head = cell.head, tile_number = cell.tile;
-    RowTile t = find_tile<kRowsLog, Span>(aa, tile_number);
+    const RowTile t = find_tile<kRowsLog, Span>(aa, tile_number);
     if (!t.there) return;
     const uint32_t m = wave * 32u + j;
     const bool is_row = m < t.rows;
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
             any_lo = min(any_lo, ranges[w][2]);
         }
         group_lo = __builtin_amdgcn_readfirstlane(group_lo); group_hi = __builtin_amdgcn_readfirstlane(group_hi);
-        t.lo = __builtin_amdgcn_readfirstlane(min(any_lo, t.hi));
+        any_lo = __builtin_amdgcn_readfirstlane(any_lo);
     } else {
         const int32_t p0 = t.position + int32_t(aa.shared.quotient(t.first_row)), p1 = t.position + int32_t(aa.shared.quotient(t.first_row + t.rows - 1u));
         group_hi = aa.causal ? p0 + 1 : t.length;
@@ -80,8 +80,10 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
         if constexpr (Span == kSpanRest) group_lo = max(group_lo, t.prefix);
     }
     const KeyPart keys_here = key_part(aa, t, part);
-    const int32_t parts = keys_here.parts, begin = keys_here.begin, end = keys_here.end;
-    if (int32_t(part) >= parts) return;
+    const int32_t parts = Span == kSpanPrefix ? 1 : keys_here.parts, end = keys_here.end;
+    if (int32_t(part) >= keys_here.parts) return;
+    // (rows of several sequences: from the first key that any of them sees)
+    const int32_t begin = Span == kSpanPrefix ? max(keys_here.begin, min(any_lo & ~31, end)) : keys_here.begin;
     const int32_t n_images = end > begin ? (end - begin + 63) / 64 : 0;
     if (tid == 0u) odd = 0u;
 
@@ -428,7 +430,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
     }
     if (!is_row) return;
     if constexpr (Span == kSpanPrefix) {
-        float *const to = prefix_sums(aa, row);
+        float *const to = prefix_sums(aa, row, part);
 #pragma unroll
         for (int c = 0; c < kTiles; ++c)
 #pragma unroll
@@ -440,20 +442,24 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel
         return;
     }
     if (Span == kSpanRest && t.prefix) {
-        const float *const from = prefix_sums(aa, row);
-        const float other = from[D], top = fmaxf(ref, other);
-        const float keep = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - top), by = other == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other - top);
-        total = total * keep + from[D + 1u] * by;
+        const uint32_t others = prefix_parts(aa, t.prefix);
+#pragma unroll 1
+        for (uint32_t p = 0; p < others; ++p) {
+            const float *const from = prefix_sums(aa, row, p);
+            const float other = from[D], top = fmaxf(ref, other);
+            const float keep = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - top), by = other == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other - top);
+            total = total * keep + from[D + 1u] * by;
 #pragma unroll
-        for (int c = 0; c < kTiles; ++c)
+            for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const uint32_t d = 32u * c + 2u * r + 4u * h;
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (d < D ? d : 0u));
+                for (int r = 0; r < 16; r += 4) {
+                    const uint32_t d = 32u * c + 2u * r + 4u * h;
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (d < D ? d : 0u));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[c][r + e] = o[c][r + e] * keep + x[e] * by;
-            }
-        ref = top;
+                    for (int e = 0; e < 4; ++e) o[c][r + e] = o[c][r + e] * keep + x[e] * by;
+                }
+            ref = top;
+        }
     }
     const bool any = !(total == 0.f);
     const float by = any ? 1.f / total : 0.f;

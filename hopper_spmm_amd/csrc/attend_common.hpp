@@ -120,16 +120,17 @@ __device__ __forceinline__ RowTile find_tile(const AttendArgs &aa, uint32_t tile
 // The keys [begin, end) of part `part` of a tile's: parts begin a multiple of 32 keys apart.  Where aa.splits parts of aa.part_keys do not reach (long spans,
 // or a sequence longer than the call said) all are longer, by the same: one token over 2^18 keys, 8 heads of 128, 1810 -> 192 us, 2^20 keys of one head 11500 -> 107.
 struct KeyPart { int32_t begin, end, parts; };
-__device__ __forceinline__ KeyPart key_part(const AttendArgs &aa, const RowTile &t, uint32_t part)
+__device__ __forceinline__ KeyPart key_part(int32_t from, int32_t hi, uint32_t part_keys, uint32_t splits, uint32_t part)
 {
-    const int32_t lo = t.lo & ~31;
-    const uint32_t span = t.hi > lo ? uint32_t(t.hi - lo) : 0u;
-    uint32_t each = aa.part_keys;
-    if (uint64_t(each) * aa.splits < span) each = ((span + aa.splits - 1u) / aa.splits + 31u) & ~31u;
+    const int32_t lo = from & ~31;
+    const uint32_t span = hi > lo ? uint32_t(hi - lo) : 0u;
+    uint32_t each = part_keys;
+    if (uint64_t(each) * splits < span) each = ((span + splits - 1u) / splits + 31u) & ~31u;
     const uint32_t parts = span ? (span + each - 1u) / each : 1u;
     const int32_t begin = lo + int32_t(part < parts ? part * each : 0u);
-    return KeyPart{begin, part + 1u < parts ? begin + int32_t(each) : t.hi, int32_t(parts)};
+    return KeyPart{begin, part + 1u < parts ? begin + int32_t(each) : hi, int32_t(parts)};
 }
+__device__ __forceinline__ KeyPart key_part(const AttendArgs &aa, const RowTile &t, uint32_t part) { return key_part(t.lo, t.hi, aa.part_keys, aa.splits, part); }
 
 // The tile and the head of a workgroup: heads side by side, as they are of one length, then tiles, then parts.  Workgroups go to the eight L2 domains and,
 // there, to groups of compute units in turn, whatever they have to do, so what repeats in the numbers must not repeat in time: where chunks fill their
@@ -176,11 +177,14 @@ __device__ __forceinline__ RowOf row_of_tile(const AttendArgs &aa, const RowTile
     return r;
 }
 
-// Where a row's sums over its group's prefix are.
-__device__ __forceinline__ float *prefix_sums(const AttendArgs &aa, const RowOf &r)
+// Where a row's sums over a part of its group's prefix are.  The launch of what is behind the prefixes adds them up, row by row: a workgroup that joined a tile's parts
+// would read as much as all of them together wrote, alone.
+__device__ __forceinline__ float *prefix_sums(const AttendArgs &aa, const RowOf &r, uint32_t part)
 {
-    return aa.prefix.sums + (size_t(r.token) * aa.q_heads + r.head) * (aa.pages.head_dim + kPrefixExtra);
+    return aa.prefix.sums + int64_t(part) * aa.prefix.part_stride + int64_t(size_t(r.token) * aa.q_heads + r.head) * (aa.pages.head_dim + kPrefixExtra);
 }
+// How many parts a prefix of so many keys has.
+__device__ __forceinline__ uint32_t prefix_parts(const AttendArgs &aa, int32_t keys) { return uint32_t(key_part(0, keys, aa.prefix.part_keys, aa.prefix.splits, 0u).parts); }
 
 // Element offset of the row of a key (kv head `head`), -1: not stored.
 __device__ __forceinline__ int64_t key_offset(const PagesArgs &pg, const int32_t *table_row, int64_t head_offset, int32_t key)

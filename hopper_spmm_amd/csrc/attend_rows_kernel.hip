@@ -246,21 +246,20 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
     RowTile t = find_tile<4, Span>(aa, cell.tile);
     if (!t.there) return;
     constexpr int32_t kKeys = K::kKeys;
-    RowOf row;
+    // this part's keys
+    const KeyPart keys_here = key_part(aa, t, part);
+    const int32_t parts = Span == kSpanPrefix ? 1 : keys_here.parts, end = keys_here.end;
+    int32_t begin = keys_here.begin;
+    if (int32_t(part) >= keys_here.parts) return;
+
+    const RowOf row = row_of_tile<Span>(aa, t, head, i);
     if constexpr (Span == kSpanPrefix) {
-        row = row_of_tile<Span>(aa, t, head, i);
-        // (rows of several sequences: the first key that any of them sees)
+        // (rows of several sequences: from the first key that any of them sees)
         int32_t low = i < t.rows ? row.lo : 0x7FFFFFFF;
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) low = min(low, __shfl_xor(low, d));
-        t.lo = __builtin_amdgcn_readfirstlane(min(low, t.hi));
+        begin = max(begin, min(__builtin_amdgcn_readfirstlane(low) & ~31, end));
     }
-    // this part's keys
-    const KeyPart keys_here = key_part(aa, t, part);
-    const int32_t parts = keys_here.parts, begin = keys_here.begin, end = keys_here.end;
-    if (int32_t(part) >= parts) return;
-
-    if constexpr (Span != kSpanPrefix) row = row_of_tile<Span>(aa, t, head, i);
     typename K::Query Q;
     K::load_query(Q, aa.q.data + (int64_t(row.token) * aa.q.token_stride + int64_t(row.head) * aa.q.head_stride) * K::kElem, i < t.rows, lane, D);
     const float scale = aa.scale * kLog2e;
@@ -541,7 +540,7 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
     if (m < t.rows) {
         const RowOf r = row_of_tile<Span>(aa, t, head, m);
         if constexpr (Span == kSpanPrefix) {
-            float *const to = prefix_sums(aa, r);
+            float *const to = prefix_sums(aa, r, part);
 #pragma unroll
             for (uint32_t e = 0; e < kEach; e += 4)
                 if (d0 + e < D) *reinterpret_cast<f32x4 *>(to + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
@@ -549,13 +548,30 @@ __global__ __launch_bounds__(64 * kRowWaves, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) v
             return;
         }
         if (Span == kSpanRest && t.prefix) {
-            const float *const from = prefix_sums(aa, r);
-            const float other = from[D], top = fmaxf(most, other);
-            const float keep = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(most - top), by = other == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other - top);
-            sum = sum * keep + from[D + 1u] * by;
+            const uint32_t others = prefix_parts(aa, t.prefix);
+            constexpr uint32_t kAtOnce = 4u;
+            for (uint32_t p0 = 0; p0 < others; p0 += kAtOnce) {
+                f32x4 x[kAtOnce][kEach / 4u];
+                float ref_of_part[kAtOnce], total_of_part[kAtOnce];
 #pragma unroll
-            for (uint32_t e = 0; e < kEach; ++e) acc[e] = acc[e] * keep + (d0 + e < D ? from[d0 + e] : 0.f) * by;
-            most = top;
+                for (uint32_t k = 0; k < kAtOnce; ++k) {
+                    const float *const from = prefix_sums(aa, r, p0 + k < others ? p0 + k : p0);
+                    ref_of_part[k] = from[D];
+                    total_of_part[k] = from[D + 1u];
+#pragma unroll
+                    for (uint32_t e = 0; e < kEach; e += 4) x[k][e / 4u] = *reinterpret_cast<const f32x4 *>(from + (d0 + e < D ? d0 + e : 0u));
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < kAtOnce; ++k) {
+                    if (p0 + k >= others) break;
+                    const float other = ref_of_part[k], top = fmaxf(most, other);
+                    const float keep = most == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(most - top), by = other == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(other - top);
+                    sum = sum * keep + total_of_part[k] * by;
+#pragma unroll
+                    for (uint32_t e = 0; e < kEach; ++e) acc[e] = acc[e] * keep + x[k][e / 4u][e % 4u] * by;
+                    most = top;
+                }
+            }
         }
         const bool any = !(sum == 0.f);
         const float by = any ? 1.f / sum : 0.f;

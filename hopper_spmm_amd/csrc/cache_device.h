@@ -43,7 +43,9 @@ hipError_t launch_rotary(int dtype, const RotaryArgs &ra, uint32_t vec, hipStrea
 struct PrefixArgs {
     const int32_t *firsts, *tokens;
     uint32_t groups;
-    float *sums;                         // per token and head of queries: sums over the prefix (kPrefixExtra floats more than head_dim)
+    uint32_t splits, part_keys;          // of the prefixes' launch
+    float *sums;                         // per part of a prefix, token and head of queries: sums over the part (kPrefixExtra floats more than head_dim)
+    int64_t part_stride;                 // from a part to the next
 };
 constexpr uint32_t kPrefixExtra = 4u;    // reference, total
 // Which keys an attention's launch has: all; those of the groups' prefixes; those behind them, after which the sums of both are added.

@@ -286,7 +286,7 @@ __global__ __launch_bounds__(kScanThreads, kHeld <= 8u ? 8 : 4) void evict_choos
     else evict_choose<kHeld>(pa, ea, blockIdx.x - ea.n);
 }
 
-constexpr uint32_t kMoveThreads = 256u, kMoveAtOnce = 8u;
+constexpr uint32_t kMoveThreads = 256u, kMoveAtOnce = 4u;
 
 // Keys or values of a layer, an entry and a head, a share of them: columns (in place) or tokens.
 template <class U>

@@ -377,7 +377,7 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
 // An attention over shared prefixes: two launches, of the prefixes with a group for a sequence, and of what is behind them.
 struct SharedShape {
     AttendShape prefix, rest;
-    uint64_t parts_bytes, bytes;         // of the workspace: counters and sums of parts, which the launches have in turn; with the prefixes' sums behind them
+    uint64_t parts_bytes, bytes;         // of the workspace: counters and sums of the second one's parts; with the sums of the prefixes' parts behind them
 };
 
 static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, const hspmm_prefix *p, const hspmm_attention *a)
@@ -389,8 +389,8 @@ static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     sh.prefix = attend_shape(c, p->groups, b->tokens, p->most_tokens ? p->most_tokens : b->tokens, common, &whole);
     // (keys behind the prefix: the longest sequence is taken to have the longest one)
     sh.rest = attend_shape(c, b->sequences, b->tokens, a->longest_chunk, std::max<uint64_t>(all - common, std::min<uint64_t>(std::max(a->longest_chunk, 1u), all)), a);
-    sh.parts_bytes = (std::max(sh.prefix.bytes, sh.rest.bytes) + 15u) & ~uint64_t(15u);
-    sh.bytes = sh.parts_bytes + uint64_t(b->tokens) * a->q_heads * (c->head_dim + kPrefixExtra) * 4u;
+    sh.parts_bytes = (sh.rest.bytes + 15u) & ~uint64_t(15u);
+    sh.bytes = sh.parts_bytes + sh.prefix.splits * uint64_t(b->tokens) * a->q_heads * (c->head_dim + kPrefixExtra) * 4u;
     return sh;
 }
 
@@ -505,7 +505,8 @@ int hspmm_cache_attend_shared(const hspmm_cache *cache, uint32_t layer, const hs
     if (int rc = check_tiles(cache, batch, sh.rest)) return rc;
     if (int rc = check_workspace(workspace, workspace_bytes, sh.bytes)) return rc;
     if (int rc = check_device()) return rc;
-    const PrefixArgs pa{prefix->firsts, prefix->tokens, prefix->groups, reinterpret_cast<float *>(static_cast<char *>(workspace) + sh.parts_bytes)};
+    const PrefixArgs pa{prefix->firsts, prefix->tokens, prefix->groups, sh.prefix.splits, sh.prefix.part_keys, reinterpret_cast<float *>(static_cast<char *>(workspace) + sh.parts_bytes),
+                        int64_t(batch->tokens) * attention->q_heads * (cache->head_dim + kPrefixExtra)};
     AttendArgs aa = attend_args(cache, layer, batch, attention, q, out, lse, sh.prefix, workspace);
     aa.prefix = pa;
     HSPMM_HIP(launch_attend(cache->dtype, aa, kSpanPrefix, sh.prefix, stream));

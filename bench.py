@@ -153,8 +153,8 @@ def cpu_baseline(A, B, N, flops_full):
 
 
 # sources that no product is made with: positions, the cache's pages and attention over it
-CACHE_SOURCES = ("attend_chunk_kernel.hip", "attend_common.hpp", "attend_rows_kernel.hip", "cache_device.h", "divisor.hpp", "evict_kernels.hip",
-                 "hspmm_cache.hip", "page_kernels.hip", "pages_common.hpp", "rotary_kernels.hip", "weigh_chunk_kernel.hip",
+CACHE_SOURCES = ("attend_chunk.hpp", "attend_chunk_kernel.hip", "attend_common.hpp", "attend_rows.hpp", "attend_rows_kernel.hip", "attend_shared_kernel.hip", "cache_device.h",
+                 "divisor.hpp", "evict_kernels.hip", "hspmm_cache.hip", "page_kernels.hip", "pages_common.hpp", "rotary_kernels.hip", "weigh_chunk_kernel.hip",
                  "weigh_common.hpp", "weigh_rows_kernel.hip")
 
 

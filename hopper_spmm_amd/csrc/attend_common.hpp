@@ -25,7 +25,8 @@ struct RowTile {
     int32_t length, position;                                    // tokens the cache holds; the position of the chunk's first token
     int32_t lo, hi;                                              // keys that any of the rows may see, as far as there are places for them
     uint32_t first_batch, end_batch;                             // kSpanPrefix: the batch's rows of the group, whose sequences' chunks the rows are of
-    int32_t prefix;                                              // keys of the group's prefix (kSpanPrefix, kSpanRest)
+    int32_t prefix;                                              // keys of the group's prefix (not kSpanAll)
+    uint32_t leader;                                             // whose row of the table has them (kSpanBoth)
     bool there;
 };
 
@@ -62,11 +63,12 @@ __device__ __forceinline__ Prefix prefix_of(const AttendArgs &aa, uint32_t g)
 }
 
 // The prefix of the group that batch row b, which has the tokens [first_token, end_token), is in.
-__device__ __forceinline__ int32_t prefix_keys(const AttendArgs &aa, uint32_t b, int32_t first_token, int32_t end_token)
+__device__ __forceinline__ Prefix prefix_of_row(const AttendArgs &aa, uint32_t b, int32_t first_token, int32_t end_token)
 {
     const uint32_t g = last_at_most(aa.prefix.groups, b, [&](uint32_t i) __attribute__((always_inline)) { return uint32_t(max(aa.prefix.firsts[i], 0)); });
-    const Prefix p = prefix_of(aa, g);
-    return b >= p.first && b < p.end && first_token >= p.first_token && end_token <= p.end_token ? p.keys : 0;
+    Prefix p = prefix_of(aa, g);
+    if (b < p.first || b >= p.end || first_token < p.first_token || end_token > p.end_token) p.keys = 0;
+    return p;
 }
 
 // Tile number `tile` of (1 << ROWS_LOG) rows.  Batch row b has the tiles from (starts[b] * shared >> ROWS_LOG) + b on: more than it needs at most by
@@ -110,9 +112,11 @@ __device__ __forceinline__ RowTile find_tile(const AttendArgs &aa, uint32_t tile
     const int32_t p0 = t.position + int32_t(aa.shared.quotient(from)), p1 = t.position + int32_t(aa.shared.quotient(from + t.rows - 1u));
     t.hi = clamp_i32(aa.causal ? p1 + 1 : t.length, 0, keys_of_row(aa.pages));
     t.lo = aa.window && int64_t(p0) + 1 > int64_t(aa.window) ? min(p0 + 1 - int32_t(aa.window), t.hi) : 0;
-    if constexpr (Span == kSpanRest) {
-        t.prefix = prefix_keys(aa, lo, first, end);
-        t.lo = min(max(t.lo, t.prefix), t.hi);
+    if constexpr (Span != kSpanAll) {
+        const Prefix p = prefix_of_row(aa, lo, first, end);
+        t.prefix = p.keys;
+        t.leader = p.sequence;
+        if (Span == kSpanRest) t.lo = min(max(t.lo, t.prefix), t.hi);
     }
     return t;
 }
@@ -177,14 +181,20 @@ __device__ __forceinline__ RowOf row_of_tile(const AttendArgs &aa, const RowTile
     return r;
 }
 
-// Where a row's sums over a part of its group's prefix are.  The launch of what is behind the prefixes adds them up, row by row: a workgroup that joined a tile's parts
-// would read as much as all of them together wrote, alone.
-__device__ __forceinline__ float *prefix_sums(const AttendArgs &aa, const RowOf &r, uint32_t part)
+// Attention over shared prefixes: where a row's sums over a part of its group's prefix, or of the keys behind it, are.  Nobody joins a tile's parts: a launch behind adds up a row's,
+// and a tile's workgroup would read alone what all of them wrote together.
+template <AttendSpan Span>
+__device__ __forceinline__ float *span_sums(const AttendArgs &aa, const RowOf &r, uint32_t part)
 {
-    return aa.prefix.sums + int64_t(part) * aa.prefix.part_stride + int64_t(size_t(r.token) * aa.q_heads + r.head) * (aa.pages.head_dim + kPrefixExtra);
+    return aa.prefix.sums + int64_t(Span == kSpanRest ? aa.prefix.splits + part : part) * aa.prefix.part_stride + int64_t(size_t(r.token) * aa.q_heads + r.head) * (aa.pages.head_dim + kPrefixExtra);
 }
-// How many parts a prefix of so many keys has.
-__device__ __forceinline__ uint32_t prefix_parts(const AttendArgs &aa, int32_t keys) { return uint32_t(key_part(0, keys, aa.prefix.part_keys, aa.prefix.splits, 0u).parts); }
+// Behind them: reference, total, and of what is behind a prefix how many parts there are of either.
+template <AttendSpan Span>
+__device__ __forceinline__ f32x4 span_header(const AttendArgs &aa, const RowTile &t, float ref, float total, int32_t parts)
+{
+    const uint32_t others = Span == kSpanRest && t.prefix ? uint32_t(key_part(0, t.prefix, aa.prefix.part_keys, aa.prefix.splits, 0u).parts) : 0u;
+    return f32x4{ref, total, __builtin_bit_cast(float, uint32_t(parts)), __builtin_bit_cast(float, others)};
+}
 
 // Element offset of the row of a key (kv head `head`), -1: not stored.
 __device__ __forceinline__ int64_t key_offset(const PagesArgs &pg, const int32_t *table_row, int64_t head_offset, int32_t key)

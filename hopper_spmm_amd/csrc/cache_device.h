@@ -43,13 +43,13 @@ hipError_t launch_rotary(int dtype, const RotaryArgs &ra, uint32_t vec, hipStrea
 struct PrefixArgs {
     const int32_t *firsts, *tokens;
     uint32_t groups;
-    uint32_t splits, part_keys;          // of the prefixes' launch
-    float *sums;                         // per part of a prefix, token and head of queries: sums over the part (kPrefixExtra floats more than head_dim)
+    uint32_t splits, part_keys;          // of the prefixes
+    float *sums;                         // per part - of the prefixes, then of what is behind -, token and head of queries: sums over the part (kPrefixExtra floats more than head_dim)
     int64_t part_stride;                 // from a part to the next
 };
-constexpr uint32_t kPrefixExtra = 4u;    // reference, total
-// Which keys an attention's launch has: all; those of the groups' prefixes; those behind them, after which the sums of both are added.
-enum AttendSpan { kSpanAll, kSpanPrefix, kSpanRest };
+constexpr uint32_t kPrefixExtra = 4u;    // reference, total, parts
+// Which keys a workgroup of an attention has: all; those of a group's prefix; those behind it; all, those of the prefix by its first sequence's pages.
+enum AttendSpan { kSpanAll, kSpanPrefix, kSpanRest, kSpanBoth };
 
 struct AttendArgs {
     PagesArgs pages;
@@ -76,9 +76,12 @@ constexpr uint32_t kAttendCounters = 16384u;
 // floats of a part of a tile's sums
 inline uint32_t attend_slot(uint32_t rows_log, uint32_t head_dim) { return (1u << rows_log) * ((head_dim <= 64u ? 64u : head_dim <= 128u ? 128u : 256u) + 4u); }
 // past: 16-bit keys and values are not kept in the L2
-hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, AttendSpan span, bool past, hipStream_t s);
+hipError_t launch_attend_rows(int dtype, const AttendArgs &aa, bool past, hipStream_t s);
 // 16-bit types; tiles of 1 << rows_log rows: 128, or 256 for heads of up to 128 elements
-hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, AttendSpan span, uint32_t rows_log, hipStream_t s);
+// both: with prefixes, by the pages of their first sequences
+hipError_t launch_attend_chunk(int dtype, const AttendArgs &aa, bool both, uint32_t rows_log, hipStream_t s);
+// Attention over shared prefixes: `prefix` has the prefixes' tiles, `rest` those of what is behind them, by the rows kernel or the chunk kernel (tiles of 128 rows) each.
+hipError_t launch_attend_shared(int dtype, const AttendArgs &prefix, const AttendArgs &rest, bool prefix_chunk, bool rest_chunk, hipStream_t s);
 
 // Attention weights that cached keys have received.
 struct WeighArgs {

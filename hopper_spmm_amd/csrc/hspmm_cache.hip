@@ -374,23 +374,52 @@ static AttendShape attend_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     return attend_shape(c, b->sequences, b->tokens, a->longest_chunk, most_keys(c, a->longest), a);
 }
 
-// An attention over shared prefixes: two launches, of the prefixes with a group for a sequence, and of what is behind them.
+// An attention over shared prefixes, by sizes alone: tiles of the prefixes, with a group for a sequence, and of what is behind them.
 struct SharedShape {
+    bool both;                           // by tiles of the sequences' own rows, all keys: `rest` is an attention's
     AttendShape prefix, rest;
-    uint64_t parts_bytes, bytes;         // of the workspace: counters and sums of the second one's parts; with the sums of the prefixes' parts behind them
+    uint64_t bytes;                      // of the workspace: sums of the parts of either
 };
 
 static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, const hspmm_prefix *p, const hspmm_attention *a)
 {
     SharedShape sh{};
     const uint64_t all = most_keys(c, a->longest), common = std::min<uint64_t>(p->longest ? p->longest : all, all);
+    // Where a sequence's own rows fill tiles of the chunk kernel there is nothing to win by others' beside them, and sums need not go through memory.  us, 16 chunks of 50 to 250
+    // tokens, 32 heads on 8, behind 3000 and 6000, bf16: 295 so; 393 by tiles of the prefixes' rows, 58 of them the launch that adds up; 8 beams over 1000 keys, a token each, 17, and 21 as an attention.
+    sh.rest = attend_shape(c, b, a);
+    sh.both = sh.rest.rows_log != kAttendRowsLog && uint64_t(std::min(a->longest_chunk, b->tokens)) * (a->q_heads / c->heads) >= 128u;
+    if (sh.both) {
+        sh.bytes = sh.rest.bytes;
+        return sh;
+    }
     hspmm_attention whole = *a;
     whole.window = 0u;
     sh.prefix = attend_shape(c, p->groups, b->tokens, p->most_tokens ? p->most_tokens : b->tokens, common, &whole);
     // (keys behind the prefix: the longest sequence is taken to have the longest one)
-    sh.rest = attend_shape(c, b->sequences, b->tokens, a->longest_chunk, std::max<uint64_t>(all - common, std::min<uint64_t>(std::max(a->longest_chunk, 1u), all)), a);
-    sh.parts_bytes = (sh.rest.bytes + 15u) & ~uint64_t(15u);
-    sh.bytes = sh.parts_bytes + sh.prefix.splits * uint64_t(b->tokens) * a->q_heads * (c->head_dim + kPrefixExtra) * 4u;
+    const uint64_t behind = std::max<uint64_t>(all - common, std::min<uint64_t>(std::max(a->longest_chunk, 1u), all));
+    sh.rest = attend_shape(c, b->sequences, b->tokens, a->longest_chunk, behind, a);
+    const uint32_t shared = a->q_heads / c->heads;
+    auto tiles_of = [&](AttendShape &x, uint32_t sequences, uint32_t log) { x.rows_log = log; x.tiles = uint32_t(attend_tiles(b->tokens, sequences, shared, log)); };
+    auto parts_of = [](AttendShape &x, uint64_t keys, uint64_t part) {
+        x.part_keys = uint32_t(std::max<uint64_t>((part + 127u) & ~uint64_t(127u), 128u));
+        x.splits = uint32_t(std::min<uint64_t>(std::max<uint64_t>((keys + 31u + x.part_keys - 1u) / x.part_keys, 1u), 256u));
+    };
+    tiles_of(sh.prefix, p->groups, std::min(sh.prefix.rows_log, 7u));
+    if (sh.prefix.rows_log == kAttendRowsLog) sh.rest.rows_log = kAttendRowsLog;
+    tiles_of(sh.rest, b->sequences, std::min(sh.rest.rows_log, 7u));
+    // Parts cost a row's sums each, written and read, but nobody waits for them.  us by keys of a prefix's part / of what is behind one's: 8 beams over 1000 keys by 128 / 256 / 512 / 1024 17.8 /
+    // 15.6 / 16.1 / 19.9; 64 sequences of up to 1500 behind 8000 by 256 / 512 / 768 / 1024 / 1536 102 / 79 / 72 / 67 / 75, and with 1024 there by 256 / 512 / 1024 / 1536 75 / 69 / 67 / 70; fp32 drafts over
+    // up to 6000 81 / 67 / - / 60 / 70 and 60 / 60 / 64 / -.
+    auto spread = [&](const AttendShape &x, uint32_t sequences, uint64_t keys) {
+        const uint64_t most = uint64_t(sequences) * ((uint64_t(std::min(&x == &sh.prefix ? (p->most_tokens ? p->most_tokens : b->tokens) : a->longest_chunk, b->tokens)) * shared + (1u << x.rows_log) - 1u) >> x.rows_log);
+        const uint64_t cells = std::max<uint64_t>(std::min<uint64_t>(most, x.tiles) * c->heads, 1u);
+        return std::min<uint64_t>(std::max<uint64_t>(cells * keys / 128u, 256u), 1024u);
+    };
+    parts_of(sh.prefix, common, spread(sh.prefix, p->groups, common));
+    parts_of(sh.rest, behind, spread(sh.rest, b->sequences, behind));
+    // (behind an attention's counters, so that one workspace serves both)
+    sh.bytes = kAttendCounters * 4u + uint64_t(sh.prefix.splits + sh.rest.splits) * b->tokens * a->q_heads * (c->head_dim + kPrefixExtra) * 4u;
     return sh;
 }
 
@@ -408,6 +437,19 @@ static int check_tiles(const hspmm_cache *c, const hspmm_batch *b, const AttendS
     if (uint64_t(sh.tiles) * c->heads < (1u << 23)) return HSPMM_OK;
     return fail(HSPMM_ERR_UNSUPPORTED, "%u tokens of %u sequences with %u heads of keys: in several calls", b->tokens, b->sequences, c->heads);
 }
+
+}  // extern "C"
+
+// (launches have fewer than 2^32 threads, 256 a workgroup)
+static int check_shared(const hspmm_cache *c, const hspmm_batch *b, const hspmm_attention *a, const SharedShape &sh)
+{
+    if (sh.both) return check_tiles(c, b, sh.rest);
+    const uint64_t groups = uint64_t(c->heads) * (uint64_t(sh.prefix.tiles) * sh.prefix.splits + uint64_t(sh.rest.tiles) * sh.rest.splits), merged = (uint64_t(b->tokens) + 15u) / 16u * a->q_heads;
+    if (groups < (1u << 23) && merged < (1u << 24)) return HSPMM_OK;
+    return fail(HSPMM_ERR_UNSUPPORTED, "%u tokens of %u sequences with %u heads of keys: in several calls", b->tokens, b->sequences, c->heads);
+}
+
+extern "C" {
 
 int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_attention *attention, uint64_t *bytes)
 {
@@ -447,12 +489,6 @@ static AttendArgs attend_args(const hspmm_cache *cache, uint32_t layer, const hs
     return aa;
 }
 
-static hipError_t launch_attend(int dtype, const AttendArgs &aa, AttendSpan span, const AttendShape &sh, void *stream)
-{
-    if (sh.rows_log == kAttendRowsLog) return launch_attend_rows(dtype, aa, span, sh.past, static_cast<hipStream_t>(stream));
-    return launch_attend_chunk(dtype, aa, span, sh.rows_log, static_cast<hipStream_t>(stream));
-}
-
 static int check_workspace(const void *workspace, uint64_t bytes, uint64_t wanted)
 {
     if (wanted && (!workspace || bytes < wanted || reinterpret_cast<uintptr_t>(workspace) % 16u))
@@ -474,7 +510,8 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     if (int rc = check_workspace(workspace, workspace_bytes, sh.bytes)) return rc;
     if (int rc = check_device()) return rc;
     const AttendArgs aa = attend_args(cache, layer, batch, attention, q, out, lse, sh, workspace);
-    HSPMM_HIP(launch_attend(cache->dtype, aa, kSpanAll, sh, stream));
+    if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, sh.past, static_cast<hipStream_t>(stream)));
+    else HSPMM_HIP(launch_attend_chunk(cache->dtype, aa, false, sh.rows_log, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
 
@@ -487,8 +524,7 @@ int hspmm_cache_attend_shared_workspace(const hspmm_cache *cache, const hspmm_ba
     if (batch->tokens == 0) { *bytes = 0; return HSPMM_OK; }
     const SharedShape sh = shared_shape(cache, batch, prefix, attention);
     *bytes = sh.bytes;
-    if (int rc = check_tiles(cache, batch, sh.prefix)) return rc;
-    return check_tiles(cache, batch, sh.rest);
+    return check_shared(cache, batch, attention, sh);
 }
 
 int hspmm_cache_attend_shared(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_prefix *prefix, const hspmm_attention *attention,
@@ -501,18 +537,17 @@ int hspmm_cache_attend_shared(const hspmm_cache *cache, uint32_t layer, const hs
     if (batch->tokens == 0) return HSPMM_OK;
     if (int rc = check_attend_tensors(cache, layer, q, out, lse)) return rc;
     const SharedShape sh = shared_shape(cache, batch, prefix, attention);
-    if (int rc = check_tiles(cache, batch, sh.prefix)) return rc;
-    if (int rc = check_tiles(cache, batch, sh.rest)) return rc;
+    if (int rc = check_shared(cache, batch, attention, sh)) return rc;
     if (int rc = check_workspace(workspace, workspace_bytes, sh.bytes)) return rc;
     if (int rc = check_device()) return rc;
-    const PrefixArgs pa{prefix->firsts, prefix->tokens, prefix->groups, sh.prefix.splits, sh.prefix.part_keys, reinterpret_cast<float *>(static_cast<char *>(workspace) + sh.parts_bytes),
-                        int64_t(batch->tokens) * attention->q_heads * (cache->head_dim + kPrefixExtra)};
-    AttendArgs aa = attend_args(cache, layer, batch, attention, q, out, lse, sh.prefix, workspace);
-    aa.prefix = pa;
-    HSPMM_HIP(launch_attend(cache->dtype, aa, kSpanPrefix, sh.prefix, stream));
-    aa = attend_args(cache, layer, batch, attention, q, out, lse, sh.rest, workspace);
-    aa.prefix = pa;
-    HSPMM_HIP(launch_attend(cache->dtype, aa, kSpanRest, sh.rest, stream));
+    AttendArgs of_prefix = attend_args(cache, layer, batch, attention, q, out, lse, sh.prefix, workspace), of_rest = attend_args(cache, layer, batch, attention, q, out, lse, sh.rest, workspace);
+    of_prefix.prefix = of_rest.prefix = PrefixArgs{prefix->firsts, prefix->tokens, prefix->groups, sh.prefix.splits, sh.prefix.part_keys, of_rest.sums,
+                                                   int64_t(batch->tokens) * attention->q_heads * (cache->head_dim + kPrefixExtra)};
+    if (sh.both) {
+        HSPMM_HIP(launch_attend_chunk(cache->dtype, of_rest, true, sh.rest.rows_log, static_cast<hipStream_t>(stream)));
+        return HSPMM_OK;
+    }
+    HSPMM_HIP(launch_attend_shared(cache->dtype, of_prefix, of_rest, sh.prefix.rows_log != kAttendRowsLog, sh.rest.rows_log != kAttendRowsLog, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
 
@@ -594,7 +629,8 @@ static WeighShape weigh_shape(const hspmm_cache *c, const hspmm_batch *b, const 
     // parts of the rows: as many as make some thousand workgroups, 256 rows at least
     sh.part_rows = uint32_t(std::max<uint64_t>(up(up(rows * sh.cells, 1536u), 64u) * 64u, 256u));
     sh.parts = uint32_t(std::min<uint64_t>(up(rows, sh.part_rows), 256u));
-    if (sh.parts > 1u) sh.bytes = ((sh.cells * 4u + 15u) & ~uint64_t(15u)) + sh.cells * sh.parts * kWeighKeys * 4u;
+    if (sh.cells > kAttendCounters) sh.parts = 1u;
+    if (sh.parts > 1u) sh.bytes = kAttendCounters * 4u + sh.cells * sh.parts * kWeighKeys * 4u;
     return sh;
 }
 
@@ -645,7 +681,7 @@ int hspmm_cache_weigh(const hspmm_cache *cache, uint32_t layer, const hspmm_batc
     }
     wa.blocks = Divisor::of(sh.blocks); wa.part_rows = sh.part_rows;
     wa.arrive = static_cast<uint32_t *>(workspace);
-    wa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + ((sh.cells * 4u + 15u) & ~uint64_t(15u)));
+    wa.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + kAttendCounters * 4u);
     HSPMM_HIP(launch_weigh_chunk(cache->dtype, wa, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
@@ -660,7 +696,7 @@ static EvictShape evict_shape(const hspmm_cache *c, uint32_t n, uint32_t keep)
     EvictShape sh{};
     sh.keep_pages = (keep + c->page_tokens - 1u) / c->page_tokens;
     const uint64_t lists = uint64_t(c->layers) * n * c->heads * keep, pages = uint64_t(n) * sh.keep_pages;
-    sh.entries = sh.arrive + 16u;
+    sh.entries = sh.arrive + kAttendCounters;                    // (an attention's, so that one workspace serves both)
     sh.rows = sh.entries + uint64_t(n) * kEvictEntry;
     sh.to = sh.rows + uint64_t(n) * c->table_pages;
     sh.free = sh.to + pages;

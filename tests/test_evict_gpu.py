@@ -285,3 +285,21 @@ def test_captured_and_on_another_stream(torch_cuda, hs):
         assert np.array_equal(kept.cpu().numpy(), lists)
         for x in ("table", "lengths", "references", "weights"):
             assert np.array_equal(after[x], want[x]), x
+
+
+@pytest.mark.parametrize("lengths,keep,first,last", [([9000, 40], 2100, 4, 300), ([16384, 8193], 8000, 0, 0), ([16385], 16384, 1, 1), ([30000, 12000], 5000, 100, 1000)])
+@pytest.mark.parametrize("kind", ["random", "ties"])
+def test_long_sequences(torch_cuda, hs, lengths, keep, first, last, kind):
+    # more tokens than a workgroup's threads have in registers, and just as many
+    m, rng = filled(torch_cuda, hs, keep, 2, 0, lengths, 64, 1, 8, 1, -(-max(lengths) // 64) + 1, 2 * len(lengths) * (-(-keep // 64)), extra=len(lengths), kind=kind)
+    n = len(lengths)
+    assert m.check(list(range(n)), list(range(n, 2 * n)), keep, first, last) == 0
+    assert m.check(list(range(n)), None, keep, first, last) == 0
+
+
+def test_many_entries(torch_cuda, hs):
+    # more entries than a workgroup has threads, in place and into others
+    n = 1100
+    m, rng = filled(torch_cuda, hs, 3, 0, 0, [5 + (7 * i) % 30 for i in range(n)], 4, 1, 8, 1, 9, 2 * n * 3, extra=n)
+    assert m.check(list(range(n)), list(range(n, 2 * n)), 9, 1, 2) == 0
+    assert m.check(list(rng.permutation(n)), None, 9, 1, 2) == 0

@@ -272,3 +272,56 @@ def test_a_captured_call_and_two_workspaces(torch_cuda, hs):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+# many rows over a long prefix: tiles of 128 rows for the prefix, of 16 or of 128 for what is behind it; heads of every kernel's size
+LARGE = [([64], [4001], [3, 60], [1], 0, 4, 8, 128, 16, 0, True), ([40, 23], [3500, 2900], [0, 33], [1], 1, 4, 8, 64, 24, 0, True), ([64], [3900], [20], [1], 0, 4, 8, 96, 32, 700, True),
+         ([50], [4100], [9], [1], 0, 4, 8, 160, 16, 0, True), ([40], [3000], [500, 400], [3], 0, 4, 16, 128, 16, 0, True), ([33], [2200], [700], [7], 1, 4, 8, 80, 48, 0, True)]
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("number", range(len(LARGE)))
+def test_many_rows_over_a_long_prefix(torch_cuda, hs, dtype, number):
+    torch = torch_cuda
+    CASES.append(LARGE[number])
+    try:
+        c = Case(torch, hs, dtype, len(CASES) - 1, order=number % 2)
+    finally:
+        CASES.pop()
+    want = c.want()
+    for layout in ("tokens", "features"):
+        out, lse = c.run(torch, hs, layout=layout)
+        assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)
+    again, _ = c.run(torch, hs, layout="gaps", lse=False)
+    assert torch.equal(out, again)
+
+
+def test_one_workspace_serves_every_call_in_turn(torch_cuda, hs):
+    # the calls leave the workspace as they want to find it, each other's among them
+    torch = torch_cuda
+    from test_cache_gpu import attend, attention_case
+    c = Case(torch, hs, 2, 5)
+    st, batch, attention, q, k, v, new, old, rows, scale, window, causal = attention_case(torch, hs, 2, 13)
+    alone, lse = attend(torch, hs, st, batch, attention, q)
+    want, _ = c.run(torch, hs)
+    weights = torch.zeros((1, st.table.shape[0], st.heads, st.table.shape[1] * st.page_tokens), device="cuda")
+    into = hs.Weights(weights.data_ptr(), *weights.stride()[:3])
+    qd, stream = device(torch, q, 2), torch.cuda.current_stream().cuda_stream
+    one = ints(torch, [int(rows[0])])
+    need = max(st.handle.attend_workspace(batch, attention), c.st.handle.attend_shared_workspace(c.batch, c.prefixes(hs), c.attention), st.handle.weigh_workspace(batch, attention),
+               st.handle.evict_workspace(1, 1500), st.handle.weigh_workspace(batch, hs.Attention(attention.q_heads, attention.scale, longest_chunk=5000, longest=2000)))
+    w = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    many = hs.Attention(attention.q_heads, attention.scale, longest_chunk=5000, longest=2000)
+    for turn in range(3):
+        out, _ = attend(torch, hs, st, batch, attention, q, workspace=w)
+        assert torch.equal(out, alone)
+        out, _ = c.run(torch, hs, workspace=w)
+        assert torch.equal(out, want)
+        for a in (attention, many):
+            weights.zero_()
+            st.handle.weigh(0, batch, a, heads_view(hs, qd), lse.data_ptr(), into, workspace=w.data_ptr(), workspace_bytes=need, stream=stream)
+            total = weights.sum().item()
+            assert abs(total - q.shape[0] * q.shape[1]) <= 1e-4 * total
+        # (as many tokens as it has: nothing happens but the choice)
+        st.handle.evict(1, one.data_ptr(), 0, into, 1500, workspace=w.data_ptr(), workspace_bytes=need, stream=stream)
+        assert not w[: 4 * 16384].any()

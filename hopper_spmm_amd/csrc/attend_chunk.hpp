@@ -51,9 +51,35 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
     const uint32_t head = cell.head, tile_number = cell.tile;
     const RowTile t = find_tile<kRowsLog, Span>(aa, tile_number);
     if (!t.there) return;
+    const KeyPart keys_here = key_part(aa, t, part);
+    constexpr bool kJoins = Span == kSpanAll || Span == kSpanBoth;
+    const int32_t parts = kJoins ? keys_here.parts : 1, end = keys_here.end;
+    if (int32_t(part) >= keys_here.parts) return;
+    if (tid == 0u) odd = 0u;
+
     const uint32_t m = wave * 32u + j;
     const bool is_row = m < t.rows;
     const RowOf row = row_of_tile<Span>(aa, t, head, m);
+    const float scale = aa.scale == 0.f ? 1.f : fabsf(aa.scale) * kLog2e;
+    const uint32_t flip = aa.scale < 0.f ? 0x80008000u : 0u;
+    u32x4 q[kSteps];
+    {
+        const char *from = aa.q.data + (int64_t(row.token) * aa.q.token_stride + int64_t(row.head) * aa.q.head_stride) * 2;
+        // (loads without conditions: one wait for all of them)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const uint32_t d = 16u * s + 8u * h;
+            q[s] = *reinterpret_cast<const u32x4 *>(from + (d < D ? d : 0u) * 2u);
+        }
+        const uint32_t keep = is_row && aa.scale != 0.f ? ~0u : 0u;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) q[s] = (q[s] ^ flip) & keep;
+        if (D < uint32_t(DP)) {
+            asm volatile("");
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) q[s] &= 16u * s + 8u * h < D ? ~0u : 0u;
+        }
+    }
     // keys that all of the wave's rows see
     int32_t all_lo = is_row ? row.lo : 0, all_hi = is_row ? row.hi : 0x7FFFFFFF, any_lo = is_row ? row.lo : 0x7FFFFFFF;
 #pragma unroll
@@ -85,10 +111,6 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
         group_lo = aa.window && int64_t(p1) + 1 > int64_t(aa.window) ? p1 + 1 - int32_t(aa.window) : 0;
         if constexpr (Span == kSpanRest) group_lo = max(group_lo, t.prefix);
     }
-    const KeyPart keys_here = key_part(aa, t, part);
-    constexpr bool kJoins = Span == kSpanAll || Span == kSpanBoth;
-    const int32_t parts = kJoins ? keys_here.parts : 1, end = keys_here.end;
-    if (int32_t(part) >= keys_here.parts) return;
     // (rows of several sequences: from the first key that any of them sees)
     const int32_t begin = Span == kSpanPrefix ? max(keys_here.begin, min(any_lo & ~31, end)) : keys_here.begin;
     // Images of 64 keys: of the prefix (kSpanBoth), by its first sequence's pages, then of what is behind it, from where a group of 16 begins.
@@ -100,28 +122,6 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
     const int32_t n_images = first_images + (end > (Span == kSpanBoth ? max(begin, t.prefix) : begin) ? (end - behind + 63) / 64 : 0);
     auto key_of = [&](int32_t n) __attribute__((always_inline)) { return Span == kSpanBoth && n < first_images ? begin + n * 64 : behind + (n - first_images) * 64; };
     auto end_of = [&](int32_t n) __attribute__((always_inline)) { return Span == kSpanBoth && n < first_images ? min(end, t.prefix) : end; };
-    if (tid == 0u) odd = 0u;
-
-    const float scale = aa.scale == 0.f ? 1.f : fabsf(aa.scale) * kLog2e;
-    const uint32_t flip = aa.scale < 0.f ? 0x80008000u : 0u;
-    u32x4 q[kSteps];
-    {
-        const char *from = aa.q.data + (int64_t(row.token) * aa.q.token_stride + int64_t(row.head) * aa.q.head_stride) * 2;
-        // (loads without conditions: one wait for all of them)
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const uint32_t d = 16u * s + 8u * h;
-            q[s] = *reinterpret_cast<const u32x4 *>(from + (d < D ? d : 0u) * 2u);
-        }
-        const uint32_t keep = is_row && aa.scale != 0.f ? ~0u : 0u;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) q[s] = (q[s] ^ flip) & keep;
-        if (D < uint32_t(DP)) {
-            asm volatile("");
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) q[s] &= 16u * s + 8u * h < D ? ~0u : 0u;
-        }
-    }
     const int32_t *table = aa.pages.table + size_t(t.sequence) * aa.pages.table_pages, *const lead = aa.pages.table + size_t(Span == kSpanBoth ? t.leader : t.sequence) * aa.pages.table_pages;
     const int64_t head_offset = int64_t(head) * aa.pages.head_stride;
     // Where keys lie, in bytes from keys and values: of groups of 16 keys, four an image, of 16 images at a time, a lane each (Whole), or of

@@ -594,11 +594,14 @@ int hspmm_cache_compact(const hspmm_cache *cache, int32_t *table_out, int32_t *r
 
 }  // extern "C"
 
-static int check_weights(const hspmm_weights *w)
+// tokens, sequences: that a head's row has at least, and that have rows which are written at a time (rows side by side are written by different workgroups).
+static int check_weights(const hspmm_cache *c, const hspmm_weights *w, uint64_t tokens, uint32_t sequences, uint32_t layers)
 {
     if (!w || !w->data) return fail(HSPMM_ERR_INVALID, "null weights");
     if (reinterpret_cast<uintptr_t>(w->data) % 4u) return fail(HSPMM_ERR_INVALID, "weights are not aligned to their elements");
     if (w->layer_stride < 0 || w->sequence_stride < 0 || w->head_stride < 0) return fail(HSPMM_ERR_INVALID, "weights: strides below 0");
+    if ((c->heads > 1u && uint64_t(w->head_stride) < tokens) || (sequences > 1u && uint64_t(w->sequence_stride) < tokens) || (layers > 1u && uint64_t(w->layer_stride) < tokens))
+        return fail(HSPMM_ERR_INVALID, "weights: rows of %llu tokens that overlap", (unsigned long long)tokens);
     return HSPMM_OK;
 }
 
@@ -658,7 +661,7 @@ int hspmm_cache_weigh(const hspmm_cache *cache, uint32_t layer, const hspmm_batc
     if (int rc = check_weigh(cache, batch, attention)) return rc;
     if (layer >= cache->layers) return fail(HSPMM_ERR_INVALID, "layer %u of %u", layer, cache->layers);
     if (!std::isfinite(decay)) return fail(HSPMM_ERR_INVALID, "decay %g", double(decay));
-    if (int rc = check_weights(weights)) return rc;
+    if (int rc = check_weights(cache, weights, 1u, batch->sequences, 1u)) return rc;
     if (batch->tokens == 0) return HSPMM_OK;
     if (int rc = check_heads("q", q, cache->dtype)) return rc;
     if (int rc = check_queries(cache, q)) return rc;
@@ -694,7 +697,7 @@ struct EvictShape { uint64_t arrive, entries, rows, to, free, kept, weights, wor
 static EvictShape evict_shape(const hspmm_cache *c, uint32_t n, uint32_t keep)
 {
     EvictShape sh{};
-    sh.keep_pages = (keep + c->page_tokens - 1u) / c->page_tokens;
+    sh.keep_pages = uint32_t((uint64_t(keep) + c->page_tokens - 1u) / c->page_tokens);
     const uint64_t lists = uint64_t(c->layers) * n * c->heads * keep, pages = uint64_t(n) * sh.keep_pages;
     sh.entries = sh.arrive + kAttendCounters;                    // (an attention's, so that one workspace serves both)
     sh.rows = sh.entries + uint64_t(n) * kEvictEntry;
@@ -710,7 +713,7 @@ static int check_eviction(const hspmm_cache *c, uint32_t n, uint32_t keep)
 {
     if (int rc = check_cache(c)) return rc;
     if (n > c->sequences) return fail(HSPMM_ERR_INVALID, "a list of %u for a cache of %u sequences", n, c->sequences);
-    if (!keep || keep > uint64_t(c->table_pages) * c->page_tokens) return fail(HSPMM_ERR_INVALID, "%u tokens to keep, of at most %llu", keep, (unsigned long long)c->table_pages * c->page_tokens);
+    if (!keep || keep > 0x7FFFFFFFu || keep > uint64_t(c->table_pages) * c->page_tokens) return fail(HSPMM_ERR_INVALID, "%u tokens to keep, of at most %llu", keep, (unsigned long long)c->table_pages * c->page_tokens);
     // (a launch has fewer than 2^32 threads, 1024 a workgroup, or 256 and up to 2 x 16384 + 1 workgroups a head)
     const uint64_t cells = uint64_t(n) * c->layers * c->heads;
     PoolArgs pa{};
@@ -734,7 +737,7 @@ int hspmm_cache_evict(const hspmm_cache *cache, uint32_t n, const int32_t *paren
 {
     if (int rc = check_eviction(cache, n, keep)) return rc;
     if (int rc = check_list(cache, n, parents, "parents")) return rc;
-    if (int rc = check_weights(weights)) return rc;
+    if (int rc = check_weights(cache, weights, uint64_t(cache->table_pages) * cache->page_tokens, cache->sequences, cache->layers)) return rc;
     if (uint64_t(first) + last > keep) return fail(HSPMM_ERR_INVALID, "the first %u and the last %u tokens, of %u to keep", first, last, keep);
     if (n == 0 && !status) return HSPMM_OK;
     const EvictShape sh = evict_shape(cache, n, keep);

@@ -196,14 +196,14 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void weigh_chunk_kerne
                     unit(masked, std::integral_constant<int, 2>{}, seen[2], base);
                     find();
                     unit(masked, std::integral_constant<int, 3>{}, seen[3], base);
-                    base = lse_ahead * -kLog2e;
+                    base = moved_by(lse_ahead);
                 }
                 return n;
             };
             static_assert(kTiles == 4, "");
             put();
             find();
-            base = lse_ahead * -kLog2e;
+            base = moved_by(lse_ahead);
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) read_q(s);
 #pragma unroll

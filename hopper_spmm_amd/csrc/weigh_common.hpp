@@ -47,6 +47,9 @@ __device__ __forceinline__ RowOf weigh_row(const WeighArgs &wa, const WeighRows 
     return r;
 }
 
+// -lse in units of ln 2: what a row's scores are moved by.  Of a row whose lse says that it sees nothing every key receives 0.
+__device__ __forceinline__ float moved_by(float lse) { return lse == -INFINITY ? -INFINITY : lse * -kLog2e; }
+
 // The rows [first, end) that may see a key of [key0, key0 + n).
 struct RowRange { uint32_t first, end; };
 __device__ __forceinline__ RowRange rows_that_see(const WeighArgs &wa, const WeighRows &w, int32_t key0, int32_t n)

@@ -118,7 +118,7 @@ __global__ __launch_bounds__(64 * kWeighWaves) void weigh_rows_kernel(const Weig
     constexpr uint32_t kBatch = Few ? 16u : kWeighBatch, kPitch = DP * K::kElem + 16u, kRowPieces = DP / K::kPiece;
     constexpr int32_t kKeys = K::kKeys;
     __shared__ __attribute__((aligned(16))) char rows_of[Few ? 16 : kBatch * kPitch];
-    __shared__ float lse_of[kBatch];
+    __shared__ float by_of[kBatch];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i = lane & 15u, D = wa.pages.head_dim;
     const uint32_t b = wa.heads.quotient(blockIdx.x), head = blockIdx.x - b * wa.heads.d;
     const WeighRows w = weigh_rows(wa, b);
@@ -141,11 +141,11 @@ __global__ __launch_bounds__(64 * kWeighWaves) void weigh_rows_kernel(const Weig
         const uint32_t end = min(w.rows, base + kBatch);
         RowOf row{};
         typename K::Query Q;
-        float lse = 0.f;
+        float by = 0.f;
         if constexpr (Few) {
             row = weigh_row(wa, w, head, base + i);
             K::load_query(Q, wa.q.data + (int64_t(row.token) * wa.q.token_stride + int64_t(row.head) * wa.q.head_stride) * K::kElem, base + i < end, lane, D);
-            lse = wa.lse[size_t(row.token) * wa.q_heads + row.head] * kLog2e;
+            by = moved_by(wa.lse[size_t(row.token) * wa.q_heads + row.head]);
         } else {
             __syncthreads();
             // (of rows behind the last one the first is read, and not used; behind a row's last element its first ones, which meet zeros of the keys)
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(64 * kWeighWaves) void weigh_rows_kernel(const Weig
             }
             if (tid < kBatch) {
                 const RowOf r = weigh_row(wa, w, head, base + tid);
-                lse_of[tid] = wa.lse[size_t(r.token) * wa.q_heads + r.head] * kLog2e;
+                by_of[tid] = moved_by(wa.lse[size_t(r.token) * wa.q_heads + r.head]);
             }
             __syncthreads();
         }
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(64 * kWeighWaves) void weigh_rows_kernel(const Weig
 #pragma unroll
                     for (int t = 0; t < K::kParts; ++t)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) sums[t][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, -lse));
+                        for (int r = 0; r < 4; ++r) sums[t][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, by));
                 } else {
                     if constexpr (!Few) row = weigh_row(wa, w, head, m0 + i < end ? m0 + i : w.rows);
                     const int32_t low = row.lo - key0 - int32_t(4u * g), high = row.hi - key0 - int32_t(4u * g);
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(64 * kWeighWaves) void weigh_rows_kernel(const Weig
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const int a = 16 * t + r;
-                            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, -lse));
+                            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, by));
                             sums[t][r] += select(bool(int(a < low) | int(a >= high) | int(!(there >> a & 1u))), 0.f, p);
                         }
                 }
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(64 * kWeighWaves) void weigh_rows_kernel(const Weig
 #pragma unroll 1
                 for (uint32_t m0 = m_first; m0 < m_end; m0 += 16u) {
                     K::load_rows(Q, rows_of + (m0 - base + i) * kPitch, lane);
-                    lse = lse_of[m0 - base + i];
+                    by = by_of[m0 - base + i];
                     f32x4 s[K::kParts];
                     k.scores(Q, s);
                     if (m0 + 16u >= m_end) request(at);

@@ -638,7 +638,9 @@ typedef struct hspmm_weights {
 } hspmm_weights;
 /* weights of `layer` <- decay * weights + sum over the batch's tokens, and the query heads that share a head of keys, of
  * exp(scale * q k - lse), for every key of the batch's sequences; the batch's own tokens begin with 0, what is behind a
- * sequence's last token stays as it is.  What a token does not see, or has no page, receives nothing from it.
+ * sequence's last token stays as it is.  What a token does not see, or has no page, receives nothing from it, and a token
+ * whose lse is -infinity (it sees nothing) gives nothing.  Keys are read by a sequence's own pages, which of a prefix of hspmm_cache_attend_shared have to be
+ * there as well.  A sequence is in the batch once, and its rows of weights do not overlap others'.
  * q, lse: those of hspmm_cache_attend (or _shared), with the same attention.  last: of a sequence's tokens in the batch only that
  * many last ones count (0: all).  Products as in attend, the rest in fp32.
  * workspace: as for attend, of hspmm_cache_weigh_workspace bytes; zero before its first use. */
@@ -668,7 +670,7 @@ int hspmm_cache_free(const hspmm_cache *cache, uint32_t n, const int32_t *rows, 
  * A sequence that is its own child and has no more than `keep` tokens stays as it is; one with more is rewritten in the pages it has, but for those that
  * others name as well, or where it is another entry's parent, too: there, and for other children, pages are given out.  A child that the pool has no pages for stays as it was; *status
  * receives how many pages were missing.  Pages released become free as in hspmm_cache_fork.
- * kept (layers x n x heads x keep, may be null): the numbers of the tokens kept, -1 behind them.
+ * kept (layers x n x heads x keep, may be null): the numbers of the tokens kept, -1 behind them; of an entry that stays as it is those that a choice had left.
  * workspace: hspmm_cache_evict_workspace bytes, aligned to 16 bytes; zero before its first use, and not used by two calls that overlap in time. */
 int hspmm_cache_evict(const hspmm_cache *cache, uint32_t n, const int32_t *parents, const int32_t *children, const hspmm_weights *weights, uint32_t keep, uint32_t first,
                       uint32_t last, int32_t *kept, int32_t *status, void *workspace, uint64_t workspace_bytes, void *stream);

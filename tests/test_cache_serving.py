@@ -108,3 +108,22 @@ def test_calls_fail_loudly_without_a_gfx950_device(hs):
     for f in (lambda: c.attend_shared(0, b, hs.Prefix(1, ADDRESS, ADDRESS), a, x, x, **big), lambda: c.weigh(0, b, a, x, ADDRESS, w, **big),
               lambda: c.evict(2, ADDRESS, 0, w, 8, **big), lambda: c.evict(0, 0, 0, w, 8, status=ADDRESS)):
         refused(hs, 2, f)
+
+
+def test_rows_of_weights_that_overlap_are_refused(hs):
+    c, b, a, x, w = cache(hs), hs.Batch(3, 4, ADDRESS), hs.Attention(8, 0.125), hs.Heads(ADDRESS, 512, 64), hs.Weights(ADDRESS, 3 * 4 * 64, 4 * 64, 64)
+    need = c.evict_workspace(2, 8)
+    for bad in (hs.Weights(ADDRESS, 768, 256, 63), hs.Weights(ADDRESS, 768, 63, 256), hs.Weights(ADDRESS, 0, 256, 64), hs.Weights(ADDRESS, 768, 256, 0)):
+        refused(hs, 1, lambda: c.evict(2, ADDRESS, 0, bad, 8, workspace=ADDRESS, workspace_bytes=need), "overlap")
+    for bad in (hs.Weights(ADDRESS, 768, 0, 64), hs.Weights(ADDRESS, 768, 256, 0)):
+        refused(hs, 1, lambda: c.weigh(0, b, a, x, ADDRESS, bad), "overlap")
+    assert w.head_stride == 64
+
+
+def test_an_eviction_of_very_many_tokens_has_room_for_its_pages(hs):
+    # (what is to be kept and a page of tokens pass 32 bits together)
+    c = cache(hs, layers=1, heads=1, head_dim=8, page_tokens=1 << 24, table_pages=256, sequences=1, pages=256)
+    keep = 0x7FFFFFFF
+    assert c.evict_workspace(1, keep) >= 4 * (2 * keep + 256 + 128 + 128)
+    for keep in (0x80000000, 0xFFFFFFFF):
+        refused(hs, 1, lambda: c.evict_workspace(1, keep), "keep")

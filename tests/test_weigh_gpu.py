@@ -260,3 +260,21 @@ def test_a_captured_call_on_another_stream(torch_cuda, hs):
                 graph.replay()
             torch.cuda.synchronize()
             assert np.array_equal(to64(c.weights), want)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("number", [4, 6, 9, 13, 24])
+def test_rows_whose_lse_is_infinite_give_nothing(torch_cuda, hs, dtype, number):
+    # every third one says that it sees nothing, though there are keys that it would see
+    c = Case(torch_cuda, hs, dtype, number, seed=5)
+    full = c.lse.clone()
+    c.lse.view(-1)[::3] = -np.inf
+    for a in [None] + hints(hs, c):
+        c.weights.copy_(torch_cuda.from_numpy(c.before))
+        got = c.run(hs, decay=0.5, attention=a)
+        assert np.isfinite(got).all()
+    # as with those rows' lse so large that nothing is left of what they give
+    c.lse = full
+    c.lse.view(-1)[::3] = 1e30
+    c.weights.copy_(torch_cuda.from_numpy(c.before))
+    assert np.array_equal(c.run(hs, decay=0.5, attention=a), got)

@@ -1,11 +1,14 @@
 """The attention block of a decoder whose four projections are pruned: sparse products, rotary positions, a paged cache and
 the attention over it, as a serving loop runs them.
 
-    python examples/pruned_attention.py [--hidden 1024] [--heads 8] [--kv-heads 2] [--keep 0.1] [--layers 2]
+    python examples/pruned_attention.py [--hidden 1024] [--heads 8] [--kv-heads 2] [--keep 0.1] [--layers 2] [--budget 40]
 
 Prompts of different lengths go through as one ragged batch, every prompt is forked into beams, the beams decode and are
 reordered, one prompt's beams end and its pages are compacted away.  Activations lie features x tokens, which is what
 `Plan.run` reads and writes; `append` and `attend` take them by their strides, so nothing is transposed in between.
+
+With a budget a sequence holds no more tokens than that: beams attend their prompt together (`attend_shared`), what every cached
+token receives is added up (`weigh`), and the tokens that received least leave (`evict`).
 """
 import argparse
 import math
@@ -172,12 +175,183 @@ def run(hidden=1024, heads=8, kv_heads=2, keep=0.1, layers=2, prompts=(70, 33, 5
     return out.cpu().double().numpy(), np.stack([w[:, -1] for w in want], 1), largest
 
 
+class BoundedDecoder(Decoder):
+    """The same with prompts that beams read together and a cache of bounded length.  Where tokens have left, a sequence's next position is no
+    longer its length: the caller says the positions, by which queries and keys are turned before they are appended."""
+
+    def __init__(self, *args):
+        super().__init__(*args)
+        self.weights = torch.zeros(len(self.layers), self.lengths.numel(), self.kv_heads, self.table.shape[1] * self.keys.shape[3], device="cuda")
+        self.received = hs.Weights(self.weights.data_ptr(), *self.weights.stride()[:3])
+
+    def reserve(self, need):
+        if need > self.workspace.numel():
+            self.workspace = torch.zeros(need, dtype=torch.uint8, device="cuda")
+        return dict(workspace=self.workspace.data_ptr(), workspace_bytes=self.workspace.numel())
+
+    def turn(self, x, positions):
+        """features x tokens, as tokens x heads x dim at their positions."""
+        y = torch.empty((x.shape[1], x.shape[0] // self.dim, self.dim), dtype=TORCH, device="cuda")
+        hs.rotate(DTYPE, self.rotary, y.shape[0], y.shape[1], self.dim, view(heads_of(x, self.dim)), view(y), positions.data_ptr(), stream=stream())
+        return y
+
+    def forward(self, x, rows, new, positions, groups=(), decay=1.0, last=0):
+        """groups: (rows of the batch, tokens) that begin alike, of all rows in order, or none; decay, last: of the weights."""
+        rows_d, new_d, starts, positions = i32(rows), i32(new), i32(np.concatenate([[0], np.cumsum(new)])), i32(positions)
+        self.cache.extend(len(rows), rows_d.data_ptr(), new_d.data_ptr(), self.status.data_ptr(), stream())
+        batch = hs.Batch(len(rows), x.shape[1], starts.data_ptr(), rows_d.data_ptr())
+        attention = hs.Attention(self.heads, 1.0 / math.sqrt(self.dim), longest_chunk=max(new), longest=self.longest)
+        firsts, tokens = i32(np.cumsum([0] + [n for n, _ in groups])), i32([t for _, t in groups])
+        prefix = hs.Prefix(len(groups), firsts.data_ptr(), tokens.data_ptr() if groups else 0, longest=max([t for _, t in groups], default=0))
+        space = self.reserve(max(self.cache.attend_shared_workspace(batch, prefix, attention), self.cache.weigh_workspace(batch, attention, last)))
+        lse = torch.empty((x.shape[1], self.heads), device="cuda")
+        for i, layer in enumerate(self.layers):
+            q, k, v = (layer.product(j, x) for j in range(3))
+            q, k = self.turn(q, positions), self.turn(k, positions)
+            self.cache.append(i, batch, view(k), view(heads_of(v, self.dim)), stream=stream())
+            mixed = torch.empty((self.heads * self.dim, x.shape[1]), dtype=TORCH, device="cuda")
+            self.cache.attend_shared(i, batch, prefix, attention, view(q), view(heads_of(mixed, self.dim)), lse=lse.data_ptr(), stream=stream(), **space)
+            self.cache.weigh(i, batch, attention, view(q), lse.data_ptr(), self.received, decay=decay, last=last, stream=stream(), **space)
+            x = x + layer.product(3, mixed)
+        if int(self.status):
+            raise RuntimeError("%d pages are missing" % int(self.status))
+        return x
+
+    def fork(self, parents, children):
+        super().fork(parents, children)
+        self.weights[:, children] = self.weights[:, parents]
+
+    def evict(self, parents, children, keep, first, last):
+        """The tokens kept, layers x entries x heads x keep."""
+        p, c, kept = i32(parents), i32(children), i32(np.empty((len(self.layers), len(parents), self.kv_heads, keep)))
+        self.cache.evict(len(parents), p.data_ptr(), c.data_ptr(), self.received, keep, first=first, last=last, kept=kept.data_ptr(), status=self.status.data_ptr(),
+                         stream=stream(), **self.reserve(self.cache.evict_workspace(len(parents), keep)))
+        if int(self.status):
+            raise RuntimeError("%d pages are missing" % int(self.status))
+        return kept.cpu().numpy()
+
+
+class Mirror:
+    """What a BoundedDecoder does, in 64 bits.  Which tokens are kept is taken from it, and looked at: `worst` is the largest
+    weight in layer 0 that left, relative to the smallest one that stayed in its place; `reach` its largest scale |q| |k|."""
+
+    def __init__(self, decoder):
+        self.decoder, self.dense = decoder, [[layer.dense(j) for j in range(4)] for layer in decoder.layers]
+        self.angles = decoder.angles.cpu().double().numpy()
+        empty = np.zeros((decoder.kv_heads, 0, decoder.dim))
+        self.held = {s: [(empty, empty, empty[:, :, 0]) for _ in decoder.layers] for s in range(decoder.lengths.numel())}
+        self.largest = self.reach = self.worst = 0.0
+
+    def turn(self, y, positions):
+        half, a = self.decoder.dim // 2, self.angles[positions]
+        return np.concatenate([y[..., :half] * a[:, :, 0] - y[..., half:] * a[:, :, 1], y[..., :half] * a[:, :, 1] + y[..., half:] * a[:, :, 0]], -1)
+
+    def forward(self, s, x, positions, decay, last):
+        d, x = self.decoder, x.astype(np.float64)
+        n, shared = x.shape[1], d.heads // d.kv_heads
+        for i, w in enumerate(self.dense):
+            q, k, v = ((w[j] @ x).reshape(-1, d.dim, n).transpose(0, 2, 1) for j in range(3))
+            keys, values, weights = self.held[s][i]
+            old = keys.shape[1]
+            q, keys, values = self.turn(q, positions), np.concatenate([keys, self.turn(k, positions)], 1), np.concatenate([values, v], 1)
+            weights = np.concatenate([weights * decay, np.zeros((d.kv_heads, n))], 1)
+            mixed = np.zeros_like(q)
+            for h in range(d.heads):
+                g = h // shared
+                scores = q[h] @ keys[g].T / math.sqrt(d.dim)
+                scores[np.arange(old + n)[None] > old + np.arange(n)[:, None]] = -np.inf
+                self.largest = max(self.largest, np.abs(scores[np.isfinite(scores)]).max())
+                if i == 0:
+                    self.reach = max(self.reach, np.linalg.norm(q[h], axis=1).max() * np.linalg.norm(keys[g], axis=1).max() / math.sqrt(d.dim))
+                p = np.exp(scores - scores.max(1, keepdims=True))
+                p /= p.sum(1, keepdims=True)
+                mixed[h] = p @ values[g]
+                weights[g] += p[-last:].sum(0)
+            self.held[s][i] = keys, values, weights
+            x = x + w[3] @ mixed.transpose(0, 2, 1).reshape(-1, n)
+        return x
+
+    def fork(self, parents, children):
+        self.held.update({c: list(h) for c, h in [(c, self.held[p]) for p, c in zip(parents, children)]})
+
+    def evict(self, parents, children, keep, first, last, kept):
+        now = {}
+        for e, (p, c) in enumerate(zip(parents, children)):
+            now[c] = []
+            for i, (keys, values, weights) in enumerate(self.held[p]):
+                n = keys.shape[1]
+                at = [list(x[x >= 0]) for x in kept[i, e]]
+                for g in range(self.decoder.kv_heads):
+                    assert len(at[g]) == min(n, keep) and at[g] == sorted(set(at[g])) and (kept[i, e, g, len(at[g]):] == -1).all()
+                    gone, sure = set(range(n)) - set(at[g]), set(range(first)) | set(range(n - last, n))
+                    assert not gone & sure
+                    chosen = [weights[g, j] for j in at[g] if j not in sure]
+                    if i == 0 and gone and chosen:
+                        self.worst = max(self.worst, max(weights[g, j] for j in gone) / min(chosen))
+                now[c].append(tuple(np.stack([x[g][at[g]] for g in range(self.decoder.kv_heads)]) for x in (keys, values, weights)))
+        self.held.update(now)
+
+
+def run_bounded(hidden=1024, heads=8, kv_heads=2, keep=0.1, layers=2, prompts=(70, 33, 90), beams=3, steps=4, page_tokens=16, budget=40, first=2, last=8, decay=0.875, window=16, seed=0):
+    """Serves `prompts` with `beams` beams each that hold `budget` tokens at most; returns the outputs of every step, what the mirror says of them, and both."""
+    rng = np.random.default_rng(seed)
+    n = len(prompts)
+    longest = max(prompts) + 3 * steps
+    decoder = BoundedDecoder(hidden, heads, kv_heads, layers, keep, 2 * n * beams * (-(-longest // page_tokens) + 1), page_tokens, n * beams, longest)
+    mirror, outs = Mirror(decoder), []
+    position = np.zeros(n * beams, int)
+
+    def forward(rows, new, groups=(), last=0):
+        x = [rng.standard_normal((hidden, m)).astype(np.float16) for m in new]
+        at = [np.arange(position[s], position[s] + m) for s, m in zip(rows, new)]
+        got = decoder.forward(torch.from_numpy(np.concatenate(x, 1)).cuda(), rows, new, np.concatenate(at), groups, decay, last)
+        want = np.concatenate([mirror.forward(s, y, p, decay, last) for s, y, p in zip(rows, x, at)], 1)
+        position[rows] += new
+        outs.append((got.cpu().double().numpy(), want))
+
+    def fork(parents, children):
+        decoder.fork(parents, children)
+        mirror.fork(parents, children)
+        position[children] = position[parents]
+
+    def evict(parents, children, keep):
+        mirror.evict(parents, children, keep, first, last, decoder.evict(parents, children, keep, first, last))
+        position[children] = position[parents]
+
+    # (of a prompt its last tokens say what is wanted)
+    begin = [i * beams for i in range(n)]
+    forward(begin, list(prompts), last=window)
+    fork([f for f in begin for _ in range(beams - 1)], [f + b for f in begin for b in range(1, beams)])
+    rows = list(range(n * beams))
+    for step in range(steps):
+        forward(rows, [1] * len(rows), [(beams, p) for p in prompts])
+        if step % 2 == 0:
+            fork([s - s % beams + int(rng.integers(beams)) for s in rows], rows)
+    # every beam keeps tokens of its own choice: nothing is shared from here on
+    evict(rows, rows, budget)
+    for step in range(steps):
+        forward(rows, [1] * len(rows))
+        if step % 2 == 0:
+            evict(rows, rows, budget)
+    # a prompt's first beam goes on in all of them, with half as many tokens
+    evict([s - s % beams for s in rows], rows, max(budget // 2, first + last))
+    for step in range(steps):
+        forward(rows, [1] * len(rows))
+    print("tokens held: %s of %s" % (decoder.lengths.tolist(), position.tolist()), flush=True)
+    return outs, decoder, mirror
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     for name, value in (("hidden", 1024), ("heads", 8), ("kv-heads", 2), ("layers", 2), ("beams", 3), ("steps", 4)):
         ap.add_argument("--" + name, type=int, default=value)
     ap.add_argument("--keep", type=float, default=0.1)
+    ap.add_argument("--budget", type=int, default=0, help="tokens that a sequence holds at most (0: all)")
     a = ap.parse_args()
+    if a.budget:
+        outs, _, _ = run_bounded(a.hidden, a.heads, a.kv_heads, a.keep, a.layers, beams=a.beams, steps=a.steps, budget=a.budget)
+        print("outputs of %d steps: relative difference to 64 bits %.2g" % (len(outs), max(np.linalg.norm(g - w) / np.linalg.norm(w) for g, w in outs)))
+        return
     got, want, _ = run(a.hidden, a.heads, a.kv_heads, a.keep, a.layers, beams=a.beams, steps=a.steps)
     print("last tokens of %d beams: relative difference to 64 bits %.2g" % (got.shape[1], np.linalg.norm(got - want) / np.linalg.norm(want)))
 

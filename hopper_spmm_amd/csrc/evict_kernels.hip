@@ -7,6 +7,9 @@
 // In place - a sequence that is its own child, its pages named by nobody else - no token moves to a higher slot, so a workgroup that has all tokens of a column and
 // loads a set of them before it stores the set in front loses none.  Everything else goes to new pages, by as many workgroups as like.
 // Two launches, as which pages are free has to be known before one is written (page_kernels.hip).
+// Moving is memory's: 1024 of up to 8000 tokens of 12 prompts, 8 layers of 8 heads of 128, bf16, 179 us for 0.8 GB, 4.5 TB/s in rows of 256 bytes that lie apart (a copy: 4.8); four rows a thread on their way
+// (two or eight: slower), stores past the L2.  Choosing is a chain of sums over the workgroup and of counts, 10 us for 700 tokens and 35 there, so each weight stays in a register (16 a thread) for all digits, and tokens follow each other in
+// a thread so that one sum puts them in order.
 #include "pages_common.hpp"
 #include <algorithm>
 
@@ -288,7 +291,7 @@ __global__ __launch_bounds__(kScanThreads, kHeld <= 8u ? 8 : 4) void evict_choos
 
 constexpr uint32_t kMoveThreads = 256u, kMoveAtOnce = 4u;
 
-// Keys or values of a layer, an entry and a head, a share of them: columns (in place) or tokens.
+// Keys or values of a layer, an entry and a head, a share of them: columns (in place) or tokens, as only what a workgroup has all tokens of can be rewritten in place.
 template <class U>
 __device__ void evict_move(const PoolArgs &pa, const EvictArgs &ea, uint32_t row, uint32_t head, uint32_t values, uint32_t share, uint32_t shares)
 {
@@ -386,6 +389,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(const PoolArgs
 hipError_t launch_evict(const PoolArgs &pa, const EvictArgs &ea, hipStream_t s)
 {
     const uint64_t cells = uint64_t(ea.n) * pa.layers * pa.heads;
+    // (two workgroups a compute unit where eight tokens a thread are enough; us, eight / sixteen: 12 prompts of up to 8000 213 / 224, 700 tokens 14.5 / 17.4)
     if (uint64_t(pa.table_pages) * pa.page_tokens.d <= 8u * kScanThreads) evict_choose_kernel<8u><<<dim3(uint32_t(ea.n + cells)), dim3(kScanThreads), 0, s>>>(pa, ea);
     else evict_choose_kernel<16u><<<dim3(uint32_t(ea.n + cells)), dim3(kScanThreads), 0, s>>>(pa, ea);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;

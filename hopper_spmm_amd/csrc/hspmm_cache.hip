@@ -618,7 +618,9 @@ static WeighShape weigh_shape(const hspmm_cache *c, const hspmm_batch *b, const 
     const uint64_t keys = most_keys(c, a->longest), heads = uint64_t(b->sequences) * c->heads;
     const uint64_t tokens = std::min(a->longest_chunk, b->tokens), rows = std::max<uint64_t>((last && last < tokens ? last : tokens) * (a->q_heads / c->heads), 1u);
     auto up = [](uint64_t n, uint64_t to) { return (n + to - 1u) / to; };
+    // (rows in registers / in LDS, us: a token for each of 48 sequences of up to 16000 178 / 234, of 3 of up to 300 6.8 / 7.0)
     sh.few = rows <= 16u;
+    // (up to the rows that the rows kernel has in LDS; us there / by the chunk kernel: 96 rows over 17 of up to 5700 keys 18 / 30, 16384 over 8192 840 / 260)
     sh.chunk = c->dtype != HSPMM_TF32 && rows > 128u;
     if (!sh.chunk) {
         // a wave has a tile of 32 keys or some.  us by 1024 / 2048 / 4096 / 8192 / 16384 workgroups: a token for each of 48 sequences of up to 16000 214 / 195 / 184 / 177 / 182;

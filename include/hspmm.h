@@ -623,7 +623,8 @@ typedef struct hspmm_prefix {
     uint32_t groups, most_tokens, longest;
     const int32_t *firsts, *tokens;
 } hspmm_prefix;
-/* hspmm_cache_attend with the groups' prefixes read once.  No groups: the same call. */
+/* hspmm_cache_attend with the groups' prefixes read once.  No groups: the same call.  workspace: as for attend, of
+ * hspmm_cache_attend_shared_workspace bytes, zero before its first use; one of the largest size serves attend, attend_shared, weigh and evict in turn. */
 int hspmm_cache_attend_shared(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_prefix *prefix, const hspmm_attention *attention,
                               const hspmm_heads *q, const hspmm_heads *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream);
 int hspmm_cache_attend_shared_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_prefix *prefix, const hspmm_attention *attention, uint64_t *bytes);

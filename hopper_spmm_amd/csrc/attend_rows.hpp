@@ -251,7 +251,8 @@ __device__ __forceinline__ void attend_rows(const AttendArgs &aa, char *lds, uin
     constexpr int32_t kKeys = K::kKeys;
     // this part's keys
     const KeyPart keys_here = key_part(aa, t, part);
-    const int32_t parts = Span != kSpanAll ? 1 : keys_here.parts, end = keys_here.end;
+    constexpr bool kJoins = Span == kSpanAll || Span == kSpanBoth;
+    const int32_t parts = kJoins ? keys_here.parts : 1, end = keys_here.end;
     int32_t begin = keys_here.begin;
     if (int32_t(part) >= keys_here.parts) return;
 
@@ -266,7 +267,9 @@ __device__ __forceinline__ void attend_rows(const AttendArgs &aa, char *lds, uin
     typename K::Query Q;
     K::load_query(Q, aa.q.data + (int64_t(row.token) * aa.q.token_stride + int64_t(row.head) * aa.q.head_stride) * K::kElem, i < t.rows, lane, D);
     const float scale = aa.scale * kLog2e;
-    const int32_t *table = aa.pages.table + size_t(t.sequence) * aa.pages.table_pages;
+    const int32_t *table = aa.pages.table + size_t(t.sequence) * aa.pages.table_pages, *const lead = aa.pages.table + size_t(Span == kSpanBoth ? t.leader : t.sequence) * aa.pages.table_pages;
+    // (key by key, as a prefix may end within a group of 16)
+    static_assert(Span != kSpanBoth || !Whole, "");
     const int64_t head_offset = int64_t(head) * aa.pages.head_stride;
     const char *keys = aa.pages.keys, *values = aa.pages.values;
     // keys that every row of the tile sees
@@ -320,7 +323,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs &aa, char *lds, uin
             pl.stored &= in;
         } else {
             const int32_t key = j0 + int32_t(lane) % kKeys;
-            pl.at[0] = key < end ? key_offset(aa.pages, table, head_offset, key) : -1;
+            pl.at[0] = key < end ? key_offset(aa.pages, Span == kSpanBoth && key < t.prefix ? lead : table, head_offset, key) : -1;
             pl.stored = uint32_t(__ballot(pl.at[0] >= 0)) & (~0u >> (32 - kKeys));
         }
     };
@@ -542,7 +545,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs &aa, char *lds, uin
     }
     if (m < t.rows) {
         const RowOf r = row_of_tile<Span>(aa, t, head, m);
-        if constexpr (Span != kSpanAll) {
+        if constexpr (!kJoins) {
             float *const to = span_sums<Span>(aa, r, part);
 #pragma unroll
             for (uint32_t e = 0; e < kEach; e += 4)

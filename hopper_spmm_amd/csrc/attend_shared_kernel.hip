@@ -4,7 +4,7 @@
 // out_r = (sum over parts p of 2^(m_p - m) o_p) / (sum of 2^(m_p - m) l_p), m the largest reference m_p of the row's parts, l_p and o_p their totals and sums of values relative to it.
 // Prefixes are bound by matrix instructions or by the L2, what is behind them by memory, so both run at a time: workgroups of the prefixes come first, as they are the longer ones.
 // A token for each of 64 sequences of up to 1500 keys behind 8000, 32 heads on 8 of 128, bf16: 57.6 us, and 10.7 to add up 17 MB of sums (one behind the other 94; by attention alone, which reads the prefix 64 times, from the L2 as far as it goes, 232);
-// 8 beams over 1000 and up to 200, fp16, 9.8 + 7.0; drafts of up to 12 tokens over 5 prompts of up to 6000, 12 heads on 4 of 64, fp32, 60 + 7.6.
+// drafts of up to 12 tokens over 5 prompts of up to 6000, 12 heads on 4 of 64, fp32, 60 + 7.6.
 #include "attend_rows.hpp"
 #include "attend_chunk.hpp"
 

@@ -386,9 +386,13 @@ static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     SharedShape sh{};
     const uint64_t all = most_keys(c, a->longest), common = std::min<uint64_t>(p->longest ? p->longest : all, all);
     // Where a sequence's own rows fill tiles of the chunk kernel there is nothing to win by others' beside them, and sums need not go through memory.  us, 16 chunks of 50 to 250
-    // tokens, 32 heads on 8, behind 3000 and 6000, bf16: 295 so; 393 by tiles of the prefixes' rows, 58 of them the launch that adds up; 8 beams over 1000 keys, a token each, 17, and 21 as an attention.
+    // tokens, 32 heads on 8, behind 3000 and 6000, bf16: 295 so; 393 by tiles of the prefixes' rows, 58 of them the launch that adds up.
     sh.rest = attend_shape(c, b, a);
-    sh.both = sh.rest.rows_log != kAttendRowsLog && uint64_t(std::min(a->longest_chunk, b->tokens)) * (a->q_heads / c->heads) >= 128u;
+    // The same where all of it is little: a launch less.  us so / by tiles of prefixes and of what is behind them, a token each, 32 heads on 8, fp16, by MB of keys and values that the sequences'
+    // own tiles read: 39 13.8 / 16.1, 72 16.7 / 19.7, 79 16.7 / 18.5, 92 20.4 / 18.0, 138 24.9 / 21.0; 12 heads on 4 of 64, fp32: 46 14.7 / 15.2, 69 19.8 / 21.8, 79 19.5 / 18.8, 144 27.9 / 22.6.
+    const uint64_t rows = uint64_t(std::min(a->longest_chunk, b->tokens)) * (a->q_heads / c->heads), tiles = uint64_t(b->sequences) * ((rows + (1u << sh.rest.rows_log) - 1u) >> sh.rest.rows_log);
+    const bool little = tiles * c->heads * all * c->head_dim * 2u * element_bytes(c->dtype) <= (uint64_t(80) << 20);
+    sh.both = little || (sh.rest.rows_log != kAttendRowsLog && rows >= 128u);
     if (sh.both) {
         sh.bytes = sh.rest.bytes;
         return sh;
@@ -510,7 +514,7 @@ int hspmm_cache_attend(const hspmm_cache *cache, uint32_t layer, const hspmm_bat
     if (int rc = check_workspace(workspace, workspace_bytes, sh.bytes)) return rc;
     if (int rc = check_device()) return rc;
     const AttendArgs aa = attend_args(cache, layer, batch, attention, q, out, lse, sh, workspace);
-    if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, sh.past, static_cast<hipStream_t>(stream)));
+    if (sh.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, aa, sh.past, false, static_cast<hipStream_t>(stream)));
     else HSPMM_HIP(launch_attend_chunk(cache->dtype, aa, false, sh.rows_log, static_cast<hipStream_t>(stream)));
     return HSPMM_OK;
 }
@@ -544,7 +548,8 @@ int hspmm_cache_attend_shared(const hspmm_cache *cache, uint32_t layer, const hs
     of_prefix.prefix = of_rest.prefix = PrefixArgs{prefix->firsts, prefix->tokens, prefix->groups, sh.prefix.splits, sh.prefix.part_keys, of_rest.sums,
                                                    int64_t(batch->tokens) * attention->q_heads * (cache->head_dim + kPrefixExtra)};
     if (sh.both) {
-        HSPMM_HIP(launch_attend_chunk(cache->dtype, of_rest, true, sh.rest.rows_log, static_cast<hipStream_t>(stream)));
+        if (sh.rest.rows_log == kAttendRowsLog) HSPMM_HIP(launch_attend_rows(cache->dtype, of_rest, false, true, static_cast<hipStream_t>(stream)));
+        else HSPMM_HIP(launch_attend_chunk(cache->dtype, of_rest, true, sh.rest.rows_log, static_cast<hipStream_t>(stream)));
         return HSPMM_OK;
     }
     HSPMM_HIP(launch_attend_shared(cache->dtype, of_prefix, of_rest, sh.prefix.rows_log != kAttendRowsLog, sh.rest.rows_log != kAttendRowsLog, static_cast<hipStream_t>(stream)));

@@ -325,3 +325,29 @@ def test_one_workspace_serves_every_call_in_turn(torch_cuda, hs):
         # (as many tokens as it has: nothing happens but the choice)
         st.handle.evict(1, one.data_ptr(), 0, into, 1500, workspace=w.data_ptr(), workspace_bytes=need, stream=stream)
         assert not w[: 4 * 16384].any()
+
+
+def widened(torch, hs, c, keys):
+    """The same cache with rows of the table that have places for so many keys: what the call is told to expect."""
+    st = c.st
+    table = torch.full((st.table.shape[0], max(-(-keys // st.page_tokens), st.table.shape[1])), -1, dtype=torch.int32, device="cuda")
+    table[:, : st.table.shape[1]] = st.table
+    st.wide = table
+    st.handle = hs.Cache(st.dtype, st.layers, st.pages, st.page_tokens, st.heads, st.head_dim, table.shape[0], table.shape[1], st.pool[0].data_ptr(), st.pool[1].data_ptr(),
+                         table.data_ptr(), st.lengths.data_ptr(), st.references.data_ptr(), st.scratch.data_ptr(), order=st.order)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("number", range(len(CASES)))
+def test_small_calls_that_expect_long_sequences(torch_cuda, hs, dtype, number):
+    # (by tiles of the prefixes' rows and of what is behind them, which else only large calls are)
+    torch = torch_cuda
+    c = Case(torch, hs, dtype, number, order=number % 2, seed=1)
+    size = 4 if dtype == 1 else 2
+    widened(torch, hs, c, -(-(1 << 27) // (c.n * c.st.heads * c.dim * 2 * size)))
+    want = c.want()
+    keys = c.st.wide.shape[1] * c.st.page_tokens
+    for chunk, longest in ((int(c.new.max()), keys), (1, 0), (5000, keys)):
+        for prefix in (c.hint, dict(most_tokens=0, longest=0), dict(most_tokens=1, longest=1)):
+            out, lse = c.run(torch, hs, c.hints(hs, chunk, longest), c.prefixes(hs, **prefix), layout="gaps" if chunk == 1 else "tokens")
+            assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)

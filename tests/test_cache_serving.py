@@ -40,10 +40,13 @@ def test_attend_shared_refuses(hs):
         refused(hs, 5, lambda: shared(hs, q=q), "q")
     refused(hs, 1, lambda: shared(hs, out=hs.Heads(ADDRESS, 1, 256, 0)), "out")
     refused(hs, 1, lambda: shared(hs, lse=ADDRESS + 2), "lse")
-    need = c.attend_shared_workspace(b, hs.Prefix(1, ADDRESS, ADDRESS), a)
+    # (a small call joins nothing; one that expects long sequences leaves sums)
+    assert c.attend_shared_workspace(b, hs.Prefix(1, ADDRESS, ADDRESS), a) == 0
+    far = cache(hs, table_pages=1 << 13)
+    need = far.attend_shared_workspace(b, hs.Prefix(1, ADDRESS, ADDRESS), a)
     assert need >= 4 * 8 * 68 * 4
     for w in ((0, need), (ADDRESS, need - 1), (ADDRESS + 8, need)):
-        refused(hs, 1, lambda: shared(hs, workspace=w[0], workspace_bytes=w[1]), "workspace")
+        refused(hs, 1, lambda: shared(hs, c=far, workspace=w[0], workspace_bytes=w[1]), "workspace")
     refused(hs, 5, lambda: shared(hs, c=cache(hs, head_dim=60)), "elements")
     wide = hs.Batch(3, 1 << 29, ADDRESS)
     refused(hs, 5, lambda: shared(hs, batch=wide, attention=hs.Attention(4, 1.0, longest_chunk=1 << 29)), "several calls")

@@ -75,7 +75,7 @@ __device__ __forceinline__ void store_words(void *p, const uint32_t (&src)[V])
 __device__ __forceinline__ uint32_t pack_half2_rn(float lo, float hi)
 {
     // float -> half conversion in the default rounding mode (nearest even), as the
-    // reference's store does (src/fp16.cu:167, cvt.rn.f16.f32).
+    // reference's store does (src/fp16.cu:167, an implicit conversion to half).
     _Float16 l = (_Float16)lo, h = (_Float16)hi;
     uint16_t lb = __builtin_bit_cast(uint16_t, l), hb = __builtin_bit_cast(uint16_t, h);
     return uint32_t(lb) | (uint32_t(hb) << 16);

@@ -62,7 +62,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void weigh_chunk_kerne
         // Rows, 32 a wave, 128 on in the next turn: where those lie follows without a division or a product (`step_heads` heads on, and some tokens), a lane finds out for row j.
         // They are loaded with a row's pieces side by side, of eight elements each, and go through the wave's own LDS to be a product's operand: loaded as that, sixteen bytes of a row
         // a lane, a turn's loads were two thirds of what a compute unit's cache can look up, 277 us of which 70 went for them (4096 tokens over 8192 keys).
-        // Of rows behind the last one the first of the tensor is read, and not used; behind a row's last element its first ones, which meet zeros of the keys.
+        // Of rows behind the last one the first of the tensor is read, and not used; behind a row's last element there are zeros, as those of the keys do not undo an infinity.
         uint32_t at_row = first_row + wave * 32u + j, at_head;
         int64_t at_q, at_lse, lse_at;
         {
@@ -76,6 +76,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void weigh_chunk_kerne
         float lse_ahead;
         auto piece_of = [&](uint32_t i) __attribute__((always_inline)) { return (lane + 64u * i) / kRowPieces; };
         auto column_of = [&](uint32_t i) __attribute__((always_inline)) { return (lane + 64u * i) % kRowPieces * 8u; };
+        // (what is read for an element behind the last one goes where nobody looks, past the row: in its own place are the zeros that are put there now)
+        auto put_column = [&](uint32_t i) __attribute__((always_inline)) { return column_of(i) < D ? column_of(i) : uint32_t(DP); };
+        if (D < uint32_t(DP)) {
+#pragma unroll 1
+            for (uint32_t i = 0; i < kRowsPieces; ++i)
+                if (column_of(i) >= D) *reinterpret_cast<u32x4 *>(rows_of[wave] + piece_of(i) * kPitch + column_of(i) * 2u) = u32x4{0u, 0u, 0u, 0u};
+        }
         auto find = [&]() __attribute__((always_inline)) {
             const bool there = at_row < w.rows;
             rows_at[wave][j] = there ? at_q : 0;
@@ -99,7 +106,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void weigh_chunk_kerne
         };
         auto put = [&]() __attribute__((always_inline)) {
 #pragma unroll
-            for (uint32_t i = 0; i < kRowsPieces; ++i) *reinterpret_cast<u32x4 *>(rows_of[wave] + piece_of(i) * kPitch + column_of(i) * 2u) = rows_piece[i];
+            for (uint32_t i = 0; i < kRowsPieces; ++i) *reinterpret_cast<u32x4 *>(rows_of[wave] + piece_of(i) * kPitch + put_column(i) * 2u) = rows_piece[i];
             // (a wave's LDS accesses are done in the order they are issued in)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
             __builtin_amdgcn_wave_barrier();

@@ -152,12 +152,12 @@ __global__ __launch_bounds__(64 * kWeighWaves) void weigh_rows_kernel(const Weig
             by = moved_by(wa.lse[size_t(row.token) * wa.q_heads + row.head]);
         } else {
             __syncthreads();
-            // (of rows behind the last one the first is read, and not used; behind a row's last element its first ones, which meet zeros of the keys)
+            // (of rows behind the last one the first is read, and not used; behind a row's last element there are zeros: those of the keys do not undo an infinity)
             for (uint32_t p = tid; p < ((end - base + 15u) & ~15u) * kRowPieces; p += 64u * kWeighWaves) {
                 const uint32_t m = p / kRowPieces, c = p % kRowPieces * K::kPiece;
                 const RowOf r = weigh_row(wa, w, head, base + m);
-                *reinterpret_cast<u32x4 *>(rows_of + m * kPitch + c * K::kElem) = *reinterpret_cast<const u32x4 *>(
-                    wa.q.data + (int64_t(r.token) * wa.q.token_stride + int64_t(r.head) * wa.q.head_stride + (c < D ? c : 0u)) * K::kElem);
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(wa.q.data + (int64_t(r.token) * wa.q.token_stride + int64_t(r.head) * wa.q.head_stride + (c < D ? c : 0u)) * K::kElem);
+                *reinterpret_cast<u32x4 *>(rows_of + m * kPitch + c * K::kElem) = x & (c < D ? ~0u : 0u);
             }
             if (tid < kBatch) {
                 const RowOf r = weigh_row(wa, w, head, base + tid);

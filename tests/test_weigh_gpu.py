@@ -278,3 +278,28 @@ def test_rows_whose_lse_is_infinite_give_nothing(torch_cuda, hs, dtype, number):
     c.lse.view(-1)[::3] = 1e30
     c.weights.copy_(torch_cuda.from_numpy(c.before))
     assert np.array_equal(c.run(hs, decay=0.5, attention=a), got)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("number", [3, 4, 6, 8, 9, 11, 13, 16, 24])
+def test_rows_whose_scores_are_all_minus_infinity_give_nothing(torch_cuda, hs, dtype, number):
+    # an infinite element of a query: whatever a kernel has behind a head's last element, that row gives nothing
+    torch = torch_cuda
+    c = Case(torch, hs, dtype, number, seed=6)
+    for b, row in enumerate(c.rows):
+        c.k[b][..., 0] = np.abs(c.k[b][..., 0]) + 0.5
+        c.st.store(c.layer, int(row), 0, c.k[b])
+    rows = c.q.reshape(-1, c.q.shape[2])
+    rows[::3, 0] = -math.inf
+    _, c.lse = attend(torch, hs, c.st, c.batch, c.attention, c.q, layer=c.layer)
+    assert torch.isneginf(c.lse.view(-1)[::3]).all()
+    got = []
+    for a in [None] + hints(hs, c):
+        c.weights.copy_(torch.from_numpy(c.before))
+        got.append(c.run(hs, decay=0.5, attention=a))
+        assert np.isfinite(got[-1]).all()
+    # to the bit what the others give where those rows are zeros
+    rows[::3] = 0.0
+    for a, x in zip([None] + hints(hs, c), got):
+        c.weights.copy_(torch.from_numpy(c.before))
+        assert np.array_equal(c.run(hs, decay=0.5, attention=a), x)

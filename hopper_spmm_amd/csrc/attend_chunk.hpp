@@ -25,12 +25,14 @@ __device__ __forceinline__ void lds_barrier()
 // TFLOP/s.  A wave has 32 rows, two waves a SIMD: one multiplies while the other one takes exponentials.
 // The scores of a half are made among the exponentials of the half in front.  Images go through LDS, kRing of them in turn: while image n is
 // multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image (with two places: two).
-// lds: chunk_lds(DP, W) bytes; number: of the workgroup among so many `numbers`; part: of its keys.
+// Lds<N>: chunk_lds(DP, W) bytes or more; number: of the workgroup among so many `numbers`; part: of its keys.
+// What one kind of call has alone stands behind `if constexpr`, and LDS is named, not pointed to: registers are short with heads of 256 elements.  1024 tokens over 2048 older keys, 16 heads on 4
+// of 256, bf16, pages of 24 tokens, 158 us with conditions that are never true and a pointer, 147 so; pages of 16 149 and 151 (without prefixes in the body at all 137 and 155).
 constexpr uint32_t chunk_image(int DP) { return 64u * (uint32_t(DP) * 2u + 16u + uint32_t(DP) * 2u + (DP % 128 == 0 || DP == 64 ? 64u : 0u)); }
 constexpr uint32_t chunk_ring(int DP, int W) { return 3u * chunk_image(DP) <= (DP <= 128 && W == 4 ? 80u : 160u) * 1024u - 256u ? 3u : 2u; }
-constexpr uint32_t chunk_lds(int DP, int W) { return chunk_ring(DP, W) * chunk_image(DP) + 16u + uint32_t(W) * 12u; }
-template <bool BF, int DP, int W, bool Whole, AttendSpan Span>
-__device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, uint32_t number, uint32_t numbers, uint32_t part)
+constexpr uint32_t chunk_lds(int DP, int W) { return chunk_ring(DP, W) * chunk_image(DP) + (uint32_t(W) * 12u + 15u) / 16u * 16u; }
+template <bool BF, int DP, int W, bool Whole, AttendSpan Span, uint32_t N>
+__device__ __forceinline__ void attend_chunk(const AttendArgs &aa, uint32_t number, uint32_t numbers, uint32_t part)
 {
     typedef typename HalfOps<BF>::elem_t T;
     constexpr uint32_t kThreads = 64u * W, kRows = 32u * W, kKeys = 64u;
@@ -39,11 +41,10 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
     constexpr uint32_t kKeyPitch = DP * 2u + 16u, kValuePitch = DP * 2u + (DP % 128 == 0 || DP == 64 ? 64u : 0u), kImage = kKeys * (kKeyPitch + kValuePitch);
     static_assert(kKeyPitch / 16u % 2u == 1u && kValuePitch / 64u % 2u == 1u && kValuePitch % 64u == 0u, "");
     constexpr uint32_t kRing = chunk_ring(DP, W);
-    static_assert(kImage == chunk_image(DP), "");
+    static_assert(kImage == chunk_image(DP) && N >= chunk_lds(DP, W), "");
     constexpr uint32_t kRowPieces = DP / 8u, kImagePieces = kKeys * kRowPieces;
     constexpr int kSteps = DP / 16, kTiles = DP / 32, kPieces = int((kImagePieces + kThreads - 1u) / kThreads);
-    char *const images = lds;
-    uint32_t &odd = *reinterpret_cast<uint32_t *>(lds + kRing * kImage), &arrived = (&odd)[1];
+    __shared__ uint32_t odd, arrived;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, j = lane & 31u;
     // (the last tiles first: where a token sees what is in front of it they are the longest)
     const uint32_t D = aa.pages.head_dim;
@@ -93,7 +94,7 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
     int32_t group_lo, group_hi;
     if constexpr (Span == kSpanPrefix) {
         // (rows of several sequences)
-        int32_t (*const ranges)[3] = reinterpret_cast<int32_t (*)[3]>(lds + kRing * kImage + 16u);
+        int32_t (*const ranges)[3] = reinterpret_cast<int32_t (*)[3]>(Lds<N>::bytes + kRing * kImage);
         if (lane == 0u) { ranges[wave][0] = all_lo; ranges[wave][1] = all_hi; ranges[wave][2] = any_lo; }
         __syncthreads();
         group_lo = all_lo; group_hi = all_hi;
@@ -107,22 +108,41 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
         any_lo = __builtin_amdgcn_readfirstlane(any_lo);
     } else {
         const int32_t p0 = t.position + int32_t(aa.shared.quotient(t.first_row)), p1 = t.position + int32_t(aa.shared.quotient(t.first_row + t.rows - 1u));
-        group_hi = aa.causal ? p0 + 1 : t.length;
-        group_lo = aa.window && int64_t(p1) + 1 > int64_t(aa.window) ? p1 + 1 - int32_t(aa.window) : 0;
+        group_hi = __builtin_amdgcn_readfirstlane(aa.causal ? p0 + 1 : t.length);
+        group_lo = __builtin_amdgcn_readfirstlane(aa.window && int64_t(p1) + 1 > int64_t(aa.window) ? p1 + 1 - int32_t(aa.window) : 0);
         if constexpr (Span == kSpanRest) group_lo = max(group_lo, t.prefix);
     }
     // (rows of several sequences: from the first key that any of them sees)
     const int32_t begin = Span == kSpanPrefix ? max(keys_here.begin, min(any_lo & ~31, end)) : keys_here.begin;
     // Images of 64 keys: of the prefix (kSpanBoth), by its first sequence's pages, then of what is behind it, from where a group of 16 begins.
-    int32_t first_images = 0, behind = begin;
-    if (Span == kSpanBoth && begin < t.prefix) {
-        first_images = (min(end, t.prefix) - begin + 63) / 64;
-        behind = t.prefix & ~15;
+    int32_t first_images = 0, behind = begin, n_images = end > begin ? (end - begin + 63) / 64 : 0;
+    if constexpr (Span == kSpanBoth) {
+        if (begin < t.prefix) {
+            first_images = (min(end, t.prefix) - begin + 63) / 64;
+            behind = t.prefix & ~15;
+            n_images = first_images + (end > t.prefix ? (end - behind + 63) / 64 : 0);
+        }
     }
-    const int32_t n_images = first_images + (end > (Span == kSpanBoth ? max(begin, t.prefix) : begin) ? (end - behind + 63) / 64 : 0);
-    auto key_of = [&](int32_t n) __attribute__((always_inline)) { return Span == kSpanBoth && n < first_images ? begin + n * 64 : behind + (n - first_images) * 64; };
-    auto end_of = [&](int32_t n) __attribute__((always_inline)) { return Span == kSpanBoth && n < first_images ? min(end, t.prefix) : end; };
     const int32_t *table = aa.pages.table + size_t(t.sequence) * aa.pages.table_pages, *const lead = aa.pages.table + size_t(Span == kSpanBoth ? t.leader : t.sequence) * aa.pages.table_pages;
+    // The first key of image n, what its keys end in front of, whose row of the table has them, and those of its 64 places that are its.
+    auto key_of = [&](int32_t n) __attribute__((always_inline)) {
+        if constexpr (Span == kSpanBoth) return n < first_images ? begin + n * 64 : behind + (n - first_images) * 64;
+        else return begin + n * 64;
+    };
+    auto end_of = [&](int32_t n) __attribute__((always_inline)) {
+        if constexpr (Span == kSpanBoth) return n < first_images ? min(end, t.prefix) : end;
+        else return end;
+    };
+    auto table_of = [&](int32_t n) __attribute__((always_inline)) {
+        if constexpr (Span == kSpanBoth) return n < first_images ? lead : table;
+        else return table;
+    };
+    auto places_of = [&](int32_t n) __attribute__((always_inline)) {
+        const int32_t left = end_of(n) - key_of(n);
+        const uint64_t in = left >= 64 ? ~uint64_t(0) : left > 0 ? (uint64_t(1) << left) - 1u : 0u;
+        if constexpr (Span == kSpanBoth) return n == first_images && behind < t.prefix ? in & ~uint64_t(0) << (t.prefix - behind) : in;
+        else return in;
+    };
     const int64_t head_offset = int64_t(head) * aa.pages.head_stride;
     // Where keys lie, in bytes from keys and values: of groups of 16 keys, four an image, of 16 images at a time, a lane each (Whole), or of
     // the keys of an image; and which of them are stored, a bit each.
@@ -130,7 +150,7 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
     uint64_t ahead_there = 0u;
     auto look_up = [&](int32_t n, int32_t in_image) __attribute__((always_inline)) {
         const int32_t key = key_of(n) + in_image;
-        const int64_t at = key < end_of(n) ? key_offset(aa.pages, Span == kSpanBoth && n < first_images ? lead : table, head_offset, key) : -1;
+        const int64_t at = key < end_of(n) ? key_offset(aa.pages, table_of(n), head_offset, key) : -1;
         ahead_there = __ballot(at >= 0);
         const uint64_t bytes = at >= 0 ? uint64_t(at) * 2u : 0u;
         ahead_low = uint32_t(bytes);
@@ -183,9 +203,7 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
     };
     // the stored keys of image n, which is in the registers
     auto stored_keys = [&](int32_t n) __attribute__((always_inline)) {
-        const int32_t left = end_of(n) - key_of(n);
-        uint64_t in = left >= 64 ? ~uint64_t(0) : left > 0 ? (uint64_t(1) << left) - 1u : 0u;
-        if (Span == kSpanBoth && n == first_images && behind < t.prefix) in &= ~uint64_t(0) << (t.prefix - behind);
+        const uint64_t in = places_of(n);
         if constexpr (!Whole) return keys_there & in;
         if (groups_there == 15u) return in;
         uint64_t there = 0u;
@@ -195,7 +213,7 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
         return there & in;
     };
     auto write_image = [&](int32_t n, uint32_t to) __attribute__((always_inline)) {
-        char *const image = images + to * kImage;
+        char *const image = Lds<N>::bytes + to * kImage;
         const uint64_t stored_there = stored_keys(n);
         if (~stored_there || D < uint32_t(DP)) {
             // (what is not stored may be anything, and no weight of zero undoes a NaN)
@@ -236,7 +254,7 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
     // The first operands of half of the scores' instructions, asked for well ahead of them.
     struct KeyOperands { u32x4 a[kSteps / 2]; };
     auto ask_keys = [&](KeyOperands &f, auto second, uint32_t image, uint32_t half) __attribute__((always_inline)) {
-        const char *const from = images + image * kImage + half * 32u * kKeyPitch + key_lane + decltype(second)::value * (kSteps / 2) * 32;
+        const char *const from = Lds<N>::bytes + image * kImage + half * 32u * kKeyPitch + key_lane + decltype(second)::value * (kSteps / 2) * 32;
 #pragma unroll
         for (int c = 0; c < kSteps / 2; ++c) f.a[c] = *reinterpret_cast<const u32x4 *>(from + c * 32);
     };
@@ -288,7 +306,7 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
     struct ValueOperands { u32x4 a[kTiles]; };
     auto ask_values = [&](ValueOperands &f, auto second, uint32_t image, uint32_t half) __attribute__((always_inline)) {
         constexpr int c = decltype(second)::value;
-        const __attribute__((address_space(3))) char *const from = (const __attribute__((address_space(3))) char *)(images + image * kImage + half * 32u * kValuePitch + value_lane);
+        const __attribute__((address_space(3))) char *const from = (const __attribute__((address_space(3))) char *)(Lds<N>::bytes + image * kImage + half * 32u * kValuePitch + value_lane);
 #pragma unroll
         for (int e = 0; e < kTiles; ++e) {
             const t_u32x2 a0 = __builtin_bit_cast(t_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tile_tr_ptr)(from + (16 * c) * kValuePitch + e * 64)));
@@ -363,7 +381,7 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
             // An infinity or a NaN that some rows do not see, which a matrix instruction would multiply by their zeros: once more, the values key by
             // key and by the rows that see it.  Slow, and off the path of finite data.
             begin_sums();
-            float *const weights = reinterpret_cast<float *>(images + kImage) + wave * 32u * 32u;
+            float *const weights = reinterpret_cast<float *>(Lds<N>::bytes + kImage) + wave * 32u * 32u;
             static_assert(W * 32u * 32u * 4u <= (kRing - 1u) * kImage, "weights in the place of the other images");
 #pragma unroll 1
             for (int32_t n = 0; n < n_images; ++n) {
@@ -390,7 +408,7 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, char *lds, ui
                     for (uint32_t a = 0; a < 32u; ++a) {
                         const int32_t key = key0 + int32_t(a);
                         const float w = weights[a * 32u + j];
-                        const T *from = reinterpret_cast<const T *>(images + kKeys * kKeyPitch + (32u * half + a) * kValuePitch) + 4u * h;
+                        const T *from = reinterpret_cast<const T *>(Lds<N>::bytes + kKeys * kKeyPitch + (32u * half + a) * kValuePitch) + 4u * h;
                         const bool hidden = int(key < row.lo) | int(key >= row.hi);
 #pragma unroll
                         for (int c = 0; c < kTiles; ++c)

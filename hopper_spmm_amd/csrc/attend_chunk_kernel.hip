@@ -8,8 +8,7 @@ namespace {
 template <bool BF, int DP, int W, bool Whole, AttendSpan Span>
 __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend_chunk_kernel(const AttendArgs aa)
 {
-    __shared__ __attribute__((aligned(16))) char lds[chunk_lds(DP, W)];
-    attend_chunk<BF, DP, W, Whole, Span>(aa, lds, blockIdx.x, gridDim.x, blockIdx.y);
+    attend_chunk<BF, DP, W, Whole, Span, chunk_lds(DP, W)>(aa, blockIdx.x, gridDim.x, blockIdx.y);
 }
 
 template <bool BF, int DP, int W, AttendSpan Span>

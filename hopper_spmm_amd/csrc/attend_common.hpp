@@ -20,6 +20,10 @@ constexpr float kReferenceSlack = 8.f;
 // a smaller one is off (from 1 on these would be 2^-14 and 2^-25, and 20000 keys of 2^-26 each had counted in the total and not in the sums).  bf16 has fp32's range.
 template <class T> constexpr float kReferenceLead = sizeof(T) == 2 && !__is_same(T, __bf16) ? 7.f : 0.f;
 
+// A workgroup's LDS for the parts of a kernel that run one instead of the other.
+template <uint32_t N> struct Lds { static __shared__ __attribute__((aligned(16))) char bytes[N]; };
+template <uint32_t N> __shared__ __attribute__((aligned(16))) char Lds<N>::bytes[N];
+
 struct RowTile {
     uint32_t sequence, first_row, rows, first_token, chunk;      // first_token of the batch; rows from first_row on
     int32_t length, position;                                    // tokens the cache holds; the position of the chunk's first token

@@ -18,16 +18,16 @@ constexpr uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
 template <class K, bool BF, int DR, int DC, bool Whole, bool PrefixChunk, bool RestChunk>
 __global__ __launch_bounds__(256, DC <= 64 && !PrefixChunk && !RestChunk ? 3 : DC <= 128 ? 2 : 1) void attend_shared_kernel(const AttendArgs prefix, const AttendArgs rest)
 {
-    __shared__ __attribute__((aligned(16))) char lds[larger(PrefixChunk || RestChunk ? chunk_lds(DC, 4) : 0u, rows_lds(DR))];
+    constexpr uint32_t kLds = larger(PrefixChunk || RestChunk ? chunk_lds(DC, 4) : 0u, rows_lds(DR));
     const uint32_t of_prefix = prefix.tiles * prefix.heads.d, of_rest = rest.tiles * rest.heads.d, n_prefix = of_prefix * prefix.splits;
     if (blockIdx.x < n_prefix) {
         const uint32_t part = blockIdx.x / of_prefix, number = blockIdx.x - part * of_prefix;
-        if constexpr (PrefixChunk) attend_chunk<BF, DC, 4, Whole, kSpanPrefix>(prefix, lds, number, of_prefix, part);
-        else attend_rows<K, Whole, DR, kSpanPrefix>(prefix, lds, number, part);
+        if constexpr (PrefixChunk) attend_chunk<BF, DC, 4, Whole, kSpanPrefix, kLds>(prefix, number, of_prefix, part);
+        else attend_rows<K, Whole, DR, kSpanPrefix>(prefix, Lds<kLds>::bytes, number, part);
     } else {
         const uint32_t part = (blockIdx.x - n_prefix) / of_rest, number = blockIdx.x - n_prefix - part * of_rest;
-        if constexpr (RestChunk) attend_chunk<BF, DC, 4, Whole, kSpanRest>(rest, lds, number, of_rest, part);
-        else attend_rows<K, Whole, DR, kSpanRest>(rest, lds, number, part);
+        if constexpr (RestChunk) attend_chunk<BF, DC, 4, Whole, kSpanRest, kLds>(rest, number, of_rest, part);
+        else attend_rows<K, Whole, DR, kSpanRest>(rest, Lds<kLds>::bytes, number, part);
     }
 }
 

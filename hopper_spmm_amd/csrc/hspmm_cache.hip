@@ -406,7 +406,7 @@ static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     const uint32_t shared = a->q_heads / c->heads;
     auto tiles_of = [&](AttendShape &x, uint32_t sequences, uint32_t log) { x.rows_log = log; x.tiles = uint32_t(attend_tiles(b->tokens, sequences, shared, log)); };
     auto parts_of = [](AttendShape &x, uint64_t keys, uint64_t part) {
-        x.part_keys = uint32_t(std::max<uint64_t>((part + 127u) & ~uint64_t(127u), 128u));
+        x.part_keys = uint32_t(std::min<uint64_t>(std::max<uint64_t>((part + 127u) & ~uint64_t(127u), 128u), 1u << 30));
         x.splits = uint32_t(std::min<uint64_t>(std::max<uint64_t>((keys + 31u + x.part_keys - 1u) / x.part_keys, 1u), 256u));
     };
     tiles_of(sh.prefix, p->groups, std::min(sh.prefix.rows_log, 7u));
@@ -415,10 +415,17 @@ static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     // Parts cost a row's sums each, written and read, but nobody waits for them.  us by keys of a prefix's part / of what is behind one's: 8 beams over 1000 keys by 128 / 256 / 512 / 1024 17.8 /
     // 15.6 / 16.1 / 19.9; 64 sequences of up to 1500 behind 8000 by 256 / 512 / 768 / 1024 / 1536 102 / 79 / 72 / 67 / 75, and with 1024 there by 256 / 512 / 1024 / 1536 75 / 69 / 67 / 70; fp32 drafts over
     // up to 6000 81 / 67 / - / 60 / 70 and 60 / 60 / 64 / -.
+    // Longer ones where tiles alone are workgroups for the chip - one and a half times those of the chunk kernel that run at a time, four times those of the rows kernel -, as sums are what parts cost
+    // then.  us (MB of workspace) by 1024 keys / 1024 / 768 / 512 workgroups of the chunk kernel, 32 heads on 8 of 128, bf16: 64 x 16 tokens behind 8000 243 (156) / 204 (87) / 193 (69) / 189 (52);
+    // 256 x 8 538 (311) / 411 (104) / 414 (104) / 397 (69); 32 x 100 715 (487) / 545 (162) / 594 (108) / 593 (108); 63 tokens and a chunk of 1000 289 (180) / 250 (108) / 225 (72) / 253 (54); 128 x 16 behind
+    // 32000 1696 (1142) / 1202 (138) / 1198 (104) / 1200 (104); 256 x 1 behind 128000 902 (549) / 668 (74) / 672 (56) / 670 (43).  By 1024 keys / 2048 workgroups of the rows kernel, fp32: 16 x 60 behind
+    // 4000 782 / 739, 16 x 64, 12 heads on 4 of 64, 185 / 181.
     auto spread = [&](const AttendShape &x, uint32_t sequences, uint64_t keys) {
         const uint64_t most = uint64_t(sequences) * ((uint64_t(std::min(&x == &sh.prefix ? (p->most_tokens ? p->most_tokens : b->tokens) : a->longest_chunk, b->tokens)) * shared + (1u << x.rows_log) - 1u) >> x.rows_log);
-        const uint64_t cells = std::max<uint64_t>(std::min<uint64_t>(most, x.tiles) * c->heads, 1u);
-        return std::min<uint64_t>(std::max<uint64_t>(cells * keys / 128u, 256u), 1024u);
+        // (whatever the call says, there are no fewer tiles than its rows fill)
+        const uint64_t tiles = std::max<uint64_t>(std::min<uint64_t>(most, x.tiles), uint64_t(b->tokens) * shared >> x.rows_log);
+        const uint64_t cells = std::max<uint64_t>(tiles, 1u) * c->heads, at_a_time = x.rows_log == kAttendRowsLog ? 2048u : 768u;
+        return std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(cells * keys / 128u, 256u), 1024u), cells * keys / at_a_time);
     };
     parts_of(sh.prefix, common, spread(sh.prefix, p->groups, common));
     parts_of(sh.rest, behind, spread(sh.rest, b->sequences, behind));

@@ -133,6 +133,8 @@ void launch16(const AttendArgs &prefix, const AttendArgs &rest, bool prefix_chun
     if (D <= 64u) launch<Rows16<BF, 64, false>, BF, 64, 64>(prefix, rest, prefix_chunk, rest_chunk, s);
     else if (D <= 96u && prefix_chunk) launch<Rows16<BF, 128, false>, BF, 128, 96>(prefix, rest, prefix_chunk, rest_chunk, s);
     else if (D <= 128u) launch<Rows16<BF, 128, false>, BF, 128, 128>(prefix, rest, prefix_chunk, rest_chunk, s);
+    // (160 / 256 elements, heads of 160, 16 heads on 4, us: 16 x 40 tokens behind 6000 122 / 270, 16 x 100 224 / 603)
+    else if (D <= 160u && prefix_chunk) launch<Rows16<BF, 256, false>, BF, 256, 160>(prefix, rest, prefix_chunk, rest_chunk, s);
     else launch<Rows16<BF, 256, false>, BF, 256, 256>(prefix, rest, prefix_chunk, rest_chunk, s);
 }
 

@@ -351,3 +351,28 @@ def test_small_calls_that_expect_long_sequences(torch_cuda, hs, dtype, number):
         for prefix in (c.hint, dict(most_tokens=0, longest=0), dict(most_tokens=1, longest=1)):
             out, lse = c.run(torch, hs, c.hints(hs, chunk, longest), c.prefixes(hs, **prefix), layout="gaps" if chunk == 1 else "tokens")
             assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)
+
+
+# heads of 129 to 160 elements: chunks of fewer rows than a tile has, of sequences that are said to be long
+MIDDLE = [([24], [700], [40, 300], [30, 9], 1, 2, 4, 160, 16, 0, True), ([11, 9], [500, 333], [77, 0, 200], [25], 0, 2, 4, 136, 24, 400, True), ([20], [650], [90, 8], [30], 0, 2, 4, 152, 32, 0, False)]
+
+
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("number", range(len(MIDDLE)))
+def test_heads_between_128_and_160(torch_cuda, hs, dtype, number):
+    torch = torch_cuda
+    CASES.append(MIDDLE[number])
+    try:
+        c = Case(torch, hs, dtype, len(CASES) - 1, order=number % 2)
+    finally:
+        CASES.pop()
+    widened(torch, hs, c, 16000)
+    keys = c.st.wide.shape[1] * c.st.page_tokens
+    attention, want = c.hints(hs, int(c.new.max()), keys), c.want()
+    # (by tiles of the prefixes' rows: sums of whole rows are left)
+    part = c.q.shape[0] * c.q.shape[1] * (c.dim + 4) * 4
+    need = c.st.handle.attend_shared_workspace(c.batch, c.prefixes(hs), attention)
+    assert need > 4 * 16384 and (need - 4 * 16384) % part == 0
+    for layout in ("tokens", "features"):
+        out, lse = c.run(torch, hs, attention, layout=layout)
+        assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)

@@ -385,14 +385,19 @@ static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, cons
 {
     SharedShape sh{};
     const uint64_t all = most_keys(c, a->longest), common = std::min<uint64_t>(p->longest ? p->longest : all, all);
-    // Where a sequence's own rows fill tiles of the chunk kernel there is nothing to win by others' beside them, and sums need not go through memory.  us, 16 chunks of 50 to 250
-    // tokens, 32 heads on 8, behind 3000 and 6000, bf16: 295 so; 393 by tiles of the prefixes' rows, 58 of them the launch that adds up.
+    // Where sequences' own rows fill some tiles of the chunk kernel each, on average, there is little to win by others' beside them, and sums need not go through memory.  (One long chunk among
+    // single tokens does not make these full.)  us so / by tiles of the prefixes' rows and of what is behind them, by rows a sequence, 32 heads on 8 of 128, bf16: 160 (40 tokens for each of 64 behind 8000)
+    // 728 / 476, (63 tokens and a chunk of 2500) 800 / 495; 256 755 / 665; 400 (100 tokens behind 8000) 732 / 589, (1500) 128 / 109; 590 (16 chunks of 50 to 250 tokens behind 3000 and 6000, features x
+    // tokens) 273 to 283 / 275 to 302; 1000 506 / 416, (1500) 209 / 221; 2000 838 / 843, (1500) 366 / 457.  fp32, whose tiles are of 16 rows either way: 2000 1681 / 1554, but there sums are twice
+    // what the call reads and writes else.
     sh.rest = attend_shape(c, b, a);
+    const uint64_t filled = uint64_t(b->tokens) * (a->q_heads / c->heads) / b->sequences;
+    const bool full = c->dtype == HSPMM_TF32 ? filled >= 4096u : sh.rest.rows_log != kAttendRowsLog && filled >= 512u;
     // The same where all of it is little: a launch less.  us so / by tiles of prefixes and of what is behind them, a token each, 32 heads on 8, fp16, by MB of keys and values that the sequences'
     // own tiles read: 39 13.8 / 16.1, 72 16.7 / 19.7, 79 16.7 / 18.5, 92 20.4 / 18.0, 138 24.9 / 21.0; 12 heads on 4 of 64, fp32: 46 14.7 / 15.2, 69 19.8 / 21.8, 79 19.5 / 18.8, 144 27.9 / 22.6.
     const uint64_t rows = uint64_t(std::min(a->longest_chunk, b->tokens)) * (a->q_heads / c->heads), tiles = uint64_t(b->sequences) * ((rows + (1u << sh.rest.rows_log) - 1u) >> sh.rest.rows_log);
     const bool little = tiles * c->heads * all * c->head_dim * 2u * element_bytes(c->dtype) <= (uint64_t(80) << 20);
-    sh.both = little || (sh.rest.rows_log != kAttendRowsLog && rows >= 128u);
+    sh.both = little || full;
     if (sh.both) {
         sh.bytes = sh.rest.bytes;
         return sh;
@@ -415,16 +420,16 @@ static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     // Parts cost a row's sums each, written and read, but nobody waits for them.  us by keys of a prefix's part / of what is behind one's: 8 beams over 1000 keys by 128 / 256 / 512 / 1024 17.8 /
     // 15.6 / 16.1 / 19.9; 64 sequences of up to 1500 behind 8000 by 256 / 512 / 768 / 1024 / 1536 102 / 79 / 72 / 67 / 75, and with 1024 there by 256 / 512 / 1024 / 1536 75 / 69 / 67 / 70; fp32 drafts over
     // up to 6000 81 / 67 / - / 60 / 70 and 60 / 60 / 64 / -.
-    // Longer ones where tiles alone are workgroups for the chip - one and a half times those of the chunk kernel that run at a time, four times those of the rows kernel -, as sums are what parts cost
+    // Longer ones where tiles alone are workgroups for the chip - as many of the chunk kernel's as run at a time, four times as many of the rows kernel's -, as sums are what parts cost
     // then.  us (MB of workspace) by 1024 keys / 1024 / 768 / 512 workgroups of the chunk kernel, 32 heads on 8 of 128, bf16: 64 x 16 tokens behind 8000 243 (156) / 204 (87) / 193 (69) / 189 (52);
     // 256 x 8 538 (311) / 411 (104) / 414 (104) / 397 (69); 32 x 100 715 (487) / 545 (162) / 594 (108) / 593 (108); 63 tokens and a chunk of 1000 289 (180) / 250 (108) / 225 (72) / 253 (54); 128 x 16 behind
     // 32000 1696 (1142) / 1202 (138) / 1198 (104) / 1200 (104); 256 x 1 behind 128000 902 (549) / 668 (74) / 672 (56) / 670 (43).  By 1024 keys / 2048 workgroups of the rows kernel, fp32: 16 x 60 behind
-    // 4000 782 / 739, 16 x 64, 12 heads on 4 of 64, 185 / 181.
+    // 4000 782 / 739, 16 x 64, 12 heads on 4 of 64, 185 / 181.  (By 768 / 512, 18 such shapes were 2 % above the best on average with either, and 512 wants a third less.)
     auto spread = [&](const AttendShape &x, uint32_t sequences, uint64_t keys) {
         const uint64_t most = uint64_t(sequences) * ((uint64_t(std::min(&x == &sh.prefix ? (p->most_tokens ? p->most_tokens : b->tokens) : a->longest_chunk, b->tokens)) * shared + (1u << x.rows_log) - 1u) >> x.rows_log);
         // (whatever the call says, there are no fewer tiles than its rows fill)
         const uint64_t tiles = std::max<uint64_t>(std::min<uint64_t>(most, x.tiles), uint64_t(b->tokens) * shared >> x.rows_log);
-        const uint64_t cells = std::max<uint64_t>(tiles, 1u) * c->heads, at_a_time = x.rows_log == kAttendRowsLog ? 2048u : 768u;
+        const uint64_t cells = std::max<uint64_t>(tiles, 1u) * c->heads, at_a_time = x.rows_log == kAttendRowsLog ? 2048u : 512u;
         return std::max<uint64_t>(std::min<uint64_t>(std::max<uint64_t>(cells * keys / 128u, 256u), 1024u), cells * keys / at_a_time);
     };
     parts_of(sh.prefix, common, spread(sh.prefix, p->groups, common));

@@ -376,3 +376,31 @@ def test_heads_between_128_and_160(torch_cuda, hs, dtype, number):
     for layout in ("tokens", "features"):
         out, lse = c.run(torch, hs, attention, layout=layout)
         assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)
+
+
+# single tokens and long chunks in one batch, behind one prefix
+MIXED = [([14], [900], [5, 130, 33], [1] * 9 + [200] + [1] * 4, 0, 2, 4, 128, 16, 0, True), ([9, 6], [500, 1300], [40, 0], [1] * 4 + [333, 1, 2] + [1] * 7 + [64], 2, 2, 4, 64, 24, 0, True),
+         ([12], [700], [60, 9], [1] * 5 + [150] + [3] * 6, 0, 1, 8, 96, 32, 250, True), ([10], [640], [17], [1] * 9 + [180], 1, 2, 2, 256, 7, 0, True)]
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("number", range(len(MIXED)))
+def test_single_tokens_and_long_chunks_together(torch_cuda, hs, dtype, number):
+    torch = torch_cuda
+    CASES.append(MIXED[number])
+    try:
+        c = Case(torch, hs, dtype, len(CASES) - 1, order=number % 2)
+    finally:
+        CASES.pop()
+    want = c.want()
+    out, lse = c.run(torch, hs)
+    assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)
+    widened(torch, hs, c, 40000)
+    keys = c.st.wide.shape[1] * c.st.page_tokens
+    attention = c.hints(hs, int(c.new.max()), keys)
+    part = c.q.shape[0] * c.q.shape[1] * (c.dim + 4) * 4
+    need = c.st.handle.attend_shared_workspace(c.batch, c.prefixes(hs), attention)
+    assert need > 4 * 16384 and (need - 4 * 16384) % part == 0
+    for layout in ("tokens", "features"):
+        out, lse = c.run(torch, hs, attention, layout=layout)
+        assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)

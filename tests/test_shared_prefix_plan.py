@@ -37,3 +37,22 @@ def test_sums_are_no_more_than_the_rows_and_a_launch_of_tiles(hs, dtype, seed):
         got, plain, part = planned(hs, dtype, groups, chunks, prefix, behind, heads, shared, dim, hint=hint)
         rows = part // (4 * (dim + 4))
         assert got <= max(plain, COUNTERS + (4 * 768 * 128 + 4 * rows) * (dim + 4) * 4), (got / part, got, plain)
+
+
+def by_prefixes(got, plain, part):
+    """Whether a call goes by tiles of the prefixes' rows: it leaves sums of all rows, and plain attention's tiles leave others."""
+    return got != plain and got > COUNTERS and (got - COUNTERS) % part == 0
+
+
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("chunk", [1, 31, 32, 33, 200, 1000, 2500])
+def test_a_long_chunk_takes_the_prefix_from_no_single_token(hs, dtype, chunk):
+    assert by_prefixes(*planned(hs, dtype, 1, [1] * 63 + [chunk], 8000, 300, 8, 4, 128))
+    assert by_prefixes(*planned(hs, dtype, 2, [1] * 40 + [chunk] + [2] * 23, 6000, 700, 4, 8, 64))
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_chunks_that_fill_tiles_leave_no_sums(hs, dtype):
+    for chunks in ([4096] * 8, [1500, 1200, 1100], [2000] * 3):
+        got, plain, _ = planned(hs, dtype, 1, chunks, 16000, 300, 8, 4, 128)
+        assert got == plain

@@ -391,11 +391,14 @@ static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, cons
     // tokens) 273 to 283 / 275 to 302; 1000 506 / 416, (1500) 209 / 221; 2000 838 / 843, (1500) 366 / 457.  fp32, whose tiles are of 16 rows either way: 2000 1681 / 1554, but there sums are twice
     // what the call reads and writes else.
     sh.rest = attend_shape(c, b, a);
-    const uint64_t filled = uint64_t(b->tokens) * (a->q_heads / c->heads) / b->sequences;
+    const uint64_t all_rows = uint64_t(b->tokens) * (a->q_heads / c->heads), filled = all_rows / b->sequences;
     const bool full = c->dtype == HSPMM_TF32 ? filled >= 4096u : sh.rest.rows_log != kAttendRowsLog && filled >= 512u;
     // The same where all of it is little: a launch less.  us so / by tiles of prefixes and of what is behind them, a token each, 32 heads on 8, fp16, by MB of keys and values that the sequences'
     // own tiles read: 39 13.8 / 16.1, 72 16.7 / 19.7, 79 16.7 / 18.5, 92 20.4 / 18.0, 138 24.9 / 21.0; 12 heads on 4 of 64, fp32: 46 14.7 / 15.2, 69 19.8 / 21.8, 79 19.5 / 18.8, 144 27.9 / 22.6.
-    const uint64_t rows = uint64_t(std::min(a->longest_chunk, b->tokens)) * (a->q_heads / c->heads), tiles = uint64_t(b->sequences) * ((rows + (1u << sh.rest.rows_log) - 1u) >> sh.rest.rows_log);
+    // (no fewer tiles than rows fill, and as many as are numbered where the longest chunk is not told)
+    const uint64_t rows = uint64_t(std::min(a->longest_chunk, b->tokens)) * (a->q_heads / c->heads);
+    const uint64_t told = a->longest_chunk ? uint64_t(b->sequences) * ((rows + (1u << sh.rest.rows_log) - 1u) >> sh.rest.rows_log) : sh.rest.tiles;
+    const uint64_t tiles = std::max<uint64_t>(std::min<uint64_t>(told, sh.rest.tiles), all_rows >> sh.rest.rows_log);
     const bool little = tiles * c->heads * all * c->head_dim * 2u * element_bytes(c->dtype) <= (uint64_t(80) << 20);
     sh.both = little || full;
     if (sh.both) {

@@ -56,3 +56,10 @@ def test_chunks_that_fill_tiles_leave_no_sums(hs, dtype):
     for chunks in ([4096] * 8, [1500, 1200, 1100], [2000] * 3):
         got, plain, _ = planned(hs, dtype, 1, chunks, 16000, 300, 8, 4, 128)
         assert got == plain
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_hints_that_are_not_there_leave_large_calls_their_prefixes(hs, dtype):
+    for groups, chunks in ((1, [1] * 64), (4, [1, 2, 3, 4] * 20), (2, [20] * 30)):
+        for hint in ((0, 0, 0, 0), (0, 9000, 0, 8000), (1, 9000, 0, 0)):
+            assert by_prefixes(*planned(hs, dtype, groups, chunks, 8000, 300, 8, 4, 128, hint=hint))

@@ -614,14 +614,21 @@ int hspmm_cache_compact(const hspmm_cache *cache, int32_t *table_out, int32_t *r
 
 }  // extern "C"
 
-// tokens, sequences: that a head's row has at least, and that have rows which are written at a time (rows side by side are written by different workgroups).
+// tokens, sequences: that a head's row has at least, and that have rows which are written at a time (rows side by side are written by different workgroups): from the smallest stride to the
+// largest each passes all rows of those below it.
 static int check_weights(const hspmm_cache *c, const hspmm_weights *w, uint64_t tokens, uint32_t sequences, uint32_t layers)
 {
     if (!w || !w->data) return fail(HSPMM_ERR_INVALID, "null weights");
     if (reinterpret_cast<uintptr_t>(w->data) % 4u) return fail(HSPMM_ERR_INVALID, "weights are not aligned to their elements");
     if (w->layer_stride < 0 || w->sequence_stride < 0 || w->head_stride < 0) return fail(HSPMM_ERR_INVALID, "weights: strides below 0");
-    if ((c->heads > 1u && uint64_t(w->head_stride) < tokens) || (sequences > 1u && uint64_t(w->sequence_stride) < tokens) || (layers > 1u && uint64_t(w->layer_stride) < tokens))
-        return fail(HSPMM_ERR_INVALID, "weights: rows of %llu tokens that overlap", (unsigned long long)tokens);
+    std::pair<uint64_t, uint32_t> rows[3] = {{uint64_t(w->head_stride), c->heads}, {uint64_t(w->sequence_stride), sequences}, {uint64_t(w->layer_stride), layers}};
+    std::sort(rows, rows + 3);
+    unsigned __int128 reach = tokens;
+    for (const auto &r : rows) {
+        if (r.second <= 1u) continue;
+        if (r.first < reach) return fail(HSPMM_ERR_INVALID, "weights: rows of %llu tokens that overlap", (unsigned long long)tokens);
+        reach += static_cast<unsigned __int128>(r.first) * (r.second - 1u);
+    }
     return HSPMM_OK;
 }
 

@@ -130,3 +130,14 @@ def test_an_eviction_of_very_many_tokens_has_room_for_its_pages(hs):
     assert c.evict_workspace(1, keep) >= 4 * (2 * keep + 256 + 128 + 128)
     for keep in (0x80000000, 0xFFFFFFFF):
         refused(hs, 1, lambda: c.evict_workspace(1, keep), "keep")
+
+
+def test_rows_of_weights_that_meet_others_of_another_kind_are_refused(hs):
+    # (2 layers of 3 sequences of 4 heads of 64 tokens; each stride passes a row, but a head's rows are where another sequence's or layer's are)
+    c = cache(hs)
+    ok = dict(workspace=ADDRESS, workspace_bytes=c.evict_workspace(2, 8))
+    for bad in ((768, 64, 64), (64, 256, 64), (64, 64, 256), (256, 256, 64), (767, 256, 64), (768, 255, 64), (191, 384, 64), (768, 64, 191)):
+        refused(hs, 1, lambda: c.evict(2, ADDRESS, 0, hs.Weights(ADDRESS, *bad), 8, **ok), "overlap")
+    # in any order, and with something between: refused for what comes behind
+    for good in ((768, 256, 64), (64, 512, 128), (256, 512, 64), (64, 128, 384), (5000, 300, 70), (1 << 62, 1 << 60, 64)):
+        refused(hs, 1, lambda: c.evict(2, ADDRESS, 0, hs.Weights(ADDRESS, *good), 8), "workspace")

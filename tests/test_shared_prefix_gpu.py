@@ -404,3 +404,77 @@ def test_single_tokens_and_long_chunks_together(torch_cuda, hs, dtype, number):
     for layout in ("tokens", "features"):
         out, lse = c.run(torch, hs, attention, layout=layout)
         assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)
+
+
+class LongCase(Case):
+    """The same with rows of the table that have places for so many keys that the call goes by tiles of the prefixes' rows and of what is behind them; a call without other hints is
+    looked at for it."""
+    def __init__(self, torch, hs, dtype, number, *args, **kw):
+        super().__init__(torch, hs, dtype, number, *args, **kw)
+        widened(torch, hs, self, -(-(1 << 27) // (self.n * self.st.heads * self.dim * 2 * (4 if dtype == 1 else 2))))
+        self.st.table = self.st.wide
+        self.attention = self.hints(hs, int(self.new.max()), self.st.wide.shape[1] * self.st.page_tokens)
+        part = self.q.shape[0] * self.q.shape[1] * (self.dim + 4) * 4
+        need = self.st.handle.attend_shared_workspace(self.batch, self.prefixes(hs), self.attention)
+        assert need > 4 * 16384 and (need - 4 * 16384) % part == 0 and need != self.st.handle.attend_workspace(self.batch, self.attention)
+
+
+@pytest.fixture
+def long_cases(monkeypatch):
+    import sys
+    monkeypatch.setattr(sys.modules[__name__], "Case", LongCase)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("number", range(len(CASES)))
+def test_attend_shared_by_prefix_tiles(torch_cuda, hs, long_cases, dtype, number):
+    test_attend_shared(torch_cuda, hs, dtype, number)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("number", [2, 3, 6, 8, 10, 14])
+def test_pages_that_are_gone_by_prefix_tiles(torch_cuda, hs, long_cases, dtype, number):
+    test_pages_that_are_gone_are_not_seen(torch_cuda, hs, dtype, number)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_chunks_that_begin_within_the_prefix_by_prefix_tiles(torch_cuda, hs, long_cases, dtype):
+    test_chunks_that_begin_within_the_prefix(torch_cuda, hs, dtype)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("number", [3, 6, 8, 9])
+def test_what_is_masked_by_prefix_tiles(torch_cuda, hs, long_cases, dtype, number):
+    test_what_is_masked_does_not_reach_the_result(torch_cuda, hs, dtype, number)
+
+
+@pytest.mark.parametrize("number", [2, 3, 6, 13])
+def test_bad_numbers_by_prefix_tiles(torch_cuda, hs, long_cases, number):
+    test_bad_numbers_stay_within_the_arrays(torch_cuda, hs, number)
+
+
+def test_a_captured_call_and_two_workspaces_by_prefix_tiles(torch_cuda, hs, long_cases):
+    test_a_captured_call_and_two_workspaces(torch_cuda, hs)
+
+
+def test_one_workspace_serves_every_call_by_prefix_tiles(torch_cuda, hs, long_cases):
+    test_one_workspace_serves_every_call_in_turn(torch_cuda, hs)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("kind", [Case, LongCase])
+@pytest.mark.parametrize("number", [2, 3, 6, 8])
+def test_rows_of_groups_that_are_none_read_their_own_pages(torch_cuda, hs, dtype, kind, number):
+    # every group is out of order or has no tokens: each row is attended by its own pages
+    torch = torch_cuda
+    c = kind(torch, hs, dtype, number, seed=6)
+    for b in range(c.n):
+        for which, x in ((0, c.k), (1, c.v)):
+            c.st.store(0, int(c.rows[b]), which, x[b])
+    want = c.want()
+    for firsts, tokens in (([-5] * len(c.firsts), c.prefix), ([c.n + 3] * len(c.firsts), c.prefix), ([c.n - 1 - i for i in range(len(c.firsts))], c.prefix), ([0x7FFFFFFF] * len(c.firsts), c.prefix),
+                           (c.firsts, np.full(len(c.prefix), -1)), (c.firsts, np.zeros(len(c.prefix))), (c.firsts, np.full(len(c.prefix), -0x80000000))):
+        c.fd.copy_(ints(torch, firsts))
+        c.pd.copy_(ints(torch, tokens))
+        out, lse = c.run(torch, hs)
+        assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)

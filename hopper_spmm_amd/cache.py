@@ -161,7 +161,8 @@ class Cache:
         return n.value
 
     def attend_shared(self, layer, batch, prefix, attention, q, out, lse=0, workspace=0, workspace_bytes=0, stream=0):
-        """hspmm_cache_attend_shared: `attend` of groups of sequences that begin with the same tokens, whose keys and values are read once."""
+        """hspmm_cache_attend_shared: `attend` of groups of sequences that begin with the same tokens, whose keys and values are read by the first
+        one's pages, and once for all of a group where each sequence has few new tokens."""
         rc = self._attend_shared(self._c, layer, batch, prefix, attention, q, out, lse, workspace, workspace_bytes, stream)
         if rc:
             _check(rc)

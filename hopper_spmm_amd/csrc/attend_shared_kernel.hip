@@ -5,6 +5,7 @@
 // Prefixes are bound by matrix instructions or by the L2, what is behind them by memory, so both run at a time: workgroups of the prefixes come first, as they are the longer ones.
 // A token for each of 64 sequences of up to 1500 keys behind 8000, 32 heads on 8 of 128, bf16: 57.6 us, and 10.7 to add up 17 MB of sums (one behind the other 94; by attention alone, which reads the prefix 64 times, from the L2 as far as it goes, 232);
 // drafts of up to 12 tokens over 5 prompts of up to 6000, 12 heads on 4 of 64, fp32, 60 + 7.6.
+// Registers are short with heads of 161 to 256 elements, whose one wave a SIMD has 512: of 16-bit types 50 to 131 of them lie in memory where either kind of tile is of 128 rows, of fp32 94 to 98.
 #include "attend_rows.hpp"
 #include "attend_chunk.hpp"
 
@@ -116,7 +117,8 @@ void launch_kinds(const AttendArgs &prefix, const AttendArgs &rest, bool prefix_
         if (prefix_chunk && rest_chunk) return attend_shared_kernel<K, BF, DR, DC, Whole, true, true><<<grid, threads, 0, s>>>(prefix, rest);
         if (prefix_chunk) return attend_shared_kernel<K, BF, DR, DC, Whole, true, false><<<grid, threads, 0, s>>>(prefix, rest);
     }
-    attend_shared_kernel<K, BF, DR, DC, Whole, false, false><<<grid, threads, 0, s>>>(prefix, rest);
+    // (heads that the chunk kernel's part has a form of its own for come here with tiles of it only)
+    if constexpr (DR == DC) attend_shared_kernel<K, BF, DR, DC, Whole, false, false><<<grid, threads, 0, s>>>(prefix, rest);
 }
 
 template <class K, bool BF, int DR, int DC>

@@ -2,10 +2,13 @@
 //
 // Per layer, list entry and head of keys: of the tokens that the parent has stored, those that are kept anyway (the first and the last ones) and, of the others, those of the
 // greatest weights, ties to the lowest number.  The smallest weight that is taken is found digit by digit (2048, 2048 and 1024 values of a
-// digit) from counts in LDS, so a row of weights is read four times, from memory once.  Then slot k of the child receives the k-th token kept.
+// digit) from counts in LDS.  Up to 16384 tokens each weight is read once, into a register; of more once a digit, and once more for the list.  Then slot k of the child receives the k-th token kept.
 //
 // In place - a sequence that is its own child, its pages named by nobody else - no token moves to a higher slot, so a workgroup that has all tokens of a column and
 // loads a set of them before it stores the set in front loses none.  Everything else goes to new pages, by as many workgroups as like.
+// Columns are shares of 64 bytes and more, and sets wait for each other, so moving all is slower than into other pages, but what keeps its place is not moved: us into others / in place (keys, values and
+// weights last used long ago), 12 sequences, 8 layers of 8 heads of 128, bf16: 1024 of up to 8000 tokens 246 / 285, 1024 of 1025 227 / 123; 32 sequences, 32 layers, 1024 of up to 1040 1953 / 1100;
+// 4 of 8192 of up to 60000 749 / 891.
 // Two launches, as which pages are free has to be known before one is written (page_kernels.hip).
 // Moving is memory's: 1024 of up to 8000 tokens of 12 prompts, 8 layers of 8 heads of 128, bf16, 179 us for 0.8 GB, 4.5 TB/s in rows of 256 bytes that lie apart (a copy: 4.8); four rows a thread on their way
 // (two or eight: slower), stores past the L2.  Choosing is a chain of sums over the workgroup and of counts, 10 us for 700 tokens and 35 there, so each weight stays in a register (16 a thread) for all digits, and tokens follow each other in

@@ -615,16 +615,20 @@ int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *ba
 
 /* Groups of a batch's rows whose sequences begin with the same tokens (a system prompt, the prompt of several beams):
  * rows firsts[g] .. firsts[g + 1] - 1 of the batch share the first tokens[g] tokens, which are read by the table row of the group's
- * first sequence, once for all of them (at most the tokens that it holds).  The other sequences' own pages of these
+ * first sequence (at most the tokens that it holds).  The other sequences' own pages of these
  * tokens are not read.  Rows of the batch that are in no group share nothing.  firsts ascends.
  * most_tokens: the most tokens of the batch that a group has; longest: of a prefix (0: not known); they choose kernels and how the work
- * is split, the result is right whatever they are. */
+ * is split, as the attention's longest_chunk and longest do (0: not known), the result is right whatever they are. */
 typedef struct hspmm_prefix {
     uint32_t groups, most_tokens, longest;
     const int32_t *firsts, *tokens;
 } hspmm_prefix;
-/* hspmm_cache_attend with the groups' prefixes read once.  No groups: the same call.  workspace: as for attend, of
- * hspmm_cache_attend_shared_workspace bytes, zero before its first use; one of the largest size serves attend, attend_shared, weigh and evict in turn. */
+/* hspmm_cache_attend of groups with their prefixes.  No groups: the same call.
+ * Where few rows a sequence meet long prefixes - new tokens, drafts, one chunk among them -, tiles of all of a group's rows read its prefix once for a tile of up to 128 rows.  Where sequences have
+ * rows enough to fill tiles of their own (512 and more on average - tokens times the query heads that share keys -; fp32: 4096), and where all that their own tiles read is at most
+ * 80 MB, these read it by the first sequence's pages, each for itself: as attend does, and no faster than attend where a sequence's own pages have the prefix as well (after hspmm_cache_fork they do).
+ * workspace: as for attend, of hspmm_cache_attend_shared_workspace bytes, zero before its first use; in the first kind of call a row's sums in fp32 for each of its parts of keys, which are no more than
+ * four times those of all rows and, for heads of 128, 140 MB.  One of the largest size serves attend, attend_shared, weigh and evict in turn. */
 int hspmm_cache_attend_shared(const hspmm_cache *cache, uint32_t layer, const hspmm_batch *batch, const hspmm_prefix *prefix, const hspmm_attention *attention,
                               const hspmm_heads *q, const hspmm_heads *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream);
 int hspmm_cache_attend_shared_workspace(const hspmm_cache *cache, const hspmm_batch *batch, const hspmm_prefix *prefix, const hspmm_attention *attention, uint64_t *bytes);
@@ -632,7 +636,7 @@ int hspmm_cache_attend_shared_workspace(const hspmm_cache *cache, const hspmm_ba
 /* The attention weight that cached keys have received: floats, layers x sequences x heads (of keys) at these strides (in
  * floats), a head's tokens side by side: those that a sequence holds, for hspmm_cache_evict table_pages * page_tokens of them.  The
  * caller's, zero at first; a row follows its sequence through hspmm_cache_evict, and is the caller's to copy or to clear where a
- * sequence is forked or freed. */
+ * sequence is forked or freed.  No two rows overlap: from the smallest stride to the largest, each passes all rows of those below it. */
 typedef struct hspmm_weights {
     float *data;
     int64_t layer_stride, sequence_stride, head_stride;

@@ -23,7 +23,7 @@ def planned(hs, dtype, groups, chunks, prefix, behind, heads, shared, dim, page=
 @pytest.mark.parametrize("seed", range(60))
 def test_sums_are_no_more_than_the_rows_and_a_launch_of_tiles(hs, dtype, seed):
     # A prefix and what is behind it are in P <= W / cells + 2 parts each, W workgroups of the chip and cells >= 1 tiles and heads, of R rows; there are no more than R (cells + heads) rows, and
-    # heads are no more than cells.  So rows times parts are at most 2 W R + 2 rows of either, W R = 768 x 128 or 2048 x 16.
+    # heads are no more than cells.  So rows times parts are at most 2 W R + 2 rows of either, W R = 512 x 128 or 2048 x 16.
     rng = random.Random(seed)
     cases = [(1, [4096] * 8, 16000, 300, 8, 4, 128), (1, [1000] * 16, 8000, 300, 8, 4, 128), (1, [250] * 16, 6000, 300, 8, 4, 128), (1, [16] * 128, 16000, 300, 8, 4, 128),
              (1, [8] * 256, 8000, 300, 8, 4, 128), (1, [1] * 256, 128000, 300, 8, 4, 128)]
@@ -36,7 +36,7 @@ def test_sums_are_no_more_than_the_rows_and_a_launch_of_tiles(hs, dtype, seed):
     for hint in (None, (1, 0, 1, 1), (0, 0, 0, 0), (100000, 0, 100000, 0)):
         got, plain, part = planned(hs, dtype, groups, chunks, prefix, behind, heads, shared, dim, hint=hint)
         rows = part // (4 * (dim + 4))
-        assert got <= max(plain, COUNTERS + (4 * 768 * 128 + 4 * rows) * (dim + 4) * 4), (got / part, got, plain)
+        assert got <= max(plain, COUNTERS + (4 * 512 * 128 + 4 * rows) * (dim + 4) * 4), (got / part, got, plain)
 
 
 def by_prefixes(got, plain, part):

@@ -616,7 +616,7 @@ int hspmm_cache_attend_workspace(const hspmm_cache *cache, const hspmm_batch *ba
 /* Groups of a batch's rows whose sequences begin with the same tokens (a system prompt, the prompt of several beams):
  * rows firsts[g] .. firsts[g + 1] - 1 of the batch share the first tokens[g] tokens, which are read by the table row of the group's
  * first sequence (at most the tokens that it holds).  The other sequences' own pages of these
- * tokens are not read.  Rows of the batch that are in no group share nothing.  firsts ascends.
+ * tokens are not read.  Rows of the batch that are in no group share nothing.  firsts ascends; there are no more groups than sequences in the batch.
  * most_tokens: the most tokens of the batch that a group has; longest: of a prefix (0: not known); they choose kernels and how the work
  * is split, as the attention's longest_chunk and longest do (0: not known), the result is right whatever they are. */
 typedef struct hspmm_prefix {

@@ -478,3 +478,24 @@ def test_rows_of_groups_that_are_none_read_their_own_pages(torch_cuda, hs, dtype
         c.pd.copy_(ints(torch, tokens))
         out, lse = c.run(torch, hs)
         assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("kind", [Case, LongCase])
+@pytest.mark.parametrize("number", [3, 6, 8, 9, 13])
+def test_rows_in_front_of_the_first_group_and_behind_the_last(torch_cuda, hs, dtype, kind, number):
+    # some of the groups only, and groups without rows among them: the other rows are attended by their own pages
+    torch = torch_cuda
+    c = kind(torch, hs, dtype, number, seed=8)
+    for b in range(c.n):
+        for which, x in ((0, c.k), (1, c.v)):
+            c.st.store(0, int(c.rows[b]), which, x[b])
+    want = c.want()
+    f, p = list(c.firsts), list(c.prefix)
+    for firsts, prefixes in ((f[:-1], p[:-1]), (f[1:], p[1:]), (f[:2], p[:1]), ([f[0]] + f, [5] + p), (f + [f[-1]], p + [9]), (f[:2] + f[1:], p[:1] + [7] + p[1:])):
+        if not 1 <= len(prefixes) <= c.n:                   # (no more groups than rows)
+            continue
+        fd, pd = ints(torch, firsts), ints(torch, prefixes)
+        prefix = hs.Prefix(len(prefixes), fd.data_ptr(), pd.data_ptr(), **c.hint)
+        out, lse = c.run(torch, hs, prefix=prefix)
+        assert_attended(dtype, out, lse, want, c.k, c.v, c.dim)

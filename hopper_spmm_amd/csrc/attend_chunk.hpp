@@ -27,7 +27,7 @@ __device__ __forceinline__ void lds_barrier()
 // multiplied, n + 1 is there and n + 2 on its way, first to registers, then to the place of n - 1; one barrier an image (with two places: two).
 // Lds<N>: chunk_lds(DP, W) bytes or more; number: of the workgroup among so many `numbers`; part: of its keys.
 // What one kind of call has alone stands behind `if constexpr`, and LDS is named, not pointed to: registers are short with heads of 256 elements.  1024 tokens over 2048 older keys, 16 heads on 4
-// of 256, bf16, pages of 24 tokens, 158 us with conditions that are never true and a pointer, 147 so; pages of 16 149 and 151 (without prefixes in the body at all 137 and 155).
+// of 256, bf16, pages of 24 tokens, 158 us with conditions that are never true and a pointer, 142 so; pages of 16 149 and 151 (without prefixes in the body at all 137 and 155).
 constexpr uint32_t chunk_image(int DP) { return 64u * (uint32_t(DP) * 2u + 16u + uint32_t(DP) * 2u + (DP % 128 == 0 || DP == 64 ? 64u : 0u)); }
 constexpr uint32_t chunk_ring(int DP, int W) { return 3u * chunk_image(DP) <= (DP <= 128 && W == 4 ? 80u : 160u) * 1024u - 256u ? 3u : 2u; }
 constexpr uint32_t chunk_lds(int DP, int W) { return chunk_ring(DP, W) * chunk_image(DP) + (uint32_t(W) * 12u + 15u) / 16u * 16u; }
@@ -54,7 +54,9 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, uint32_t numb
     if (!t.there) return;
     const KeyPart keys_here = key_part(aa, t, part);
     constexpr bool kJoins = Span == kSpanAll || Span == kSpanBoth;
-    const int32_t parts = kJoins ? keys_here.parts : 1, end = keys_here.end;
+    // (where pages are no multiples of 16 tokens what is alike in all lanes is kept in scalar registers: 1024 tokens over 2048 older keys, heads of 256, 147 -> 142 us; else 151 -> 160)
+    auto uniform = [](int32_t x) __attribute__((always_inline)) { return Whole ? x : __builtin_amdgcn_readfirstlane(x); };
+    const int32_t parts = kJoins ? keys_here.parts : 1, end = uniform(keys_here.end);
     if (int32_t(part) >= keys_here.parts) return;
     if (tid == 0u) odd = 0u;
 
@@ -113,7 +115,7 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, uint32_t numb
         if constexpr (Span == kSpanRest) group_lo = max(group_lo, t.prefix);
     }
     // (rows of several sequences: from the first key that any of them sees)
-    const int32_t begin = Span == kSpanPrefix ? max(keys_here.begin, min(any_lo & ~31, end)) : keys_here.begin;
+    const int32_t begin = uniform(Span == kSpanPrefix ? max(keys_here.begin, min(any_lo & ~31, end)) : keys_here.begin);
     // Images of 64 keys: of the prefix (kSpanBoth), by its first sequence's pages, then of what is behind it, from where a group of 16 begins.
     int32_t first_images = 0, behind = begin, n_images = end > begin ? (end - begin + 63) / 64 : 0;
     if constexpr (Span == kSpanBoth) {
@@ -168,12 +170,20 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, uint32_t numb
     };
     auto piece_column = [&](int i) __attribute__((always_inline)) { return (tid + kThreads * i) % kRowPieces * 8u; };
     auto is_piece = [&](int i) __attribute__((always_inline)) { return kImagePieces % kThreads == 0u || tid + kThreads * i < kImagePieces; };
-    uint32_t in_group[kPieces];
+    // A piece's bytes from where its group of 16 begins (Whole), or its key: the latter is made anew, and is one for all of a thread's pieces where its columns are.
+    uint32_t in_group_of[Whole ? kPieces : 1];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < (Whole ? kPieces : 1); ++i) {
         const uint32_t c = piece_column(i);
-        in_group[i] = (Whole ? uint32_t(int64_t(piece_row(i) % 16u) * aa.pages.token_stride) * 2u : 0u) + (c < D ? c : 0u) * 2u;
+        in_group_of[i] = (Whole ? uint32_t(int64_t(piece_row(i) % 16u) * aa.pages.token_stride) * 2u : 0u) + (c < D ? c : 0u) * 2u;
     }
+    auto in_group = [&](int i) __attribute__((always_inline)) {
+        if constexpr (Whole || kThreads % kRowPieces == 0u) return in_group_of[Whole ? i : 0];
+        else {
+            const uint32_t c = piece_column(i);
+            return (c < D ? c : 0u) * 2u;
+        }
+    };
     auto request = [&](int32_t n) __attribute__((always_inline)) {
         if constexpr (Whole) {
             if (n % 16 == 0) look_up(n + int32_t(lane / 4u), int32_t(lane % 4u) * 16);
@@ -197,8 +207,8 @@ __device__ __forceinline__ void attend_chunk(const AttendArgs &aa, uint32_t numb
                 const int at = int(piece_row(i));
                 from = uint64_t(uint32_t(__shfl(int(ahead_low), at))) | uint64_t(uint32_t(__shfl(int(ahead_high), at))) << 32;
             }
-            k_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.keys + from + in_group[i]);
-            v_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.values + from + in_group[i]);
+            k_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.keys + from + in_group(i));
+            v_piece[i] = *reinterpret_cast<const u32x4 *>(aa.pages.values + from + in_group(i));
         }
     };
     // the stored keys of image n, which is in the registers

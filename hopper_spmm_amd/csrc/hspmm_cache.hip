@@ -385,8 +385,8 @@ static SharedShape shared_shape(const hspmm_cache *c, const hspmm_batch *b, cons
 {
     SharedShape sh{};
     const uint64_t all = most_keys(c, a->longest), common = std::min<uint64_t>(p->longest ? p->longest : all, all);
-    // Where sequences' own rows fill some tiles of the chunk kernel each, on average, there is little to win by others' beside them, and sums need not go through memory.  (One long chunk among
-    // single tokens does not make these full.)  us so / by tiles of the prefixes' rows and of what is behind them, by rows a sequence, 32 heads on 8 of 128, bf16: 160 (40 tokens for each of 64 behind 8000)
+    // Where sequences' own rows fill some tiles of the chunk kernel each, on average, there is little to win by others' beside them, and sums need not go through memory.  (A chunk of some thousand
+    // tokens among 63 single ones does not make these full.)  us so / by tiles of the prefixes' rows and of what is behind them, by rows a sequence, 32 heads on 8 of 128, bf16: 160 (40 tokens for each of 64 behind 8000)
     // 728 / 476, (63 tokens and a chunk of 2500) 800 / 495; 256 755 / 665; 400 (100 tokens behind 8000) 732 / 589, (1500) 128 / 109; 590 (16 chunks of 50 to 250 tokens behind 3000 and 6000, features x
     // tokens) 273 to 283 / 275 to 302; 1000 506 / 416, (1500) 209 / 221; 2000 838 / 843, (1500) 366 / 457.  fp32, whose tiles are of 16 rows either way: 2000 1681 / 1554, but there sums are twice
     // what the call reads and writes else.
